@@ -29,6 +29,13 @@ ABORT_TOKEN = 0x10
 ABORT_ATTN_WAIT = 0x20
 ABORT_BAD_ID = 0x40
 ABORT_STEP_WAIT = 0x80
+ABORT_NO_PAGE = 0x100
+ABORT_BAD_PAGE = 0x200
+
+CACHE_ROW = 576
+CACHE_PAGE_TOKENS = 64
+CACHE_BLOCK_TOKENS = 16
+CACHE_PAGE_BYTES = 36992
 
 
 class FleetMoeDims(ctypes.Structure):
@@ -61,6 +68,13 @@ class FleetStepModel(ctypes.Structure):
     _fields_ = [("layers", c_void_p), ("n_layers", c_int32), ("max_pos", c_int32),
                 ("embed", c_void_p), ("final_norm", c_void_p), ("lm_head", c_void_p),
                 ("rope_cos", c_void_p), ("rope_sin", c_void_p)]
+
+
+class FleetCache(ctypes.Structure):
+    """struct fleet_cache (device pointers)."""
+    _fields_ = [("pool", c_void_p), ("table", c_void_p), ("lens", c_void_p), ("refs", c_void_p),
+                ("n_pages", c_int32), ("n_layers", c_int32), ("n_seqs", c_int32),
+                ("max_pages", c_int32)]
 
 
 # (name, restype, argtypes) of every symbol the header declares.
@@ -108,6 +122,23 @@ SYMBOLS = [
     ("fleet_lm_head_argmax", c_int,
      [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
       c_size_t, POINTER(FleetMoeDims), c_void_p]),
+    ("fleet_cache_workspace_bytes", c_size_t, [c_int32, c_int32]),
+    ("fleet_cache_remap", c_int, [POINTER(FleetCache), c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("fleet_cache_grow", c_int, [POINTER(FleetCache), c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("fleet_cache_compact", c_int, [POINTER(FleetCache), c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("fleet_cache_append", c_int,
+     [POINTER(FleetCache), c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int32,
+      c_void_p, c_size_t, c_void_p]),
+    ("fleet_cache_read", c_int,
+     [POINTER(FleetCache), c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int32,
+      c_void_p, c_size_t, c_void_p]),
+    ("fleet_cache_attend", c_int,
+     [POINTER(FleetCache), c_int32, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32,
+      c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("fleet_beam_workspace_bytes", c_size_t, [c_int32, c_int32, c_int32, c_int32]),
+    ("fleet_beam_select", c_int,
+     [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,
+      c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     ("fleet_moe_stream_read", c_int, [c_void_p, c_size_t, c_void_p, c_void_p]),
     ("fleet_moe_workspace_status", c_int, [c_void_p, POINTER(c_uint32), c_void_p]),
     ("fleet_moe_error_string", c_char_p, [c_int]),

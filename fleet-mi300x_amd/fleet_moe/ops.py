@@ -51,6 +51,33 @@ def _need(t: torch.Tensor, dtype, shape, name: str) -> None:
                          f"got {t.dtype} {tuple(t.shape)}")
 
 
+class _Here:
+    """The context of a call whose tensors are on the current device: none."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(device: torch.device):
+    """A context in which `device` is the current one: launches go there, and a
+    call without a stream takes that device's current one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+def _same_device(owner: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != owner.device:
+            raise ValueError(f"{name} is on {t.device}, not on {owner.device}")
+
+
 @dataclass
 class DeviceLayer:
     """One packed MoE layer resident in device memory."""
@@ -369,6 +396,54 @@ class AttnDecoder:
                                                     _stream(stream))
         _lib.check(rc, "fleet_moe_workspace_status")
         return int(v.value)
+
+
+class BeamSelector:
+    """The best continuations of groups of beams (fleet_beam_select), beside
+    lm_head_into()'s single greedy pick, with its own workspace. Calls on one
+    selector must be ordered on one stream."""
+
+    def __init__(self, n_groups: int, n_beams: int, n_out: int | None = None,
+                 vocab: int | None = None, eos: int = -1, device="cuda"):
+        from .layout import VOCAB
+        self.n_groups, self.n_beams = int(n_groups), int(n_beams)
+        self.n_out = self.n_beams if n_out is None else int(n_out)
+        self.vocab = VOCAB if vocab is None else int(vocab)
+        self.eos = int(eos)
+        n = _lib.load().fleet_beam_workspace_bytes(self.n_groups, self.n_beams, self.n_out,
+                                                   self.vocab)
+        if n == 0 or self.eos >= self.vocab:
+            raise ValueError(f"unsupported beam sizes: {self.n_groups} groups of {self.n_beams} "
+                             f"beams, {self.n_out} out, vocab {self.vocab}, eos {self.eos}")
+        self.workspace = torch.empty(n, dtype=torch.uint8, device=device)
+
+    def select(self, logits: torch.Tensor, scores: torch.Tensor,
+               finished: torch.Tensor | None = None, stream=None) -> dict:
+        """logits fp32 [groups * beams, vocab] (unit column stride), scores fp32
+        [groups, beams], finished uint8 [groups, beams] or None. Returns
+        dict(scores fp32, parents int32, tokens int32, finished uint8), each
+        [groups, n_out], best first; a parent is a row of logits."""
+        g, b, k = self.n_groups, self.n_beams, self.n_out
+        if (not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2
+                or logits.shape != (g * b, self.vocab) or logits.stride(1) != 1
+                or (g * b > 1 and logits.stride(0) < self.vocab)):
+            raise ValueError(f"logits: expected fp32 [{g * b}, {self.vocab}] on the device with "
+                             f"unit column stride, got {logits.dtype} {tuple(logits.shape)}")
+        _need(scores, torch.float32, (g, b), "scores")
+        if finished is not None:
+            _need(finished, torch.uint8, (g, b), "finished")
+        _same_device(self.workspace, logits=logits, scores=scores, finished=finished)
+        out = torch.empty((g, k), dtype=torch.float32, device=logits.device)
+        picks = torch.empty((2, g, k), dtype=torch.int32, device=logits.device)
+        ended = torch.empty((g, k), dtype=torch.uint8, device=logits.device)
+        with _on(self.workspace.device):
+            rc = _lib.load().fleet_beam_select(
+                _ptr(logits), max(int(logits.stride(0)), self.vocab), _ptr(scores),
+                _ptr(finished), g, b, k, self.vocab, self.eos, _ptr(out), picks.data_ptr(),
+                picks.data_ptr() + 4 * g * k, _ptr(ended), _ptr(self.workspace),
+                self.workspace.numel(), _stream(stream))
+        _lib.check(rc, "fleet_beam_select")
+        return {"scores": out, "parents": picks[0], "tokens": picks[1], "finished": ended}
 
 
 class Decoder:

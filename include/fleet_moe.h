@@ -351,6 +351,151 @@ int fleet_lm_head_argmax(const float* x, const uint16_t* final_norm, const uint1
                          int32_t* pos_advance, void* workspace, size_t workspace_bytes,
                          const fleet_moe_dims* dims, hipStream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Several sequences of one model: their latent cache in pages of 8-bit rows,
+ * the attention over it, and the choice of beams (no counterpart in the
+ * reference, which decodes one sequence greedily). A step of beam search is
+ * fleet_beam_select, fleet_cache_remap by the chosen parents,
+ * fleet_cache_grow by one position, and per layer fleet_cache_append and
+ * fleet_cache_attend. Everything is enqueued on `stream`, nothing is
+ * allocated or read back, and every call may be captured in a graph. */
+
+#define FLEET_CACHE_ROW 576           /* values of one position: c (512), k_pe (64) */
+#define FLEET_CACHE_PAGE_TOKENS 64    /* positions of a page */
+#define FLEET_CACHE_BLOCK_TOKENS 16   /* positions that share a part's scale */
+#define FLEET_CACHE_PAGE_BYTES 36992  /* one layer of a page */
+#define FLEET_CACHE_MAX_SEQS 1024
+#define FLEET_CACHE_MAX_HEADS 128
+
+/* A cache. One layer of a page is FLEET_CACHE_PAGE_BYTES: four blocks of 16
+ * positions, each [36 chunks][16 positions][16 bytes] of e4m3 codes (value
+ * 16 * chunk + byte of a row), then fp32 scales [4 blocks][2], of c and of
+ * k_pe, powers of two in [2^-110, 2^120], and 96 unused bytes. A row's value is
+ * code * scale. Sequence s holds positions 0 .. lens[s] - 1 in the pages
+ * table[s][0 ..]; table[s][j] = -1 from page ceil(lens[s] / 64) on. refs[p] is
+ * the number of table entries that name page p, 0 for a free page. All
+ * sequences empty: table all -1, lens and refs zero (the pool may hold
+ * anything). n_pages <= 2^24, n_seqs <= 1024, n_layers <= 64, max_pages <=
+ * 2^20. */
+typedef struct fleet_cache {
+    uint8_t* pool;      /* [n_pages][n_layers][FLEET_CACHE_PAGE_BYTES], 16-byte aligned */
+    int32_t* table;     /* [n_seqs][max_pages] */
+    int32_t* lens;      /* [n_seqs] */
+    int32_t* refs;      /* [n_pages] */
+    int32_t n_pages;
+    int32_t n_layers;
+    int32_t n_seqs;
+    int32_t max_pages;
+} fleet_cache;
+
+/* Workspace bytes of the fleet_cache_* calls (one workspace serves all; about
+ * 34 MB). 0 for sizes outside the limits above. Its status word (fleet_moe_workspace_
+ * status) collects the FLEET_MOE_ABORT_* bits named below. */
+size_t fleet_cache_workspace_bytes(int32_t n_pages, int32_t n_seqs);
+
+/* Reorders, forks and frees sequences: row i of table and lens becomes what row
+ * parents[i] (device int32[n_seqs]) was, or empty where parents[i] is -1; refs
+ * follow, and a page that no row names any more is free. Pages are shared, not
+ * copied. A parent outside [-1, n_seqs) counts as -1 and sets
+ * FLEET_MOE_ABORT_BAD_ID. */
+int fleet_cache_remap(const fleet_cache* cache, const int32_t* parents, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream);
+
+/* Adds n_new[s] >= 0 (device int32[n_seqs]) positions to every sequence s, to be
+ * written by fleet_cache_append: lens grows, and pages are taken from the free
+ * ones, lowest first, for sequence 0, then 1, and so on. A last page that is
+ * partly filled and shared is copied (the filled blocks, every layer) into the
+ * first page its sequence takes, unless all its other holders left it in this
+ * call before. All sequences grow or none: too few free pages or a table row
+ * that is too short set FLEET_MOE_ABORT_NO_PAGE, a negative count or length
+ * FLEET_MOE_ABORT_POSITION, a last page outside the pool
+ * FLEET_MOE_ABORT_BAD_PAGE, and nothing changes. */
+int fleet_cache_grow(const fleet_cache* cache, const int32_t* n_new, void* workspace,
+                     size_t workspace_bytes, hipStream_t stream);
+
+/* Moves the used pages to the front of the pool: with U of them in use, the k-th
+ * used page at or behind U moves into the k-th free one before it; table and
+ * refs follow. n_used: device int32 that receives U, or NULL. */
+int fleet_cache_compact(const fleet_cache* cache, int32_t* n_used, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+
+/* Writes the newest positions of each sequence, of layers layer0 .. layer0 +
+ * n_layers - 1. rows: bf16 [n_layers][n_rows][576], rows row_stride and layers
+ * layer_stride elements apart (multiples of 8, so that a row is 16-byte
+ * aligned). start: device int32[n_seqs + 1], not decreasing, start[n_seqs] <=
+ * n_rows: rows start[s] .. start[s + 1] - 1 are the last of the lens[s]
+ * positions of sequence s; NULL: one row for each sequence (n_rows == n_seqs).
+ * A block's scale is the least power of two that takes its new finite values
+ * within the largest code, 448, and no less than the scale of older positions
+ * in the block; where those have a smaller scale they are rounded again to the
+ * new one. Rounding is to nearest even; an infinity becomes +-448 times the
+ * scale, NaN stays NaN. More rows than positions, or a length outside the
+ * table, set FLEET_MOE_ABORT_POSITION, a page outside the pool or one that
+ * another sequence holds too FLEET_MOE_ABORT_BAD_PAGE; such rows are not
+ * written. */
+int fleet_cache_append(const fleet_cache* cache, int32_t layer0, int32_t n_layers,
+                       const uint16_t* rows, int64_t row_stride, int64_t layer_stride,
+                       const int32_t* start, int32_t n_rows, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/* The reverse: rows receives the newest positions of each sequence as bf16 (the
+ * values the codes stand for). Rows that name no position or a page outside the
+ * pool (status as above), and those behind start[n_seqs], are left as they
+ * were. */
+int fleet_cache_read(const fleet_cache* cache, int32_t layer0, int32_t n_layers, uint16_t* rows,
+                     int64_t row_stride, int64_t layer_stride, const int32_t* start,
+                     int32_t n_rows, void* workspace, size_t workspace_bytes,
+                     hipStream_t stream);
+
+/* Absorbed-MLA attention of one layer over the cache. q: bf16 [n_tokens][n_heads]
+ * [576] (the absorbed query, then its rotated part), tokens q_stride elements
+ * apart (a multiple of 8); start as above: token start[s] + j stands at position
+ * lens[s] - (start[s+1] - start[s]) + j of sequence s. It sees the positions p up
+ * to its own, with window > 0 only those above its own - window and those
+ * below sinks. out[token][head][0..511] = sum_p softmax_p(scale * q . row_p)
+ * c_p as bf16, lse[token][head] (fp32, may be NULL) = log sum_p exp(scale * q .
+ * row_p); a token that sees nothing gets out = 0, lse = -infinity. NaN reaches
+ * only the tokens that see it. Products are of bf16 values with fp32 sums; the
+ * probabilities are rounded to bf16 before the second product. max_len: a bound
+ * on lens that the host knows, for the division of the work (longer sequences
+ * are still right), or 0. Outputs of tokens behind start[n_seqs] are left as
+ * they were. A length outside the table sets FLEET_MOE_ABORT_POSITION, and the
+ * sequence's tokens see nothing; positions in a page outside the pool are not
+ * seen, and set FLEET_MOE_ABORT_BAD_PAGE. 1 <= n_heads <= 128, n_tokens * n_heads
+ * <= 2^26, 0 < scale. */
+int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const uint16_t* q,
+                       int64_t q_stride, const int32_t* start, int32_t n_tokens,
+                       int32_t n_heads, int32_t max_len, int32_t window, int32_t sinks,
+                       float scale, uint16_t* out, float* lse, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+#define FLEET_BEAM_MAX_BEAMS 64
+#define FLEET_BEAM_MAX_OUT 64
+
+/* Workspace bytes of fleet_beam_select (0: outside its limits). */
+size_t fleet_beam_workspace_bytes(int32_t n_groups, int32_t n_beams, int32_t n_out,
+                                  int32_t vocab);
+
+/* The n_out best continuations of each group of n_beams beams. logits: fp32 rows
+ * of vocab, ld elements apart, row g * n_beams + b of beam b of group g; scores:
+ * fp32 [n_groups][n_beams], the beams' log probabilities so far; finished:
+ * uint8 [n_groups][n_beams] or NULL. Beam b offers every token t with the score
+ * scores[b] + log softmax(logits[b])[t], a finished beam one continuation, eos
+ * with its own score. Order: higher score (64 bits), then lower beam, higher
+ * logit, lower token. A logit of NaN or -infinity is not offered, +infinity
+ * counts as the largest finite number; a beam whose score is NaN or -infinity
+ * offers nothing. out_scores fp32, parents int32 (row g * n_beams + b, as
+ * fleet_cache_remap takes it), tokens int32 and out_finished uint8 (the parent
+ * was finished, or the token is eos; may be NULL) are [n_groups][n_out], best first;
+ * where a group offers fewer: -infinity, -1, -1, 0. eos < 0: no such token (a finished
+ * beam then offers token -1). 1 <= n_beams, n_out <= 64, n_groups * n_beams <= 65535,
+ * 1 <= vocab <= 2^24. Two launches; the workspace needs no clearing. */
+int fleet_beam_select(const float* logits, int64_t ld, const float* scores,
+                      const uint8_t* finished, int32_t n_groups, int32_t n_beams, int32_t n_out,
+                      int32_t vocab, int32_t eos, float* out_scores, int32_t* parents,
+                      int32_t* tokens, uint8_t* out_finished, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream);
+
 /* Copies the workspace's sticky status word to *status (0 = healthy; a
  * nonzero value names a bounded wait that expired, see FLEET_MOE_ABORT_*),
  * synchronising `stream`. The reference's equivalent is the sticky rt.abort
@@ -367,6 +512,9 @@ int fleet_moe_workspace_status(const void* workspace, uint32_t* status, hipStrea
                                              was clamped into range (output unspecified) */
 #define FLEET_MOE_ABORT_STEP_WAIT 0x80u   /* fleet_decode_step: a stage's input residual
                                              (or an lm_head candidate) never arrived */
+#define FLEET_MOE_ABORT_NO_PAGE 0x100u    /* fleet_cache_grow: too few free pages */
+#define FLEET_MOE_ABORT_BAD_PAGE 0x200u   /* fleet_cache_*: a table entry outside the pool,
+                                             or a shared page to be written */
 
 /* Diagnostic: reads `bytes` of device memory with the weight-streaming load
  * pattern of the kernels above (16-byte non-temporal loads, 1 KB per wave
