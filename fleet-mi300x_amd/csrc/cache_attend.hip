@@ -33,83 +33,98 @@ struct AttendParams {
     const int32_t* start;
     uint16_t* out;
     float* lse;
-    float* part;                // fp32 [tile][split][16][512], then [tile][split][16][2..]
+    float* part;                // partial O, fp32 [slot][rows][512]
+    f32x4* stat;                // [slot][rows]: reference, sum, rounded sum
+    int4* meta;                 // [unit]: first slot, next workgroup, number of slots
     Header* h;
     int64_t q_stride;
-    int layer, n_tokens, n_heads, window, sinks, splits, pad;
+    int layer, n_tokens, n_heads, window, sinks, pad, units;
+    int shares;                 // workgroups, or splits of a unit
     float scale;                // times log2(e)
 };
 
-// 32 positions, the k of a 16x16x32 product, are a tile.
-constexpr int kTile = 32;
-constexpr int kRows = 16;
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
+constexpr float kSlack = 8.f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// A workgroup's rows and the positions they see: sink tiles [0, n_sink), then
-// tiles [main, main + n - n_sink).
+// A unit: up to R rows (token, head) of a sequence, and the steps of S positions
+// that some of them see: the first n_sink steps from position 0 on, the others from
+// step `main` on.
 struct Work {
     int seq, row0, rows;        // rows row0 .. of the sequence's `rows`
-    int tok0;                   // its first token
-    int len, n_new;
+    int tok0, n_new, len;       // its first token, its tokens, its positions
     int n_sink, main, n;
 };
+template <int S>
+__device__ __forceinline__ int step_of(const Work& w, int i) {
+    return i < w.n_sink ? i : w.main + i - w.n_sink;
+}
 
-template <int R>
-__device__ __forceinline__ bool find_work(const AttendParams& P, int64_t u, Work& w) {
-    const fleet_cache& c = P.c;
-    w.seq = find_seq(P.start, c.n_seqs, P.n_tokens, u, P.n_heads, R, P.pad);
-    if (w.seq < 0) return false;
-    const int a = P.start ? clamp_row(P.start[w.seq], P.n_tokens) : w.seq;
-    const int z = P.start ? clamp_row(P.start[w.seq + 1], P.n_tokens) : w.seq + 1;
-    if (z <= a) return false;
-    w.tok0 = a;
-    w.n_new = z - a;
-    w.rows = w.n_new * P.n_heads;
-    const int64_t r = (u - first_unit(a, w.seq, P.n_heads, R, P.pad)) * R;
-    if (r >= w.rows) return false;
-    w.row0 = (int)r;
-    int len = c.lens[w.seq];
-    w.len = checked_len(len, c.max_pages);
-    // the positions of the tile's first and last token
-    const int last_row = w.row0 + R - 1 < w.rows ? w.row0 + R - 1 : w.rows - 1;
-    const int p0 = w.len - w.n_new + w.row0 / P.n_heads;
-    const int p1 = w.len - w.n_new + last_row / P.n_heads;
+// The steps of a unit: everything but the sequence's tokens and length set here.
+template <int R, int S>
+__device__ __forceinline__ void see(const AttendParams& P, Work& w) {
     w.n_sink = w.main = w.n = 0;
-    if (w.len < 0) {
-        if (threadIdx.x == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
-        return true;
-    }
-    if (p1 < 0) return true;
+    const int last = w.row0 + R - 1 < w.rows ? w.row0 + R - 1 : w.rows - 1;
+    const int p0 = w.len - w.n_new + w.row0 / P.n_heads;
+    const int p1 = w.len - w.n_new + last / P.n_heads;
+    if (w.len < 0 || p1 < 0) return;
     const Seen s = seen_of(p0 < 0 ? 0 : p0, P.window, P.sinks);
-    const int end = (p1 + kTile) / kTile;                 // p1 + 1 positions
-    w.main = s.lo / kTile;
-    const int sink = (s.sink + kTile - 1) / kTile;
+    const int end = (p1 + S) / S;                         // steps of p1 + 1 positions
+    w.main = s.lo / S;
+    const int sink = (s.sink + S - 1) / S;
     w.n_sink = sink < w.main ? sink : w.main;
     w.n = w.n_sink + end - w.main;
-    return true;
+}
+__device__ __forceinline__ void open_seq(const AttendParams& P, int seq, Work& w) {
+    const int a = P.start ? clamp_row(ld_global(P.start + seq), P.n_tokens) : seq;
+    const int z = P.start ? clamp_row(ld_global(P.start + seq + 1), P.n_tokens) : seq + 1;
+    w.seq = seq;
+    w.row0 = 0;
+    w.tok0 = a;
+    w.n_new = z > a ? z - a : 0;
+    w.rows = w.n_new * P.n_heads;
+    w.len = checked_len(ld_global(P.c.lens + seq), P.c.max_pages);
 }
 
-// The share of one of `splits` workgroups in n tiles, whole rounds of the waves.
-// Fewer tiles than that leave the last workgroups without any.
-__device__ __forceinline__ int split_size(int n, int splits) {
-    const int each = (n + splits - 1) / splits;
-    return (each + kWaves - 1) / kWaves * kWaves;
-}
-
-// LDS, per wave two tiles of two blocks. The second block sits 64 bytes off, so
-// that the two halves of a transposing read fall into different banks.
-constexpr int kBlockStep = kBlockBytes + 64;
-constexpr int kScaleAt = 2 * kBlockStep;
-constexpr int kTileBytes = kScaleAt + 256;
-struct AttendLds {
-    union {
-        __attribute__((aligned(16))) uint8_t tile[kWaves][2][kTileBytes];
-        f32x4 sum[kWaves][kC / 16][64];
-    };
-    float stat[kWaves][3][kRows];
+// A lane's row, and what it sees.
+struct Row {
+    int64_t at;                 // token * heads + head; -1: no row
+    int pos;
+    Seen seen;
 };
+__device__ __forceinline__ Row row_of(const AttendParams& P, const Work& w, int row) {
+    Row r;
+    const bool live = row < w.rows;
+    const int tok = live ? row / P.n_heads : 0;
+    r.at = live ? (int64_t)w.tok0 * P.n_heads + row : -1;
+    r.pos = live && w.len >= 0 ? w.len - w.n_new + tok : -1;
+    r.seen = seen_of(r.pos < 0 ? 0 : r.pos, P.window, P.sinks);
+    return r;
+}
+// Its query as the right operand: the k order of the products is that of the bytes
+// a lane of group g takes of a row: chunks g, 4 + g, ..
+__device__ __forceinline__ void load_q(const AttendParams& P, const Row& r, int g,
+                                       bf16x8 (&q)[kChunks / 2]) {
+    const int64_t tok = r.at < 0 ? 0 : r.at / P.n_heads;
+    const int head = r.at < 0 ? 0 : (int)(r.at % P.n_heads);
+#pragma unroll
+    for (int i = 0; i < kChunks / 4; ++i) {
+        u32x4 a{0, 0, 0, 0}, b{0, 0, 0, 0};
+        if (r.at >= 0) {
+            const u32x4* src = reinterpret_cast<const u32x4*>(P.q + tok * P.q_stride + head * kRow +
+                                                              (4 * i + g) * 16);
+            a = ld_global(src);
+            b = ld_global(src + 1);
+        }
+        q[2 * i] = __builtin_bit_cast(bf16x8, a);
+        q[2 * i + 1] = __builtin_bit_cast(bf16x8, b);
+    }
+}
+
+// Blocks in LDS lie 64 bytes further apart than they are long, so that the two
+// halves of a transposing read, from neighbouring blocks, fall into different banks.
+constexpr int kBlockStep = kBlockBytes + 64;
 
 // Copies 16 bytes per lane from global memory to LDS, kN times 1 KB: lane's `src`
 // + 1024 i to `lds` + 1024 i + 16 lane (the offset counts on both sides). There is
@@ -144,23 +159,12 @@ template <int kLeft>
 __device__ __forceinline__ void wait_copies() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
 }
-constexpr int kCopies = 2 * kBlockBytes / 1024 + 1;       // of a tile
-
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
-
-// One tile of a page's layer into LDS; `src` is the page's layer, half 0 or 1.
-__device__ __forceinline__ void load_tile(const uint8_t* src, int half, uint32_t lds, int lane) {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        const uint8_t* at = src + (2 * half + b) * kBlockBytes + lane * 16;
-        const uint32_t to = lds + b * kBlockStep;
-        copy_kb<4>(at, to);
-        copy_kb<4>(at + 4096, to + 4096);
-        copy_kb<1>(at + 8192, to + 8192);
-    }
-    copy_words(src + kCodeBytes + (lane & 7) * 4, lds + kScaleAt);
+// The workgroup's barrier, without waiting for copies in flight.
+__device__ __forceinline__ void barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi, float slo, float shi) {
@@ -202,263 +206,596 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// 16 rows against a share of the positions. Four waves take the tiles in turn,
-// each with its own maximum, sum and O^T (16 rows x 512 in 128 registers), from two
-// buffers of its own that copies fill a tile ahead: no wave waits for another
-// before the end. At 576 bytes per position for 16 rows the memory bounds it, the
-// products take about a third of the time; the LDS (2 x 18 KB per wave) is sized
-// for what has to be in flight.
-__global__ __launch_bounds__(kThreads, 1) void attend_kernel(AttendParams P) {
-    __shared__ AttendLds L;
-    const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
-    const int split = blockIdx.x % P.splits;
-    Work w;
-    if (!find_work<kRows>(P, blockIdx.x / P.splits, w)) return;
-    const int each = split_size(w.n, P.splits);
-    const int t0 = split * each;
-    const int t1 = t0 + each < w.n ? t0 + each : w.n;
-    if (split > 0 && t0 >= w.n) return;
-    const bool whole = each >= w.n;             // no other workgroup has these rows
+// Four weights as bf16.
+__device__ __forceinline__ uint2 weights(const float (&p)[4]) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    bf16x2 a, b;
+    a[0] = (__bf16)p[0];
+    a[1] = (__bf16)p[1];
+    b[0] = (__bf16)p[2];
+    b[1] = (__bf16)p[3];
+    return make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+}
 
-    // this lane's row, and what it sees
-    const int g = lane >> 4, row = w.row0 + (lane & 15);
-    const bool live = row < w.rows;
-    const int tok = live ? row / P.n_heads : 0, head = live ? row % P.n_heads : 0;
-    const int pos = live ? w.len - w.n_new + tok : -1;
-    const Seen seen = seen_of(pos < 0 ? 0 : pos, P.window, P.sinks);
-    bf16x8 q[2 * kChunks / 4];
+// The transposing read: 8 positions of one of the 16 dimensions of chunk i. `col`
+// is what column_at() gives: lane r of a group of 16 points at row r / 2 of 8,
+// positions 4g .. 4g + 3 of two neighbouring blocks.
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+__device__ __forceinline__ const uint8_t* column_at(const uint8_t* block, int lane) {
+    const int r = (lane & 15) >> 1;
+    return block + (r < 4 ? 0 : kBlockStep) + (4 * (lane >> 4) + (r & 3)) * 16 + (lane & 1) * 8;
+}
+__device__ __forceinline__ i32x2 column(const uint8_t* col, int i) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (lds_i32x2*)(const __attribute__((address_space(3))) uint8_t*)(col + i * 256));
+}
+
+// A block's NaN codes as zeros, by one wave. A NaN in a row makes the score, and
+// so the weight, of every row of q that sees it NaN; a row that does not see it
+// has the weight 0, and must not meet 0 * NaN.
+__device__ __forceinline__ void clean(uint8_t* block, int lane) {
+    for (int i = 0; i < kC / 64; ++i) {
+        u32x4* at = reinterpret_cast<u32x4*>(block + i * 1024 + lane * 16);
+        u32x4 v = *at;
 #pragma unroll
-    for (int i = 0; i < kChunks / 4; ++i) {
-        u32x4 a{0, 0, 0, 0}, b{0, 0, 0, 0};
-        if (live) {
-            const u32x4* src = reinterpret_cast<const u32x4*>(
-                P.q + (int64_t)(w.tok0 + tok) * P.q_stride + head * kRow + (4 * i + g) * 16);
-            a = ld_global(src);
-            b = ld_global(src + 1);
-        }
-        q[2 * i] = __builtin_bit_cast(bf16x8, a);
-        q[2 * i + 1] = __builtin_bit_cast(bf16x8, b);
+        for (int j = 0; j < 4; ++j) v[j] = drop_nan(v[j]);
+        *at = v;
     }
-    f32x4 acc[kC / 16];
+}
+
+__device__ __forceinline__ uint32_t bf16x2_bits(float a, float b) {
+    return bf16_bits(a) | bf16_bits(b) << 16;
+}
+__device__ __forceinline__ void put(uint16_t* out, const f32x4& o, float inv) {
+    const uint64_t b = (uint64_t)bf16x2_bits(o[0] * inv, o[1] * inv) |
+                       (uint64_t)bf16x2_bits(o[2] * inv, o[3] * inv) << 32;
+    st_global(reinterpret_cast<uint64_t*>(out), b);
+}
+__device__ __forceinline__ float lse_of(float m, float sum) {
+    return sum == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+constexpr uint32_t kOnes = 0x3f803f80u;                   // bf16 1, 1
+
+// Pages of the next 64 steps, one per lane.
+struct Pages {
+    int held, from;
+    int page;
+};
+template <int S>
+__device__ __forceinline__ int page_of(const AttendParams& P, const Work& w, Pages& h, int i,
+                                       int end, int lane) {
+    if (i >= h.held) {
+        h.from = i;
+        h.held = i + 64;
+        h.page = i + lane < end ? ld_global(P.c.table + (int64_t)w.seq * P.c.max_pages +
+                                            step_of<S>(w, i + lane) * S / kPage)
+                                : 0;
+    }
+    return __builtin_amdgcn_readlane(h.page, i - h.from);
+}
+
+// ---------------------------------------------------------------- few rows
+
+// Sequences with a token or two: 16 rows a unit, a page a step. The bytes of the
+// pages bound it (576 a position for 16 rows, 60 flops a byte), so what matters is
+// that they keep coming: each wave copies its own block of the page into LDS and
+// takes the scores of its 16 positions; after one barrier every wave has all
+// weights and adds its 128 columns of O over the whole page. O needs 32 registers
+// a lane this way, q 72, and no sum over waves at the end; two workgroups share a
+// CU, and one's copies run beside the other's products.
+//
+// The work is divided into equal shares of steps over all units, whatever their
+// lengths: a workgroup takes a range of the concatenated steps, across units where it
+// has to. A unit that several have a part in leaves partial results, which
+// join_kernel adds in order.
+struct FewLds {
+    __attribute__((aligned(16))) uint8_t tile[2][4 * kBlockStep];
+    uint32_t scale[2][kWaves][64];
+    u32x4 p[2][2][64];          // [step parity][half of the page][lane]
+    float top[2][kWaves][16];
+    int flag[2][kWaves];
+    int64_t before[kWaves];
+    int seq, row0;
+    int64_t off;
+};
+static_assert(sizeof(FewLds) <= 80 * 1024, "two workgroups share a CU");
+constexpr int kFew = 16;        // rows
+
+constexpr int kNeedMax = 1, kHasNan = 2;
+
+// The steps of all units of a sequence, an empty unit as one.
+__device__ __forceinline__ int64_t seq_steps(const AttendParams& P, Work& w) {
+    int64_t n = 0;
+    for (w.row0 = 0; w.row0 < w.rows; w.row0 += kFew) {
+        see<kFew, kPage>(P, w);
+        n += w.n > 0 ? w.n : 1;
+    }
+    return n;
+}
+
+// The total of steps, and where step `at` of them lies: sequence, row and step of
+// the unit (in L). `at` is a function of the total.
+template <class F>
+__device__ __forceinline__ int64_t locate(const AttendParams& P, FewLds& L, F at) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int each = (P.c.n_seqs + kThreads - 1) / kThreads;
+    Work w;
+    int64_t mine = 0;
+    for (int i = 0; i < each; ++i) {
+        const int s = t * each + i;
+        if (s >= P.c.n_seqs) break;
+        open_seq(P, s, w);
+        mine += seq_steps(P, w);
+    }
+    int64_t incl = mine;
 #pragma unroll
-    for (int i = 0; i < kC / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    f32x4 ones = f32x4{0.f, 0.f, 0.f, 0.f};     // the sum of the rounded weights
-    const u32x4 one_bits{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-    float m = -INFINITY, l = 0.f;
-
-    // the wave's tiles: t0 + wave, + kWaves, ..; lane k holds the page of the k-th
-    // of the next 64
-    const int32_t* table = P.c.table + (int64_t)w.seq * P.c.max_pages;
-    const auto tile_of = [&](int i) { return i < w.n_sink ? i : w.main + i - w.n_sink; };
-    int pages = 0, held = 0, asked = 0;         // `held` pages from the asked-th tile on
-    const int mine = t1 - t0 - wave > 0 ? (t1 - t0 - wave + kWaves - 1) / kWaves : 0;
-    const auto page_of = [&](int k) {           // of the wave's k-th tile
-        if (k >= held) {
-            asked = k;
-            held = k + 64;
-            const int i = k + lane;
-            pages = i < mine ? ld_global(table + tile_of(t0 + wave + i * kWaves) / 2) : 0;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t o = __shfl_up((long long)incl, d);
+        if (lane >= d) incl += o;
+    }
+    if (lane == 63) L.before[wave] = incl;
+    __syncthreads();
+    int64_t total = 0, first = incl - mine;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        if (i < wave) first += L.before[i];
+        total += L.before[i];
+    }
+    int64_t want = at(total) - first;
+    if (want >= 0 && want < mine) {
+        for (int i = 0; i < each; ++i) {
+            open_seq(P, t * each + i, w);
+            const int64_t n = seq_steps(P, w);
+            if (want < n) break;
+            want -= n;
         }
-        return __builtin_amdgcn_readlane(pages, k - asked);
-    };
-    const auto issue = [&](int k) {
-        const int page = page_of(k);
-        const int tile = tile_of(t0 + wave + k * kWaves);
-        const int64_t at = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
-        load_tile(P.c.pool + (at < 0 ? 0 : at), tile & 1, lds_addr(L.tile[wave][k & 1]), lane);
-        return at >= 0;
-    };
-    // bit k & 1: whether the tile in that buffer is one of the pool's
-    int good = 0;
-    if (mine > 0) good |= issue(0) ? 1 : 0;
-    if (mine > 1) good |= issue(1) ? 2 : 0;
-    for (int k = 0; k < mine; ++k) {
-        if (k + 1 < mine) wait_copies<kCopies>();
-        else wait_copies<0>();
-        const uint8_t* buf = L.tile[wave][k & 1];
-        const int tile = tile_of(t0 + wave + k * kWaves);
-        const uint32_t* sc = reinterpret_cast<const uint32_t*>(buf + kScaleAt) + 4 * (tile & 1);
-        const float sc0 = any_scale(sc[0]), sp0 = any_scale(sc[1]);
-        const float sc1 = any_scale(sc[2]), sp1 = any_scale(sc[3]);
+        for (w.row0 = 0;; w.row0 += kFew) {
+            see<kFew, kPage>(P, w);
+            const int n = w.n > 0 ? w.n : 1;
+            if (want < n) break;
+            want -= n;
+        }
+        L.seq = w.seq;
+        L.row0 = w.row0;
+        L.off = want;
+    }
+    __syncthreads();
+    return total;
+}
 
-        f32x4 s0{0.f, 0.f, 0.f, 0.f}, s1{0.f, 0.f, 0.f, 0.f};
+__global__ __launch_bounds__(kThreads, 2) void few_kernel(AttendParams P) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    FewLds& L = *reinterpret_cast<FewLds*>(lds);
+    const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int wg = blockIdx.x;
+    // (no share is empty: the join counts on it)
+    const auto share = [&](int64_t all, int i) { return all * i / (all < P.shares ? all : P.shares); };
+    const int64_t total = locate(P, L, [&](int64_t all) { return all ? share(all, wg) : 0; });
+    const int shares = total < P.shares ? (int)total : P.shares;
+    if (wg >= shares) return;
+    int64_t at = share(total, wg);
+    const int64_t end = share(total, wg + 1);
+    Work w;
+    open_seq(P, wave_bcast(L.seq), w);
+    w.row0 = wave_bcast(L.row0);
+    int off = wave_bcast((int)L.off);
+    for (bool lead = true;; lead = false) {
+        see<kFew, kPage>(P, w);
+        const int all = w.n > 0 ? w.n : 1;
+        const int take = all - off < end - at ? all - off : (int)(end - at);
+        const int until = off + take < w.n ? off + take : w.n;
+        const int cnt = until > off ? until - off : 0;
+        const Row r = row_of(P, w, w.row0 + n);
+        if (w.len < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
+
+        bf16x8 q[kChunks / 2];
+        load_q(P, r, g, q);
+        f32x4 acc[kC / 16 / kWaves];
+#pragma unroll
+        for (auto& a : acc) a = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 ones{0.f, 0.f, 0.f, 0.f};         // the sum of the rounded weights
+        float m = -INFINITY, l = 0.f;
+        Pages pages{0, 0, 0};
+        int good = 0;                           // bit: whether that buffer's page is one
+        const auto issue = [&](int k) {
+            const int page = page_of<kPage>(P, w, pages, off + k, until, lane);
+            const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
+            const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
+            const uint8_t* from = src + wave * kBlockBytes + lane * 16;
+            const uint32_t to = lds_addr(L.tile[k & 1]) + wave * kBlockStep;
+            copy_kb<4>(from, to);
+            copy_kb<4>(from + 4096, to + 4096);
+            copy_kb<1>(from + 8192, to + 8192);
+            copy_words(src + kCodeBytes + (lane & 7) * 4, lds_addr(L.scale[k & 1][wave]));
+            const int bit = 1 << (k & 1);
+            good = base >= 0 ? good | bit : good & ~bit;
+            if (base < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
+        };
+        if (cnt > 0) issue(0);
+        if (cnt > 1) issue(1);
+        for (int k = 0; k < cnt; ++k) {
+            const int b = k & 1;
+            if (k == 0 && cnt > 1) wait_copies<10>();
+            else wait_copies<0>();
+            const uint8_t* block = L.tile[b] + wave * kBlockStep;
+            f32x4 z{0.f, 0.f, 0.f, 0.f}, z2{0.f, 0.f, 0.f, 0.f};
+            {
+                const float sc = any_scale(L.scale[b][wave][2 * wave]);
+                const float sp = any_scale(L.scale[b][wave][2 * wave + 1]);
+#pragma unroll
+                for (int i = 0; i < kChunks / 4; ++i) {
+                    const u32x4 a = *reinterpret_cast<const u32x4*>(block + i * 1024 + lane * 16);
+                    const float s = i < kC / 64 ? sc : sp;
+                    z = mfma(widen(a.x, a.y, s, s), q[2 * i], z);
+                    z2 = mfma(widen(a.z, a.w, s, s), q[2 * i + 1], z2);
+                }
+            }
+            float s[4], p[4], top = -INFINITY;
+            bool nan = false;
+            const bool ok = good >> b & 1;
+            const int base = step_of<kPage>(w, off + k) * kPage + wave * kBlock + 4 * g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float v = (z[j] + z2[j]) * P.scale;
+                nan |= v != v;
+                const int pos = base + j;
+                s[j] = ok && pos <= r.pos && (pos >= r.seen.lo || pos < r.seen.sink) ? v : -INFINITY;
+                top = fmaxf(top, s[j]);
+            }
+            top = xor32_max(xor16_max(top));
+            // m is any reference not far below the maximum: weights up to 2^kSlack are
+            // as exact as those up to 1, and moving it costs a pass over O and a
+            // barrier
+            const auto weigh = [&] {
+                const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[j] = exp2_(s[j] - ref);
+                reinterpret_cast<uint2*>(&L.p[b][wave >> 1][lane])[wave & 1] = weights(p);
+            };
+            weigh();
+            if (lane < 16) L.top[b][wave][lane] = top;
+            const int flag = (__ballot(top > m + kSlack) ? kNeedMax : 0) |
+                             (__ballot(nan) ? kHasNan : 0);
+            if (lane == 0) L.flag[b][wave] = flag;
+            barrier();                          // every block is there, every weight
+            if (k > 0 && k + 1 < cnt) issue(k + 1);       // where the page before was
+            const int any = wave_bcast((L.flag[b][0] | L.flag[b][1]) | (L.flag[b][2] | L.flag[b][3]));
+            if (any) {
+                if (any & kNeedMax) {
+                    float to = m;
+#pragma unroll
+                    for (int i = 0; i < kWaves; ++i) to = fmaxf(to, L.top[b][i][n]);
+                    const float shrink = to == -INFINITY ? 1.f : exp2_(m - to);
+                    m = to;
+                    l *= shrink;
+                    ones *= shrink;
+#pragma unroll
+                    for (auto& a : acc) a *= shrink;
+                    weigh();
+                }
+                if (any & kHasNan) clean(L.tile[b] + wave * kBlockStep, lane);
+                barrier();
+            }
+            l += (p[0] + p[1]) + (p[2] + p[3]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[b][h][lane]);
+                const float sa = any_scale(L.scale[b][wave][4 * h]);
+                const float sb = any_scale(L.scale[b][wave][4 * h + 2]);
+                const uint8_t* col = column_at(L.tile[b] + 2 * h * kBlockStep, lane) +
+                                     wave * (kC / kWaves / 16) * 256;
+#pragma unroll
+                for (int i = 0; i < kC / 16 / kWaves; ++i) {
+                    const i32x2 v = column(col, i);
+                    acc[i] = mfma(widen((uint32_t)v.x, (uint32_t)v.y, sa, sb), pb, acc[i]);
+                }
+                ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}), pb, ones);
+            }
+        }
+        // the waves' sums
+        l = xor32_sum(xor16_sum(l));
+        barrier();
+        if (lane < 16) L.top[0][wave][lane] = l;
+        barrier();
+        const float sum = (L.top[0][0][n] + L.top[0][1][n]) + (L.top[0][2][n] + L.top[0][3][n]);
+        const bool whole = take == all;
+        const int column0 = wave * (kC / kWaves) + 4 * g;
+        if (whole) {
+            if (r.at >= 0) {
+                const float inv = ones[0] == 0.f ? 0.f : 1.f / ones[0];
+#pragma unroll
+                for (int i = 0; i < kC / 16 / kWaves; ++i)
+                    put(P.out + r.at * kC + column0 + i * 16, acc[i], inv);
+                if (P.lse && wave == 0 && g == 0) P.lse[r.at] = lse_of(m, sum);
+            }
+        } else {
+            // a workgroup has at most two such: its first, and its last
+            const int64_t slot = 2 * (int64_t)wg + (lead ? 0 : 1);
+            float* part = P.part + (slot * kFew + n) * kC + column0;
+#pragma unroll
+            for (int i = 0; i < kC / 16 / kWaves; ++i)
+                st_global(reinterpret_cast<f32x4*>(part + i * 16), acc[i]);
+            if (wave == 0 && g == 0) st_global(P.stat + slot * kFew + n, f32x4{m, sum, ones[0], 0.f});
+        }
+        if (off == 0 && t == 0) {
+            const int64_t u = first_unit(w.tok0, w.seq, P.n_heads, kFew, P.pad) + w.row0 / kFew;
+            // the workgroup of the unit's last step: the last with its first step there
+            const int64_t last = ((at + all) * shares + total - 1) / total - 1;
+            P.meta[u] = make_int4(2 * wg + (lead ? 0 : 1), wg + 1, whole ? 1 : (int)(last - wg) + 1, 0);
+        }
+        at += take;
+        if (at >= end) return;
+        // the next unit
+        off = 0;
+        w.row0 += kFew;
+        while (w.row0 >= w.rows) {
+            if (w.seq + 1 >= P.c.n_seqs) return;
+            open_seq(P, w.seq + 1, w);
+        }
+        barrier();                              // L.top is free again
+    }
+}
+
+// Adds the parts of a row, in order: a workgroup per row, four groups of threads
+// with a quarter of the parts each.
+constexpr int kJoinGroups = 4;
+constexpr int kJoinThreads = kC / 4 * kJoinGroups;
+template <int R>
+__device__ __forceinline__ void join(const AttendParams& P, int64_t row_at, int row, int64_t slot0,
+                                     int64_t rest, int64_t step, int count) {
+    __shared__ f32x4 sum_o[kJoinGroups][kC / 4];
+    const int t = threadIdx.x % (kC / 4), part = threadIdx.x / (kC / 4);
+    const auto slot = [&](int i) { return (i == 0 ? slot0 : rest + (i - 1) * step) * R + row; };
+    float top = -INFINITY;
+    for (int i = 0; i < count; ++i) top = fmaxf(top, ld_global(P.stat + slot(i))[0]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, rounded = 0.f;
+    for (int i = 0; i < count; ++i) {
+        const f32x4 st = ld_global(P.stat + slot(i));
+        const float f = exp2_(st[0] - ref);
+        sum += f * st[1];
+        rounded += f * st[2];
+    }
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    const int each = (count + kJoinGroups - 1) / kJoinGroups;
+    const int end = (part + 1) * each < count ? (part + 1) * each : count;
+#pragma unroll 4
+    for (int i = part * each; i < end; ++i) {
+        const float f = exp2_(ld_global(P.stat + slot(i))[0] - ref);
+        o += ld_global(reinterpret_cast<const f32x4*>(P.part + slot(i) * kC) + t) * f;
+    }
+    sum_o[part][t] = o;
+    __syncthreads();
+    if (part) return;
+    o = (sum_o[0][t] + sum_o[1][t]) + (sum_o[2][t] + sum_o[3][t]);
+    put(P.out + row_at * kC + 4 * t, o, rounded == 0.f ? 0.f : 1.f / rounded);
+    if (P.lse && threadIdx.x == 0) P.lse[row_at] = lse_of(top, sum);
+}
+
+// The unit of number u, if there is one.
+template <int R, int S>
+__device__ __forceinline__ bool find_work(const AttendParams& P, int64_t u, Work& w) {
+    const int seq = find_seq(P.start, P.c.n_seqs, P.n_tokens, u, P.n_heads, R, P.pad);
+    if (seq < 0) return false;
+    open_seq(P, seq, w);
+    const int64_t r = (u - first_unit(w.tok0, seq, P.n_heads, R, P.pad)) * R;
+    if (r >= w.rows) return false;
+    w.row0 = (int)r;
+    see<R, S>(P, w);
+    return true;
+}
+
+__global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams P) {
+    const int64_t u = blockIdx.x / kFew;
+    Work w;
+    if (!find_work<kFew, kPage>(P, u, w)) return;
+    const int row = blockIdx.x % kFew;
+    if (w.row0 + row >= w.rows) return;
+    const int4 m = P.meta[u];
+    if (m.z <= 1) return;
+    join<kFew>(P, (int64_t)w.tok0 * P.n_heads + w.row0 + row, row, m.x, 2 * (int64_t)m.y, 2, m.z);
+}
+
+// ---------------------------------------------------------------- many rows
+
+// Prompts, and whatever else has 64 rows or more for a sequence: 64 rows a unit, 32
+// positions a step. The products bound it, so K is read from LDS by four waves that
+// have 16 rows each, and each widened V operand serves all 64 rows: a wave takes
+// the scores of its 16 rows, and adds its 128 columns of O for all 64 (128
+// registers). One barrier a step: behind it are the weights of this step and the
+// copies of the next, so the second product of a step and the first of the next
+// fill the matrix pipes together; two workgroups share a CU.
+struct ManyLds {
+    __attribute__((aligned(16))) uint8_t tile[3][2 * kBlockStep];
+    uint32_t scale[3][kWaves][64];
+    u32x4 p[2][kWaves][64];     // [step parity][16 rows][lane]
+    float shrink[2][kWaves][16];
+    int flag[2][kWaves];
+};
+static_assert(sizeof(ManyLds) <= 80 * 1024, "two workgroups share a CU");
+constexpr int kMany = 64;       // rows
+constexpr int kStep = 32;       // positions
+
+__global__ __launch_bounds__(kThreads, 2) void many_kernel(AttendParams P) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    ManyLds& L = *reinterpret_cast<ManyLds*>(lds);
+    const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int unit = P.units - 1 - blockIdx.x / P.shares, split = blockIdx.x % P.shares;
+    Work w;
+    if (!find_work<kMany, kStep>(P, unit, w)) return;
+    const int each = (w.n + P.shares - 1) / P.shares;
+    const int off = split * each;
+    const int cnt = off + each < w.n ? each : w.n - off;
+    if (split > 0 && cnt <= 0) return;
+    const bool whole = each >= w.n;             // no other workgroup has these rows
+    const Row r = row_of(P, w, w.row0 + wave * 16 + n);
+    if (w.len < 0 && t == 0 && split == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
+
+    bf16x8 q[kChunks / 2];
+    load_q(P, r, g, q);
+    constexpr int kCols = kC / 16 / kWaves;     // of 16
+    f32x4 acc[kWaves][kCols];
+#pragma unroll
+    for (auto& a : acc)
+#pragma unroll
+        for (auto& b : a) b = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 ones{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    Pages pages{0, 0, 0};
+    int good = 0;
+    const auto issue = [&](int k) {
+        const int page = page_of<kStep>(P, w, pages, off + k, off + cnt, lane);
+        const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
+        const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
+        const int half = step_of<kStep>(w, off + k) & 1;
+        // eighteen pieces of 1 KB: two waves take five, two take four
+        const uint32_t to = lds_addr(L.tile[k % 3]);
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            const int piece = wave + kWaves * i;
+            if (piece < 18)
+                copy_kb<1>(src + half * 2 * kBlockBytes + piece * 1024 + lane * 16,
+                           to + piece * 1024 + (piece >= 9 ? kBlockStep - kBlockBytes : 0));
+        }
+        copy_words(src + kCodeBytes + half * 16 + (lane & 3) * 4, lds_addr(L.scale[k % 3][wave]));
+        const int bit = 1 << (k % 3);
+        good = base >= 0 ? good | bit : good & ~bit;
+        if (base < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
+    };
+    // the scores and weights of step k
+    const auto score = [&](int k) {
+        const uint8_t* buf = L.tile[k % 3];
+        const float sc0 = any_scale(L.scale[k % 3][wave][0]), sp0 = any_scale(L.scale[k % 3][wave][1]);
+        const float sc1 = any_scale(L.scale[k % 3][wave][2]), sp1 = any_scale(L.scale[k % 3][wave][3]);
+        f32x4 z0{0.f, 0.f, 0.f, 0.f}, z1{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < kChunks / 4; ++i) {
             const u32x4 a = *reinterpret_cast<const u32x4*>(buf + i * 1024 + lane * 16);
             const u32x4 b = *reinterpret_cast<const u32x4*>(buf + kBlockStep + i * 1024 + lane * 16);
             const float sa = i < kC / 64 ? sc0 : sp0, sb = i < kC / 64 ? sc1 : sp1;
-            s0 = mfma(widen(a.x, a.y, sa, sa), q[2 * i], s0);
-            s1 = mfma(widen(b.x, b.y, sb, sb), q[2 * i], s1);
-            s0 = mfma(widen(a.z, a.w, sa, sa), q[2 * i + 1], s0);
-            s1 = mfma(widen(b.z, b.w, sb, sb), q[2 * i + 1], s1);
+            z0 = mfma(widen(a.x, a.y, sa, sa), q[2 * i], z0);
+            z1 = mfma(widen(b.x, b.y, sb, sb), q[2 * i], z1);
+            z0 = mfma(widen(a.z, a.w, sa, sa), q[2 * i + 1], z0);
+            z1 = mfma(widen(b.z, b.w, sb, sb), q[2 * i + 1], z1);
         }
-        float s[8];
+        float s0[4], s1[4], top = m;
         bool nan = false;
-        const int base = tile * kTile + 4 * g;
-        const bool ok = good >> (k & 1) & 1;
-        if (!ok && lane == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float v = (j < 4 ? s0[j & 3] : s1[j & 3]) * P.scale;
-            const int p = base + (j & 3) + (j < 4 ? 0 : kBlock);
-            nan |= v != v;
-            s[j] = ok && p <= pos && (p >= seen.lo || p < seen.sink) ? v : -INFINITY;
-        }
-        float top = m;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j]);
-        top = xor32_max(xor16_max(top));
-        const float base_m = top == -INFINITY ? 0.f : top;
-        const float shrink = exp2_(m - base_m);
-        if (__ballot(top != m)) {
-            l *= shrink;
-            ones *= shrink;
-#pragma unroll
-            for (int i = 0; i < kC / 16; ++i) acc[i] *= shrink;
-        }
-        m = top;
-        u32x4 pb;
+        const bool ok = good >> (k % 3) & 1;
+        const int base = step_of<kStep>(w, off + k) * kStep + 4 * g;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float a = exp2_(s[2 * j] - base_m), b = exp2_(s[2 * j + 1] - base_m);
-            l += a + b;
-            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-            bf16x2 r;
-            r[0] = (__bf16)a;
-            r[1] = (__bf16)b;
-            pb[j] = __builtin_bit_cast(uint32_t, r);
+            const float a = z0[j] * P.scale, b = z1[j] * P.scale;
+            const int pa = base + j, pb = base + kBlock + j;
+            nan |= a != a || b != b;
+            s0[j] = ok && pa <= r.pos && (pa >= r.seen.lo || pa < r.seen.sink) ? a : -INFINITY;
+            s1[j] = ok && pb <= r.pos && (pb >= r.seen.lo || pb < r.seen.sink) ? b : -INFINITY;
+            top = fmaxf(top, fmaxf(s0[j], s1[j]));
         }
-        const bf16x8 p = __builtin_bit_cast(bf16x8, pb);
-        ones = mfma(__builtin_bit_cast(bf16x8, one_bits), p, ones);
-        // lane r of its group of 16 points at row r / 2 of 8: positions 4g .. 4g + 3 of
-        // both blocks
-        const int r8 = (lane & 15) >> 1;
-        const uint8_t* col = buf + (r8 < 4 ? 0 : kBlockStep) + (4 * g + (r8 & 3)) * 16 +
-                             (lane & 1) * 8;
-        typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-        if (__ballot(nan) == 0) {
+        top = xor32_max(xor16_max(top));
+        int flag = __ballot(nan) ? kHasNan : 0;
+        if (__ballot(top > m + kSlack)) {
+            flag |= kNeedMax;
+            const float shrink = top == -INFINITY ? 1.f : exp2_(m - top);
+            m = top;
+            l *= shrink;
+            ones *= shrink;
+            if (lane < 16) L.shrink[k & 1][wave][lane] = shrink;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int i = 0; i < kC / 16; ++i) {
-                const i32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (lds_i32x2*)(const __attribute__((address_space(3))) uint8_t*)(col + i * 256));
-                acc[i] = mfma(widen((uint32_t)v.x, (uint32_t)v.y, sc0, sc1), p, acc[i]);
-            }
-        } else {
-            // A NaN in a row: every row of q that sees it has a NaN weight, and
-            // those that do not must not meet 0 * NaN.
+        for (int j = 0; j < 4; ++j) {
+            s0[j] = exp2_(s0[j] - ref);
+            s1[j] = exp2_(s1[j] - ref);
+        }
+        l += ((s0[0] + s0[1]) + (s0[2] + s0[3])) + ((s1[0] + s1[1]) + (s1[2] + s1[3]));
+        const uint2 a = weights(s0), b = weights(s1);
+        const u32x4 p{a.x, a.y, b.x, b.y};
+        L.p[k & 1][wave][lane] = p;
+        if (lane == 0) L.flag[k & 1][wave] = flag;
+        ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}),
+                    __builtin_bit_cast(bf16x8, p), ones);
+    };
+    if (cnt > 0) issue(0);
+    if (cnt > 1) issue(1);
+    wait_copies<0>();
+    barrier();
+    if (cnt > 0) score(0);
+    for (int k = 0; k < cnt; ++k) {
+        wait_copies<0>();
+        barrier();              // this step's weights, and the next one's tile
+        if (k + 2 < cnt) issue(k + 2);          // where the tile before was
+        const int any = wave_bcast((L.flag[k & 1][0] | L.flag[k & 1][1]) |
+                                   (L.flag[k & 1][2] | L.flag[k & 1][3]));
+        if (any) {
+            if (any & kNeedMax) {
 #pragma unroll
-            for (int i = 0; i < kC / 16; ++i) {
-                const i32x2 v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (lds_i32x2*)(const __attribute__((address_space(3))) uint8_t*)(col + i * 256));
-                acc[i] = mfma(widen(drop_nan((uint32_t)v.x), drop_nan((uint32_t)v.y), sc0, sc1), p,
-                              acc[i]);
+                for (int i = 0; i < kWaves; ++i) {
+                    if (!(wave_bcast(L.flag[k & 1][i]) & kNeedMax)) continue;
+                    const float f = L.shrink[k & 1][i][n];
+#pragma unroll
+                    for (auto& a : acc[i]) a *= f;
+                }
+            }
+            if (any & kHasNan) {
+                if (wave < 2) clean(L.tile[k % 3] + wave * kBlockStep, lane);
+                barrier();
             }
         }
-        if (k + 2 < mine) {
-            // every LDS read of this buffer has returned before it is filled again
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            const int bit = 1 << (k & 1);
-            good = issue(k + 2) ? good | bit : good & ~bit;
+        const float sa = any_scale(L.scale[k % 3][wave][0]), sb = any_scale(L.scale[k % 3][wave][2]);
+        bf16x8 p[kWaves];
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) p[i] = __builtin_bit_cast(bf16x8, L.p[k & 1][i][lane]);
+        const uint8_t* col = column_at(L.tile[k % 3], lane) + wave * kCols * 256;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) {
+            const i32x2 v = column(col, i);
+            const bf16x8 a = widen((uint32_t)v.x, (uint32_t)v.y, sa, sb);
+#pragma unroll
+            for (int j = 0; j < kWaves; ++j) acc[j][i] = mfma(a, p[j], acc[j][i]);
         }
+        if (k + 1 < cnt) score(k + 1);
     }
+    // every wave needs the sums of all rows
     l = xor32_sum(xor16_sum(l));
-
-    // The waves' results: each takes 128 of the 512 columns of all four.
-    if (lane < kRows) {
-        L.stat[wave][0][lane] = m;
-        L.stat[wave][1][lane] = l;
-        L.stat[wave][2][lane] = ones[0];
-    }
-    __syncthreads();                            // (and every wave is done with its tiles)
-    const int n = lane & 15;
-    float top = L.stat[0][0][n];
-#pragma unroll
-    for (int i = 1; i < kWaves; ++i) top = fmaxf(top, L.stat[i][0][n]);
-    const float base_m = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, rounded = 0.f;
+    barrier();
+    f32x4* stat = reinterpret_cast<f32x4*>(&L.p[0][0][0]);
+    if (lane < 16) stat[wave * 16 + lane] = f32x4{m, l, ones[0], 0.f};
+    barrier();
+    const int64_t slot = (int64_t)unit * P.shares + split;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-        const float f = exp2_(L.stat[i][0][n] - base_m);
-        sum += f * L.stat[i][1][n];
-        rounded += f * L.stat[i][2][n];
-    }
-    const float f = exp2_(m - base_m);
+        const int row = i * 16 + n;
+        const f32x4 st = stat[row];
+        const int column0 = wave * (kC / kWaves) + 4 * g;
+        if (whole) {
+            if (w.row0 + row >= w.rows) continue;
+            const int64_t at = (int64_t)w.tok0 * P.n_heads + w.row0 + row;
+            const float inv = st[2] == 0.f ? 0.f : 1.f / st[2];
 #pragma unroll
-    for (int i = 0; i < kC / 16; ++i) L.sum[wave][i][lane] = acc[i] * f;
-    __syncthreads();
-    constexpr int kMine = kC / 16 / kWaves;
-    f32x4 o[kMine];
+            for (int j = 0; j < kCols; ++j) put(P.out + at * kC + column0 + j * 16, acc[i][j], inv);
+            if (P.lse && wave == 0 && g == 0) P.lse[at] = lse_of(st[0], st[1]);
+        } else {
+            float* part = P.part + (slot * kMany + row) * kC + column0;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-        const int ch = wave * kMine + i;
-        o[i] = (L.sum[0][ch][lane] + L.sum[1][ch][lane]) + (L.sum[2][ch][lane] + L.sum[3][ch][lane]);
-    }
-    if (whole) {
-        if (!live) return;
-        const int64_t at = (int64_t)(w.tok0 + tok) * P.n_heads + head;
-        const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            const uint64_t b = (uint64_t)(bf16_bits(o[i][0] * inv) | bf16_bits(o[i][1] * inv) << 16) |
-                               (uint64_t)(bf16_bits(o[i][2] * inv) | bf16_bits(o[i][3] * inv) << 16)
-                                   << 32;
-            st_global(reinterpret_cast<uint64_t*>(P.out + at * kC + (wave * kMine + i) * 16 + 4 * g), b);
+            for (int j = 0; j < kCols; ++j)
+                st_global(reinterpret_cast<f32x4*>(part + j * 16), acc[i][j]);
+            if (wave == 0 && g == 0) st_global(P.stat + slot * kMany + row, st);
         }
-        if (P.lse && wave == 0 && g == 0)
-            P.lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
-        return;
-    }
-    const int64_t slot = (int64_t)(blockIdx.x / P.splits) * P.splits + split;
-    float* part = P.part + slot * kRows * kC;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i)
-        st_global(reinterpret_cast<f32x4*>(part + n * kC + (wave * kMine + i) * 16 + 4 * g), o[i]);
-    if (wave == 0 && g == 0) {
-        float* stat = P.part + (int64_t)kPartRows * kC + (slot * kRows + n) * 4;
-        stat[0] = top;
-        stat[1] = sum;
-        stat[2] = rounded;
     }
 }
 
-// Joins the splits of a row: a workgroup per row, each thread four columns. The splits
-// are read in order, so the result does not depend on timing.
-constexpr int kJoinThreads = 128;
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams P) {
+__global__ __launch_bounds__(kJoinThreads) void join_many_kernel(AttendParams P) {
+    const int64_t u = blockIdx.x / kMany;
     Work w;
-    const int64_t u = blockIdx.x / kRows;
-    const int n = blockIdx.x % kRows;
-    if (!find_work<kRows>(P, u, w)) return;
-    const int each = split_size(w.n, P.splits);
+    if (!find_work<kMany, kStep>(P, u, w)) return;
+    const int row = blockIdx.x % kMany;
+    if (w.row0 + row >= w.rows) return;
+    const int each = (w.n + P.shares - 1) / P.shares;
     if (each >= w.n) return;
-    const int row = w.row0 + n;
-    if (row >= w.rows) return;
-    const int used = (w.n + each - 1) / each;
-    const int64_t slot0 = u * P.splits;
-    const f32x4* stat = reinterpret_cast<const f32x4*>(P.part + (int64_t)kPartRows * kC) +
-                        slot0 * kRows + n;
-    float top = -INFINITY;
-    for (int i = 0; i < used; ++i) top = fmaxf(top, stat[(int64_t)i * kRows][0]);
-    const float base_m = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, rounded = 0.f;
-    f32x4 o{0.f, 0.f, 0.f, 0.f};
-    const f32x4* part = reinterpret_cast<const f32x4*>(P.part + (slot0 * kRows + n) * kC) +
-                        threadIdx.x;
-#pragma unroll 8
-    for (int i = 0; i < used; ++i) {
-        const f32x4 st = stat[(int64_t)i * kRows];
-        const float f = exp2_(st[0] - base_m);
-        sum += f * st[1];
-        rounded += f * st[2];
-        o += part[(int64_t)i * kRows * kC / 4] * f;
-    }
-    const int64_t at = (int64_t)w.tok0 * P.n_heads + row;
-    const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
-    const uint64_t b = (uint64_t)(bf16_bits(o[0] * inv) | bf16_bits(o[1] * inv) << 16) |
-                       (uint64_t)(bf16_bits(o[2] * inv) | bf16_bits(o[3] * inv) << 16) << 32;
-    st_global(reinterpret_cast<uint64_t*>(P.out + at * kC + threadIdx.x * 4), b);
-    if (P.lse && threadIdx.x == 0)
-        P.lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    join<kMany>(P, (int64_t)w.tok0 * P.n_heads + w.row0 + row, row, u * P.shares,
+                u * P.shares + 1, 1, (w.n + each - 1) / each);
 }
 
 }  // namespace cache
@@ -468,6 +805,23 @@ using namespace fleet_moe;
 using namespace fleet_moe::cache;
 
 int fleet_moe_check_device(int min_cus);
+
+// More than 64 KB of dynamic LDS has to be asked for. (The LDS is dynamic so that
+// the compiler keeps to the registers of two waves on a SIMD, and takes O as an
+// operand of the matrix instructions from them; where it knows that LDS allows one
+// only, it moves O to accumulation registers and back, 400 moves a step.)
+template <class K>
+static int launch(K kernel, int64_t grid, int threads, size_t lds, const AttendParams& P,
+                  hipStream_t stream) {
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)lds);
+        if (e != hipSuccess) return (int)e;
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, stream, P);
+    return (int)hipGetLastError();
+}
 
 extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const uint16_t* q,
                                   int64_t q_stride, const int32_t* start, int32_t n_tokens,
@@ -491,9 +845,11 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     P.start = start;
     P.out = out;
     P.lse = lse;
-    char* ws = static_cast<char*>(workspace);
-    P.h = reinterpret_cast<Header*>(ws);
-    P.part = reinterpret_cast<float*>(ws + parts_at(cache->n_seqs, cache->n_pages));
+    char* ws = static_cast<char*>(workspace) + parts_at(cache->n_seqs, cache->n_pages);
+    P.h = static_cast<Header*>(workspace);
+    P.part = reinterpret_cast<float*>(ws);
+    P.stat = reinterpret_cast<f32x4*>(ws + kPartBytes);
+    P.meta = reinterpret_cast<int4*>(ws + kPartBytes + kStatBytes);
     P.q_stride = q_stride;
     P.layer = layer;
     P.n_tokens = n_tokens;
@@ -501,21 +857,28 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     P.window = window;
     P.sinks = sinks;
     P.scale = scale * 1.4426950408889634f;
-    P.pad = n_heads % kRows != 0;
-    const int64_t units = first_unit(n_tokens, cache->n_seqs, n_heads, kRows, P.pad);
+    // positions that a row may see, as far as the host knows
     int64_t seen = (int64_t)cache->max_pages * kPage;
     if (max_len > 0 && max_len < seen) seen = max_len;
-    if (window > 0 && (int64_t)window + sinks + n_tokens < seen) seen = (int64_t)window + sinks + n_tokens;
-    const int64_t rounds = (seen + kTile * kWaves - 1) / (kTile * kWaves);
-    int64_t splits = 512 / units;
-    if (splits > rounds) splits = rounds;
-    if (splits > 64) splits = 64;
-    if (splits < 1) splits = 1;
-    P.splits = (int)splits;
-    hipLaunchKernelGGL(attend_kernel, dim3((unsigned)(units * splits)), dim3(kThreads), 0, stream,
-                       P);
-    if (splits > 1)
-        hipLaunchKernelGGL(join_kernel, dim3((unsigned)(units * kRows)), dim3(kJoinThreads), 0,
-                           stream, P);
-    return (int)hipGetLastError();
+    if (window > 0 && (int64_t)window + sinks + n_tokens < seen)
+        seen = (int64_t)window + sinks + n_tokens;
+    const int64_t rows = (int64_t)n_tokens * n_heads;
+    P.pad = n_heads % kFew != 0;
+    const int64_t few = first_unit(n_tokens, cache->n_seqs, n_heads, kFew, P.pad);
+    if (rows <= 2 * kFew * (int64_t)cache->n_seqs && few <= kMaxUnits) {
+        P.units = (int)few;
+        const int64_t steps = few * ((seen + kPage - 1) / kPage);
+        P.shares = (int)(steps < kShares ? steps : kShares);
+        if (int e = launch(few_kernel, P.shares, kThreads, sizeof(FewLds), P, stream)) return e;
+        return launch(join_few_kernel, few * kFew, kJoinThreads, 0, P, stream);
+    }
+    P.pad = n_heads % kMany != 0;
+    const int64_t units = first_unit(n_tokens, cache->n_seqs, n_heads, kMany, P.pad);
+    P.units = (int)units;
+    int64_t splits = kShares / 2 / units;
+    const int64_t most = (seen + 4 * kStep - 1) / (4 * kStep);
+    if (splits > most) splits = most;
+    P.shares = splits < 1 ? 1 : (int)splits;
+    if (int e = launch(many_kernel, units * P.shares, kThreads, sizeof(ManyLds), P, stream)) return e;
+    return P.shares > 1 ? launch(join_many_kernel, units * kMany, kJoinThreads, 0, P, stream) : 0;
 }

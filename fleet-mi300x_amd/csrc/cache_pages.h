@@ -97,11 +97,14 @@ struct Copy {
 
 __device__ __forceinline__ void raise(Header* h, uint32_t bit) { atomicOr(&h->status, bit); }
 
-// The partial results the attention may hold: 16-row tiles of fp32 [16][512] and
-// each row's maximum and sums [4].
-constexpr int kPartTiles = 1024;
-constexpr int kPartRows = kPartTiles * 16;
-constexpr size_t kPartBytes = (size_t)kPartRows * (kC + 4) * 4;
+// What the attention's second launch joins: partial results of up to 1024 times 16
+// rows (fp32 [512] each), their maxima and sums, and where a unit's lie.
+constexpr int kShares = 512;
+constexpr int kMaxUnits = 4096;
+constexpr int kPartRows = 2 * kShares * 16;
+constexpr size_t kPartBytes = (size_t)kPartRows * kC * 4;
+constexpr size_t kStatBytes = (size_t)kPartRows * 16;
+constexpr size_t kMetaBytes = (size_t)kMaxUnits * 16;
 
 __host__ __device__ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 __host__ __device__ inline size_t copies_at() { return sizeof(Header); }
@@ -113,7 +116,7 @@ __host__ __device__ inline size_t parts_at(int n_seqs, int n_pages) {
     return list_at(n_seqs, n_pages) + up256((size_t)n_pages * 4);
 }
 inline size_t workspace_size(int n_seqs, int n_pages) {
-    return parts_at(n_seqs, n_pages) + up256(kPartBytes);
+    return parts_at(n_seqs, n_pages) + kPartBytes + kStatBytes + kMetaBytes;
 }
 
 // The checks every call makes of a cache.
