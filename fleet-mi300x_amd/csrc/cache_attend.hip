@@ -38,6 +38,7 @@ struct AttendParams {
     int4* meta;                 // [unit]: first slot, next workgroup, number of slots
     Header* h;
     int64_t q_stride;
+    uint64_t per_head;          // floor(2^40 / n_heads) + 1
     int layer, n_tokens, n_heads, window, sinks, pad, units;
     int shares;                 // workgroups, or splits of a unit
     float scale;                // times log2(e)
@@ -47,6 +48,11 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr float kSlack = 8.f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+// row / n_heads: exact for row < 2^33 (n_heads * per_head is over 2^40 by n_heads at most).
+__device__ __forceinline__ int token_of(const AttendParams& P, int row) {
+    return (int)((uint64_t)(uint32_t)row * P.per_head >> 40);
+}
 
 // A unit: up to R rows (token, head) of a sequence, and the steps of S positions
 // that some of them see: the first n_sink steps from position 0 on, the others from
@@ -66,8 +72,8 @@ template <int R, int S>
 __device__ __forceinline__ void see(const AttendParams& P, Work& w) {
     w.n_sink = w.main = w.n = 0;
     const int last = w.row0 + R - 1 < w.rows ? w.row0 + R - 1 : w.rows - 1;
-    const int p0 = w.len - w.n_new + w.row0 / P.n_heads;
-    const int p1 = w.len - w.n_new + last / P.n_heads;
+    const int p0 = w.len - w.n_new + token_of(P, w.row0);
+    const int p1 = w.len - w.n_new + token_of(P, last);
     if (w.len < 0 || p1 < 0) return;
     const Seen s = seen_of(p0 < 0 ? 0 : p0, P.window, P.sinks);
     const int end = (p1 + S) / S;                         // steps of p1 + 1 positions
@@ -89,64 +95,52 @@ __device__ __forceinline__ void open_seq(const AttendParams& P, int seq, Work& w
 
 // A lane's row, and what it sees.
 struct Row {
-    int64_t at;                 // token * heads + head; -1: no row
+    bool live;
+    int tok, head;              // of the sequence's; dead rows: the unit's first
     int pos;
     Seen seen;
 };
 __device__ __forceinline__ Row row_of(const AttendParams& P, const Work& w, int row) {
     Row r;
-    const bool live = row < w.rows;
-    const int tok = live ? row / P.n_heads : 0;
-    r.at = live ? (int64_t)w.tok0 * P.n_heads + row : -1;
-    r.pos = live && w.len >= 0 ? w.len - w.n_new + tok : -1;
+    r.live = row < w.rows;
+    if (!r.live) row = w.row0;
+    r.tok = token_of(P, row);
+    r.head = row - r.tok * P.n_heads;
+    r.pos = r.live && w.len >= 0 ? w.len - w.n_new + r.tok : -1;
     r.seen = seen_of(r.pos < 0 ? 0 : r.pos, P.window, P.sinks);
     return r;
 }
 // Its query as the right operand: the k order of the products is that of the bytes
 // a lane of group g takes of a row: chunks g, 4 + g, ..
-__device__ __forceinline__ void load_q(const AttendParams& P, const Row& r, int g,
-                                       bf16x8 (&q)[kChunks / 2]) {
-    const int64_t tok = r.at < 0 ? 0 : r.at / P.n_heads;
-    const int head = r.at < 0 ? 0 : (int)(r.at % P.n_heads);
+template <int N>                // N of the 18 steps of 32 values, from `step` on
+__device__ __forceinline__ void load_q(const AttendParams& P, const Work& w, const Row& r, int g,
+                                       int step, bf16x8 (&q)[N]) {
+    const uint16_t* src = P.q + (int64_t)(w.tok0 + r.tok) * P.q_stride + r.head * kRow + g * 16;
 #pragma unroll
-    for (int i = 0; i < kChunks / 4; ++i) {
-        u32x4 a{0, 0, 0, 0}, b{0, 0, 0, 0};
-        if (r.at >= 0) {
-            const u32x4* src = reinterpret_cast<const u32x4*>(P.q + tok * P.q_stride + head * kRow +
-                                                              (4 * i + g) * 16);
-            a = ld_global(src);
-            b = ld_global(src + 1);
-        }
-        q[2 * i] = __builtin_bit_cast(bf16x8, a);
-        q[2 * i + 1] = __builtin_bit_cast(bf16x8, b);
-    }
+    for (int i = 0; i < N; ++i)
+        q[i] = __builtin_bit_cast(bf16x8, ld_global(reinterpret_cast<const u32x4*>(
+                                              src + (step + i) / 2 * 64 + (step + i) % 2 * 8)));
+}
+__device__ __forceinline__ int64_t out_row(const AttendParams& P, const Work& w, int row) {
+    return (int64_t)w.tok0 * P.n_heads + row;
 }
 
 // Blocks in LDS lie 64 bytes further apart than they are long, so that the two
 // halves of a transposing read, from neighbouring blocks, fall into different banks.
 constexpr int kBlockStep = kBlockBytes + 64;
 
-// Copies 16 bytes per lane from global memory to LDS, kN times 1 KB: lane's `src`
-// + 1024 i to `lds` + 1024 i + 16 lane (the offset counts on both sides). There is
-// no register for the data, so none is in flight behind the compiler's back. In asm,
-// because the compiler would wait for every copy in flight before each LDS read;
-// wait_copies() orders them.
-template <int kN>
+// Copies 16 bytes per lane from global memory to LDS, 1 KB in all: to `lds` + 16 lane.
+// There is no register for the data, so none is in flight behind the compiler's
+// back. In asm, because the compiler would wait for every copy in flight before each
+// LDS read; wait_copies() orders them.
+template <bool kOnce>           // read once: kept out of the caches
 __device__ __forceinline__ void copy_kb(const uint8_t* src, uint32_t lds) {
-    static_assert(kN == 1 || kN == 4, "");
-    if constexpr (kN == 4)
-        asm volatile(
-            "s_nop 0\n\t"
-            "global_load_lds_dwordx4 %0, off\n\t"
-            "global_load_lds_dwordx4 %0, off offset:1024\n\t"
-            "global_load_lds_dwordx4 %0, off offset:2048\n\t"
-            "global_load_lds_dwordx4 %0, off offset:3072" ::"v"(src), "{m0}"(lds)
-            : "memory");
+    if constexpr (kOnce)
+        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "{m0}"(lds)
+                     : "memory");
     else
-        asm volatile(
-            "s_nop 0\n\t"
-            "global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds)
-            : "memory");
+        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds)
+                     : "memory");
 }
 // The same with 4 bytes per lane.
 __device__ __forceinline__ void copy_words(const uint8_t* src, uint32_t lds) {
@@ -278,251 +272,319 @@ __device__ __forceinline__ int page_of(const AttendParams& P, const Work& w, Pag
 
 // Sequences with a token or two: 16 rows a unit, a page a step. The bytes of the
 // pages bound it (576 a position for 16 rows, 60 flops a byte), so what matters is
-// that they keep coming: each wave copies its own block of the page into LDS and
-// takes the scores of its 16 positions; after one barrier every wave has all
-// weights and adds its 128 columns of O over the whole page. O needs 32 registers
-// a lane this way, q 72, and no sum over waves at the end; two workgroups share a
-// CU, and one's copies run beside the other's products.
+// that they keep coming: four pages fit in LDS, two or three of them on their way.
+// Eight waves, two on a SIMD (one alone issues a vector instruction every six
+// cycles, two every three). A block's scores are shared by two waves, half of the 576
+// products each; the first four waves add the halves up and make the weights while
+// the other four issue the copies (a copy of 1 KB occupies the address unit for 24
+// cycles, so a page's hold a wave up for a thousand). Then each wave adds its 64
+// columns of O over the whole page: 16 registers a lane, and no sum over waves at the
+// end.
 //
 // The work is divided into equal shares of steps over all units, whatever their
 // lengths: a workgroup takes a range of the concatenated steps, across units where it
 // has to. A unit that several have a part in leaves partial results, which
-// join_kernel adds in order.
+// join_few_kernel adds in order.
+constexpr int kDeep = 4;        // pages in LDS
+constexpr int kFewWaves = 8;
+constexpr int kFewThreads = kFewWaves * 64;
 struct FewLds {
-    __attribute__((aligned(16))) uint8_t tile[2][4 * kBlockStep];
-    uint32_t scale[2][kWaves][64];
+    __attribute__((aligned(16))) uint8_t tile[kDeep][4 * kBlockStep];
+    uint32_t scale[kDeep][64];
+    f32x4 half[4][64];          // the second half of a block's scores
     u32x4 p[2][2][64];          // [step parity][half of the page][lane]
-    float top[2][kWaves][16];
-    int flag[2][kWaves];
-    int64_t before[kWaves];
-    int seq, row0;
-    int64_t off;
+    float top[2][4][16];
+    int flag[2][4];
 };
-static_assert(sizeof(FewLds) <= 80 * 1024, "two workgroups share a CU");
+static_assert(sizeof(FewLds) <= 160 * 1024, "");
 constexpr int kFew = 16;        // rows
 
+constexpr int kPageCopies = 10; // of each of four waves: 9 KB of codes, and the scales
 constexpr int kNeedMax = 1, kHasNan = 2;
 
 // The steps of all units of a sequence, an empty unit as one.
-__device__ __forceinline__ int64_t seq_steps(const AttendParams& P, Work& w) {
-    int64_t n = 0;
+__device__ __forceinline__ int seq_steps(const AttendParams& P, Work& w) {
+    int n = 0;
     for (w.row0 = 0; w.row0 < w.rows; w.row0 += kFew) {
         see<kFew, kPage>(P, w);
         n += w.n > 0 ? w.n : 1;
     }
     return n;
 }
-
-// The total of steps, and where step `at` of them lies: sequence, row and step of
-// the unit (in L). `at` is a function of the total.
-template <class F>
-__device__ __forceinline__ int64_t locate(const AttendParams& P, FewLds& L, F at) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int each = (P.c.n_seqs + kThreads - 1) / kThreads;
-    Work w;
-    int64_t mine = 0;
-    for (int i = 0; i < each; ++i) {
-        const int s = t * each + i;
-        if (s >= P.c.n_seqs) break;
-        open_seq(P, s, w);
-        mine += seq_steps(P, w);
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t o = __shfl_up((long long)incl, d);
-        if (lane >= d) incl += o;
-    }
-    if (lane == 63) L.before[wave] = incl;
-    __syncthreads();
-    int64_t total = 0, first = incl - mine;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        if (i < wave) first += L.before[i];
-        total += L.before[i];
-    }
-    int64_t want = at(total) - first;
-    if (want >= 0 && want < mine) {
-        for (int i = 0; i < each; ++i) {
-            open_seq(P, t * each + i, w);
-            const int64_t n = seq_steps(P, w);
-            if (want < n) break;
-            want -= n;
-        }
-        for (w.row0 = 0;; w.row0 += kFew) {
-            see<kFew, kPage>(P, w);
-            const int n = w.n > 0 ? w.n : 1;
-            if (want < n) break;
-            want -= n;
-        }
-        L.seq = w.seq;
-        L.row0 = w.row0;
-        L.off = want;
-    }
-    __syncthreads();
-    return total;
+__device__ __forceinline__ int lane_of(int v, int lane) {
+    return __builtin_amdgcn_readlane(v, lane);
+}
+__device__ __forceinline__ Work lane_of(const Work& v, int lane) {
+    Work w{};
+    w.seq = lane_of(v.seq, lane);
+    w.rows = lane_of(v.rows, lane);
+    w.tok0 = lane_of(v.tok0, lane);
+    w.n_new = lane_of(v.n_new, lane);
+    w.len = lane_of(v.len, lane);
+    return w;
 }
 
-__global__ __launch_bounds__(kThreads, 2) void few_kernel(AttendParams P) {
+// A range of n things in `shares` parts that differ by one at most.
+struct Shares {
+    int each, more;             // the first `more` have each + 1
+    __device__ Shares(int n, int shares) : each(n / shares), more(n % shares) {}
+    __device__ int first(int i) const { return i * each + (i < more ? i : more); }
+    __device__ int holder(int at) const {
+        const int big = more * (each + 1);
+        return at < big ? at / (each + 1) : more + (at - big) / each;
+    }
+};
+
+// The total of all units' steps; its division (no share is empty: the join counts
+// on it); and the unit in which workgroup wg's part begins, and where. Every
+// wave for itself, a lane per sequence (or for several, then once more a lane for each
+// of the one lane's): no barrier, and one round of loads for 64 sequences.
+__device__ __forceinline__ bool locate(const AttendParams& P, int wg, Work& w, int& off, int& total,
+                                       int& shares) {
+    const int lane = threadIdx.x & 63;
+    const int each = (P.c.n_seqs + 63) / 64;
+    Work mine{};
+    int n = 0;
+    for (int i = 0; i < each; ++i) {
+        const int s = lane * each + i;
+        if (s < P.c.n_seqs) {
+            open_seq(P, s, mine);
+            n += seq_steps(P, mine);
+        }
+    }
+    int incl = wave_incl_scan(n);
+    total = lane_of(incl, 63);
+    shares = total < P.shares ? total : P.shares;
+    if (wg >= shares) return false;
+    off = Shares(total, shares).first(wg);
+    int owner = __popcll(__ballot(incl <= off));
+    off -= lane_of(incl - n, owner);
+    if (each > 1) {
+        const int s = owner * each + lane;
+        mine.seq = s;
+        n = 0;
+        if (lane < each && s < P.c.n_seqs) {
+            open_seq(P, s, mine);
+            n = seq_steps(P, mine);
+        }
+        incl = wave_incl_scan(n);
+        owner = __popcll(__ballot(incl <= off));
+        off -= lane_of(incl - n, owner);
+    }
+    w = lane_of(mine, owner);
+    for (w.row0 = 0;; w.row0 += kFew) {
+        see<kFew, kPage>(P, w);
+        const int all = w.n > 0 ? w.n : 1;
+        if (off < all) return true;
+        off -= all;
+    }
+}
+
+__global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     FewLds& L = *reinterpret_cast<FewLds*>(lds);
     const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
-    const int g = lane >> 4, n = lane & 15;
+    const int g = lane >> 4, n = lane & 15, blk = wave & 3;
     const int wg = blockIdx.x;
-    // (no share is empty: the join counts on it)
-    const auto share = [&](int64_t all, int i) { return all * i / (all < P.shares ? all : P.shares); };
-    const int64_t total = locate(P, L, [&](int64_t all) { return all ? share(all, wg) : 0; });
-    const int shares = total < P.shares ? (int)total : P.shares;
-    if (wg >= shares) return;
-    int64_t at = share(total, wg);
-    const int64_t end = share(total, wg + 1);
     Work w;
-    open_seq(P, wave_bcast(L.seq), w);
-    w.row0 = wave_bcast(L.row0);
-    int off = wave_bcast((int)L.off);
+    int off, total, shares;
+    if (!locate(P, wg, w, off, total, shares)) return;
+    const Shares share(total, shares);
+    int at = share.first(wg);
+    const int end = share.first(wg + 1);
     for (bool lead = true;; lead = false) {
         see<kFew, kPage>(P, w);
         const int all = w.n > 0 ? w.n : 1;
-        const int take = all - off < end - at ? all - off : (int)(end - at);
+        const int take = all - off < end - at ? all - off : end - at;
         const int until = off + take < w.n ? off + take : w.n;
         const int cnt = until > off ? until - off : 0;
         const Row r = row_of(P, w, w.row0 + n);
         if (w.len < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
 
-        bf16x8 q[kChunks / 2];
-        load_q(P, r, g, q);
-        f32x4 acc[kC / 16 / kWaves];
+        constexpr int kHalf = kChunks / 4;      // steps of 32 values, of 18
+        bf16x8 q[kHalf];
+        load_q(P, w, r, g, wave < 4 ? 0 : kHalf, q);
+        constexpr int kCols = kC / 16 / kFewWaves;
+        f32x4 acc[kCols];
 #pragma unroll
         for (auto& a : acc) a = f32x4{0.f, 0.f, 0.f, 0.f};
         f32x4 ones{0.f, 0.f, 0.f, 0.f};         // the sum of the rounded weights
+        f32x4 z;
         float m = -INFINITY, l = 0.f;
+        float s[4], p[4];
         Pages pages{0, 0, 0};
-        int good = 0;                           // bit: whether that buffer's page is one
+        // copies page k: waves 4 .. 7
         const auto issue = [&](int k) {
             const int page = page_of<kPage>(P, w, pages, off + k, until, lane);
             const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
             const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
-            const uint8_t* from = src + wave * kBlockBytes + lane * 16;
-            const uint32_t to = lds_addr(L.tile[k & 1]) + wave * kBlockStep;
-            copy_kb<4>(from, to);
-            copy_kb<4>(from + 4096, to + 4096);
-            copy_kb<1>(from + 8192, to + 8192);
-            copy_words(src + kCodeBytes + (lane & 7) * 4, lds_addr(L.scale[k & 1][wave]));
-            const int bit = 1 << (k & 1);
-            good = base >= 0 ? good | bit : good & ~bit;
-            if (base < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
-        };
-        if (cnt > 0) issue(0);
-        if (cnt > 1) issue(1);
-        for (int k = 0; k < cnt; ++k) {
-            const int b = k & 1;
-            if (k == 0 && cnt > 1) wait_copies<10>();
-            else wait_copies<0>();
-            const uint8_t* block = L.tile[b] + wave * kBlockStep;
-            f32x4 z{0.f, 0.f, 0.f, 0.f}, z2{0.f, 0.f, 0.f, 0.f};
-            {
-                const float sc = any_scale(L.scale[b][wave][2 * wave]);
-                const float sp = any_scale(L.scale[b][wave][2 * wave + 1]);
+            const uint8_t* from = src + blk * kBlockBytes + lane * 16;
+            const int b = k % kDeep;
+            const uint32_t to = lds_addr(L.tile[b]) + blk * kBlockStep;
 #pragma unroll
-                for (int i = 0; i < kChunks / 4; ++i) {
-                    const u32x4 a = *reinterpret_cast<const u32x4*>(block + i * 1024 + lane * 16);
-                    const float s = i < kC / 64 ? sc : sp;
-                    z = mfma(widen(a.x, a.y, s, s), q[2 * i], z);
-                    z2 = mfma(widen(a.z, a.w, s, s), q[2 * i + 1], z2);
+            for (int i = 0; i < kBlockBytes / 1024; ++i) copy_kb<true>(from + i * 1024, to + i * 1024);
+            copy_words(src + kCodeBytes + (lane & 7) * 4, lds_addr(L.scale[b]));
+        };
+        // this wave's half of its block's scores
+        const auto score = [&](int k) {
+            const int b = k % kDeep;
+            const uint8_t* block = L.tile[b] + blk * kBlockStep + lane * 16;
+            const float sc = any_scale(L.scale[b][2 * blk]);
+            f32x4 z0{0.f, 0.f, 0.f, 0.f}, z1{0.f, 0.f, 0.f, 0.f};
+            const auto chunk = [&](int i) { return *reinterpret_cast<const u32x4*>(block + i * 1024); };
+            if (wave < 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const u32x4 a = chunk(i);
+                    z0 = mfma(widen(a.x, a.y, sc, sc), q[2 * i], z0);
+                    z1 = mfma(widen(a.z, a.w, sc, sc), q[2 * i + 1], z1);
                 }
+                const u32x4 a = chunk(4);
+                z0 = mfma(widen(a.x, a.y, sc, sc), q[8], z0);
+            } else {
+                const float sp = any_scale(L.scale[b][2 * blk + 1]);
+                u32x4 a = chunk(4);
+                z0 = mfma(widen(a.z, a.w, sc, sc), q[0], z0);
+#pragma unroll
+                for (int i = 5; i < 8; ++i) {
+                    a = chunk(i);
+                    z1 = mfma(widen(a.x, a.y, sc, sc), q[2 * i - 9], z1);
+                    z0 = mfma(widen(a.z, a.w, sc, sc), q[2 * i - 8], z0);
+                }
+                a = chunk(8);
+                z1 = mfma(widen(a.x, a.y, sp, sp), q[7], z1);
+                z0 = mfma(widen(a.z, a.w, sp, sp), q[8], z0);
             }
-            float s[4], p[4], top = -INFINITY;
+            z = z0 + z1;
+            if (wave >= 4) L.half[blk][lane] = z;
+        };
+        // the weights of step k under the reference m: waves 0 .. 3
+        const auto weigh = [&](int k) {
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = exp2_(s[j] - ref);
+            reinterpret_cast<uint2*>(&L.p[k & 1][blk >> 1][lane])[blk & 1] = weights(p);
+        };
+        const auto finish = [&](int k) {
+            z += L.half[blk][lane];
+            float top = -INFINITY;
             bool nan = false;
-            const bool ok = good >> b & 1;
-            const int base = step_of<kPage>(w, off + k) * kPage + wave * kBlock + 4 * g;
+            const int page = page_of<kPage>(P, w, pages, off + k, until, lane);
+            const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
+            if (!ok && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
+            const int base = step_of<kPage>(w, off + k) * kPage + blk * kBlock + 4 * g;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float v = (z[j] + z2[j]) * P.scale;
+                const float v = z[j] * P.scale;
                 nan |= v != v;
                 const int pos = base + j;
                 s[j] = ok && pos <= r.pos && (pos >= r.seen.lo || pos < r.seen.sink) ? v : -INFINITY;
                 top = fmaxf(top, s[j]);
             }
             top = xor32_max(xor16_max(top));
-            // m is any reference not far below the maximum: weights up to 2^kSlack are
-            // as exact as those up to 1, and moving it costs a pass over O and a
-            // barrier
-            const auto weigh = [&] {
-                const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) p[j] = exp2_(s[j] - ref);
-                reinterpret_cast<uint2*>(&L.p[b][wave >> 1][lane])[wave & 1] = weights(p);
-            };
-            weigh();
-            if (lane < 16) L.top[b][wave][lane] = top;
+            weigh(k);
+            if (lane < 16) L.top[k & 1][blk][lane] = top;
             const int flag = (__ballot(top > m + kSlack) ? kNeedMax : 0) |
                              (__ballot(nan) ? kHasNan : 0);
-            if (lane == 0) L.flag[b][wave] = flag;
-            barrier();                          // every block is there, every weight
-            if (k > 0 && k + 1 < cnt) issue(k + 1);       // where the page before was
-            const int any = wave_bcast((L.flag[b][0] | L.flag[b][1]) | (L.flag[b][2] | L.flag[b][3]));
+            if (lane == 0) L.flag[k & 1][blk] = flag;
+        };
+        // Step k: behind barrier A the weights of k and page k + 1 are there, behind
+        // B both halves of the scores of k + 1.
+        if (wave >= 4) {
+            for (int k = 0; k < kDeep - 1 && k < cnt; ++k) issue(k);
+            if (cnt > 2) wait_copies<2 * kPageCopies>();
+            else if (cnt > 1) wait_copies<kPageCopies>();
+            else wait_copies<0>();
+        }
+        barrier();
+        for (int k = -1; k < cnt; ++k) {
+            if (k + 1 < cnt) {
+                score(k + 1);
+                barrier();                      // B
+                if (wave < 4) {
+                    finish(k + 1);
+                } else {
+                    // into the buffer of page k - 1
+                    if (k >= 0 && k + kDeep - 1 < cnt) issue(k + kDeep - 1);
+                    // page k + 2; the one behind it may be on its way
+                    if (cnt - k > 3) wait_copies<kPageCopies>();
+                    else wait_copies<0>();
+                }
+            }
+            if (k >= 0) {
+                const int b = k % kDeep, par = k & 1;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[par][h][lane]);
+                    const float sa = any_scale(L.scale[b][4 * h]);
+                    const float sb = any_scale(L.scale[b][4 * h + 2]);
+                    const uint8_t* col = column_at(L.tile[b] + 2 * h * kBlockStep, lane) +
+                                         wave * kCols * 256;
+#pragma unroll
+                    for (int i = 0; i < kCols; ++i) {
+                        const i32x2 v = column(col, i);
+                        acc[i] = mfma(widen((uint32_t)v.x, (uint32_t)v.y, sa, sb), pb, acc[i]);
+                    }
+                    ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}), pb,
+                                ones);
+                }
+            }
+            if (k + 1 == cnt) break;
+            barrier();                          // A
+            const int par = (k + 1) & 1;
+            const int any = wave_bcast((L.flag[par][0] | L.flag[par][1]) |
+                                       (L.flag[par][2] | L.flag[par][3]));
             if (any) {
+                // m is any reference not far below the maximum: weights up to 2^kSlack
+                // are as exact as those up to 1, and moving it costs a pass over O and a
+                // barrier
                 if (any & kNeedMax) {
                     float to = m;
 #pragma unroll
-                    for (int i = 0; i < kWaves; ++i) to = fmaxf(to, L.top[b][i][n]);
+                    for (int i = 0; i < 4; ++i) to = fmaxf(to, L.top[par][i][n]);
                     const float shrink = to == -INFINITY ? 1.f : exp2_(m - to);
                     m = to;
                     l *= shrink;
                     ones *= shrink;
 #pragma unroll
                     for (auto& a : acc) a *= shrink;
-                    weigh();
+                    if (wave < 4) weigh(k + 1);
                 }
-                if (any & kHasNan) clean(L.tile[b] + wave * kBlockStep, lane);
+                if ((any & kHasNan) && wave < 4)
+                    clean(L.tile[(k + 1) % kDeep] + blk * kBlockStep, lane);
                 barrier();
             }
-            l += (p[0] + p[1]) + (p[2] + p[3]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[b][h][lane]);
-                const float sa = any_scale(L.scale[b][wave][4 * h]);
-                const float sb = any_scale(L.scale[b][wave][4 * h + 2]);
-                const uint8_t* col = column_at(L.tile[b] + 2 * h * kBlockStep, lane) +
-                                     wave * (kC / kWaves / 16) * 256;
-#pragma unroll
-                for (int i = 0; i < kC / 16 / kWaves; ++i) {
-                    const i32x2 v = column(col, i);
-                    acc[i] = mfma(widen((uint32_t)v.x, (uint32_t)v.y, sa, sb), pb, acc[i]);
-                }
-                ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}), pb, ones);
-            }
+            if (wave < 4) l += (p[0] + p[1]) + (p[2] + p[3]);
         }
-        // the waves' sums
+        // the sums of the four blocks
         l = xor32_sum(xor16_sum(l));
         barrier();
-        if (lane < 16) L.top[0][wave][lane] = l;
+        if (wave < 4 && lane < 16) L.top[0][blk][lane] = l;
         barrier();
         const float sum = (L.top[0][0][n] + L.top[0][1][n]) + (L.top[0][2][n] + L.top[0][3][n]);
         const bool whole = take == all;
-        const int column0 = wave * (kC / kWaves) + 4 * g;
+        const int column0 = wave * kCols * 16 + 4 * g;
         if (whole) {
-            if (r.at >= 0) {
+            if (r.live) {
+                const int64_t to = out_row(P, w, w.row0 + n);
                 const float inv = ones[0] == 0.f ? 0.f : 1.f / ones[0];
 #pragma unroll
-                for (int i = 0; i < kC / 16 / kWaves; ++i)
-                    put(P.out + r.at * kC + column0 + i * 16, acc[i], inv);
-                if (P.lse && wave == 0 && g == 0) P.lse[r.at] = lse_of(m, sum);
+                for (int i = 0; i < kCols; ++i) put(P.out + to * kC + column0 + i * 16, acc[i], inv);
+                if (P.lse && wave == 0 && g == 0) P.lse[to] = lse_of(m, sum);
             }
         } else {
             // a workgroup has at most two such: its first, and its last
-            const int64_t slot = 2 * (int64_t)wg + (lead ? 0 : 1);
-            float* part = P.part + (slot * kFew + n) * kC + column0;
+            const int slot = 2 * wg + (lead ? 0 : 1);
+            float* part = P.part + ((int64_t)slot * kFew + n) * kC + column0;
 #pragma unroll
-            for (int i = 0; i < kC / 16 / kWaves; ++i)
+            for (int i = 0; i < kCols; ++i)
                 st_global(reinterpret_cast<f32x4*>(part + i * 16), acc[i]);
             if (wave == 0 && g == 0) st_global(P.stat + slot * kFew + n, f32x4{m, sum, ones[0], 0.f});
         }
         if (off == 0 && t == 0) {
             const int64_t u = first_unit(w.tok0, w.seq, P.n_heads, kFew, P.pad) + w.row0 / kFew;
-            // the workgroup of the unit's last step: the last with its first step there
-            const int64_t last = ((at + all) * shares + total - 1) / total - 1;
-            P.meta[u] = make_int4(2 * wg + (lead ? 0 : 1), wg + 1, whole ? 1 : (int)(last - wg) + 1, 0);
+            const int last = share.holder(at + all - 1);
+            P.meta[u] = make_int4(2 * wg + (lead ? 0 : 1), wg + 1, whole ? 1 : last - wg + 1, 0);
         }
         at += take;
         if (at >= end) return;
@@ -547,24 +609,28 @@ __device__ __forceinline__ void join(const AttendParams& P, int64_t row_at, int 
     __shared__ f32x4 sum_o[kJoinGroups][kC / 4];
     const int t = threadIdx.x % (kC / 4), part = threadIdx.x / (kC / 4);
     const auto slot = [&](int i) { return (i == 0 ? slot0 : rest + (i - 1) * step) * R + row; };
+    // the parts' weights: a lane per part
+    __shared__ float factor[kShares];
+    const int lane = threadIdx.x & 63;
     float top = -INFINITY;
-    for (int i = 0; i < count; ++i) top = fmaxf(top, ld_global(P.stat + slot(i))[0]);
+    for (int i = lane; i < count; i += 64) top = fmaxf(top, ld_global(P.stat + slot(i))[0]);
+    top = wave_max(top);
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f, rounded = 0.f;
-    for (int i = 0; i < count; ++i) {
+    for (int i = lane; i < count; i += 64) {
         const f32x4 st = ld_global(P.stat + slot(i));
         const float f = exp2_(st[0] - ref);
+        if (threadIdx.x < 64) factor[i] = f;
         sum += f * st[1];
         rounded += f * st[2];
     }
+    sum = wave_sum(sum);
+    rounded = wave_sum(rounded);
+    __syncthreads();
     f32x4 o{0.f, 0.f, 0.f, 0.f};
-    const int each = (count + kJoinGroups - 1) / kJoinGroups;
-    const int end = (part + 1) * each < count ? (part + 1) * each : count;
 #pragma unroll 4
-    for (int i = part * each; i < end; ++i) {
-        const float f = exp2_(ld_global(P.stat + slot(i))[0] - ref);
-        o += ld_global(reinterpret_cast<const f32x4*>(P.part + slot(i) * kC) + t) * f;
-    }
+    for (int i = part; i < count; i += kJoinGroups)
+        o += ld_global(reinterpret_cast<const f32x4*>(P.part + slot(i) * kC) + t) * factor[i];
     sum_o[part][t] = o;
     __syncthreads();
     if (part) return;
@@ -594,7 +660,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams P) 
     if (w.row0 + row >= w.rows) return;
     const int4 m = P.meta[u];
     if (m.z <= 1) return;
-    join<kFew>(P, (int64_t)w.tok0 * P.n_heads + w.row0 + row, row, m.x, 2 * (int64_t)m.y, 2, m.z);
+    join<kFew>(P, out_row(P, w, w.row0 + row), row, m.x, 2 * (int64_t)m.y, 2, m.z);
 }
 
 // ---------------------------------------------------------------- many rows
@@ -634,7 +700,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(AttendParams P) {
     if (w.len < 0 && t == 0 && split == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
 
     bf16x8 q[kChunks / 2];
-    load_q(P, r, g, q);
+    load_q(P, w, r, g, 0, q);
     constexpr int kCols = kC / 16 / kWaves;     // of 16
     f32x4 acc[kWaves][kCols];
 #pragma unroll
@@ -656,7 +722,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(AttendParams P) {
         for (int i = 0; i < 5; ++i) {
             const int piece = wave + kWaves * i;
             if (piece < 18)
-                copy_kb<1>(src + half * 2 * kBlockBytes + piece * 1024 + lane * 16,
+                copy_kb<false>(src + half * 2 * kBlockBytes + piece * 1024 + lane * 16,
                            to + piece * 1024 + (piece >= 9 ? kBlockStep - kBlockBytes : 0));
         }
         copy_words(src + kCodeBytes + half * 16 + (lane & 3) * 4, lds_addr(L.scale[k % 3][wave]));
@@ -771,7 +837,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(AttendParams P) {
         const int column0 = wave * (kC / kWaves) + 4 * g;
         if (whole) {
             if (w.row0 + row >= w.rows) continue;
-            const int64_t at = (int64_t)w.tok0 * P.n_heads + w.row0 + row;
+            const int64_t at = out_row(P, w, w.row0 + row);
             const float inv = st[2] == 0.f ? 0.f : 1.f / st[2];
 #pragma unroll
             for (int j = 0; j < kCols; ++j) put(P.out + at * kC + column0 + j * 16, acc[i][j], inv);
@@ -794,7 +860,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_many_kernel(AttendParams P)
     if (w.row0 + row >= w.rows) return;
     const int each = (w.n + P.shares - 1) / P.shares;
     if (each >= w.n) return;
-    join<kMany>(P, (int64_t)w.tok0 * P.n_heads + w.row0 + row, row, u * P.shares,
+    join<kMany>(P, out_row(P, w, w.row0 + row), row, u * P.shares,
                 u * P.shares + 1, 1, (w.n + each - 1) / each);
 }
 
@@ -854,6 +920,7 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     P.layer = layer;
     P.n_tokens = n_tokens;
     P.n_heads = n_heads;
+    P.per_head = ((uint64_t)1 << 40) / n_heads + 1;
     P.window = window;
     P.sinks = sinks;
     P.scale = scale * 1.4426950408889634f;
@@ -865,17 +932,18 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     const int64_t rows = (int64_t)n_tokens * n_heads;
     P.pad = n_heads % kFew != 0;
     const int64_t few = first_unit(n_tokens, cache->n_seqs, n_heads, kFew, P.pad);
-    if (rows <= 2 * kFew * (int64_t)cache->n_seqs && few <= kMaxUnits) {
+    if (rows <= 2 * kFew * (int64_t)cache->n_seqs && few <= kMaxUnits &&
+        few * cache->max_pages < (1 << 30)) {
         P.units = (int)few;
         const int64_t steps = few * ((seen + kPage - 1) / kPage);
         P.shares = (int)(steps < kShares ? steps : kShares);
-        if (int e = launch(few_kernel, P.shares, kThreads, sizeof(FewLds), P, stream)) return e;
+        if (int e = launch(few_kernel, P.shares, kFewThreads, sizeof(FewLds), P, stream)) return e;
         return launch(join_few_kernel, few * kFew, kJoinThreads, 0, P, stream);
     }
     P.pad = n_heads % kMany != 0;
     const int64_t units = first_unit(n_tokens, cache->n_seqs, n_heads, kMany, P.pad);
     P.units = (int)units;
-    int64_t splits = kShares / 2 / units;
+    int64_t splits = kShares / units;
     const int64_t most = (seen + 4 * kStep - 1) / (4 * kStep);
     if (splits > most) splits = most;
     P.shares = splits < 1 ? 1 : (int)splits;
