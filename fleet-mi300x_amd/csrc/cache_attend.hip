@@ -270,43 +270,42 @@ __device__ __forceinline__ int page_of(const AttendParams& P, const Work& w, Pag
 
 // ---------------------------------------------------------------- few rows
 
-// Sequences with a token or two: 16 rows a unit, a page a step. The bytes of the
-// pages bound it (576 a position for 16 rows, 60 flops a byte), so what matters is
-// that they keep coming: four pages fit in LDS, two or three of them on their way.
-// Eight waves, two on a SIMD (one alone issues a vector instruction every six
-// cycles, two every three). A block's scores are shared by two waves, half of the 576
-// products each; the first four waves add the halves up and make the weights while
-// the other four issue the copies (a copy of 1 KB occupies the address unit for 24
-// cycles, so a page's hold a wave up for a thousand). Then each wave adds its 64
-// columns of O over the whole page: 16 registers a lane, and no sum over waves at the
-// end.
+// Sequences with a token or two: 16 rows a unit, 32 positions (two blocks, half a
+// page) a step. The bytes of the pages bound it (576 a position for 16 rows, 60 flops
+// a byte), so what matters is that they keep coming: four steps fit in LDS, two or
+// three of them on their way, and two workgroups share a CU, so that one's
+// barriers and latencies are the other's time. A block's scores are shared by two
+// waves, half of the 576 products each; the first two waves add the halves up and
+// make the weights while the other two issue the copies (a copy of 1 KB occupies the
+// address unit for 24 cycles, so that holds a wave up). Then each wave adds its 128
+// columns of O: 32 registers a lane, and no sum over waves at the end.
 //
 // The work is divided into equal shares of steps over all units, whatever their
 // lengths: a workgroup takes a range of the concatenated steps, across units where it
 // has to. A unit that several have a part in leaves partial results, which
 // join_few_kernel adds in order.
-constexpr int kDeep = 4;        // pages in LDS
-constexpr int kFewWaves = 8;
-constexpr int kFewThreads = kFewWaves * 64;
+constexpr int kDeep = 4;        // steps in LDS
+constexpr int kStep = 32;       // positions
 struct FewLds {
-    __attribute__((aligned(16))) uint8_t tile[kDeep][4 * kBlockStep];
+    __attribute__((aligned(16))) uint8_t tile[kDeep][2 * kBlockStep];
     uint32_t scale[kDeep][64];
-    f32x4 half[4][64];          // the second half of a block's scores
-    u32x4 p[2][2][64];          // [step parity][half of the page][lane]
-    float top[2][4][16];
-    int flag[2][4];
+    f32x4 half[2][64];          // the second half of a block's scores
+    u32x4 p[2][64];             // [step parity][lane]
+    float top[2][2][16];
+    int flag[2][2];
+    float sum[2][16];
 };
-static_assert(sizeof(FewLds) <= 160 * 1024, "");
+static_assert(sizeof(FewLds) <= 80 * 1024, "two workgroups share a CU");
 constexpr int kFew = 16;        // rows
 
-constexpr int kPageCopies = 10; // of each of four waves: 9 KB of codes, and the scales
+constexpr int kStepCopies = 10; // of each of two waves: 9 KB of codes, and the scales
 constexpr int kNeedMax = 1, kHasNan = 2;
 
 // The steps of all units of a sequence, an empty unit as one.
 __device__ __forceinline__ int seq_steps(const AttendParams& P, Work& w) {
     int n = 0;
     for (w.row0 = 0; w.row0 < w.rows; w.row0 += kFew) {
-        see<kFew, kPage>(P, w);
+        see<kFew, kStep>(P, w);
         n += w.n > 0 ? w.n : 1;
     }
     return n;
@@ -373,18 +372,19 @@ __device__ __forceinline__ bool locate(const AttendParams& P, int wg, Work& w, i
     }
     w = lane_of(mine, owner);
     for (w.row0 = 0;; w.row0 += kFew) {
-        see<kFew, kPage>(P, w);
+        see<kFew, kStep>(P, w);
         const int all = w.n > 0 ? w.n : 1;
         if (off < all) return true;
         off -= all;
     }
 }
 
-__global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
+__global__ __launch_bounds__(kThreads, 2) void few_kernel(AttendParams P) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     FewLds& L = *reinterpret_cast<FewLds*>(lds);
     const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
-    const int g = lane >> 4, n = lane & 15, blk = wave & 3;
+    const int g = lane >> 4, n = lane & 15, blk = wave & 1;
+    const bool first = wave < 2;
     const int wg = blockIdx.x;
     Work w;
     int off, total, shares;
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
     int at = share.first(wg);
     const int end = share.first(wg + 1);
     for (bool lead = true;; lead = false) {
-        see<kFew, kPage>(P, w);
+        see<kFew, kStep>(P, w);
         const int all = w.n > 0 ? w.n : 1;
         const int take = all - off < end - at ? all - off : end - at;
         const int until = off + take < w.n ? off + take : w.n;
@@ -403,8 +403,8 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
 
         constexpr int kHalf = kChunks / 4;      // steps of 32 values, of 18
         bf16x8 q[kHalf];
-        load_q(P, w, r, g, wave < 4 ? 0 : kHalf, q);
-        constexpr int kCols = kC / 16 / kFewWaves;
+        load_q(P, w, r, g, first ? 0 : kHalf, q);
+        constexpr int kCols = kC / 16 / kWaves;
         f32x4 acc[kCols];
 #pragma unroll
         for (auto& a : acc) a = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -413,17 +413,17 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
         float m = -INFINITY, l = 0.f;
         float s[4], p[4];
         Pages pages{0, 0, 0};
-        // copies page k: waves 4 .. 7
+        // copies step k: the last two waves
         const auto issue = [&](int k) {
-            const int page = page_of<kPage>(P, w, pages, off + k, until, lane);
+            const int page = page_of<kStep>(P, w, pages, off + k, until, lane);
             const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
             const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
-            const uint8_t* from = src + blk * kBlockBytes + lane * 16;
-            const int b = k % kDeep;
+            const int b = k % kDeep, half = step_of<kStep>(w, off + k) & 1;
+            const uint8_t* from = src + (2 * half + blk) * kBlockBytes + lane * 16;
             const uint32_t to = lds_addr(L.tile[b]) + blk * kBlockStep;
 #pragma unroll
             for (int i = 0; i < kBlockBytes / 1024; ++i) copy_kb<true>(from + i * 1024, to + i * 1024);
-            copy_words(src + kCodeBytes + (lane & 7) * 4, lds_addr(L.scale[b]));
+            copy_words(src + kCodeBytes + half * 16 + (lane & 3) * 4, lds_addr(L.scale[b]));
         };
         // this wave's half of its block's scores
         const auto score = [&](int k) {
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
             const float sc = any_scale(L.scale[b][2 * blk]);
             f32x4 z0{0.f, 0.f, 0.f, 0.f}, z1{0.f, 0.f, 0.f, 0.f};
             const auto chunk = [&](int i) { return *reinterpret_cast<const u32x4*>(block + i * 1024); };
-            if (wave < 4) {
+            if (first) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const u32x4 a = chunk(i);
@@ -456,23 +456,23 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
                 z0 = mfma(widen(a.z, a.w, sp, sp), q[8], z0);
             }
             z = z0 + z1;
-            if (wave >= 4) L.half[blk][lane] = z;
+            if (!first) L.half[blk][lane] = z;
         };
-        // the weights of step k under the reference m: waves 0 .. 3
+        // the weights of step k under the reference m: the first two waves
         const auto weigh = [&](int k) {
             const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int j = 0; j < 4; ++j) p[j] = exp2_(s[j] - ref);
-            reinterpret_cast<uint2*>(&L.p[k & 1][blk >> 1][lane])[blk & 1] = weights(p);
+            reinterpret_cast<uint2*>(&L.p[k & 1][lane])[blk] = weights(p);
         };
         const auto finish = [&](int k) {
             z += L.half[blk][lane];
             float top = -INFINITY;
             bool nan = false;
-            const int page = page_of<kPage>(P, w, pages, off + k, until, lane);
+            const int page = page_of<kStep>(P, w, pages, off + k, until, lane);
             const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
             if (!ok && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
-            const int base = step_of<kPage>(w, off + k) * kPage + blk * kBlock + 4 * g;
+            const int base = step_of<kStep>(w, off + k) * kStep + blk * kBlock + 4 * g;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float v = z[j] * P.scale;
@@ -488,12 +488,12 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
                              (__ballot(nan) ? kHasNan : 0);
             if (lane == 0) L.flag[k & 1][blk] = flag;
         };
-        // Step k: behind barrier A the weights of k and page k + 1 are there, behind
+        // Step k: behind barrier A the weights of k and the rows of k + 1 are there, behind
         // B both halves of the scores of k + 1.
-        if (wave >= 4) {
+        if (!first) {
             for (int k = 0; k < kDeep - 1 && k < cnt; ++k) issue(k);
-            if (cnt > 2) wait_copies<2 * kPageCopies>();
-            else if (cnt > 1) wait_copies<kPageCopies>();
+            if (cnt > 2) wait_copies<2 * kStepCopies>();
+            else if (cnt > 1) wait_copies<kStepCopies>();
             else wait_copies<0>();
         }
         barrier();
@@ -501,39 +501,32 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
             if (k + 1 < cnt) {
                 score(k + 1);
                 barrier();                      // B
-                if (wave < 4) {
+                if (first) {
                     finish(k + 1);
                 } else {
-                    // into the buffer of page k - 1
+                    // into the buffer of step k - 1
                     if (k >= 0 && k + kDeep - 1 < cnt) issue(k + kDeep - 1);
-                    // page k + 2; the one behind it may be on its way
-                    if (cnt - k > 3) wait_copies<kPageCopies>();
+                    // step k + 2; the one behind it may be on its way
+                    if (cnt - k > 3) wait_copies<kStepCopies>();
                     else wait_copies<0>();
                 }
             }
             if (k >= 0) {
                 const int b = k % kDeep, par = k & 1;
+                const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[par][lane]);
+                const float sa = any_scale(L.scale[b][0]), sb = any_scale(L.scale[b][2]);
+                const uint8_t* col = column_at(L.tile[b], lane) + wave * kCols * 256;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[par][h][lane]);
-                    const float sa = any_scale(L.scale[b][4 * h]);
-                    const float sb = any_scale(L.scale[b][4 * h + 2]);
-                    const uint8_t* col = column_at(L.tile[b] + 2 * h * kBlockStep, lane) +
-                                         wave * kCols * 256;
-#pragma unroll
-                    for (int i = 0; i < kCols; ++i) {
-                        const i32x2 v = column(col, i);
-                        acc[i] = mfma(widen((uint32_t)v.x, (uint32_t)v.y, sa, sb), pb, acc[i]);
-                    }
-                    ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}), pb,
-                                ones);
+                for (int i = 0; i < kCols; ++i) {
+                    const i32x2 v = column(col, i);
+                    acc[i] = mfma(widen((uint32_t)v.x, (uint32_t)v.y, sa, sb), pb, acc[i]);
                 }
+                ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}), pb, ones);
             }
             if (k + 1 == cnt) break;
             barrier();                          // A
             const int par = (k + 1) & 1;
-            const int any = wave_bcast((L.flag[par][0] | L.flag[par][1]) |
-                                       (L.flag[par][2] | L.flag[par][3]));
+            const int any = wave_bcast(L.flag[par][0] | L.flag[par][1]);
             if (any) {
                 // m is any reference not far below the maximum: weights up to 2^kSlack
                 // are as exact as those up to 1, and moving it costs a pass over O and a
@@ -541,27 +534,26 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
                 if (any & kNeedMax) {
                     float to = m;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) to = fmaxf(to, L.top[par][i][n]);
+                    for (int i = 0; i < 2; ++i) to = fmaxf(to, L.top[par][i][n]);
                     const float shrink = to == -INFINITY ? 1.f : exp2_(m - to);
                     m = to;
                     l *= shrink;
                     ones *= shrink;
 #pragma unroll
                     for (auto& a : acc) a *= shrink;
-                    if (wave < 4) weigh(k + 1);
+                    if (first) weigh(k + 1);
                 }
-                if ((any & kHasNan) && wave < 4)
+                if ((any & kHasNan) && first)
                     clean(L.tile[(k + 1) % kDeep] + blk * kBlockStep, lane);
                 barrier();
             }
-            if (wave < 4) l += (p[0] + p[1]) + (p[2] + p[3]);
+            if (first) l += (p[0] + p[1]) + (p[2] + p[3]);
         }
-        // the sums of the four blocks
+        // the sums of the two blocks
         l = xor32_sum(xor16_sum(l));
+        if (first && lane < 16) L.sum[blk][lane] = l;
         barrier();
-        if (wave < 4 && lane < 16) L.top[0][blk][lane] = l;
-        barrier();
-        const float sum = (L.top[0][0][n] + L.top[0][1][n]) + (L.top[0][2][n] + L.top[0][3][n]);
+        const float sum = L.sum[0][n] + L.sum[1][n];
         const bool whole = take == all;
         const int column0 = wave * kCols * 16 + 4 * g;
         if (whole) {
@@ -595,7 +587,7 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_kernel(AttendParams P) {
             if (w.seq + 1 >= P.c.n_seqs) return;
             open_seq(P, w.seq + 1, w);
         }
-        barrier();                              // L.top is free again
+        barrier();                              // LDS is free again
     }
 }
 
@@ -655,7 +647,7 @@ __device__ __forceinline__ bool find_work(const AttendParams& P, int64_t u, Work
 __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams P) {
     const int64_t u = blockIdx.x / kFew;
     Work w;
-    if (!find_work<kFew, kPage>(P, u, w)) return;
+    if (!find_work<kFew, kStep>(P, u, w)) return;
     const int row = blockIdx.x % kFew;
     if (w.row0 + row >= w.rows) return;
     const int4 m = P.meta[u];
@@ -681,7 +673,6 @@ struct ManyLds {
 };
 static_assert(sizeof(ManyLds) <= 80 * 1024, "two workgroups share a CU");
 constexpr int kMany = 64;       // rows
-constexpr int kStep = 32;       // positions
 
 __global__ __launch_bounds__(kThreads, 2) void many_kernel(AttendParams P) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -933,17 +924,17 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     P.pad = n_heads % kFew != 0;
     const int64_t few = first_unit(n_tokens, cache->n_seqs, n_heads, kFew, P.pad);
     if (rows <= 2 * kFew * (int64_t)cache->n_seqs && few <= kMaxUnits &&
-        few * cache->max_pages < (1 << 30)) {
+        2 * few * cache->max_pages < (1 << 30)) {
         P.units = (int)few;
-        const int64_t steps = few * ((seen + kPage - 1) / kPage);
+        const int64_t steps = few * ((seen + kStep - 1) / kStep);
         P.shares = (int)(steps < kShares ? steps : kShares);
-        if (int e = launch(few_kernel, P.shares, kFewThreads, sizeof(FewLds), P, stream)) return e;
+        if (int e = launch(few_kernel, P.shares, kThreads, sizeof(FewLds), P, stream)) return e;
         return launch(join_few_kernel, few * kFew, kJoinThreads, 0, P, stream);
     }
     P.pad = n_heads % kMany != 0;
     const int64_t units = first_unit(n_tokens, cache->n_seqs, n_heads, kMany, P.pad);
     P.units = (int)units;
-    int64_t splits = kShares / units;
+    int64_t splits = kShares / 2 / units;
     const int64_t most = (seen + 4 * kStep - 1) / (4 * kStep);
     if (splits > most) splits = most;
     P.shares = splits < 1 ? 1 : (int)splits;

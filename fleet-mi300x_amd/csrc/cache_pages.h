@@ -99,7 +99,7 @@ __device__ __forceinline__ void raise(Header* h, uint32_t bit) { atomicOr(&h->st
 
 // What the attention's second launch joins: partial results of up to 1024 times 16
 // rows (fp32 [512] each), their maxima and sums, and where a unit's lie.
-constexpr int kShares = 256;           // workgroups: one a CU
+constexpr int kShares = 512;           // workgroups: two a CU
 constexpr int kMaxUnits = 4096;
 constexpr int kPartRows = 1024 * 16;
 constexpr size_t kPartBytes = (size_t)kPartRows * kC * 4;
