@@ -110,16 +110,50 @@ __device__ __forceinline__ Row row_of(const AttendParams& P, const Work& w, int 
     r.seen = seen_of(r.pos < 0 ? 0 : r.pos, P.window, P.sinks);
     return r;
 }
-// Its query as the right operand: the k order of the products is that of the bytes
-// a lane of group g takes of a row: chunks g, 4 + g, ..
-template <int N>                // N of the 18 steps of 32 values, from `step` on
-__device__ __forceinline__ void load_q(const AttendParams& P, const Work& w, const Row& r, int g,
-                                       int step, bf16x8 (&q)[N]) {
-    const uint16_t* src = P.q + (int64_t)(w.tok0 + r.tok) * P.q_stride + r.head * kRow + g * 16;
+// (no short cuts: three comparisons cost less than a branch)
+__device__ __forceinline__ bool sees(const Row& r, int pos) {
+    return (pos <= r.pos) & ((pos >= r.seen.lo) | (pos < r.seen.sink));
+}
+// Whether all rows of a wave see all of the positions [a, a + n): what they all see,
+// apart from the dead ones.
+struct Common {
+    int pos, lo, sink;
+    __device__ __forceinline__ explicit Common(const Row& r) {
+        pos = r.live ? r.pos : 0x7fffffff;
+        lo = r.live ? r.seen.lo : 0;
+        sink = r.live ? r.seen.sink : 0x7fffffff;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        q[i] = __builtin_bit_cast(bf16x8, ld_global(reinterpret_cast<const u32x4*>(
-                                              src + (step + i) / 2 * 64 + (step + i) % 2 * 8)));
+        for (int d = 1; d < 16; d <<= 1) {
+            const int a = __shfl_xor(pos, d), b = __shfl_xor(lo, d), c = __shfl_xor(sink, d);
+            pos = a < pos ? a : pos;
+            lo = b > lo ? b : lo;
+            sink = c < sink ? c : sink;
+        }
+        pos = wave_bcast(pos);
+        lo = wave_bcast(lo);
+        sink = wave_bcast(sink);
+    }
+    __device__ __forceinline__ bool all(int a, int n) const {
+        return a + n - 1 <= pos && (a >= lo || a + n <= sink);
+    }
+};
+// Its query as the right operand. The k order of the products is that of the bytes a
+// lane of group g takes of a row: its chunks 4i + g, 16 values each, i = 0 .. 8, make
+// two of 18 steps. Two waves share the products: wave `half` of them has those of i =
+// half, 2 + half, 4 + half, 6 + half, and one step of i = 8, which is k_pe.
+constexpr int kHalf = kChunks / 4;              // steps of a wave
+__device__ __forceinline__ void load_q(const AttendParams& P, const Work& w, const Row& r, int g,
+                                       int half, bf16x8 (&q)[kHalf]) {
+    const uint16_t* src = P.q + (int64_t)(w.tok0 + r.tok) * P.q_stride + r.head * kRow + g * 16;
+    const auto at = [&](int v) {
+        return __builtin_bit_cast(bf16x8, ld_global(reinterpret_cast<const u32x4*>(src + v)));
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        q[2 * i] = at((2 * i + half) * 64);
+        q[2 * i + 1] = at((2 * i + half) * 64 + 8);
+    }
+    q[8] = at(8 * 64 + half * 8);
 }
 __device__ __forceinline__ int64_t out_row(const AttendParams& P, const Work& w, int row) {
     return (int64_t)w.tok0 * P.n_heads + row;
@@ -141,13 +175,6 @@ __device__ __forceinline__ void copy_kb(const uint8_t* src, uint32_t lds) {
     else
         asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds)
                      : "memory");
-}
-// The same with 4 bytes per lane.
-__device__ __forceinline__ void copy_words(const uint8_t* src, uint32_t lds) {
-    asm volatile(
-        "s_nop 0\n\t"
-        "global_load_lds_dword %0, off" ::"v"(src), "{m0}"(lds)
-        : "memory");
 }
 template <int kLeft>
 __device__ __forceinline__ void wait_copies() {
@@ -268,38 +295,265 @@ __device__ __forceinline__ int page_of(const AttendParams& P, const Work& w, Pag
     return __builtin_amdgcn_readlane(h.page, i - h.from);
 }
 
+// ---------------------------------------------------------------- the products
+//
+// A workgroup of four waves has 16 rows (few_kernel) or 32 (many_kernel), kTiles tiles
+// of 16, and takes 32 positions a step, two blocks, half a page. Wave (block, half)
+// takes half of the 576 products of its block's scores with all rows, so that each
+// widened K operand is used once per tile and no wave widens what another does;
+// halves meet in LDS, and the weights are made: with two tiles by every wave for one
+// tile and its block, with one by the first wave of each block. Then each wave adds
+// its 128 columns of O for all rows: 32 registers a lane and tile, and no sum over waves
+// at the end. Two workgroups share a CU, so that one's barriers and latencies are the
+// other's time; a wave alone on a SIMD issues a vector instruction every six cycles,
+// two every three.
+constexpr int kStep = 32;       // positions
+
+template <int kTiles>
+struct Lds {
+    // steps: one row tile lives off HBM, where three copies have to be on their way
+    static constexpr int kRing = kTiles == 1 ? 4 : 3;
+    __attribute__((aligned(16))) uint8_t tile[kRing][2 * kBlockStep];
+    uint32_t scale[kRing][4];   // c and k_pe of either block
+    f32x4 half[kWaves][64];     // half of the scores of a block and tile, for another wave
+    u32x4 p[2][kTiles][64];     // [step parity][tile][lane]
+    int flag[2][kWaves];
+    float top[kTiles][2][16];
+    float sum[kTiles][2][16];
+};
+static_assert(sizeof(Lds<1>) <= 80 * 1024 && sizeof(Lds<2>) <= 80 * 1024,
+              "two workgroups share a CU");
+
+// Steps off .. off + cnt - 1 of a unit, and its results: to `out` and `lse`, or as the
+// partial results of slot `slot` if that is not negative.
+template <int kTiles>
+__device__ __forceinline__ void attend(const AttendParams& P, Lds<kTiles>& L, const Work& w, int off,
+                                       int cnt, int slot) {
+    constexpr int kRing = Lds<kTiles>::kRing;
+    constexpr int kCols = kC / 16 / kWaves;     // of 16
+    constexpr bool kFirst = kTiles == 1;        // one wave of two makes the weights
+    // copies a wave issues for a step: nine of 1 KB and the scales, or half of them
+    constexpr int kCopies = kFirst ? 10 : 5;
+    const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
+    const int g = lane >> 4, n = lane & 15, blk = wave & 1, half = wave >> 1;
+    const int mine = kFirst ? 0 : half;         // the tile whose weights this wave makes
+    const bool weighs = !kFirst || half == 0, copies = !kFirst || half == 1;
+
+    const Row r = row_of(P, w, w.row0 + mine * 16 + n);
+    const Common common(r);
+    bf16x8 q[kTiles][kHalf];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) load_q(P, w, row_of(P, w, w.row0 + i * 16 + n), g, half, q[i]);
+    f32x4 acc[kTiles][kCols], ones[kTiles];     // O, and the sums of the rounded weights
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+        ones[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (auto& a : acc[i]) a = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // Every row's reference, as a score and as it is in the exponent: any score not far
+    // below the maximum, because weights up to 2^kSlack are as exact as those up to 1,
+    // and moving it costs a pass over O and a barrier. All waves keep all of them.
+    float m[kTiles], ref[kTiles], l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) m[i] = ref[i] = -INFINITY;
+    const float slack = kSlack / P.scale;
+    f32x4 z, next;              // the scores of `mine` and the block, and the next step's
+    bool nan = false;           // of the wave
+    float p[4];
+    Pages pages{0, 0, 0};
+    if (cnt > 0) page_of<kStep>(P, w, pages, off, off + cnt, lane);
+    // q and the pages are there before a copy is issued, as far as the compiler counts
+    __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0)
+
+    const auto issue = [&](int k) {
+        const int page = page_of<kStep>(P, w, pages, off + k, off + cnt, lane);
+        const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
+        const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
+        const int b = k % kRing, part = step_of<kStep>(w, off + k) & 1;
+        const uint8_t* from = src + (2 * part + blk) * kBlockBytes + lane * 16;
+        const uint32_t to = lds_addr(L.tile[b]) + blk * kBlockStep;
+        const int first = kFirst ? 0 : half * 5;
+        constexpr int kPieces = kFirst ? 9 : 5;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+            if (first + i < 9) copy_kb<kFirst>(from + (first + i) * 1024, to + (first + i) * 1024);
+        if ((kFirst || half == 1) && lane == 0)
+            copy_kb<false>(src + kCodeBytes + part * 16, lds_addr(L.scale[b]));
+    };
+    const auto score = [&](int k) {
+        const int b = k % kRing;
+        const uint8_t* block = L.tile[b] + blk * kBlockStep + lane * 16;
+        const float sc = any_scale(L.scale[b][2 * blk]), sp = any_scale(L.scale[b][2 * blk + 1]);
+        // two chains a tile: a product's result is not the next one's operand
+        f32x4 y[kTiles][2];
+#pragma unroll
+        for (auto& a : y) a[0] = a[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u32x4 a = *reinterpret_cast<const u32x4*>(block + (2 * i + half) * 1024);
+            const bf16x8 lo = widen(a.x, a.y, sc, sc), hi = widen(a.z, a.w, sc, sc);
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) y[j][0] = mfma(lo, q[j][2 * i], y[j][0]);
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) y[j][1] = mfma(hi, q[j][2 * i + 1], y[j][1]);
+        }
+        const uint2 a = *reinterpret_cast<const uint2*>(block + 8 * 1024 + half * 8);
+        const bf16x8 pe = widen(a.x, a.y, sp, sp);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) y[j][0] = mfma(pe, q[j][8], y[j][0]);
+        next = y[0][0] + y[0][1];
+        if constexpr (kFirst) {
+            if (half == 1) L.half[wave][lane] = next;
+        } else {
+            // (no index that is not a constant: y stays in registers)
+            const f32x4 y0 = next, y1 = y[1][0] + y[1][1];
+            next = half ? y1 : y0;
+            L.half[wave][lane] = half ? y0 : y1;
+        }
+    };
+    const auto weigh = [&](int k) {
+        const float own = kTiles == 1 || half == 0 ? ref[0] : ref[kTiles - 1];
+        const float down = own == -INFINITY ? 0.f : own;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = exp2_(fmaf(z[j], P.scale, -down));
+        reinterpret_cast<uint2*>(&L.p[k & 1][mine][lane])[blk] = weights(p);
+    };
+    const auto finish = [&](int k) {
+        z = next + L.half[wave ^ 2][lane];
+        const int page = page_of<kStep>(P, w, pages, off + k, off + cnt, lane);
+        const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
+        const int base = step_of<kStep>(w, off + k) * kStep + blk * kBlock;
+        const bool bad = (z[0] != z[0]) | (z[1] != z[1]) | (z[2] != z[2]) | (z[3] != z[3]);
+        if (!(ok && common.all(base, kBlock))) {
+            asm volatile("");                   // a branch, not twenty instructions every step
+            if (!ok && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[j] = (ok & sees(r, base + 4 * g + j)) ? z[j] : -INFINITY;
+        }
+        weigh(k);
+        const float own = kTiles == 1 || half == 0 ? m[0] : m[kTiles - 1];
+        const float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+        nan = __ballot(bad) != 0;
+        const bool high = __ballot(top > own + slack) != 0;
+        if (lane == 0) L.flag[k & 1][wave] = nan | high;
+    };
+    // What is rare: a row's scores beyond its reference, or a NaN, in step k.
+    const auto mend = [&](int k) {
+        if (weighs) {
+            float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+            top = xor32_max(xor16_max(top));
+            if (lane < 16) L.top[mine][blk][lane] = top;
+            if (nan && half == 0) clean(L.tile[k % kRing] + blk * kBlockStep, lane);
+        }
+        barrier();
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            const float to = fmaxf(m[i], fmaxf(L.top[i][0][n], L.top[i][1][n]));
+            const float scaled = to * P.scale;
+            const float shrink = to == -INFINITY ? 1.f : exp2_(ref[i] - scaled);
+            m[i] = to;
+            ref[i] = scaled;
+            if (i == mine) l *= shrink;
+            ones[i] *= shrink;
+#pragma unroll
+            for (auto& a : acc[i]) a *= shrink;
+        }
+        if (weighs) weigh(k);
+        barrier();
+    };
+    // O over step k
+    const auto add = [&](int k) {
+        const int b = k % kRing;
+        bf16x8 pb[kTiles];
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) pb[j] = __builtin_bit_cast(bf16x8, L.p[k & 1][j][lane]);
+        const float sa = any_scale(L.scale[b][0]), sb = any_scale(L.scale[b][2]);
+        const uint8_t* col = column_at(L.tile[b], lane) + wave * kCols * 256;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) {
+            const i32x2 v = column(col, i);
+            const bf16x8 a = widen((uint32_t)v.x, (uint32_t)v.y, sa, sb);
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) acc[j][i] = mfma(a, pb[j], acc[j][i]);
+        }
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+            ones[j] = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}), pb[j],
+                           ones[j]);
+    };
+
+    // The first step's copies are waited for here, the others' kRing - 2 steps after
+    // they are issued.
+    if (copies) {
+        for (int k = 0; k < kRing - 1 && k < cnt; ++k) issue(k);
+        if (kRing > 3 && cnt > 2) wait_copies<2 * kCopies>();
+        else if (cnt > 1) wait_copies<kCopies>();
+        else wait_copies<0>();
+    }
+    barrier();
+    // Step k: behind barrier A the weights of k and the rows of k + 1 are there, behind
+    // B both halves of the scores of k + 1.
+    for (int k = -1; k < cnt; ++k) {
+        const int par = k & 1;
+        int flags = 0;
+        if (k >= 0)
+            flags = kFirst ? L.flag[par][0] | L.flag[par][1]
+                           : (L.flag[par][0] | L.flag[par][1]) | (L.flag[par][2] | L.flag[par][3]);
+        // into the buffer of step k - 1
+        const bool more = k >= 0 && k + kRing - 1 < cnt;
+        if (!kFirst && more) issue(k + kRing - 1);
+        if (k + 1 < cnt) score(k + 1);
+        if (k >= 0) {
+            if (wave_bcast(flags)) mend(k);
+            if (weighs) l += (p[0] + p[1]) + (p[2] + p[3]);
+            add(k);
+        }
+        if (k + 1 == cnt) break;
+        barrier();                              // B
+        if (kFirst && copies && more) issue(k + kRing - 1);
+        if (weighs) finish(k + 1);
+        // step k + 2; with four buffers the one behind it may be on its way
+        if (kRing > 3 && cnt - k > 3) wait_copies<kCopies>();
+        else wait_copies<0>();
+        barrier();                              // A
+    }
+    // the sums of the two blocks
+    l = xor32_sum(xor16_sum(l));
+    if (weighs && lane < 16) L.sum[mine][blk][lane] = l;
+    barrier();
+    const int column0 = wave * kCols * 16 + 4 * g;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+        const int row = i * 16 + n;
+        const float sum = L.sum[i][0][n] + L.sum[i][1][n];
+        if (slot < 0) {
+            if (w.row0 + row < w.rows) {
+                const int64_t to = out_row(P, w, w.row0 + row);
+                const float inv = ones[i][0] == 0.f ? 0.f : 1.f / ones[i][0];
+#pragma unroll
+                for (int j = 0; j < kCols; ++j)
+                    put(P.out + to * kC + column0 + j * 16, acc[i][j], inv);
+                if (P.lse && wave == 0 && g == 0) P.lse[to] = lse_of(ref[i], sum);
+            }
+        } else {
+            const int64_t at = (int64_t)slot * (16 * kTiles) + row;
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+                st_global(reinterpret_cast<f32x4*>(P.part + at * kC + column0 + j * 16), acc[i][j]);
+            if (wave == 0 && g == 0) st_global(P.stat + at, f32x4{ref[i], sum, ones[i][0], 0.f});
+        }
+    }
+}
+
 // ---------------------------------------------------------------- few rows
 
-// Sequences with a token or two: 16 rows a unit, 32 positions (two blocks, half a
-// page) a step. The bytes of the pages bound it (576 a position for 16 rows, 60 flops
-// a byte), so what matters is that they keep coming: four steps fit in LDS, two or
-// three of them on their way, and two workgroups share a CU, so that one's
-// barriers and latencies are the other's time. A block's scores are shared by two
-// waves, half of the 576 products each; the first two waves add the halves up and
-// make the weights while the other two issue the copies (a copy of 1 KB occupies the
-// address unit for 24 cycles, so that holds a wave up). Then each wave adds its 128
-// columns of O: 32 registers a lane, and no sum over waves at the end.
-//
-// The work is divided into equal shares of steps over all units, whatever their
-// lengths: a workgroup takes a range of the concatenated steps, across units where it
-// has to. A unit that several have a part in leaves partial results, which
-// join_few_kernel adds in order.
-constexpr int kDeep = 4;        // steps in LDS
-constexpr int kStep = 32;       // positions
-struct FewLds {
-    __attribute__((aligned(16))) uint8_t tile[kDeep][2 * kBlockStep];
-    uint32_t scale[kDeep][64];
-    f32x4 half[2][64];          // the second half of a block's scores
-    u32x4 p[2][64];             // [step parity][lane]
-    float top[2][2][16];
-    int flag[2][2];
-    float sum[2][16];
-};
-static_assert(sizeof(FewLds) <= 80 * 1024, "two workgroups share a CU");
+// Sequences with a token or two: 16 rows a unit. The bytes of the pages bound it (576 a
+// position for 16 rows, 60 flops a byte), so the work is divided into equal shares of
+// steps over all units, whatever their lengths: a workgroup takes a range of the
+// concatenated steps, across units where it has to. A unit that several have a part
+// in leaves partial results, which join_few_kernel adds in order.
 constexpr int kFew = 16;        // rows
-
-constexpr int kStepCopies = 10; // of each of two waves: 9 KB of codes, and the scales
-constexpr int kNeedMax = 1, kHasNan = 2;
 
 // The steps of all units of a sequence, an empty unit as one.
 __device__ __forceinline__ int seq_steps(const AttendParams& P, Work& w) {
@@ -381,11 +635,8 @@ __device__ __forceinline__ bool locate(const AttendParams& P, int wg, Work& w, i
 
 __global__ __launch_bounds__(kThreads, 2) void few_kernel(AttendParams P) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    FewLds& L = *reinterpret_cast<FewLds*>(lds);
-    const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
-    const int g = lane >> 4, n = lane & 15, blk = wave & 1;
-    const bool first = wave < 2;
-    const int wg = blockIdx.x;
+    Lds<1>& L = *reinterpret_cast<Lds<1>*>(lds);
+    const int t = threadIdx.x, wg = blockIdx.x;
     Work w;
     int off, total, shares;
     if (!locate(P, wg, w, off, total, shares)) return;
@@ -397,186 +648,15 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(AttendParams P) {
         const int all = w.n > 0 ? w.n : 1;
         const int take = all - off < end - at ? all - off : end - at;
         const int until = off + take < w.n ? off + take : w.n;
-        const int cnt = until > off ? until - off : 0;
-        const Row r = row_of(P, w, w.row0 + n);
         if (w.len < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
-
-        constexpr int kHalf = kChunks / 4;      // steps of 32 values, of 18
-        bf16x8 q[kHalf];
-        load_q(P, w, r, g, first ? 0 : kHalf, q);
-        constexpr int kCols = kC / 16 / kWaves;
-        f32x4 acc[kCols];
-#pragma unroll
-        for (auto& a : acc) a = f32x4{0.f, 0.f, 0.f, 0.f};
-        f32x4 ones{0.f, 0.f, 0.f, 0.f};         // the sum of the rounded weights
-        f32x4 z;
-        float m = -INFINITY, l = 0.f;
-        float s[4], p[4];
-        Pages pages{0, 0, 0};
-        // copies step k: the last two waves
-        const auto issue = [&](int k) {
-            const int page = page_of<kStep>(P, w, pages, off + k, until, lane);
-            const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
-            const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
-            const int b = k % kDeep, half = step_of<kStep>(w, off + k) & 1;
-            const uint8_t* from = src + (2 * half + blk) * kBlockBytes + lane * 16;
-            const uint32_t to = lds_addr(L.tile[b]) + blk * kBlockStep;
-#pragma unroll
-            for (int i = 0; i < kBlockBytes / 1024; ++i) copy_kb<true>(from + i * 1024, to + i * 1024);
-            copy_words(src + kCodeBytes + half * 16 + (lane & 3) * 4, lds_addr(L.scale[b]));
-        };
-        // this wave's half of its block's scores
-        const auto score = [&](int k) {
-            const int b = k % kDeep;
-            const uint8_t* block = L.tile[b] + blk * kBlockStep + lane * 16;
-            const float sc = any_scale(L.scale[b][2 * blk]);
-            f32x4 z0{0.f, 0.f, 0.f, 0.f}, z1{0.f, 0.f, 0.f, 0.f};
-            const auto chunk = [&](int i) { return *reinterpret_cast<const u32x4*>(block + i * 1024); };
-            if (first) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const u32x4 a = chunk(i);
-                    z0 = mfma(widen(a.x, a.y, sc, sc), q[2 * i], z0);
-                    z1 = mfma(widen(a.z, a.w, sc, sc), q[2 * i + 1], z1);
-                }
-                const u32x4 a = chunk(4);
-                z0 = mfma(widen(a.x, a.y, sc, sc), q[8], z0);
-            } else {
-                const float sp = any_scale(L.scale[b][2 * blk + 1]);
-                u32x4 a = chunk(4);
-                z0 = mfma(widen(a.z, a.w, sc, sc), q[0], z0);
-#pragma unroll
-                for (int i = 5; i < 8; ++i) {
-                    a = chunk(i);
-                    z1 = mfma(widen(a.x, a.y, sc, sc), q[2 * i - 9], z1);
-                    z0 = mfma(widen(a.z, a.w, sc, sc), q[2 * i - 8], z0);
-                }
-                a = chunk(8);
-                z1 = mfma(widen(a.x, a.y, sp, sp), q[7], z1);
-                z0 = mfma(widen(a.z, a.w, sp, sp), q[8], z0);
-            }
-            z = z0 + z1;
-            if (!first) L.half[blk][lane] = z;
-        };
-        // the weights of step k under the reference m: the first two waves
-        const auto weigh = [&](int k) {
-            const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = exp2_(s[j] - ref);
-            reinterpret_cast<uint2*>(&L.p[k & 1][lane])[blk] = weights(p);
-        };
-        const auto finish = [&](int k) {
-            z += L.half[blk][lane];
-            float top = -INFINITY;
-            bool nan = false;
-            const int page = page_of<kStep>(P, w, pages, off + k, until, lane);
-            const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
-            if (!ok && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
-            const int base = step_of<kStep>(w, off + k) * kStep + blk * kBlock + 4 * g;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float v = z[j] * P.scale;
-                nan |= v != v;
-                const int pos = base + j;
-                s[j] = ok && pos <= r.pos && (pos >= r.seen.lo || pos < r.seen.sink) ? v : -INFINITY;
-                top = fmaxf(top, s[j]);
-            }
-            top = xor32_max(xor16_max(top));
-            weigh(k);
-            if (lane < 16) L.top[k & 1][blk][lane] = top;
-            const int flag = (__ballot(top > m + kSlack) ? kNeedMax : 0) |
-                             (__ballot(nan) ? kHasNan : 0);
-            if (lane == 0) L.flag[k & 1][blk] = flag;
-        };
-        // Step k: behind barrier A the weights of k and the rows of k + 1 are there, behind
-        // B both halves of the scores of k + 1.
-        if (!first) {
-            for (int k = 0; k < kDeep - 1 && k < cnt; ++k) issue(k);
-            if (cnt > 2) wait_copies<2 * kStepCopies>();
-            else if (cnt > 1) wait_copies<kStepCopies>();
-            else wait_copies<0>();
-        }
-        barrier();
-        for (int k = -1; k < cnt; ++k) {
-            if (k + 1 < cnt) {
-                score(k + 1);
-                barrier();                      // B
-                if (first) {
-                    finish(k + 1);
-                } else {
-                    // into the buffer of step k - 1
-                    if (k >= 0 && k + kDeep - 1 < cnt) issue(k + kDeep - 1);
-                    // step k + 2; the one behind it may be on its way
-                    if (cnt - k > 3) wait_copies<kStepCopies>();
-                    else wait_copies<0>();
-                }
-            }
-            if (k >= 0) {
-                const int b = k % kDeep, par = k & 1;
-                const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[par][lane]);
-                const float sa = any_scale(L.scale[b][0]), sb = any_scale(L.scale[b][2]);
-                const uint8_t* col = column_at(L.tile[b], lane) + wave * kCols * 256;
-#pragma unroll
-                for (int i = 0; i < kCols; ++i) {
-                    const i32x2 v = column(col, i);
-                    acc[i] = mfma(widen((uint32_t)v.x, (uint32_t)v.y, sa, sb), pb, acc[i]);
-                }
-                ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}), pb, ones);
-            }
-            if (k + 1 == cnt) break;
-            barrier();                          // A
-            const int par = (k + 1) & 1;
-            const int any = wave_bcast(L.flag[par][0] | L.flag[par][1]);
-            if (any) {
-                // m is any reference not far below the maximum: weights up to 2^kSlack
-                // are as exact as those up to 1, and moving it costs a pass over O and a
-                // barrier
-                if (any & kNeedMax) {
-                    float to = m;
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) to = fmaxf(to, L.top[par][i][n]);
-                    const float shrink = to == -INFINITY ? 1.f : exp2_(m - to);
-                    m = to;
-                    l *= shrink;
-                    ones *= shrink;
-#pragma unroll
-                    for (auto& a : acc) a *= shrink;
-                    if (first) weigh(k + 1);
-                }
-                if ((any & kHasNan) && first)
-                    clean(L.tile[(k + 1) % kDeep] + blk * kBlockStep, lane);
-                barrier();
-            }
-            if (first) l += (p[0] + p[1]) + (p[2] + p[3]);
-        }
-        // the sums of the two blocks
-        l = xor32_sum(xor16_sum(l));
-        if (first && lane < 16) L.sum[blk][lane] = l;
-        barrier();
-        const float sum = L.sum[0][n] + L.sum[1][n];
         const bool whole = take == all;
-        const int column0 = wave * kCols * 16 + 4 * g;
-        if (whole) {
-            if (r.live) {
-                const int64_t to = out_row(P, w, w.row0 + n);
-                const float inv = ones[0] == 0.f ? 0.f : 1.f / ones[0];
-#pragma unroll
-                for (int i = 0; i < kCols; ++i) put(P.out + to * kC + column0 + i * 16, acc[i], inv);
-                if (P.lse && wave == 0 && g == 0) P.lse[to] = lse_of(m, sum);
-            }
-        } else {
-            // a workgroup has at most two such: its first, and its last
-            const int slot = 2 * wg + (lead ? 0 : 1);
-            float* part = P.part + ((int64_t)slot * kFew + n) * kC + column0;
-#pragma unroll
-            for (int i = 0; i < kCols; ++i)
-                st_global(reinterpret_cast<f32x4*>(part + i * 16), acc[i]);
-            if (wave == 0 && g == 0) st_global(P.stat + slot * kFew + n, f32x4{m, sum, ones[0], 0.f});
-        }
+        // a workgroup has at most two parts: its first, and its last
+        const int slot = 2 * wg + (lead ? 0 : 1);
+        attend<1>(P, L, w, off, until > off ? until - off : 0, whole ? -1 : slot);
         if (off == 0 && t == 0) {
             const int64_t u = first_unit(w.tok0, w.seq, P.n_heads, kFew, P.pad) + w.row0 / kFew;
             const int last = share.holder(at + all - 1);
-            P.meta[u] = make_int4(2 * wg + (lead ? 0 : 1), wg + 1, whole ? 1 : last - wg + 1, 0);
+            P.meta[u] = make_int4(slot, wg + 1, whole ? 1 : last - wg + 1, 0);
         }
         at += take;
         if (at >= end) return;
@@ -657,188 +737,258 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams P) 
 
 // ---------------------------------------------------------------- many rows
 
-// Prompts, and whatever else has 64 rows or more for a sequence: 64 rows a unit, 32
-// positions a step. The products bound it, so K is read from LDS by four waves that
-// have 16 rows each, and each widened V operand serves all 64 rows: a wave takes
-// the scores of its 16 rows, and adds its 128 columns of O for all 64 (128
-// registers). One barrier a step: behind it are the weights of this step and the
-// copies of the next, so the second product of a step and the first of the next
-// fill the matrix pipes together; two workgroups share a CU.
-struct ManyLds {
-    __attribute__((aligned(16))) uint8_t tile[3][2 * kBlockStep];
-    uint32_t scale[3][kWaves][64];
-    u32x4 p[2][kWaves][64];     // [step parity][16 rows][lane]
-    float shrink[2][kWaves][16];
-    int flag[2][kWaves];
-};
-static_assert(sizeof(ManyLds) <= 80 * 1024, "two workgroups share a CU");
+// Prompts, and whatever else has more than 32 rows for a sequence: 64 rows a unit, four
+// tiles of 16, a page a step, eight waves. The products bound it, so the step is large
+// (a barrier's latency counts once for 64 x 64 scores) and the widening is shared: wave
+// (tile pair, half, block pair) takes half of the 576 products of 32 rows with 32
+// positions, so that each widened K operand serves two tiles; it exchanges halves with
+// its partner, makes the weights of one tile and 32 positions, and adds its 64 columns
+// of O for all 64 rows over the whole page, where each widened V operand serves four
+// tiles. 72 registers of q, 64 of O: two waves a SIMD.
+//
+// A workgroup per unit, or several with a share of the unit's steps where there are
+// few units. The last units come first: a causal prompt's are the longest.
 constexpr int kMany = 64;       // rows
+constexpr int kManyWaves = 8;
+constexpr int kManyThreads = kManyWaves * 64;
+constexpr int kManyRing = 3;
+struct ManyLds {
+    __attribute__((aligned(16))) uint8_t tile[kManyRing][4 * kBlockStep];
+    uint32_t scale[kManyRing][8];
+    f32x4 half[kManyWaves][2][64];  // half of the scores of a tile and two blocks
+    u32x4 p[2][4][2][64];       // [step parity][tile][half of the page][lane]
+    int flag[2][kManyWaves];
+    float m[4][16], top[4][2][16], sum[4][2][16], rounded[4][2][16];
+};
+static_assert(sizeof(ManyLds) <= 160 * 1024, "");
 
-__global__ __launch_bounds__(kThreads, 2) void many_kernel(AttendParams P) {
+__global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     ManyLds& L = *reinterpret_cast<ManyLds*>(lds);
+    constexpr int kCols = kC / 16 / kManyWaves; // of 16
     const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
     const int g = lane >> 4, n = lane & 15;
+    const int bp = wave & 1, half = wave >> 1 & 1, tp = wave >> 2;
+    const int mine = 2 * tp + half;             // the tile whose weights this wave makes
     const int unit = P.units - 1 - blockIdx.x / P.shares, split = blockIdx.x % P.shares;
     Work w;
-    if (!find_work<kMany, kStep>(P, unit, w)) return;
+    if (!find_work<kMany, kPage>(P, unit, w)) return;
     const int each = (w.n + P.shares - 1) / P.shares;
     const int off = split * each;
     const int cnt = off + each < w.n ? each : w.n - off;
     if (split > 0 && cnt <= 0) return;
     const bool whole = each >= w.n;             // no other workgroup has these rows
-    const Row r = row_of(P, w, w.row0 + wave * 16 + n);
     if (w.len < 0 && t == 0 && split == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
 
-    bf16x8 q[kChunks / 2];
-    load_q(P, w, r, g, 0, q);
-    constexpr int kCols = kC / 16 / kWaves;     // of 16
-    f32x4 acc[kWaves][kCols];
+    const Row r = row_of(P, w, w.row0 + mine * 16 + n);
+    const Common common(r);
+    bf16x8 q[2][kHalf];                         // of the tile pair
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        load_q(P, w, row_of(P, w, w.row0 + (2 * tp + i) * 16 + n), g, half, q[i]);
+    f32x4 acc[4][kCols];
 #pragma unroll
     for (auto& a : acc)
 #pragma unroll
         for (auto& b : a) b = f32x4{0.f, 0.f, 0.f, 0.f};
+    // the sum of the rounded weights of tile wave & 3 and half of the page wave >> 2
     f32x4 ones{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    // the references of the wave's tile (see attend())
+    float m = -INFINITY, ref = -INFINITY, l = 0.f;
+    const float slack = kSlack / P.scale;
+    f32x4 z[2];                                 // the scores of `mine` and the two blocks
+    float p0[4], p1[4];
+    bool nan = false;
+    if (t < 64) L.m[t >> 4][n] = -INFINITY;
     Pages pages{0, 0, 0};
-    int good = 0;
+    if (cnt > 0) page_of<kPage>(P, w, pages, off, off + cnt, lane);
+    __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0): see attend()
+
     const auto issue = [&](int k) {
-        const int page = page_of<kStep>(P, w, pages, off + k, off + cnt, lane);
+        const int page = page_of<kPage>(P, w, pages, off + k, off + cnt, lane);
         const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
         const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
-        const int half = step_of<kStep>(w, off + k) & 1;
-        // eighteen pieces of 1 KB: two waves take five, two take four
-        const uint32_t to = lds_addr(L.tile[k % 3]);
+        const uint32_t to = lds_addr(L.tile[k % kManyRing]);
 #pragma unroll
         for (int i = 0; i < 5; ++i) {
-            const int piece = wave + kWaves * i;
-            if (piece < 18)
-                copy_kb<false>(src + half * 2 * kBlockBytes + piece * 1024 + lane * 16,
-                           to + piece * 1024 + (piece >= 9 ? kBlockStep - kBlockBytes : 0));
+            const int piece = wave + kManyWaves * i;
+            if (piece < 36)
+                copy_kb<false>(src + piece * 1024 + lane * 16,
+                               to + piece * 1024 + piece / 9 * (kBlockStep - kBlockBytes));
         }
-        copy_words(src + kCodeBytes + half * 16 + (lane & 3) * 4, lds_addr(L.scale[k % 3][wave]));
-        const int bit = 1 << (k % 3);
-        good = base >= 0 ? good | bit : good & ~bit;
-        if (base < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
+        if (wave == 4 && lane < 2)
+            copy_kb<false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[k % kManyRing]));
     };
-    // the scores and weights of step k
     const auto score = [&](int k) {
-        const uint8_t* buf = L.tile[k % 3];
-        const float sc0 = any_scale(L.scale[k % 3][wave][0]), sp0 = any_scale(L.scale[k % 3][wave][1]);
-        const float sc1 = any_scale(L.scale[k % 3][wave][2]), sp1 = any_scale(L.scale[k % 3][wave][3]);
-        f32x4 z0{0.f, 0.f, 0.f, 0.f}, z1{0.f, 0.f, 0.f, 0.f};
+        const int b = k % kManyRing;
+        f32x4 y[2][2];                          // [tile][block]
 #pragma unroll
-        for (int i = 0; i < kChunks / 4; ++i) {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(buf + i * 1024 + lane * 16);
-            const u32x4 b = *reinterpret_cast<const u32x4*>(buf + kBlockStep + i * 1024 + lane * 16);
-            const float sa = i < kC / 64 ? sc0 : sp0, sb = i < kC / 64 ? sc1 : sp1;
-            z0 = mfma(widen(a.x, a.y, sa, sa), q[2 * i], z0);
-            z1 = mfma(widen(b.x, b.y, sb, sb), q[2 * i], z1);
-            z0 = mfma(widen(a.z, a.w, sa, sa), q[2 * i + 1], z0);
-            z1 = mfma(widen(b.z, b.w, sb, sb), q[2 * i + 1], z1);
-        }
-        float s0[4], s1[4], top = m;
-        bool nan = false;
-        const bool ok = good >> (k % 3) & 1;
-        const int base = step_of<kStep>(w, off + k) * kStep + 4 * g;
+        for (int j = 0; j < 2; ++j) {
+            const uint8_t* block = L.tile[b] + (2 * bp + j) * kBlockStep + lane * 16;
+            const float sc = any_scale(L.scale[b][2 * (2 * bp + j)]);
+            const float sp = any_scale(L.scale[b][2 * (2 * bp + j) + 1]);
+            y[0][j] = y[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float a = z0[j] * P.scale, b = z1[j] * P.scale;
-            const int pa = base + j, pb = base + kBlock + j;
-            nan |= a != a || b != b;
-            s0[j] = ok && pa <= r.pos && (pa >= r.seen.lo || pa < r.seen.sink) ? a : -INFINITY;
-            s1[j] = ok && pb <= r.pos && (pb >= r.seen.lo || pb < r.seen.sink) ? b : -INFINITY;
-            top = fmaxf(top, fmaxf(s0[j], s1[j]));
+            for (int i = 0; i < 4; ++i) {
+                const u32x4 a = *reinterpret_cast<const u32x4*>(block + (2 * i + half) * 1024);
+                const bf16x8 lo = widen(a.x, a.y, sc, sc), hi = widen(a.z, a.w, sc, sc);
+                y[0][j] = mfma(lo, q[0][2 * i], y[0][j]);
+                y[1][j] = mfma(lo, q[1][2 * i], y[1][j]);
+                y[0][j] = mfma(hi, q[0][2 * i + 1], y[0][j]);
+                y[1][j] = mfma(hi, q[1][2 * i + 1], y[1][j]);
+            }
+            const uint2 a = *reinterpret_cast<const uint2*>(block + 8 * 1024 + half * 8);
+            const bf16x8 pe = widen(a.x, a.y, sp, sp);
+            y[0][j] = mfma(pe, q[0][8], y[0][j]);
+            y[1][j] = mfma(pe, q[1][8], y[1][j]);
         }
-        top = xor32_max(xor16_max(top));
-        int flag = __ballot(nan) ? kHasNan : 0;
-        if (__ballot(top > m + kSlack)) {
-            flag |= kNeedMax;
-            const float shrink = top == -INFINITY ? 1.f : exp2_(m - top);
-            m = top;
-            l *= shrink;
-            ones *= shrink;
-            if (lane < 16) L.shrink[k & 1][wave][lane] = shrink;
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s0[j] = exp2_(s0[j] - ref);
-            s1[j] = exp2_(s1[j] - ref);
+        for (int j = 0; j < 2; ++j) {
+            z[j] = half ? y[1][j] : y[0][j];
+            L.half[wave][j][lane] = half ? y[0][j] : y[1][j];
         }
-        l += ((s0[0] + s0[1]) + (s0[2] + s0[3])) + ((s1[0] + s1[1]) + (s1[2] + s1[3]));
-        const uint2 a = weights(s0), b = weights(s1);
-        const u32x4 p{a.x, a.y, b.x, b.y};
-        L.p[k & 1][wave][lane] = p;
-        if (lane == 0) L.flag[k & 1][wave] = flag;
-        ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}),
-                    __builtin_bit_cast(bf16x8, p), ones);
     };
-    if (cnt > 0) issue(0);
-    if (cnt > 1) issue(1);
+    const auto weigh = [&](int k) {
+        const float down = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            p0[j] = exp2_(fmaf(z[0][j], P.scale, -down));
+            p1[j] = exp2_(fmaf(z[1][j], P.scale, -down));
+        }
+        const uint2 a = weights(p0), b = weights(p1);
+        L.p[k & 1][mine][bp][lane] = u32x4{a.x, a.y, b.x, b.y};
+    };
+    const auto finish = [&](int k) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) z[j] += L.half[wave ^ 2][j][lane];
+        const int page = page_of<kPage>(P, w, pages, off + k, off + cnt, lane);
+        const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
+        const int base = step_of<kPage>(w, off + k) * kPage + bp * 32;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= (z[0][j] != z[0][j]) | (z[1][j] != z[1][j]);
+        if (!(ok && common.all(base, 32))) {
+            asm volatile("");                   // a branch, not forty instructions every step
+            if (!ok && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    z[j][i] = (ok & sees(r, base + kBlock * j + 4 * g + i)) ? z[j][i] : -INFINITY;
+        }
+        weigh(k);
+        const float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
+                                fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
+        nan = __ballot(bad) != 0;
+        const bool high = __ballot(top > m + slack) != 0;
+        if (lane == 0) L.flag[k & 1][wave] = nan | high;
+    };
+    // What is rare: a row's scores beyond its reference, or a NaN, in step k.
+    const auto mend = [&](int k) {
+        float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
+                          fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
+        top = xor32_max(xor16_max(top));
+        if (lane < 16) L.top[mine][bp][lane] = top;
+        if (nan && half == 0 && tp == 0)
+            for (int j = 0; j < 2; ++j)
+                clean(L.tile[k % kManyRing] + (2 * bp + j) * kBlockStep, lane);
+        barrier();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float was = L.m[i][n];
+            const float to = fmaxf(was, fmaxf(L.top[i][0][n], L.top[i][1][n]));
+            const float shrink = to == -INFINITY ? 1.f : exp2_(was * P.scale - to * P.scale);
+            if (i == mine) {
+                m = to;
+                ref = to * P.scale;
+                l *= shrink;
+            }
+            if (i == (wave & 3)) ones *= shrink;
+#pragma unroll
+            for (auto& a : acc[i]) a *= shrink;
+        }
+        weigh(k);
+        barrier();
+        if (bp == 0 && lane < 16) L.m[mine][lane] = m;
+    };
+    // O over step k
+    const auto add = [&](int k) {
+        const int b = k % kManyRing;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            bf16x8 pb[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pb[j] = __builtin_bit_cast(bf16x8, L.p[k & 1][j][h][lane]);
+            const float sa = any_scale(L.scale[b][4 * h]), sb = any_scale(L.scale[b][4 * h + 2]);
+            const uint8_t* col = column_at(L.tile[b] + 2 * h * kBlockStep, lane) + wave * kCols * 256;
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) {
+                const i32x2 v = column(col, i);
+                const bf16x8 a = widen((uint32_t)v.x, (uint32_t)v.y, sa, sb);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j][i] = mfma(a, pb[j], acc[j][i]);
+            }
+        }
+        ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}),
+                    __builtin_bit_cast(bf16x8, L.p[k & 1][wave & 3][wave >> 2][lane]), ones);
+    };
+
+    for (int k = 0; k < kManyRing - 1 && k < cnt; ++k) issue(k);
     wait_copies<0>();
     barrier();
-    if (cnt > 0) score(0);
-    for (int k = 0; k < cnt; ++k) {
-        wait_copies<0>();
-        barrier();              // this step's weights, and the next one's tile
-        if (k + 2 < cnt) issue(k + 2);          // where the tile before was
-        const int any = wave_bcast((L.flag[k & 1][0] | L.flag[k & 1][1]) |
-                                   (L.flag[k & 1][2] | L.flag[k & 1][3]));
-        if (any) {
-            if (any & kNeedMax) {
-#pragma unroll
-                for (int i = 0; i < kWaves; ++i) {
-                    if (!(wave_bcast(L.flag[k & 1][i]) & kNeedMax)) continue;
-                    const float f = L.shrink[k & 1][i][n];
-#pragma unroll
-                    for (auto& a : acc[i]) a *= f;
-                }
-            }
-            if (any & kHasNan) {
-                if (wave < 2) clean(L.tile[k % 3] + wave * kBlockStep, lane);
-                barrier();
-            }
-        }
-        const float sa = any_scale(L.scale[k % 3][wave][0]), sb = any_scale(L.scale[k % 3][wave][2]);
-        bf16x8 p[kWaves];
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) p[i] = __builtin_bit_cast(bf16x8, L.p[k & 1][i][lane]);
-        const uint8_t* col = column_at(L.tile[k % 3], lane) + wave * kCols * 256;
-#pragma unroll
-        for (int i = 0; i < kCols; ++i) {
-            const i32x2 v = column(col, i);
-            const bf16x8 a = widen((uint32_t)v.x, (uint32_t)v.y, sa, sb);
-#pragma unroll
-            for (int j = 0; j < kWaves; ++j) acc[j][i] = mfma(a, p[j], acc[j][i]);
-        }
-        if (k + 1 < cnt) score(k + 1);
+    if (cnt > 0) {
+        score(0);
+        barrier();
+        finish(0);
     }
-    // every wave needs the sums of all rows
+    // Step k: behind barrier A the weights of k and the rows of k + 1 are there, behind
+    // B both halves of the scores of k + 1.
+    for (int k = 0; k < cnt; ++k) {
+        wait_copies<0>();                       // step k + 1
+        barrier();                              // A
+        const int* f = L.flag[k & 1];
+        const int flags = ((f[0] | f[1]) | (f[2] | f[3])) | ((f[4] | f[5]) | (f[6] | f[7]));
+        if (k + kManyRing - 1 < cnt) issue(k + kManyRing - 1);      // where step k - 1 was
+        if (wave_bcast(flags)) mend(k);
+        l += ((p0[0] + p0[1]) + (p0[2] + p0[3])) + ((p1[0] + p1[1]) + (p1[2] + p1[3]));
+        if (k + 1 < cnt) score(k + 1);
+        add(k);
+        if (k + 1 < cnt) {
+            barrier();                          // B
+            finish(k + 1);
+        }
+    }
+    // the sums of the blocks, and of the page's halves
     l = xor32_sum(xor16_sum(l));
-    barrier();
-    f32x4* stat = reinterpret_cast<f32x4*>(&L.p[0][0][0]);
-    if (lane < 16) stat[wave * 16 + lane] = f32x4{m, l, ones[0], 0.f};
+    if (lane < 16) {
+        L.sum[mine][bp][lane] = l;
+        L.rounded[wave & 3][wave >> 2][lane] = ones[0];
+        if (bp == 0) L.m[mine][lane] = m;
+    }
     barrier();
     const int64_t slot = (int64_t)unit * P.shares + split;
+    const int column0 = wave * kCols * 16 + 4 * g;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const int row = i * 16 + n;
-        const f32x4 st = stat[row];
-        const int column0 = wave * (kC / kWaves) + 4 * g;
+        const float sum = L.sum[i][0][n] + L.sum[i][1][n];
+        const float rounded = L.rounded[i][0][n] + L.rounded[i][1][n];
+        const float scaled = L.m[i][n] * P.scale;
         if (whole) {
-            if (w.row0 + row >= w.rows) continue;
-            const int64_t at = out_row(P, w, w.row0 + row);
-            const float inv = st[2] == 0.f ? 0.f : 1.f / st[2];
+            if (w.row0 + row < w.rows) {
+                const int64_t to = out_row(P, w, w.row0 + row);
+                const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) put(P.out + at * kC + column0 + j * 16, acc[i][j], inv);
-            if (P.lse && wave == 0 && g == 0) P.lse[at] = lse_of(st[0], st[1]);
+                for (int j = 0; j < kCols; ++j)
+                    put(P.out + to * kC + column0 + j * 16, acc[i][j], inv);
+                if (P.lse && wave == 0 && g == 0) P.lse[to] = lse_of(scaled, sum);
+            }
         } else {
-            float* part = P.part + (slot * kMany + row) * kC + column0;
+            const int64_t at = slot * kMany + row;
 #pragma unroll
             for (int j = 0; j < kCols; ++j)
-                st_global(reinterpret_cast<f32x4*>(part + j * 16), acc[i][j]);
-            if (wave == 0 && g == 0) st_global(P.stat + slot * kMany + row, st);
+                st_global(reinterpret_cast<f32x4*>(P.part + at * kC + column0 + j * 16), acc[i][j]);
+            if (wave == 0 && g == 0) st_global(P.stat + at, f32x4{scaled, sum, rounded, 0.f});
         }
     }
 }
@@ -846,7 +996,7 @@ __global__ __launch_bounds__(kThreads, 2) void many_kernel(AttendParams P) {
 __global__ __launch_bounds__(kJoinThreads) void join_many_kernel(AttendParams P) {
     const int64_t u = blockIdx.x / kMany;
     Work w;
-    if (!find_work<kMany, kStep>(P, u, w)) return;
+    if (!find_work<kMany, kPage>(P, u, w)) return;
     const int row = blockIdx.x % kMany;
     if (w.row0 + row >= w.rows) return;
     const int each = (w.n + P.shares - 1) / P.shares;
@@ -928,16 +1078,16 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
         P.units = (int)few;
         const int64_t steps = few * ((seen + kStep - 1) / kStep);
         P.shares = (int)(steps < kShares ? steps : kShares);
-        if (int e = launch(few_kernel, P.shares, kThreads, sizeof(FewLds), P, stream)) return e;
+        if (int e = launch(few_kernel, P.shares, kThreads, sizeof(Lds<1>), P, stream)) return e;
         return launch(join_few_kernel, few * kFew, kJoinThreads, 0, P, stream);
     }
     P.pad = n_heads % kMany != 0;
     const int64_t units = first_unit(n_tokens, cache->n_seqs, n_heads, kMany, P.pad);
     P.units = (int)units;
     int64_t splits = kShares / 2 / units;
-    const int64_t most = (seen + 4 * kStep - 1) / (4 * kStep);
+    const int64_t most = (seen + 4 * kPage - 1) / (4 * kPage);
     if (splits > most) splits = most;
     P.shares = splits < 1 ? 1 : (int)splits;
-    if (int e = launch(many_kernel, units * P.shares, kThreads, sizeof(ManyLds), P, stream)) return e;
+    if (int e = launch(many_kernel, units * P.shares, kManyThreads, sizeof(ManyLds), P, stream)) return e;
     return P.shares > 1 ? launch(join_many_kernel, units * kMany, kJoinThreads, 0, P, stream) : 0;
 }

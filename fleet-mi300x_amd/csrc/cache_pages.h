@@ -97,11 +97,11 @@ struct Copy {
 
 __device__ __forceinline__ void raise(Header* h, uint32_t bit) { atomicOr(&h->status, bit); }
 
-// What the attention's second launch joins: partial results of up to 1024 times 16
-// rows (fp32 [512] each), their maxima and sums, and where a unit's lie.
+// What the attention's second launch joins: partial results (fp32 [512] a row), the
+// rows' references and sums, and where a unit's lie.
 constexpr int kShares = 512;           // workgroups: two a CU
 constexpr int kMaxUnits = 4096;
-constexpr int kPartRows = 1024 * 16;
+constexpr int kPartRows = 1024 * 16;   // two parts of 16 rows a workgroup, or one of 32
 constexpr size_t kPartBytes = (size_t)kPartRows * kC * 4;
 constexpr size_t kStatBytes = (size_t)kPartRows * 16;
 constexpr size_t kMetaBytes = (size_t)kMaxUnits * 16;
