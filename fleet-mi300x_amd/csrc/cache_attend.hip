@@ -821,24 +821,35 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     };
     const auto score = [&](int k) {
         const int b = k % kManyRing;
-        f32x4 y[2][2];                          // [tile][block]
+        u32x4 c[2][4];
+        uint2 e[2];
+        uint32_t f[2][2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const uint8_t* block = L.tile[b] + (2 * bp + j) * kBlockStep + lane * 16;
-            const float sc = any_scale(L.scale[b][2 * (2 * bp + j)]);
-            const float sp = any_scale(L.scale[b][2 * (2 * bp + j) + 1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                c[j][i] = *reinterpret_cast<const u32x4*>(block + (2 * i + half) * 1024);
+            e[j] = *reinterpret_cast<const uint2*>(block + 8 * 1024 + half * 8);
+            f[j][0] = L.scale[b][2 * (2 * bp + j)];
+            f[j][1] = L.scale[b][2 * (2 * bp + j) + 1];
+        }
+        __builtin_amdgcn_sched_barrier(0);      // every read on its way
+        f32x4 y[2][2];                          // [tile][block]
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float sc = any_scale(f[j][0]), sp = any_scale(f[j][1]);
             y[0][j] = y[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const u32x4 a = *reinterpret_cast<const u32x4*>(block + (2 * i + half) * 1024);
+                const u32x4 a = c[j][i];
                 const bf16x8 lo = widen(a.x, a.y, sc, sc), hi = widen(a.z, a.w, sc, sc);
                 y[0][j] = mfma(lo, q[0][2 * i], y[0][j]);
                 y[1][j] = mfma(lo, q[1][2 * i], y[1][j]);
                 y[0][j] = mfma(hi, q[0][2 * i + 1], y[0][j]);
                 y[1][j] = mfma(hi, q[1][2 * i + 1], y[1][j]);
             }
-            const uint2 a = *reinterpret_cast<const uint2*>(block + 8 * 1024 + half * 8);
-            const bf16x8 pe = widen(a.x, a.y, sp, sp);
+            const bf16x8 pe = widen(e[j].x, e[j].y, sp, sp);
             y[0][j] = mfma(pe, q[0][8], y[0][j]);
             y[1][j] = mfma(pe, q[1][8], y[1][j]);
         }
@@ -914,19 +925,28 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     // O over step k
     const auto add = [&](int k) {
         const int b = k % kManyRing;
+        bf16x8 pb[2][4];
+        i32x2 v[2][kCols];
+        uint32_t f[2][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            bf16x8 pb[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) pb[j] = __builtin_bit_cast(bf16x8, L.p[k & 1][j][h][lane]);
-            const float sa = any_scale(L.scale[b][4 * h]), sb = any_scale(L.scale[b][4 * h + 2]);
             const uint8_t* col = column_at(L.tile[b] + 2 * h * kBlockStep, lane) + wave * kCols * 256;
 #pragma unroll
-            for (int i = 0; i < kCols; ++i) {
-                const i32x2 v = column(col, i);
-                const bf16x8 a = widen((uint32_t)v.x, (uint32_t)v.y, sa, sb);
+            for (int i = 0; i < kCols; ++i) v[h][i] = column(col, i);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j][i] = mfma(a, pb[j], acc[j][i]);
+            for (int j = 0; j < 4; ++j) pb[h][j] = __builtin_bit_cast(bf16x8, L.p[k & 1][j][h][lane]);
+            f[h][0] = L.scale[b][4 * h];
+            f[h][1] = L.scale[b][4 * h + 2];
+        }
+        __builtin_amdgcn_sched_barrier(0);      // every read on its way
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float sa = any_scale(f[h][0]), sb = any_scale(f[h][1]);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) {
+                const bf16x8 a = widen((uint32_t)v[h][i].x, (uint32_t)v[h][i].y, sa, sb);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j][i] = mfma(a, pb[h][j], acc[j][i]);
             }
         }
         ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}),
