@@ -163,13 +163,31 @@ __device__ __forceinline__ int64_t out_row(const AttendParams& P, const Work& w,
 // halves of a transposing read, from neighbouring blocks, fall into different banks.
 constexpr int kBlockStep = kBlockBytes + 64;
 
-// Copies 16 bytes per lane from global memory to LDS, 1 KB in all: to `lds` + 16 lane.
-// There is no register for the data, so none is in flight behind the compiler's
-// back. In asm, because the compiler would wait for every copy in flight before each
-// LDS read; wait_copies() orders them.
-template <bool kOnce>           // read once: kept out of the caches
+// Copies kN times 1 KB from global memory to LDS, 16 bytes a lane: from `src` (the
+// lane's) + 1024 i to `lds` + 1024 i + 16 lane (the offset counts on both sides). There
+// is no register for the data, so none is in flight behind the compiler's back. In
+// asm, because the compiler would wait for every copy in flight before each LDS read;
+// wait_copies() orders them. kOnce: not kept in the caches.
+template <int kN, bool kOnce>
 __device__ __forceinline__ void copy_kb(const uint8_t* src, uint32_t lds) {
-    if constexpr (kOnce)
+    static_assert(kN == 1 || kN == 4, "");
+    if constexpr (kN == 4 && kOnce)
+        asm volatile(
+            "s_nop 0\n\t"
+            "global_load_lds_dwordx4 %0, off nt\n\t"
+            "global_load_lds_dwordx4 %0, off offset:1024 nt\n\t"
+            "global_load_lds_dwordx4 %0, off offset:2048 nt\n\t"
+            "global_load_lds_dwordx4 %0, off offset:3072 nt" ::"v"(src), "{m0}"(lds)
+            : "memory");
+    else if constexpr (kN == 4)
+        asm volatile(
+            "s_nop 0\n\t"
+            "global_load_lds_dwordx4 %0, off\n\t"
+            "global_load_lds_dwordx4 %0, off offset:1024\n\t"
+            "global_load_lds_dwordx4 %0, off offset:2048\n\t"
+            "global_load_lds_dwordx4 %0, off offset:3072" ::"v"(src), "{m0}"(lds)
+            : "memory");
+    else if constexpr (kOnce)
         asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "{m0}"(lds)
                      : "memory");
     else
@@ -291,6 +309,9 @@ __device__ __forceinline__ int page_of(const AttendParams& P, const Work& w, Pag
         h.page = i + lane < end ? ld_global(P.c.table + (int64_t)w.seq * P.c.max_pages +
                                             step_of<S>(w, i + lane) * S / kPage)
                                 : 0;
+        // here, not at the use: there the compiler would wait, every step, for
+        // whatever copies are in flight
+        __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0)
     }
     return __builtin_amdgcn_readlane(h.page, i - h.from);
 }
@@ -363,7 +384,7 @@ __device__ __forceinline__ void attend(const AttendParams& P, Lds<kTiles>& L, co
     float p[4];
     Pages pages{0, 0, 0};
     if (cnt > 0) page_of<kStep>(P, w, pages, off, off + cnt, lane);
-    // q and the pages are there before a copy is issued, as far as the compiler counts
+    // q is there before a copy is issued, also as far as the compiler counts
     __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0)
 
     const auto issue = [&](int k) {
@@ -373,13 +394,11 @@ __device__ __forceinline__ void attend(const AttendParams& P, Lds<kTiles>& L, co
         const int b = k % kRing, part = step_of<kStep>(w, off + k) & 1;
         const uint8_t* from = src + (2 * part + blk) * kBlockBytes + lane * 16;
         const uint32_t to = lds_addr(L.tile[b]) + blk * kBlockStep;
-        const int first = kFirst ? 0 : half * 5;
-        constexpr int kPieces = kFirst ? 9 : 5;
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-            if (first + i < 9) copy_kb<kFirst>(from + (first + i) * 1024, to + (first + i) * 1024);
-        if ((kFirst || half == 1) && lane == 0)
-            copy_kb<false>(src + kCodeBytes + part * 16, lds_addr(L.scale[b]));
+        static_assert(kFirst && kBlockBytes == 9 * 1024, "");
+        copy_kb<4, true>(from, to);
+        copy_kb<4, true>(from + 4096, to + 4096);
+        copy_kb<1, true>(from + 8192, to + 8192);
+        if (lane == 0) copy_kb<1, true>(src + kCodeBytes + part * 16, lds_addr(L.scale[b]));
     };
     const auto score = [&](int k) {
         const int b = k % kRing;
@@ -808,16 +827,15 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         const int page = page_of<kPage>(P, w, pages, off + k, off + cnt, lane);
         const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
         const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
-        const uint32_t to = lds_addr(L.tile[k % kManyRing]);
-#pragma unroll
-        for (int i = 0; i < 5; ++i) {
-            const int piece = wave + kManyWaves * i;
-            if (piece < 36)
-                copy_kb<false>(src + piece * 1024 + lane * 16,
-                               to + piece * 1024 + piece / 9 * (kBlockStep - kBlockBytes));
-        }
-        if (wave == 4 && lane < 2)
-            copy_kb<false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[k % kManyRing]));
+        // two waves a block: five pieces of 1 KB, and four; one of the others the scales
+        const uint8_t* from = src + (wave >> 1) * kBlockBytes + (wave & 1) * 5120 + lane * 16;
+        const uint32_t to = lds_addr(L.tile[k % kManyRing]) + (wave >> 1) * kBlockStep +
+                            (wave & 1) * 5120;
+        copy_kb<4, false>(from, to);
+        if ((wave & 1) == 0)
+            copy_kb<1, false>(from + 4096, to + 4096);
+        else if (wave == 1 && lane < 2)
+            copy_kb<1, false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[k % kManyRing]));
     };
     const auto score = [&](int k) {
         const int b = k % kManyRing;
