@@ -607,28 +607,41 @@ struct Shares {
     }
 };
 
+// A unit counts kSetup steps besides its own where shares are long: beginning one in
+// the middle of a share takes as long (queries, page numbers and the first copies
+// one after the other: 7 us of 64 sequences' 45, which the workgroups that had two
+// units ended later).
+constexpr int kSetup = 6;
+
 // The total of all units' steps; its division (no share is empty: the join counts
 // on it); and the unit in which workgroup wg's part begins, and where. Every
 // wave for itself, a lane per sequence (or for several, then once more a lane for each
 // of the one lane's): no barrier, and one round of loads for 64 sequences.
-__device__ __forceinline__ bool locate(const AttendParams& P, int wg, Work& w, int& off, int& total,
-                                       int& shares) {
+struct Place {
+    int off, total, shares, setup;
+};
+__device__ __forceinline__ bool locate(const AttendParams& P, int wg, Work& w, Place& at) {
     const int lane = threadIdx.x & 63;
     const int each = (P.c.n_seqs + 63) / 64;
     Work mine{};
-    int n = 0;
+    int n = 0, units = 0;
     for (int i = 0; i < each; ++i) {
         const int s = lane * each + i;
         if (s < P.c.n_seqs) {
             open_seq(P, s, mine);
             n += seq_steps(P, mine);
+            units += (mine.rows + kFew - 1) / kFew;
         }
     }
     int incl = wave_incl_scan(n);
-    total = lane_of(incl, 63);
-    shares = total < P.shares ? total : P.shares;
-    if (wg >= shares) return false;
-    off = Shares(total, shares).first(wg);
+    const int plain = lane_of(incl, 63);
+    at.setup = plain >= 2 * kSetup * P.shares ? kSetup : 0;
+    n += at.setup * units;
+    incl = wave_incl_scan(n);
+    at.total = lane_of(incl, 63);
+    at.shares = at.total < P.shares ? at.total : P.shares;
+    if (wg >= at.shares) return false;
+    int off = Shares(at.total, at.shares).first(wg);
     int owner = __popcll(__ballot(incl <= off));
     off -= lane_of(incl - n, owner);
     if (each > 1) {
@@ -637,7 +650,7 @@ __device__ __forceinline__ bool locate(const AttendParams& P, int wg, Work& w, i
         n = 0;
         if (lane < each && s < P.c.n_seqs) {
             open_seq(P, s, mine);
-            n = seq_steps(P, mine);
+            n = seq_steps(P, mine) + at.setup * ((mine.rows + kFew - 1) / kFew);
         }
         incl = wave_incl_scan(n);
         owner = __popcll(__ballot(incl <= off));
@@ -646,10 +659,12 @@ __device__ __forceinline__ bool locate(const AttendParams& P, int wg, Work& w, i
     w = lane_of(mine, owner);
     for (w.row0 = 0;; w.row0 += kFew) {
         see<kFew, kStep>(P, w);
-        const int all = w.n > 0 ? w.n : 1;
-        if (off < all) return true;
+        const int all = (w.n > 0 ? w.n : 1) + at.setup;
+        if (off < all) break;
         off -= all;
     }
+    at.off = off;
+    return true;
 }
 
 __global__ __launch_bounds__(kThreads, 2) void few_kernel(AttendParams P) {
@@ -657,21 +672,23 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(AttendParams P) {
     Lds<1>& L = *reinterpret_cast<Lds<1>*>(lds);
     const int t = threadIdx.x, wg = blockIdx.x;
     Work w;
-    int off, total, shares;
-    if (!locate(P, wg, w, off, total, shares)) return;
-    const Shares share(total, shares);
-    int at = share.first(wg);
+    Place place;
+    if (!locate(P, wg, w, place)) return;
+    const Shares share(place.total, place.shares);
+    int at = share.first(wg), off = place.off;
     const int end = share.first(wg + 1);
     for (bool lead = true;; lead = false) {
         see<kFew, kStep>(P, w);
-        const int all = w.n > 0 ? w.n : 1;
+        const int all = (w.n > 0 ? w.n : 1) + place.setup;
         const int take = all - off < end - at ? all - off : end - at;
-        const int until = off + take < w.n ? off + take : w.n;
+        // the unit's own steps among them
+        const int from = off > place.setup ? off - place.setup : 0;
+        const int to = off + take - place.setup < w.n ? off + take - place.setup : w.n;
         if (w.len < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
         const bool whole = take == all;
         // a workgroup has at most two parts: its first, and its last
         const int slot = 2 * wg + (lead ? 0 : 1);
-        attend<1>(P, L, w, off, until > off ? until - off : 0, whole ? -1 : slot);
+        attend<1>(P, L, w, from, to > from ? to - from : 0, whole ? -1 : slot);
         if (off == 0 && t == 0) {
             const int64_t u = first_unit(w.tok0, w.seq, P.n_heads, kFew, P.pad) + w.row0 / kFew;
             const int last = share.holder(at + all - 1);
@@ -691,18 +708,28 @@ __global__ __launch_bounds__(kThreads, 2) void few_kernel(AttendParams P) {
 }
 
 // Adds the parts of a row, in order: a workgroup per row, four groups of threads
-// with a quarter of the parts each.
+// with a quarter of the parts each, the first few loaded before their weights are
+// known. Latency bounds it.
 constexpr int kJoinGroups = 4;
 constexpr int kJoinThreads = kC / 4 * kJoinGroups;
+constexpr int kJoinAhead = 4;
 template <int R>
 __device__ __forceinline__ void join(const AttendParams& P, int64_t row_at, int row, int64_t slot0,
                                      int64_t rest, int64_t step, int count) {
     __shared__ f32x4 sum_o[kJoinGroups][kC / 4];
-    const int t = threadIdx.x % (kC / 4), part = threadIdx.x / (kC / 4);
-    const auto slot = [&](int i) { return (i == 0 ? slot0 : rest + (i - 1) * step) * R + row; };
-    // the parts' weights: a lane per part
     __shared__ float factor[kShares];
+    const int t = threadIdx.x % (kC / 4), part = threadIdx.x / (kC / 4);
     const int lane = threadIdx.x & 63;
+    const auto slot = [&](int i) { return (i == 0 ? slot0 : rest + (i - 1) * step) * R + row; };
+    const auto load = [&](int i) {
+        return ld_global(reinterpret_cast<const f32x4*>(P.part + slot(i) * kC) + t);
+    };
+    f32x4 v[kJoinAhead];
+#pragma unroll
+    for (int i = 0; i < kJoinAhead; ++i)
+        v[i] = part + i * kJoinGroups < count ? load(part + i * kJoinGroups)
+                                              : f32x4{0.f, 0.f, 0.f, 0.f};
+    // the parts' weights: a lane per part
     float top = -INFINITY;
     for (int i = lane; i < count; i += 64) top = fmaxf(top, ld_global(P.stat + slot(i))[0]);
     top = wave_max(top);
@@ -719,9 +746,11 @@ __device__ __forceinline__ void join(const AttendParams& P, int64_t row_at, int 
     rounded = wave_sum(rounded);
     __syncthreads();
     f32x4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kJoinAhead; ++i)
+        if (part + i * kJoinGroups < count) o += v[i] * factor[part + i * kJoinGroups];
 #pragma unroll 4
-    for (int i = part; i < count; i += kJoinGroups)
-        o += ld_global(reinterpret_cast<const f32x4*>(P.part + slot(i) * kC) + t) * factor[i];
+    for (int i = part + kJoinAhead * kJoinGroups; i < count; i += kJoinGroups) o += load(i) * factor[i];
     sum_o[part][t] = o;
     __syncthreads();
     if (part) return;
@@ -745,13 +774,19 @@ __device__ __forceinline__ bool find_work(const AttendParams& P, int64_t u, Work
 
 __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams P) {
     const int64_t u = blockIdx.x / kFew;
-    Work w;
-    if (!find_work<kFew, kStep>(P, u, w)) return;
     const int row = blockIdx.x % kFew;
-    if (w.row0 + row >= w.rows) return;
+    int64_t to = u * kFew + row;                // where units follow each other without gaps
     const int4 m = P.meta[u];
-    if (m.z <= 1) return;
-    join<kFew>(P, out_row(P, w, w.row0 + row), row, m.x, 2 * (int64_t)m.y, 2, m.z);
+    if (P.pad == 0) {
+        const int tokens = P.start ? clamp_row(ld_global(P.start + P.c.n_seqs), P.n_tokens)
+                                   : P.n_tokens;
+        if (to >= (int64_t)tokens * P.n_heads) return;
+    } else {
+        Work w;
+        if (!find_work<kFew, kStep>(P, u, w) || w.row0 + row >= w.rows) return;
+        to = out_row(P, w, w.row0 + row);
+    }
+    if (m.z > 1) join<kFew>(P, to, row, m.x, 2 * (int64_t)m.y, 2, m.z);
 }
 
 // ---------------------------------------------------------------- many rows
