@@ -4,7 +4,9 @@
 // registers): their maximum, sum of exponentials, and n_out best. Second launch, a
 // workgroup per group: each beam's log sum, and the n_out best of what its parts
 // kept. Reading the logits bounds it (HBM for many beams; for few, the two
-// launches' latency).
+// launches' latency). Measured, 102,400 logits a beam: 32 groups of 8 beams, 16
+// outputs each, 22 + 7 us (105 MB; the loads by themselves take 15.5); 4 beams,
+// 5.3 + 4.8. With 32 logits a thread the two take 22.8 + 6.1 us: the same.
 //
 // The best of many without sorting them: let T be a value that at least n_out of
 // the threads' maxima reach. Every one of the n_out best is then >= T, and few
@@ -43,6 +45,7 @@ struct Params {
     int32_t* parents;
     int32_t* tokens;
     uint8_t* out_finished;
+    uint64_t per_beam;          // floor(2^44 / (parts * n_out)) + 1
     int n_beams, n_out, vocab, parts, eos;
 };
 
@@ -100,7 +103,8 @@ __global__ __launch_bounds__(kThreads) void part_kernel(Params P) {
     __shared__ PartLds L;
     const int row = blockIdx.y, part = blockIdx.x, t = threadIdx.x;
     const int lane = t & 63, wave = t >> 6;
-    if ((P.finished && P.finished[row]) || !has_score(P.scores[row])) return;
+    const bool done = P.finished && P.finished[row];
+    if (!has_score(P.scores[row]) | done) return;
     const float* x = P.logits + (int64_t)row * P.ld;
     const int base = part * kPart;
     const int n = P.vocab - base < kPart ? P.vocab - base : kPart;
@@ -120,10 +124,12 @@ __global__ __launch_bounds__(kThreads) void part_kernel(Params P) {
                 v[4 * i + j] = at + j < n ? ld_global(x + base + at + j) : -INFINITY;
         }
     }
-    float top = -INFINITY;
+    float top = -INFINITY, lowest = -INFINITY;
+    asm("" : "+v"(lowest));                               // (or med3 becomes min and max)
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        v[i] = v[i] == v[i] ? fminf(v[i], 3.402823466e38f) : -INFINITY;
+        // of three values with a NaN, med3 is the lesser of the others
+        v[i] = __builtin_amdgcn_fmed3f(v[i], lowest, 3.402823466e38f);
         top = fmaxf(top, v[i]);
     }
     L.top[t] = top == -INFINITY ? 0 : order32(top);
@@ -145,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void part_kernel(Params P) {
     }
     if (wave == 0) {
         const uint32_t T = reach(L.top, kThreads, P.n_out);
-        if (lane == 0) L.reach = T ? T : 1;
+        if (lane == 0) L.reach = T > 0x00800000u ? T : 0x00800000u;     // order32(-FLT_MAX)
     }
     __syncthreads();
     const int64_t slot = (int64_t)row * P.parts + part;
@@ -153,17 +159,28 @@ __global__ __launch_bounds__(kThreads) void part_kernel(Params P) {
         P.max[slot] = m;
         P.sum[slot] = (L.sum[0] + L.sum[1]) + (L.sum[2] + L.sum[3]);
     }
-    const uint32_t T = L.reach;
+    const float least = unorder32(L.reach);               // -FLT_MAX or more: no -inf
     const auto key = [&](int i) {
         const int token = base + (i / 4) * 4 * kThreads + 4 * t + i % 4;
         return (uint64_t)order32(v[i]) << 32 | (uint32_t)~token;
     };
+    uint64_t who[kPer];
+    int hits = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        if (v[i] != -INFINITY && order32(v[i]) >= T) {
-            const int at = atomicAdd(&L.n, 1);
-            if (at < kHold) L.hold[at] = key(i);
-        }
+        who[i] = __ballot(v[i] >= least);
+        hits += __popcll(who[i]);
+    }
+    int at = 0;
+    if (lane == 0 && hits) at = atomicAdd(&L.n, hits);
+    at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        if (who[i] == 0) continue;
+        const int mine = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(who[i] >> 32),
+                                 __builtin_amdgcn_mbcnt_lo((uint32_t)who[i], 0));
+        if (v[i] >= least && mine < kHold) L.hold[mine] = key(i);
+        at += __popcll(who[i]);
     }
     __syncthreads();
     const int found = L.n;
@@ -172,6 +189,7 @@ __global__ __launch_bounds__(kThreads) void part_kernel(Params P) {
         for (int i = t; i < found; i += kThreads) {
             const uint64_t mine = L.hold[i];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < found; ++j) rank += L.hold[j] > mine;
             if (rank < P.n_out) best[rank] = mine;
         }
@@ -208,76 +226,108 @@ struct Best {
     int beam;
 };
 __device__ __forceinline__ bool ahead(const Best& a, const Best& b) {
-    if (a.score != b.score) return a.score > b.score;
-    if (a.beam != b.beam) return a.beam < b.beam;
-    return a.key > b.key;
+    return (a.score > b.score) |
+           ((a.score == b.score) &
+            ((a.beam < b.beam) | ((a.beam == b.beam) & (a.key > b.key))));
 }
 
+// A group's candidates, the n_out best of every part of every beam: four a thread in
+// registers, all their loads in flight at once. More than that (many beams, parts or
+// outputs) are read once more.
+constexpr int kGroupThreads = 1024;
+constexpr int kGroupWaves = kGroupThreads / 64;
+constexpr int kGroupPer = 4;
 struct GroupLds {
     double lse[kMaxBeams];      // log of the sum of exp(x - max)
-    float max[kMaxBeams];
+    float max[kMaxBeams], score[kMaxBeams];
+    uint8_t kind[kMaxBeams];
     uint32_t top[kThreads];
-    uint64_t score[kHold], key[kHold];
+    uint64_t rank_score[kHold], key[kHold];
     uint8_t beam[kHold];
-    Best one[kWaves];
+    Best one[kGroupWaves];
     uint32_t reach;
     int n;
 };
+enum : uint8_t { kNothing, kItself, kTokens };
 
-__global__ __launch_bounds__(kThreads) void group_kernel(Params P) {
+__global__ __launch_bounds__(kGroupThreads) void group_kernel(Params P) {
     __shared__ GroupLds L;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int row0 = blockIdx.x * P.n_beams;
-    for (int b = wave; b < P.n_beams; b += kWaves) {
+    const int each = P.parts * P.n_out;
+    const int n = P.n_beams * each;
+    // beam of candidate i: i * per_beam >> 44, exact for i < 64 * each <= 2^24
+    const auto beam_of = [&](int i) { return (int)((uint64_t)(uint32_t)i * P.per_beam >> 44); };
+    const uint64_t* best = P.best + (int64_t)row0 * each;
+    uint64_t keys[kGroupPer];
+#pragma unroll
+    for (int k = 0; k < kGroupPer; ++k) {
+        const int i = t + k * kGroupThreads;
+        keys[k] = i < n ? ld_global(best + i) : 0;
+    }
+    for (int b = wave; b < P.n_beams; b += kGroupWaves) {
         const int row = row0 + b;
-        if ((P.finished && P.finished[row]) || !has_score(P.scores[row])) continue;
-        float m = -INFINITY;
-        for (int i = lane; i < P.parts; i += 64) m = fmaxf(m, P.max[(int64_t)row * P.parts + i]);
-        m = wave_max(m);
-        double s = 0.0;
-        if (m != -INFINITY)
-            for (int i = lane; i < P.parts; i += 64) {
-                const int64_t at = (int64_t)row * P.parts + i;
-                s += P.sum[at] * exp((double)P.max[at] - (double)m);
-            }
-        s = wave_sum64(s);
+        // (a beam that kept nothing has whatever is there for its maxima and sums: not used)
+        const float* max = P.max + (int64_t)row * P.parts;
+        const double* sum = P.sum + (int64_t)row * P.parts;
+        float own_max = lane < P.parts ? ld_global(max + lane) : -INFINITY;
+        double own_sum = lane < P.parts ? ld_global(sum + lane) : 0.0;
+        const float score = ld_global(P.scores + row);
+        const bool done = P.finished && P.finished[row];
+        for (int i = lane + 64; i < P.parts; i += 64) {
+            const float x = ld_global(max + i);
+            const double y = ld_global(sum + i);
+            const float both = fmaxf(own_max, x);
+            if (both != -INFINITY)
+                own_sum = own_sum * exp((double)own_max - (double)both) +
+                          y * exp((double)x - (double)both);
+            own_max = both;
+        }
+        const uint8_t kind = !has_score(score) ? kNothing : done ? kItself : kTokens;
+        const float m = wave_max(own_max);
+        const double s = wave_sum64(
+            own_max == -INFINITY ? 0.0 : own_sum * exp((double)own_max - (double)m));
         if (lane == 0) {
             L.lse[b] = log(s);
             L.max[b] = m;
+            L.score[b] = score;
+            L.kind[b] = kind;
         }
     }
     if (t == 0) L.n = 0;
+    if (t < kThreads) L.top[t] = 0;
     __syncthreads();
-    // candidate i of the group: beam i / each, the rest its part and place
-    const int each = P.parts * P.n_out;
-    const int64_t n = (int64_t)P.n_beams * each;
-    const auto candidate = [&](int64_t i) {
+    const auto candidate = [&](int i, uint64_t key) {
         Best c;
-        c.beam = (int)(i / each);
+        c.beam = beam_of(i);
+        c.key = key;
         c.score = 0;
-        const int row = row0 + c.beam;
-        const float score = P.scores[row];
-        c.key = 0;
-        if (!has_score(score)) return c;
-        if (P.finished && P.finished[row]) {
-            if (i % each == 0) {
-                c.key = 1ull << 63 | (uint32_t)~(P.eos < 0 ? -1 : P.eos);
-                c.score = order64((double)score);
-            }
-            return c;
+        const uint8_t kind = L.kind[c.beam];
+        const double score = (double)L.score[c.beam];
+        if (kind == kItself && i == c.beam * each) {
+            c.key = 1ull << 63 | (uint32_t)~(P.eos < 0 ? -1 : P.eos);
+            c.score = order64(score);
+        } else if (kind == kTokens && key) {
+            const double x = unorder32((uint32_t)(key >> 32));
+            c.score = order64(score + ((x - (double)L.max[c.beam]) - L.lse[c.beam]));
         }
-        c.key = P.best[(int64_t)row * each + i % each];
-        if (c.key == 0) return c;
-        const double x = unorder32((uint32_t)(c.key >> 32));
-        c.score = order64((double)score + ((x - (double)L.max[c.beam]) - L.lse[c.beam]));
         return c;
     };
-    Best mine{0, 0, 0};
-    for (int64_t i = t; i < n; i += kThreads) {
-        const Best c = candidate(i);
-        if (c.score > mine.score) mine = c;
+    Best held[kGroupPer];
+    uint64_t high = 0;
+#pragma unroll
+    for (int k = 0; k < kGroupPer; ++k) {
+        const int i = t + k * kGroupThreads;
+        held[k] = i < n ? candidate(i, keys[k]) : Best{0, 0, 0};
+        high = held[k].score > high ? held[k].score : high;
     }
-    L.top[t] = (uint32_t)(mine.score >> 32);
+    constexpr int kHeld = kGroupPer * kGroupThreads;
+    for (int i = t + kHeld; i < n; i += kGroupThreads) {
+        const uint64_t s = candidate(i, ld_global(best + i)).score;
+        high = s > high ? s : high;
+    }
+    // (four threads share a word: reach() takes kThreads of them)
+    atomicMax(&L.top[t % kThreads], (uint32_t)(high >> 32));
     __syncthreads();
     if (wave == 0) {
         const uint32_t T = reach(L.top, kThreads, P.n_out);
@@ -285,16 +335,18 @@ __global__ __launch_bounds__(kThreads) void group_kernel(Params P) {
     }
     __syncthreads();
     const uint32_t T = L.reach;
-    for (int64_t i = t; i < n; i += kThreads) {
-        const Best c = candidate(i);
-        if (c.score == 0 || (uint32_t)(c.score >> 32) < T) continue;
+    const auto hold = [&](const Best& c) {
+        if (c.score == 0 || (uint32_t)(c.score >> 32) < T) return;
         const int at = atomicAdd(&L.n, 1);
         if (at < kHold) {
-            L.score[at] = c.score;
+            L.rank_score[at] = c.score;
             L.key[at] = c.key;
             L.beam[at] = (uint8_t)c.beam;
         }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < kGroupPer; ++k) hold(held[k]);
+    for (int i = t + kHeld; i < n; i += kGroupThreads) hold(candidate(i, ld_global(best + i)));
     __syncthreads();
     const auto put = [&](int k, const Best& c) {
         const int64_t at = (int64_t)blockIdx.x * P.n_out + k;
@@ -304,25 +356,27 @@ __global__ __launch_bounds__(kThreads) void group_kernel(Params P) {
         P.parents[at] = there ? row : -1;
         P.tokens[at] = there ? token : -1;
         if (P.out_finished)
-            P.out_finished[at] = there && ((P.finished && P.finished[row]) ||
+            P.out_finished[at] = there && (L.kind[c.beam] == kItself ||
                                            (P.eos >= 0 && token == P.eos));
     };
     const int found = L.n;
     if (found <= kHold) {
-        for (int i = t; i < found; i += kThreads) {
-            const Best c{L.score[i], L.key[i], L.beam[i]};
+        for (int i = wave; i < found; i += kGroupWaves) {
+            const Best c{L.rank_score[i], L.key[i], L.beam[i]};
             int rank = 0;
-            for (int j = 0; j < found; ++j) rank += ahead(Best{L.score[j], L.key[j], L.beam[j]}, c);
-            if (rank < P.n_out) put(rank, c);
+            for (int j = lane; j - lane < found; j += 64)
+                rank += __popcll(__ballot(
+                    j < found && ahead(Best{L.rank_score[j], L.key[j], L.beam[j]}, c)));
+            if (lane == 0 && rank < P.n_out) put(rank, c);
         }
-        for (int i = found + t; i < P.n_out; i += kThreads) put(i, Best{0, 0, 0});
+        for (int i = found + t; i < P.n_out; i += kGroupThreads) put(i, Best{0, 0, 0});
         return;
     }
     Best last{~0ull, ~0ull, -1};
     for (int k = 0; k < P.n_out; ++k) {
         Best top{0, 0, kMaxBeams};
-        for (int64_t i = t; i < n; i += kThreads) {
-            const Best c = candidate(i);
+        for (int i = t; i < n; i += kGroupThreads) {
+            const Best c = candidate(i, ld_global(best + i));
             if (c.score != 0 && ahead(last, c) && ahead(c, top)) top = c;
         }
 #pragma unroll
@@ -335,8 +389,9 @@ __global__ __launch_bounds__(kThreads) void group_kernel(Params P) {
         __syncthreads();
         last = L.one[0];
 #pragma unroll
-        for (int i = 1; i < kWaves; ++i)
+        for (int i = 1; i < kGroupWaves; ++i)
             if (ahead(L.one[i], last)) last = L.one[i];
+        if (last.score == 0) last.beam = 0;
         if (t == 0) put(k, last);
         __syncthreads();
     }
@@ -409,8 +464,10 @@ extern "C" int fleet_beam_select(const float* logits, int64_t ld, const float* s
     P.vocab = vocab;
     P.parts = l.parts;
     P.eos = eos;
+    P.per_beam = ((uint64_t)1 << 44) / ((uint64_t)l.parts * n_out) + 1;
     hipLaunchKernelGGL(beam::part_kernel, dim3(l.parts, n_groups * n_beams), dim3(beam::kThreads),
                        0, stream, P);
-    hipLaunchKernelGGL(beam::group_kernel, dim3(n_groups), dim3(beam::kThreads), 0, stream, P);
+    hipLaunchKernelGGL(beam::group_kernel, dim3(n_groups), dim3(beam::kGroupThreads), 0, stream,
+                       P);
     return (int)hipGetLastError();
 }
