@@ -613,6 +613,21 @@ struct Shares {
 // units ended later).
 constexpr int kSetup = 6;
 
+// How many shares. A share of few steps is short, but each is a part to join: n steps
+// of a unit in parts of m take some m + n / 16 m of a step, least where m is a
+// quarter of n's root. One workgroup a CU, two where each has 4 steps or more of its
+// own (shorter ones wait for each other's first copies). Measured over 27 layers in
+// turn, against 512 shares wherever there are as many steps: one sequence of 16,384
+// positions 20 and 35 us, of 65,536 29 and 40; 16 of 1,000 16.9 and 21.4; 8 of 4,100
+// 22.5 and 25.7 (with another workspace for every call 22.3 and 21); 64 of 1,500 the
+// same 30.1, with one workgroup a CU 31.6.
+__device__ __forceinline__ int shares_of(int total, int steps, int units, int most) {
+    const int least = (int)(sqrtf((float)steps / (float)units) * 0.25f);
+    if (steps < 4 * kShares && most > kShares / 2) most = kShares / 2;
+    if (least > 1) total = (total + least - 1) / least;
+    return total < most ? total : most;
+}
+
 // The total of all units' steps; its division (no share is empty: the join counts
 // on it); and the unit in which workgroup wg's part begins, and where. Every
 // wave for itself, a lane per sequence (or for several, then once more a lane for each
@@ -639,7 +654,7 @@ __device__ __forceinline__ bool locate(const AttendParams& P, int wg, Work& w, P
     n += at.setup * units;
     incl = wave_incl_scan(n);
     at.total = lane_of(incl, 63);
-    at.shares = at.total < P.shares ? at.total : P.shares;
+    at.shares = shares_of(at.total, plain, lane_of(wave_incl_scan(units), 63), P.shares);
     if (wg >= at.shares) return false;
     int off = Shares(at.total, at.shares).first(wg);
     int owner = __popcll(__ballot(incl <= off));

@@ -369,6 +369,22 @@ def test_attention(case):
     assert torch.equal(o, out) and torch.equal(e, lse)
 
 
+@pytest.mark.parametrize("lens, counts, heads, window, sinks", [
+    # many parts of few rows, few parts of more rows, a bound far above the lengths,
+    # sequences of which only one is divided, a window and first positions
+    ([5000], [3], 16, 0, 0), ([1500], [40], 16, 0, 0), ([700, 3], [9, 3], 16, 0, 0),
+    ([2600, 40, 0], [20, 33, 2], 16, 0, 0), ([3000], [12], 5, 1500, 70), ([2049], [70], 1, 0, 0)])
+def test_attention_of_many_rows_in_parts(lens, counts, heads, window, sinks):
+    b, rng = filled(sum(lens) + heads, lens, max_pages=-(-max(lens) // 64) + 50)
+    q = ref.bf16(rng.normal(size=(sum(counts), heads, ref.ROW)) * 0.5)
+    say(f"lens {lens} new {counts} heads {heads} window {window} sinks {sinks}")
+    for bound in (max(lens), 0):
+        out, lse = b.dev.attend(to_dev(q), starts(counts), window=window, sinks=sinks,
+                                max_len=bound)
+        compare(b, q, counts, out, lse, window=window, sinks=sinks)
+    assert b.dev.status() == 0
+
+
 def test_attention_layers_strides_and_given_outputs():
     b, rng = filled(1, [90, 200], n_layers=3)
     q = ref.bf16(rng.normal(size=(5, 16, ref.ROW)))
