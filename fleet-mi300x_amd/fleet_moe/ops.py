@@ -12,6 +12,7 @@ inputs, and `route` is its router + top-k (:271-278). Errors are raised as
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 
 import numpy as np
@@ -70,6 +71,12 @@ def _on(device: torch.device):
     if device.index is None or device.index == torch.cuda.current_device():
         return _HERE
     return torch.cuda.device(device)
+
+
+def _own(stream):
+    """A context for the outputs of a call on `stream`: they belong to it, so that
+    their memory is not used again before its work is done."""
+    return _HERE if stream is None else torch.cuda.stream(stream)
 
 
 def _same_device(owner: torch.Tensor, **tensors) -> None:
@@ -433,21 +440,23 @@ class BeamSelector:
         if finished is not None:
             _need(finished, torch.uint8, (g, b), "finished")
         _same_device(self.workspace, logits=logits, scores=scores, finished=finished)
-        out = torch.empty((g, k), dtype=torch.float32, device=logits.device)
-        picks = torch.empty((2, g, k), dtype=torch.int32, device=logits.device)
-        ended = torch.empty((g, k), dtype=torch.uint8, device=logits.device)
+        with _own(stream):
+            out = torch.empty((g, k), dtype=torch.float32, device=logits.device)
+            parents, tokens = torch.empty((2, g, k), dtype=torch.int32,
+                                          device=logits.device).unbind(0)
+            ended = torch.empty((g, k), dtype=torch.uint8, device=logits.device)
         with _on(self.workspace.device):
             rc = _lib.load().fleet_beam_select(
                 _ptr(logits), max(int(logits.stride(0)), self.vocab), _ptr(scores),
-                _ptr(finished), g, b, k, self.vocab, self.eos, _ptr(out), picks.data_ptr(),
-                picks.data_ptr() + 4 * g * k, _ptr(ended), _ptr(self.workspace),
-                self.workspace.numel(), _stream(stream))
+                _ptr(finished), g, b, k, self.vocab, self.eos, _ptr(out), _ptr(parents),
+                _ptr(tokens), _ptr(ended), _ptr(self.workspace), self.workspace.numel(),
+                _stream(stream))
         _lib.check(rc, "fleet_beam_select")
-        return {"scores": out, "parents": picks[0], "tokens": picks[1], "finished": ended}
+        return {"scores": out, "parents": parents, "tokens": tokens, "finished": ended}
 
 
 class Decoder:
-    """Batch-1 greedy decode of the whole model on the GPU.
+    """Batch-1 greedy decode of the whole model on the GPU (and beam_search()).
 
     `blob` is the packed uint8 device tensor of `layout`
     (fleet_moe.layout.model_layout). Per token (reference_decode.py:294-302
@@ -609,6 +618,73 @@ class Decoder:
             self.step()
             out[j:j + 1].copy_(self.token_out)
         return out
+
+    def beam_search(self, tokens: torch.Tensor, n_beams: int, n_steps: int, eos: int = -1):
+        """The n_beams best continuations of the prompt `tokens` (device int32 [n]) by
+        n_steps tokens, or up to `eos` (which then fills the rest). Returns
+        (int32 [n_beams, n_steps], scores fp32 [n_beams]: sums of log
+        probabilities), best first. The beams' caches are pages of 8-bit rows
+        (PagedCache), shared as far as the beams agree; every step reads a beam's
+        rows into `cache`, so that the rest of the decoder's state (cache, token,
+        pos, x) is afterwards that of the last step. Synchronises once a step."""
+        from .layout import VOCAB
+        from .paged import PAGE, PagedCache
+        n, dev = tokens.numel(), self.blob.device
+        if tokens.dim() != 1 or n < 1 or n_steps < 1 or n + n_steps - 1 > self.max_pos:
+            raise ValueError(f"a prompt [n] and {n_steps} steps must take 1 to {self.max_pos} "
+                             f"positions: got {tuple(tokens.shape)}")
+        select = BeamSelector(1, n_beams, eos=eos, device=dev)
+        n_max = -(-(n + n_steps - 1) // PAGE)
+        shared = n // PAGE
+        pages = PagedCache.empty(shared + n_beams * (n_max - shared + 1), n_beams, n_max,
+                                 self.n_layers, dev)
+        i32 = dict(dtype=torch.int32, device=dev)
+        self.prefill(tokens)
+        # the prompt into the first beam, and the others its heirs
+        first = torch.zeros(n_beams, **i32)
+        ones = torch.ones(n_beams, **i32)
+        count = first.clone()
+        count[0] = n
+        start = torch.full((n_beams + 1,), n, **i32)
+        start[0] = 0
+        pages.grow(count)
+        pages.append(self.cache[:, :n], start)
+        pages.remap(first)
+        logits = torch.zeros((n_beams, VOCAB), dtype=torch.float32, device=dev)
+        self.attn.lm_head_into(self.x, self._addr("final_norm"), self._addr("lm_head"), logits[0],
+                               self.token_out)
+        scores = torch.full((1, n_beams), -math.inf, device=dev)
+        scores[0, 0] = 0.0
+        finished = torch.zeros((1, n_beams), dtype=torch.uint8, device=dev)
+        found = torch.zeros((n_beams, n_steps), **i32)
+        rows = torch.empty((self.n_layers, n_beams, 576), dtype=torch.int16, device=dev)
+        for step in range(n_steps):
+            at = n + step - 1           # the row of the last picks
+            if step:
+                for b in range(n_beams):
+                    start.fill_(at)
+                    start[:b + 1] = 0
+                    pages.read(self.cache[:, :at], start)
+                    self.reset(at)
+                    self.token.copy_(found[b, step - 1:step])
+                    self.enqueue_step(logits[b], feed_back=False)
+                    rows[:, b].copy_(self.cache[:, at])
+                pages.grow(ones)
+                pages.append(rows)
+            best = select.select(logits, scores, finished)
+            # (a beam without a score, where too few tokens have one, repeats the first)
+            parents = best["parents"][0].clamp(min=0)
+            pages.remap(parents)
+            found = found[parents.long()]
+            found[:, step] = best["tokens"][0].clamp(min=0)
+            scores, finished = best["scores"], best["finished"]
+            if eos >= 0 and bool(finished.all()):
+                found[:, step:] = eos
+                break
+        st = pages.status() | self.status()
+        if st:
+            raise RuntimeError(f"beam_search: status 0x{st:x}")
+        return found, scores[0]
 
     def status(self) -> int:
         st = self.attn.status() | self.ffn.status()

@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib
-from .ops import _need, _on, _ptr, _same_device, _stream
+from .ops import _need, _on, _own, _ptr, _same_device, _stream
 
 ROW = _lib.CACHE_ROW
 LORA = 512
@@ -93,7 +93,8 @@ class PagedCache:
 
     def compact(self, stream=None) -> torch.Tensor:
         """Moves the used pages to the front; returns their number, int32 [1]."""
-        used = torch.empty(1, dtype=torch.int32, device=self.device)
+        with _own(stream):
+            used = torch.empty(1, dtype=torch.int32, device=self.device)
         self._call("fleet_cache_compact", _ptr(used), stream=stream)
         return used
 
@@ -151,11 +152,13 @@ class PagedCache:
                              f"contiguous heads, got {q.dtype} {tuple(q.shape)}")
         n, heads = int(q.shape[0]), int(q.shape[1])
         if out is None:
-            out = torch.empty((n, heads, LORA), dtype=torch.int16, device=q.device)
+            with _own(stream):
+                out = torch.empty((n, heads, LORA), dtype=torch.int16, device=q.device)
         else:
             _need(out, torch.int16, (n, heads, LORA), "out")
         if lse is None:
-            lse = torch.empty((n, heads), dtype=torch.float32, device=q.device)
+            with _own(stream):
+                lse = torch.empty((n, heads), dtype=torch.float32, device=q.device)
         else:
             _need(lse, torch.float32, (n, heads), "lse")
         if n == 0:
