@@ -89,7 +89,7 @@ __device__ __forceinline__ void open_seq(const AttendParams& P, int seq, Work& w
     w.row0 = 0;
     w.tok0 = a;
     w.n_new = z > a ? z - a : 0;
-    w.rows = w.n_new * P.n_heads;
+    w.rows = z < a ? -1 : w.n_new * P.n_heads;            // -1: not a start at all
     w.len = checked_len(ld_global(P.c.lens + seq), P.c.max_pages);
 }
 
@@ -588,13 +588,23 @@ __device__ __forceinline__ bool locate(const AttendParams& P, int wg, Work& w, P
     const int each = (P.c.n_seqs + 63) / 64;
     Work mine{};
     int n = 0, units = 0;
+    bool bad = false;
     for (int i = 0; i < each; ++i) {
         const int s = lane * each + i;
         if (s < P.c.n_seqs) {
             open_seq(P, s, mine);
+            bad |= mine.rows < 0;
             n += seq_steps(P, mine);
             units += (mine.rows + kFew - 1) / kFew;
         }
+    }
+    // starts that decrease: more rows than there are, nothing is done
+    if (__ballot(bad)) {
+        if (wg == 0) {
+            for (int i = threadIdx.x; i < P.units; i += kThreads) P.meta[i] = make_int4(0, 0, 0, 0);
+            if (threadIdx.x == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
+        }
+        return false;
     }
     int incl = wave_incl_scan(n);
     const int plain = lane_of(incl, 63);
@@ -729,7 +739,7 @@ __device__ __forceinline__ bool find_work(const AttendParams& P, int64_t u, Work
     if (seq < 0) return false;
     open_seq(P, seq, w);
     const int64_t r = (u - first_unit(w.tok0, seq, P.n_heads, R, P.pad)) * R;
-    if (r >= w.rows) return false;
+    if (r < 0 || r >= w.rows) return false;
     w.row0 = (int)r;
     see<R, S>(P, w);
     return true;
@@ -741,9 +751,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams P) 
     int64_t to = u * kFew + row;                // where units follow each other without gaps
     const int4 m = P.meta[u];
     if (P.pad == 0) {
-        const int tokens = P.start ? clamp_row(ld_global(P.start + P.c.n_seqs), P.n_tokens)
-                                   : P.n_tokens;
-        if (to >= (int64_t)tokens * P.n_heads) return;
+        // (what is not between the first and the last start is no unit of this call)
+        const int a = P.start ? clamp_row(ld_global(P.start), P.n_tokens) : 0;
+        const int z = P.start ? clamp_row(ld_global(P.start + P.c.n_seqs), P.n_tokens)
+                              : P.n_tokens;
+        if (to < (int64_t)a * P.n_heads || to >= (int64_t)z * P.n_heads) return;
     } else {
         Work w;
         if (!find_work<kFew, kStep>(P, u, w) || w.row0 + row >= w.rows) return;

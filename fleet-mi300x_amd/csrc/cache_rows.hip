@@ -38,7 +38,7 @@ __device__ __forceinline__ bool block_at(const RowParams& P, BlockAt& b) {
     if (b.seq < 0) return false;
     const int a = P.start ? clamp_row(P.start[b.seq], P.n_rows) : b.seq;
     const int z = P.start ? clamp_row(P.start[b.seq + 1], P.n_rows) : b.seq + 1;
-    if (z <= a) return false;
+    if (z <= a || u < first_unit(a, b.seq, 1, kBlock, 2)) return false;
     b.len = checked_len(c.lens[b.seq], c.max_pages);
     b.first = b.len - (z - a);
     b.row0 = a;
@@ -205,7 +205,10 @@ static int rows_call(bool append, const fleet_cache* cache, int32_t layer0, int3
     if (!rows || (uintptr_t)rows % 16 || row_stride < kRow || row_stride % 8 ||
         row_stride > ((int64_t)1 << 32) || layer_stride % 8 || layer_stride < 0 ||
         layer_stride > ((int64_t)1 << 48) ||
-        (n_layers > 1 && layer_stride < (int64_t)(n_rows - 1) * row_stride + kRow))
+        (n_layers > 1 && layer_stride < kRow) ||
+        // rows of a layer behind each other, or the layers of a row
+        (n_layers > 1 && layer_stride < (int64_t)(n_rows - 1) * row_stride + kRow &&
+         row_stride < (int64_t)(n_layers - 1) * layer_stride + kRow))
         return FLEET_MOE_ERR_ARG;
     if (int e = fleet_moe_check_device(1)) return e;
     RowParams P{};

@@ -422,9 +422,10 @@ int fleet_cache_compact(const fleet_cache* cache, int32_t* n_used, void* workspa
 /* Writes the newest positions of each sequence, of layers layer0 .. layer0 +
  * n_layers - 1. rows: bf16 [n_layers][n_rows][576], rows row_stride and layers
  * layer_stride elements apart (multiples of 8, so that a row is 16-byte
- * aligned). start: device int32[n_seqs + 1], not decreasing, start[n_seqs] <=
+ * aligned; all rows of a layer before the next layer's, or all layers of a row before
+ * the next row's). start: device int32[n_seqs + 1], not decreasing, start[n_seqs] <=
  * n_rows: rows start[s] .. start[s + 1] - 1 are the last of the lens[s]
- * positions of sequence s; NULL: one row for each sequence (n_rows == n_seqs).
+ * positions of sequence s (rows before start[0] are nobody's); NULL: one row for each sequence (n_rows == n_seqs).
  * A block's scale is the least power of two that takes its new finite values
  * within the largest code, 448, and no less than the scale of older positions
  * in the block; where those have a smaller scale they are rounded again to the
@@ -440,8 +441,8 @@ int fleet_cache_append(const fleet_cache* cache, int32_t layer0, int32_t n_layer
 
 /* The reverse: rows receives the newest positions of each sequence as bf16 (the
  * values the codes stand for). Rows that name no position or a page outside the
- * pool (status as above), and those behind start[n_seqs], are left as they
- * were. */
+ * pool (status as above), and those before start[0] or behind start[n_seqs], are
+ * left as they were. */
 int fleet_cache_read(const fleet_cache* cache, int32_t layer0, int32_t n_layers, uint16_t* rows,
                      int64_t row_stride, int64_t layer_stride, const int32_t* start,
                      int32_t n_rows, void* workspace, size_t workspace_bytes,
@@ -458,8 +459,8 @@ int fleet_cache_read(const fleet_cache* cache, int32_t layer0, int32_t n_layers,
  * only the tokens that see it. Products are of bf16 values with fp32 sums; the
  * probabilities are rounded to bf16 before the second product. max_len: a bound
  * on lens that the host knows, for the division of the work (longer sequences
- * are still right), or 0. Outputs of tokens behind start[n_seqs] are left as
- * they were. A length outside the table sets FLEET_MOE_ABORT_POSITION, and the
+ * are still right), or 0. Outputs of tokens before start[0] or behind
+ * start[n_seqs] are left as they were. A length outside the table sets FLEET_MOE_ABORT_POSITION, and the
  * sequence's tokens see nothing; positions in a page outside the pool are not
  * seen, and set FLEET_MOE_ABORT_BAD_PAGE. 1 <= n_heads <= 128, n_tokens * n_heads
  * <= 2^26, 0 < scale. */

@@ -161,6 +161,74 @@ def test_rows_with_strides():
     assert (got[:, :3] == 0).all() and (got[:, 73:] == 0).all() and (got[..., ref.ROW:] == 0).all()
 
 
+def test_rows_of_all_layers_together():
+    """The layers of a position behind each other: [positions][layers][576]."""
+    rng = np.random.default_rng(8)
+    wide = torch.from_numpy(ref.bits(normal(rng, (40, 3, ref.ROW)))).cuda()
+    b = Both(4, 2, 2, 3)
+    assert b.grow([33, 7])
+    b.ref.append(ref.values(wide.transpose(0, 1).cpu().numpy()), [0, 33, 40])
+    b.dev.append(wide.transpose(0, 1), starts([33, 7]))
+    b.check()
+    out = torch.zeros_like(wide)
+    b.dev.read(out.transpose(0, 1), starts([33, 7]))
+    got = ref.values(out.cpu().numpy())
+    for k in range(3):
+        for s, (a, n) in enumerate(((0, 33), (33, 7))):
+            assert np.array_equal(got[a:a + n, k], b.ref.values(s, k).astype(np.float32))
+
+
+@pytest.mark.parametrize("heads, counts", [(16, [1, 1, 1]), (5, [1, 2, 1]), (16, [0, 1, 0]),
+                                           (16, [40, 0, 3]), (3, [70, 1, 30])])
+def test_rows_before_the_first_start(heads, counts):
+    """A batch whose first rows belong to no sequence, and so do its last."""
+    lens = [900, 64, 130]
+    b, rng = filled(heads + sum(counts), lens, max_pages=20)
+    lead, n = 7, sum(counts)
+    at = i32(lead + np.concatenate([[0], np.cumsum(counts)]))
+    q = ref.bf16(rng.normal(size=(n, heads, ref.ROW)) * 0.5)
+    wide = torch.full((lead + n + 2, heads, ref.ROW), 0x7fff, dtype=torch.int16, device="cuda")
+    wide[lead:lead + n] = to_dev(q)
+    out = torch.full((lead + n + 2, heads, 512), 0x55, dtype=torch.int16, device="cuda")
+    lse = torch.full((lead + n + 2, heads), 3.0, device="cuda")
+    say(f"heads {heads} counts {counts}")
+    for bound in (900, 0):
+        b.dev.attend(wide, at, max_len=bound, out=out, lse=lse)
+        compare(b, q, counts, out[lead:lead + n], lse[lead:lead + n])
+        for t, v in ((out, 0x55), (lse, 3.0)):
+            assert (t[:lead] == v).all() and (t[lead + n:] == v).all()
+    rows = torch.full((1, lead + n + 2, ref.ROW), 0x55, dtype=torch.int16, device="cuda")
+    b.dev.read(rows, at)
+    assert (rows[:, :lead] == 0x55).all() and (rows[:, lead + n:] == 0x55).all()
+    got, k = ref.values(rows.cpu().numpy())[0, lead:], 0
+    for s, c in enumerate(counts):
+        assert np.array_equal(got[k:k + c], b.ref.values(s)[lens[s] - c:].astype(np.float32))
+        k += c
+    assert b.dev.status() == 0
+
+
+def test_starts_that_decrease():
+    """Not allowed, and on the device: reported by the attention of few rows, which then
+    does nothing, and within bounds everywhere."""
+    lens = [300, 64, 130]
+    b, rng = filled(77, lens)
+    q = to_dev(ref.bf16(rng.normal(size=(6, 16, ref.ROW))))
+    out = torch.full((6, 16, 512), 0x55, dtype=torch.int16, device="cuda")
+    b.dev.attend(q, i32([0, 4, 1, 6]), out=out)
+    assert (out == 0x55).all() and b.dev.status() == _lib.ABORT_POSITION
+    big = to_dev(ref.bf16(rng.normal(size=(60, 16, ref.ROW))))
+    rows = torch.zeros((1, 60, ref.ROW), dtype=torch.int16, device="cuda")
+    for at in ([0, 50, 10, 60], [60, 0, 60, 0], [5, 5, 60, 1], [60, 40, 20, 0]):
+        say(f"starts {at}")
+        b.dev.attend(big, i32(at))
+        b.dev.attend(big[:6], i32(at))
+        b.dev.read(rows, i32(at))
+        torch.cuda.synchronize()
+    q = ref.bf16(rng.normal(size=(3, 16, ref.ROW)) * 0.5)
+    out, lse = b.dev.attend(to_dev(q))
+    compare(b, q, [1, 1, 1], out, lse)
+
+
 def test_one_row_each_without_start():
     rng = np.random.default_rng(6)
     b = Both(6, 5, 1, 1)
