@@ -29,8 +29,8 @@ ABORT_TOKEN = 0x10
 ABORT_ATTN_WAIT = 0x20
 ABORT_BAD_ID = 0x40
 ABORT_STEP_WAIT = 0x80
-ABORT_NO_PAGE = 0x100
-ABORT_BAD_PAGE = 0x200
+ABORT_NO_PAGE = 0x400
+ABORT_BAD_PAGE = 0x800
 
 CACHE_ROW = 576
 CACHE_PAGE_TOKENS = 64

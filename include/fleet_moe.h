@@ -513,8 +513,8 @@ int fleet_moe_workspace_status(const void* workspace, uint32_t* status, hipStrea
                                              was clamped into range (output unspecified) */
 #define FLEET_MOE_ABORT_STEP_WAIT 0x80u   /* fleet_decode_step: a stage's input residual
                                              (or an lm_head candidate) never arrived */
-#define FLEET_MOE_ABORT_NO_PAGE 0x100u    /* fleet_cache_grow: too few free pages */
-#define FLEET_MOE_ABORT_BAD_PAGE 0x200u   /* fleet_cache_*: a table entry outside the pool,
+#define FLEET_MOE_ABORT_NO_PAGE 0x400u    /* fleet_cache_grow: too few free pages */
+#define FLEET_MOE_ABORT_BAD_PAGE 0x800u   /* fleet_cache_*: a table entry outside the pool,
                                              or a shared page to be written */
 
 /* Diagnostic: reads `bytes` of device memory with the weight-streaming load

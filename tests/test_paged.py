@@ -4,6 +4,7 @@ share (compiled for the host), and the tests' own restatement."""
 from __future__ import annotations
 
 import ctypes
+import re
 import subprocess
 from pathlib import Path
 
@@ -213,3 +214,19 @@ def test_restated_pages():
     assert not c.grow([0, 0, 200])                           # wider than the table
     c.remap([-1, 1, 5])
     assert c.compact() == 2 and c.rows == [[], [0, 1], []]
+
+
+def test_status_bits_are_one_thing_each():
+    """The header's bits, and those that kernels keep to themselves."""
+    bits = {}
+    files = [ROOT / "include" / "fleet_moe.h"] + sorted((ROOT / "fleet-mi300x_amd" / "csrc").iterdir())
+    for f in files:
+        if f.suffix not in (".h", ".hip"):
+            continue
+        for name, v in re.findall(r"(FLEET_MOE_ABORT_\w+|kAbort\w+)\s*(?:=\s*)?(0x[0-9a-fA-F]+)u?\b",
+                                  f.read_text()):
+            bits.setdefault(name, int(v, 16))
+    assert {"FLEET_MOE_ABORT_NO_PAGE", "kAbortRouteMismatch"} <= set(bits)
+    assert len(set(bits.values())) == len(bits) and all(v & (v - 1) == 0 for v in bits.values())
+    for name in ("NO_PAGE", "BAD_PAGE", "POSITION", "BAD_ID"):
+        assert getattr(_lib, f"ABORT_{name}") == bits[f"FLEET_MOE_ABORT_{name}"]
