@@ -295,7 +295,9 @@ __device__ __forceinline__ float lse_of(float m, float sum) {
 }
 constexpr uint32_t kOnes = 0x3f803f80u;                   // bf16 1, 1
 
-// Pages of the next 64 steps, one per lane.
+// Pages of 64 steps, one per lane: the next ones, and the few before that a copy's
+// step is ahead of the one whose scores are finished.
+constexpr int kBehind = 4;
 struct Pages {
     int held, from;
     int page;
@@ -304,11 +306,13 @@ template <int S>
 __device__ __forceinline__ int page_of(const AttendParams& P, const Work& w, Pages& h, int i,
                                        int end, int lane) {
     if (i >= h.held) {
-        h.from = i;
-        h.held = i + 64;
-        h.page = i + lane < end ? ld_global(P.c.table + (int64_t)w.seq * P.c.max_pages +
-                                            step_of<S>(w, i + lane) * S / kPage)
-                                : 0;
+        h.from = i - kBehind;
+        h.held = h.from + 64;
+        const int mine = h.from + lane;
+        h.page = mine >= 0 && mine < end
+                     ? ld_global(P.c.table + (int64_t)w.seq * P.c.max_pages +
+                                 step_of<S>(w, mine) * S / kPage)
+                     : 0;
         // here, not at the use: there the compiler would wait, every step, for
         // whatever copies are in flight
         __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0)

@@ -537,6 +537,28 @@ def test_attention_with_bad_tables():
     assert (out[0] == 0).all() and torch.isneginf(l2[0]).all() and torch.equal(out[1], good[1])
 
 
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_attention_with_a_bad_page_far_into_a_share(tokens):
+    """One workgroup walks the whole sequence (the bound says it is short), looks its
+    pages up 64 steps at a time, and sees every page that is none."""
+    n = 4500
+    b, rng = filled(21 + tokens, [n])
+    q = ref.bf16(rng.normal(size=(tokens, 16, ref.ROW)) * 0.5)
+    rows = b.ref.values(0)
+    table = b.dev.table.clone()
+    for bad in (0, 29, 30, 31, 32, 33, 61, 62, 63, 64, 65, 69):
+        say(f"tokens {tokens} page {bad}")
+        b.dev.table.copy_(table)
+        b.dev.table[0, bad] = b.dev.n_pages + 3
+        out, lse = b.dev.attend(to_dev(q), starts([tokens]), max_len=1)
+        good = np.concatenate([rows[:bad * 64], rows[bad * 64 + 64:]])
+        want, wl, tol, tl = ref.attend(good, q, range(len(good) - tokens, len(good)), SCALE)
+        assert (np.abs(ref.values(out.cpu().numpy()) - want) <= tol).all(), bad
+        assert (np.abs(lse.cpu().numpy() - wl) <= tl).all(), bad
+        assert b.dev.status() == _lib.ABORT_BAD_PAGE
+        b.dev.workspace[:256].zero_()
+
+
 def test_offsets_beyond_32_bits():
     """A pool of 5 GB: rows and attention in its last pages and layer."""
     layers, pages = 27, 5100
