@@ -184,3 +184,21 @@ def test_a_server_of_beams(seed):
     used = want.compact()
     assert int(dev.compact().item()) == used
     assert np.array_equal(dev.table.cpu().numpy(), want.table())
+
+
+def test_search_up_to_the_last_position(decoder):
+    check(decoder, MAX_POS - 3, 2, 4)
+
+
+def test_search_of_a_decoder_with_separate_launches(decoder):
+    """The same tokens and scores, also where steps are replayed from a graph, and from
+    a prompt on the host or in 64 bits."""
+    want = decoder.beam_search(prompt_of(30), 3, 4)
+    other = ops.Decoder(decoder.blob, decoder.layout, DSV2_LITE, max_pos=MAX_POS, fused=False)
+    for p in (prompt_of(30), prompt_of(30).cpu(), prompt_of(30).long()):
+        got = other.beam_search(p, 3, 4)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    other.capture()
+    got = other.beam_search(prompt_of(30), 3, 4)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert other.status() == 0
