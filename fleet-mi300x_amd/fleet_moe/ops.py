@@ -80,9 +80,10 @@ def _own(stream):
 
 
 def _same_device(owner: torch.Tensor, **tensors) -> None:
+    dev = owner.device
     for name, t in tensors.items():
-        if t is not None and t.device != owner.device:
-            raise ValueError(f"{name} is on {t.device}, not on {owner.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, not on {dev}")
 
 
 @dataclass
@@ -441,9 +442,9 @@ class BeamSelector:
             _need(finished, torch.uint8, (g, b), "finished")
         _same_device(self.workspace, logits=logits, scores=scores, finished=finished)
         with _own(stream):
-            out = torch.empty((g, k), dtype=torch.float32, device=logits.device)
-            parents, tokens = torch.empty((2, g, k), dtype=torch.int32,
-                                          device=logits.device).unbind(0)
+            out, parents, tokens = torch.empty((3, g, k), dtype=torch.int32,
+                                               device=logits.device).unbind(0)
+            out = out.view(torch.float32)
             ended = torch.empty((g, k), dtype=torch.uint8, device=logits.device)
         with _on(self.workspace.device):
             rc = _lib.load().fleet_beam_select(

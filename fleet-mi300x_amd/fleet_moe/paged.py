@@ -62,6 +62,9 @@ class PagedCache:
         # only the status word has to start as zero
         self.workspace = torch.empty(n, dtype=torch.uint8, device=self.device)
         self.workspace[:256].zero_()
+        self._ws = (self.workspace.data_ptr(), n)
+        self._fn = {name: getattr(_lib.load(), name) for name, *_ in _lib.SYMBOLS
+                    if name.startswith("fleet_cache_")}
 
     @classmethod
     def empty(cls, n_pages: int, n_seqs: int, max_pages: int, n_layers: int,
@@ -73,9 +76,9 @@ class PagedCache:
 
     def _call(self, name: str, *args, stream=None) -> None:
         with _on(self.device):
-            rc = getattr(_lib.load(), name)(self._ref, *args, self.workspace.data_ptr(),
-                                            self.workspace.numel(), _stream(stream))
-        _lib.check(rc, name)
+            rc = self._fn[name](self._ref, *args, *self._ws, _stream(stream))
+        if rc:
+            _lib.check(rc, name)
 
     def remap(self, parents: torch.Tensor, stream=None) -> None:
         """Sequence i becomes what sequence parents[i] (int32 [n_seqs]) was, or empty
@@ -150,22 +153,23 @@ class PagedCache:
                 or (q.numel() and (q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != ROW)))):
             raise ValueError(f"q: expected device int16 (bf16 bits) [tokens][heads][{ROW}] with "
                              f"contiguous heads, got {q.dtype} {tuple(q.shape)}")
-        n, heads = int(q.shape[0]), int(q.shape[1])
-        if out is None:
-            with _own(stream):
-                out = torch.empty((n, heads, LORA), dtype=torch.int16, device=q.device)
-        else:
+        n, heads = q.shape[0], q.shape[1]
+        if out is not None:
             _need(out, torch.int16, (n, heads, LORA), "out")
-        if lse is None:
-            with _own(stream):
-                lse = torch.empty((n, heads), dtype=torch.float32, device=q.device)
-        else:
+        if lse is not None:
             _need(lse, torch.float32, (n, heads), "lse")
+        if n:
+            self._check_start(start, n)
+        _same_device(self.pool, q=q, start=start, out=out, lse=lse)
+        if out is None or lse is None:
+            with _own(stream):
+                if out is None:
+                    out = torch.empty((n, heads, LORA), dtype=torch.int16, device=self.device)
+                if lse is None:
+                    lse = torch.empty((n, heads), dtype=torch.float32, device=self.device)
         if n == 0:
             return out, lse
-        self._check_start(start, n)
-        _same_device(self.pool, q=q, start=start, out=out, lse=lse)
-        stride = int(q.stride(0)) if n > 1 else heads * ROW
+        stride = q.stride(0) if n > 1 else heads * ROW
         self._call("fleet_cache_attend", int(layer), _ptr(q), stride, _ptr(start), n, heads,
                    int(max_len), int(window), int(sinks), float(scale), _ptr(out), _ptr(lse),
                    stream=stream)
