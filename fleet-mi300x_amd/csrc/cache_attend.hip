@@ -736,6 +736,61 @@ __device__ __forceinline__ void join(const AttendParams& P, int64_t row_at, int 
     if (P.lse && threadIdx.x == 0) P.lse[row_at] = lse_of(top, sum);
 }
 
+// The same by one wave, kJoinWave parts at a time: enough where a row has hardly more, and
+// four rows share a workgroup. (96 units of two parts joined by a workgroup a row, 6,144
+// of them, four for each place on the chip: 22 us; by a wave a row 6.)
+constexpr int kJoinWave = 16, kWaveParts = 16;
+template <int R>
+__device__ __forceinline__ void join_wave(const AttendParams& P, int64_t row_at, int row,
+                                          int64_t slot0, int64_t rest, int64_t step, int count) {
+    const int lane = threadIdx.x & 63;
+    const auto slot = [&](int i) { return (i == 0 ? slot0 : rest + (i - 1) * step) * R + row; };
+    f32x4 v[kJoinWave][2];
+    const auto load = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < kJoinWave; ++i) {
+            if (i0 + i >= count) break;
+            const f32x4* at = reinterpret_cast<const f32x4*>(P.part + slot(i0 + i) * kC) + lane;
+            v[i][0] = ld_global(at);
+            v[i][1] = ld_global(at + 64);
+        }
+    };
+    load(0);
+    float top = -INFINITY;
+    for (int i = lane; i < count; i += 64) top = fmaxf(top, ld_global(P.stat + slot(i))[0]);
+    top = wave_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float f = 0.f, sum = 0.f, rounded = 0.f;
+    f32x4 o[2]{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int i0 = 0;;) {
+        if (i0 % 64 == 0) {                     // the weights of 64 parts, a lane each
+            f32x4 st{-INFINITY, 0.f, 0.f, 0.f};
+            if (i0 + lane < count) st = ld_global(P.stat + slot(i0 + lane));
+            f = exp2_(st[0] - ref);
+            sum += f * st[1];
+            rounded += f * st[2];
+        }
+#pragma unroll
+        for (int i = 0; i < kJoinWave; ++i) {
+            if (i0 + i >= count) break;
+            const float weight = __builtin_bit_cast(
+                float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i0 % 64 + i));
+            o[0] += v[i][0] * weight;
+            o[1] += v[i][1] * weight;
+        }
+        i0 += kJoinWave;
+        if (i0 >= count) break;
+        load(i0);
+    }
+    static_assert(64 % kJoinWave == 0, "");
+    sum = wave_sum(sum);
+    rounded = wave_sum(rounded);
+    const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
+    put(P.out + row_at * kC + 4 * lane, o[0], inv);
+    put(P.out + row_at * kC + 4 * lane + 256, o[1], inv);
+    if (P.lse && lane == 0) P.lse[row_at] = lse_of(top, sum);
+}
+
 // The unit of number u, if there is one.
 template <int R, int S>
 __device__ __forceinline__ bool find_work(const AttendParams& P, int64_t u, Work& w) {
@@ -749,9 +804,11 @@ __device__ __forceinline__ bool find_work(const AttendParams& P, int64_t u, Work
     return true;
 }
 
-__global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams P) {
-    const int64_t u = blockIdx.x / kFew;
-    const int row = blockIdx.x % kFew;
+template <bool kWave>
+__global__ __launch_bounds__(kWave ? 256 : kJoinThreads) void join_few_kernel(AttendParams P) {
+    constexpr int kRows = kWave ? 4 : 1;
+    const int64_t u = blockIdx.x / (kFew / kRows);
+    const int row = blockIdx.x % (kFew / kRows) * kRows + (kWave ? wave_bcast(threadIdx.x >> 6) : 0);
     int64_t to = u * kFew + row;                // where units follow each other without gaps
     const int4 m = P.meta[u];
     if (P.pad == 0) {
@@ -765,7 +822,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams P) 
         if (!find_work<kFew, kStep>(P, u, w) || w.row0 + row >= w.rows) return;
         to = out_row(P, w, w.row0 + row);
     }
-    if (m.z > 1) join<kFew>(P, to, row, m.x, 2 * (int64_t)m.y, 2, m.z);
+    if (m.z <= 1) return;
+    if constexpr (kWave) join_wave<kFew>(P, to, row, m.x, 2 * (int64_t)m.y, 2, m.z);
+    else join<kFew>(P, to, row, m.x, 2 * (int64_t)m.y, 2, m.z);
 }
 
 // ---------------------------------------------------------------- many rows
@@ -1052,54 +1111,19 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     }
 }
 
-// The parts of a row, in order: a workgroup per row, or a wave per row where there are
-// so few parts that one has them all on their way at once. (96 units of two parts
-// joined by 6,144 workgroups: 22 us, four for each place on the chip, one after the other.)
-constexpr int kJoinWave = 8;
 template <bool kWave>
 __global__ __launch_bounds__(kWave ? 256 : kJoinThreads) void join_many_kernel(AttendParams P) {
     constexpr int kRows = kWave ? 4 : 1;
     const int64_t u = blockIdx.x / (kMany / kRows);
+    const int row = blockIdx.x % (kMany / kRows) * kRows + (kWave ? wave_bcast(threadIdx.x >> 6) : 0);
     Work w;
-    if (!find_work<kMany, kPage>(P, u, w)) return;
-    const int wave = wave_bcast(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int row = blockIdx.x % (kMany / kRows) * kRows + (kWave ? wave : 0);
-    if (w.row0 + row >= w.rows) return;
+    if (!find_work<kMany, kPage>(P, u, w) || w.row0 + row >= w.rows) return;
     const int each = (w.n + P.shares - 1) / P.shares;
     if (each >= w.n) return;
     const int count = (w.n + each - 1) / each;
-    const int64_t to = out_row(P, w, w.row0 + row);
-    if constexpr (!kWave) {
-        join<kMany>(P, to, row, u * P.shares, u * P.shares + 1, 1, count);
-        return;
-    }
-    const int64_t first = u * P.shares * kMany + row;
-    f32x4 v[kJoinWave][2];
-#pragma unroll
-    for (int i = 0; i < kJoinWave; ++i) {
-        if (i >= count) break;
-        const f32x4* at = reinterpret_cast<const f32x4*>(P.part + (first + i * kMany) * kC) + lane;
-        v[i][0] = ld_global(at);
-        v[i][1] = ld_global(at + 64);
-    }
-    f32x4 st{-INFINITY, 0.f, 0.f, 0.f};
-    if (lane < count) st = ld_global(P.stat + first + lane * kMany);
-    const float top = wave_max(st[0]);
-    const float f = top == -INFINITY ? 0.f : exp2_(st[0] - top);
-    const float sum = wave_sum(f * st[1]), rounded = wave_sum(f * st[2]);
-    f32x4 o[2]{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-    for (int i = 0; i < kJoinWave; ++i) {
-        if (i >= count) break;
-        const float weight = __builtin_bit_cast(
-            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
-        o[0] += v[i][0] * weight;
-        o[1] += v[i][1] * weight;
-    }
-    const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
-    put(P.out + to * kC + 4 * lane, o[0], inv);
-    put(P.out + to * kC + 4 * lane + 256, o[1], inv);
-    if (P.lse && lane == 0) P.lse[to] = lse_of(top, sum);
+    const int64_t to = out_row(P, w, w.row0 + row), first = u * P.shares;
+    if constexpr (kWave) join_wave<kMany>(P, to, row, first, first + 1, 1, count);
+    else join<kMany>(P, to, row, first, first + 1, 1, count);
 }
 
 }  // namespace cache
@@ -1176,7 +1200,11 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
         const int64_t steps = few * ((seen + kStep - 1) / kStep);
         P.shares = (int)(steps < kShares ? steps : kShares);
         if (int e = launch(few_kernel, P.shares, kThreads, sizeof(FewLds), P, stream)) return e;
-        return launch(join_few_kernel, few * kFew, kJoinThreads, 0, P, stream);
+        // A wave a row where the mean is up to 16 parts (64 sequences of 4,000 positions 42
+        // to 41 us, of 1,000 25.4 to 23.9; 16 of 1,000 the same), a workgroup a row for more.
+        if (P.shares <= kWaveParts * few)
+            return launch(join_few_kernel<true>, few * (kFew / 4), 256, 0, P, stream);
+        return launch(join_few_kernel<false>, few * kFew, kJoinThreads, 0, P, stream);
     }
     P.pad = n_heads % kMany != 0;
     const int64_t units = first_unit(n_tokens, cache->n_seqs, n_heads, kMany, P.pad);
@@ -1192,7 +1220,8 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     P.shares = (int)splits;
     if (int e = launch(many_kernel, units * P.shares, kManyThreads, sizeof(ManyLds), P, stream)) return e;
     if (P.shares == 1) return 0;
-    if (P.shares <= kJoinWave)
+    // (the same to a few percent from 4 parts to 16: 45.7 to 46.5 us of 8,192 positions)
+    if (P.shares <= kWaveParts)
         return launch(join_many_kernel<true>, units * (kMany / 4), 256, 0, P, stream);
     return launch(join_many_kernel<false>, units * kMany, kJoinThreads, 0, P, stream);
 }

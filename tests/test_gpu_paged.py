@@ -453,6 +453,20 @@ def test_attention_of_many_rows_in_parts(lens, counts, heads, window, sinks):
     assert b.dev.status() == 0
 
 
+@pytest.mark.parametrize("lens, heads, window", [
+    ([9000] + [20] * 24, 16, 0), ([20] * 24 + [9000, 7], 5, 0), ([6000, 3000] + [1] * 20, 16, 0),
+    ([9000] * 2 + [20] * 24, 16, 7000)])
+def test_attention_of_one_long_sequence_among_short_ones(lens, heads, window):
+    """Few parts a sequence in the mean, and hundreds for one of them."""
+    b, rng = filled(len(lens) + heads, lens)
+    n = len(lens)
+    q = ref.bf16(rng.normal(size=(n, heads, ref.ROW)) * 0.5)
+    say(f"{n} sequences up to {max(lens)} heads {heads} window {window}")
+    out, lse = b.dev.attend(to_dev(q), window=window)
+    compare(b, q, [1] * n, out, lse, window=window)
+    assert b.dev.status() == 0
+
+
 def test_attention_layers_strides_and_given_outputs():
     b, rng = filled(1, [90, 200], n_layers=3)
     q = ref.bf16(rng.normal(size=(5, 16, ref.ROW)))
