@@ -5,8 +5,8 @@
 // workgroup per group: each beam's log sum, and the n_out best of what its parts
 // kept. Reading the logits bounds it (HBM for many beams; for few, the two
 // launches' latency). Measured, 102,400 logits a beam: 32 groups of 8 beams, 16
-// outputs each, 22 + 7 us (105 MB; the loads by themselves take 15.5); 4 beams,
-// 5.3 + 4.8. With 32 logits a thread the two take 22.8 + 6.1 us: the same.
+// outputs each, 20 + 7 us (105 MB; the loads by themselves take 15.5); 4 beams,
+// 5.2 + 4.8. (With 32 logits a thread 22.8 + 6.1 us where 16 took 22.0 + 7.)
 //
 // The best of many without sorting them: let T be a value that at least n_out of
 // the threads' maxima reach. Every one of the n_out best is then >= T, and few
@@ -68,29 +68,43 @@ __device__ __forceinline__ double unorder64(uint64_t k) {
 // A beam that offers nothing, or only itself.
 __device__ __forceinline__ bool has_score(float s) { return s == s && s != -INFINITY; }
 
-// The greatest T that at least k of the kThreads words in `keys` reach, to as many
-// leading bits as leave at most k + 16 of them. Run by one wave.
-__device__ __forceinline__ uint32_t reach(const uint32_t* keys, int n, int k) {
-    const int lane = threadIdx.x & 63;
-    uint32_t v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i * 64 + lane < n ? keys[i * 64 + lane] : 0;
+// The greatest T that at least k of the N * 64 words in v reach, to as many leading
+// bits as leave at most k + 16 of them. Run by one wave.
+template <int N>
+__device__ __forceinline__ uint32_t reach_of(const uint32_t (&v)[N], int k) {
     uint32_t T = 0;
     for (int bit = 31; bit >= 0; --bit) {
         const uint32_t c = T | 1u << bit;
         int count = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) count += __popcll(__ballot(v[i] >= c));
+        for (int i = 0; i < N; ++i) count += __popcll(__ballot(v[i] >= c));
         if (count >= k) {
             T = c;
-            if (count <= k + 16) break;
+            if (count <= k + (N > 1 ? 16 : 0)) break;
         }
     }
     return T;
 }
+// Of the kThreads words in `keys`; with kFours, for few outputs, of the 64 maxima of four
+// each: where neighbours have nothing to do with each other hardly more values reach
+// that T (of 4,096 for 16 outputs some 18 instead of 17), and each bit costs one comparison
+// instead of four. (First launch 22.0 to 20.3 us; the second's neighbours are the best of
+// one part, in order, and it went from 7.0 to 8.1.)
+template <bool kFours>
+__device__ __forceinline__ uint32_t reach(const uint32_t* keys, int k) {
+    static_assert(kThreads == 4 * 64 && kMaxOut <= 64, "");
+    const u32x4 w = reinterpret_cast<const u32x4*>(keys)[threadIdx.x & 63];
+    if (kFours && k <= 16) {
+        const uint32_t a = w.x > w.y ? w.x : w.y, b = w.z > w.w ? w.z : w.w;
+        const uint32_t v[1] = {a > b ? a : b};
+        return reach_of(v, k);
+    }
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    return reach_of(v, k);
+}
 
 struct PartLds {
-    uint32_t top[kThreads];
+    __attribute__((aligned(16))) uint32_t top[kThreads];
     uint64_t hold[kHold];
     float max[kWaves];
     double sum[kWaves];
@@ -150,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void part_kernel(Params P) {
         L.sum[wave] = 0.0;
     }
     if (wave == 0) {
-        const uint32_t T = reach(L.top, kThreads, P.n_out);
+        const uint32_t T = reach<true>(L.top, P.n_out);
         if (lane == 0) L.reach = T > 0x00800000u ? T : 0x00800000u;     // order32(-FLT_MAX)
     }
     __syncthreads();
@@ -241,7 +255,7 @@ struct GroupLds {
     double lse[kMaxBeams];      // log of the sum of exp(x - max)
     float max[kMaxBeams], score[kMaxBeams];
     uint8_t kind[kMaxBeams];
-    uint32_t top[kThreads];
+    __attribute__((aligned(16))) uint32_t top[kThreads];
     uint64_t rank_score[kHold], key[kHold];
     uint8_t beam[kHold];
     Best one[kGroupWaves];
@@ -330,7 +344,7 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Params P) {
     atomicMax(&L.top[t % kThreads], (uint32_t)(high >> 32));
     __syncthreads();
     if (wave == 0) {
-        const uint32_t T = reach(L.top, kThreads, P.n_out);
+        const uint32_t T = reach<false>(L.top, P.n_out);
         if (lane == 0) L.reach = T;
     }
     __syncthreads();
