@@ -177,7 +177,7 @@ __device__ __forceinline__ void copy_kb(const uint8_t* src, uint32_t lds) {
             "global_load_lds_dwordx4 %0, off nt\n\t"
             "global_load_lds_dwordx4 %0, off offset:1024 nt\n\t"
             "global_load_lds_dwordx4 %0, off offset:2048 nt\n\t"
-            "global_load_lds_dwordx4 %0, off offset:3072 nt" ::"v"(src), "{m0}"(lds)
+            "global_load_lds_dwordx4 %0, off offset:%2 nt" ::"v"(src), "{m0}"(lds), "n"(3 * 1024)
             : "memory");
     else if constexpr (kN == 4)
         asm volatile(
@@ -185,7 +185,7 @@ __device__ __forceinline__ void copy_kb(const uint8_t* src, uint32_t lds) {
             "global_load_lds_dwordx4 %0, off\n\t"
             "global_load_lds_dwordx4 %0, off offset:1024\n\t"
             "global_load_lds_dwordx4 %0, off offset:2048\n\t"
-            "global_load_lds_dwordx4 %0, off offset:3072" ::"v"(src), "{m0}"(lds)
+            "global_load_lds_dwordx4 %0, off offset:%2" ::"v"(src), "{m0}"(lds), "n"(3 * 1024)
             : "memory");
     else if constexpr (kOnce)
         asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(src), "{m0}"(lds)

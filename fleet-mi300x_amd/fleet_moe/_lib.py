@@ -34,7 +34,6 @@ ABORT_BAD_PAGE = 0x800
 
 CACHE_ROW = 576
 CACHE_PAGE_TOKENS = 64
-CACHE_BLOCK_TOKENS = 16
 CACHE_PAGE_BYTES = 36992
 
 
