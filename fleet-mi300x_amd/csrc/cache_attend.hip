@@ -1069,12 +1069,12 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         if (k + kManyRing - 1 < cnt) issue(k + kManyRing - 1);      // where step k - 1 was
         if (wave_bcast(flags)) mend(k);
         l += ((p0[0] + p0[1]) + (p0[2] + p0[3])) + ((p1[0] + p1[1]) + (p1[2] + p1[3]));
-        if (k + 1 < cnt) score(k + 1);
-        add(k);
         if (k + 1 < cnt) {
+            score(k + 1);
             barrier();                          // B
             finish(k + 1);
         }
+        add(k);
     }
     // the sums of the blocks, and of the page's halves
     l = xor32_sum(xor16_sum(l));
