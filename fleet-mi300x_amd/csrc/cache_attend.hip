@@ -907,14 +907,13 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         const int page = page_of<kPage>(P, w, pages, off + k, off + cnt, lane);
         const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
         const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
-        // two waves a block: five pieces of 1 KB, and four; one of the others the scales
-        const uint8_t* from = src + (wave >> 1) * kBlockBytes + (wave & 1) * 5120 + lane * 16;
-        const uint32_t to = lds_addr(L.tile[k % kManyRing]) + (wave >> 1) * kBlockStep +
-                            (wave & 1) * 5120;
+        // a wave a block; the first the scales too
+        const uint8_t* from = src + wave * kBlockBytes + lane * 16;
+        const uint32_t to = lds_addr(L.tile[k % kManyRing]) + wave * kBlockStep;
         copy_kb<4, false>(from, to);
-        if ((wave & 1) == 0)
-            copy_kb<1, false>(from + 4096, to + 4096);
-        else if (wave == 1 && lane < 2)
+        copy_kb<4, false>(from + 4096, to + 4096);
+        copy_kb<1, false>(from + 8192, to + 8192);
+        if (wave == 0 && lane < 2)
             copy_kb<1, false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[k % kManyRing]));
     };
     const auto score = [&](int k) {
@@ -1051,7 +1050,8 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
                     __builtin_bit_cast(bf16x8, L.p[k & 1][wave & 3][wave >> 2][lane]), ones);
     };
 
-    for (int k = 0; k < kManyRing - 1 && k < cnt; ++k) issue(k);
+    if (tp == 0)
+        for (int k = 0; k < kManyRing - 1 && k < cnt; ++k) issue(k);
     wait_copies<0>();
     barrier();
     if (cnt > 0) {
@@ -1066,7 +1066,7 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         barrier();                              // A
         const int* f = L.flag[k & 1];
         const int flags = ((f[0] | f[1]) | (f[2] | f[3])) | ((f[4] | f[5]) | (f[6] | f[7]));
-        if (k + kManyRing - 1 < cnt) issue(k + kManyRing - 1);      // where step k - 1 was
+        if (tp == 0 && k + kManyRing - 1 < cnt) issue(k + kManyRing - 1);      // where step k - 1 was
         if (wave_bcast(flags)) mend(k);
         l += ((p0[0] + p0[1]) + (p0[2] + p0[3])) + ((p1[0] + p1[1]) + (p1[2] + p1[3]));
         if (k + 1 < cnt) {
