@@ -216,9 +216,8 @@ __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi, float slo, flo
 }
 
 // A block that holds no position yet may hold any bytes: its weights are zero, and
-// with a scale in range so are the products.
+// with a positive scale in range, whatever its other bits, so are the products.
 __device__ __forceinline__ float any_scale(uint32_t w) {
-    w &= 0x7f800000u;
     return __uint_as_float(w < 0x7b800000u ? w : 0x7b800000u);      // 2^120
 }
 
@@ -256,17 +255,17 @@ __device__ __forceinline__ uint2 weights(const float (&p)[4]) {
     return make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
 }
 
-// The transposing read: 8 positions of one of the 16 dimensions of chunk i. `col`
-// is what column_at() gives: lane r of a group of 16 points at row r / 2 of 8,
-// positions 4g .. 4g + 3 of two neighbouring blocks.
+// The transposing read: 8 positions of one of the 16 dimensions of chunk i, from the LDS
+// address `col` of the first block and column_at(): lane r of a group of 16 points at row
+// r / 2 of 8, positions 4g .. 4g + 3 of two neighbouring blocks. (Addresses as numbers: then
+// the chunk is the instruction's own offset, not two additions.)
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-__device__ __forceinline__ const uint8_t* column_at(const uint8_t* block, int lane) {
+__device__ __forceinline__ uint32_t column_at(int lane) {
     const int r = (lane & 15) >> 1;
-    return block + (r < 4 ? 0 : kBlockStep) + (4 * (lane >> 4) + (r & 3)) * 16 + (lane & 1) * 8;
+    return (r < 4 ? 0 : kBlockStep) + (4 * (lane >> 4) + (r & 3)) * 16 + (lane & 1) * 8;
 }
-__device__ __forceinline__ i32x2 column(const uint8_t* col, int i) {
-    return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-        (lds_i32x2*)(const __attribute__((address_space(3))) uint8_t*)(col + i * 256));
+__device__ __forceinline__ i32x2 column(uint32_t col, int i) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(uintptr_t)(col + i * 256));
 }
 
 // A block's NaN codes as zeros, by one wave. A NaN in a row makes the score, and
@@ -454,7 +453,7 @@ __device__ __forceinline__ void attend(const AttendParams& P, FewLds& L, const W
         const int b = k % kRing;
         const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[k & 1][lane]);
         const float sa = any_scale(L.scale[b][0]), sb = any_scale(L.scale[b][2]);
-        const uint8_t* col = column_at(L.tile[b], lane) + wave * kCols * 256;
+        const uint32_t col = lds_addr(L.tile[b]) + wave * kCols * 256 + column_at(lane);
 #pragma unroll
         for (int i = 0; i < kCols; ++i) {
             const i32x2 v = column(col, i);
@@ -881,10 +880,9 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
 
     const Row r = row_of(P, w, w.row0 + mine * 16 + n);
     const Common common(r);
-    bf16x8 q[2][kHalf];                         // of the tile pair
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        load_q(P, w, row_of(P, w, w.row0 + (2 * tp + i) * 16 + n), g, half, q[i]);
+    bf16x8 q[2][kHalf];                         // of `mine` and of the pair's other tile
+    load_q(P, w, r, g, half, q[0]);
+    load_q(P, w, row_of(P, w, w.row0 + (mine ^ 1) * 16 + n), g, half, q[1]);
     f32x4 acc[4][kCols];
 #pragma unroll
     for (auto& a : acc)
@@ -952,8 +950,8 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            z[j] = half ? y[1][j] : y[0][j];
-            L.half[wave][j][lane] = half ? y[0][j] : y[1][j];
+            z[j] = y[0][j];
+            L.half[wave][j][lane] = y[1][j];
         }
     };
     const auto weigh = [&](int k) {
@@ -1027,7 +1025,8 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         uint32_t f[2][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint8_t* col = column_at(L.tile[b] + 2 * h * kBlockStep, lane) + wave * kCols * 256;
+            const uint32_t col = lds_addr(L.tile[b]) + wave * kCols * 256 + column_at(lane) +
+                                 2 * h * kBlockStep;
 #pragma unroll
             for (int i = 0; i < kCols; ++i) v[h][i] = column(col, i);
 #pragma unroll
