@@ -901,21 +901,22 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     if (cnt > 0) page_of<kPage>(P, w, pages, off, off + cnt, lane);
     __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0): see attend()
 
-    const auto issue = [&](int k) {
+    // (b is k % kManyRing, counted: of a remainder the compiler makes two products and a
+    // difference for every address)
+    const auto issue = [&](int k, int b) {
         const int page = page_of<kPage>(P, w, pages, off + k, off + cnt, lane);
         const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
         const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
         // a wave a block; the first the scales too
         const uint8_t* from = src + wave * kBlockBytes + lane * 16;
-        const uint32_t to = lds_addr(L.tile[k % kManyRing]) + wave * kBlockStep;
+        const uint32_t to = lds_addr(L.tile[b]) + wave * kBlockStep;
         copy_kb<4, false>(from, to);
         copy_kb<4, false>(from + 4096, to + 4096);
         copy_kb<1, false>(from + 8192, to + 8192);
         if (wave == 0 && lane < 2)
-            copy_kb<1, false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[k % kManyRing]));
+            copy_kb<1, false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[b]));
     };
-    const auto score = [&](int k) {
-        const int b = k % kManyRing;
+    const auto score = [&](int b) {
         u32x4 c[2][4];
         uint2 e[2];
         uint32_t f[2][2];
@@ -990,14 +991,14 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         if (lane == 0) L.flag[k & 1][wave] = nan | high;
     };
     // What is rare: a row's scores beyond its reference, or a NaN, in step k.
-    const auto mend = [&](int k) {
+    const auto mend = [&](int k, int b) {
         float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
                           fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
         top = xor32_max(xor16_max(top));
         if (lane < 16) L.top[mine][bp][lane] = top;
         if (nan && half == 0 && tp == 0)
             for (int j = 0; j < 2; ++j)
-                clean(L.tile[k % kManyRing] + (2 * bp + j) * kBlockStep, lane);
+                clean(L.tile[b] + (2 * bp + j) * kBlockStep, lane);
         barrier();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1018,15 +1019,15 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         if (bp == 0 && lane < 16) L.m[mine][lane] = m;
     };
     // O over step k
-    const auto add = [&](int k) {
-        const int b = k % kManyRing;
+    const auto add = [&](int k, int b) {
+        uint32_t first = lds_addr(L.tile[b]) + wave * kCols * 256 + column_at(lane);
+        asm("" : "+v"(first));                // one address, the rest is offsets
         bf16x8 pb[2][4];
         i32x2 v[2][kCols];
         uint32_t f[2][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t col = lds_addr(L.tile[b]) + wave * kCols * 256 + column_at(lane) +
-                                 2 * h * kBlockStep;
+            const uint32_t col = first + 2 * h * kBlockStep;
 #pragma unroll
             for (int i = 0; i < kCols; ++i) v[h][i] = column(col, i);
 #pragma unroll
@@ -1050,7 +1051,7 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     };
 
     if (tp == 0)
-        for (int k = 0; k < kManyRing - 1 && k < cnt; ++k) issue(k);
+        for (int k = 0; k < kManyRing - 1 && k < cnt; ++k) issue(k, k);
     wait_copies<0>();
     barrier();
     if (cnt > 0) {
@@ -1060,20 +1061,24 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     }
     // Step k: behind barrier A the weights of k and the rows of k + 1 are there, behind
     // B both halves of the scores of k + 1.
+    int b = 0;                                  // of step k
     for (int k = 0; k < cnt; ++k) {
+        const int b1 = b == kManyRing - 1 ? 0 : b + 1, b2 = b1 == kManyRing - 1 ? 0 : b1 + 1;
         wait_copies<0>();                       // step k + 1
         barrier();                              // A
         const int* f = L.flag[k & 1];
         const int flags = ((f[0] | f[1]) | (f[2] | f[3])) | ((f[4] | f[5]) | (f[6] | f[7]));
-        if (tp == 0 && k + kManyRing - 1 < cnt) issue(k + kManyRing - 1);      // where step k - 1 was
-        if (wave_bcast(flags)) mend(k);
+        if (tp == 0 && k + kManyRing - 1 < cnt) issue(k + kManyRing - 1, b2);      // where step k - 1 was
+        if (wave_bcast(flags)) mend(k, b);
         l += ((p0[0] + p0[1]) + (p0[2] + p0[3])) + ((p1[0] + p1[1]) + (p1[2] + p1[3]));
         if (k + 1 < cnt) {
-            score(k + 1);
+            score(b1);
             barrier();                          // B
             finish(k + 1);
         }
-        add(k);
+        add(k, b);
+        b = b1;
+        asm("" : "+s"(b));
     }
     // the sums of the blocks, and of the page's halves
     l = xor32_sum(xor16_sum(l));
