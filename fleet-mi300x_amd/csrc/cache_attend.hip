@@ -840,12 +840,14 @@ __global__ __launch_bounds__(kWave ? 256 : kJoinThreads) void join_few_kernel(At
 // A workgroup per unit, or several with a share of the unit's steps where there are
 // few units. The last units come first: a causal prompt's are the longest.
 //
-// Measured: the last 500 tokens of four sequences of up to 4,096 positions 280 us, 750
+// Measured: the last 500 tokens of four sequences of up to 4,096 positions 251 us, 837
 // TFLOP/s of the 1,212 that a library product of 8,192 cubed reaches. A step takes
-// 5,700 cycles, 2,300 of them matrix instructions; reads of LDS, widening and softmax
-// are the others, and the second round of 455 units leaves a tenth of the chip idle.
-// Tried: 32 rows and four waves, two workgroups a CU 363 us (the copies of 32 rows
-// take a third of the time), 64 rows and four waves 288. A prompt of 384: 27 us.
+// 5,000 cycles, 2,300 of them matrix instructions; two waves a SIMD issue the others
+// (widening, softmax, reads of LDS: some 500 a wave) at one in three to four cycles, and
+// the second round of 455 units leaves a tenth of the chip idle. Tried: 32 rows and four
+// waves, two workgroups a CU 363 us (the copies of 32 rows take a third of the time), 64
+// rows and four waves 288, two groups of four waves half a step apart 305 where this took
+// 280. A prompt of 384: 26 us.
 constexpr int kMany = 64;       // rows
 constexpr int kManyWaves = 8;
 constexpr int kManyThreads = kManyWaves * 64;
