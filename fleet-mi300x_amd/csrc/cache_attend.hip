@@ -215,17 +215,21 @@ __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi, float slo, flo
     return __builtin_bit_cast(bf16x8, r);
 }
 
-// A block that holds no position yet may hold any bytes: its weights are zero, and
-// with a positive scale in range, whatever its other bits, so are the products.
+// The scale of a block, or of one that holds no position yet and may have any bytes: a
+// power of two up to the largest that append writes.
+constexpr uint32_t kMaxScale = 0x7b800000u;     // 2^120
 __device__ __forceinline__ float any_scale(uint32_t w) {
-    return __uint_as_float(w < 0x7b800000u ? w : 0x7b800000u);      // 2^120
+    w &= 0x7f800000u;
+    return __uint_as_float(w < kMaxScale ? w : kMaxScale);
 }
 
-// NaN codes (0x7f, 0xff) of a word as zeros.
-__device__ __forceinline__ uint32_t drop_nan(uint32_t w) {
-    const uint32_t n = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+// The codes of a word that stand for no finite value as zeros: NaN (0x7f, 0xff) and,
+// with the largest scale, 256 and more, which are infinite in bf16.
+__device__ __forceinline__ uint32_t drop_infinite(uint32_t w, bool largest) {
+    const uint32_t n = ((w & 0x7f7f7f7fu) + (largest ? 0x08080808u : 0x01010101u)) & 0x80808080u;
     return w & ~(n | (n - (n >> 7)));
 }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 
 __device__ __forceinline__ float xor16_max(float v) {
     const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v),
@@ -268,15 +272,17 @@ __device__ __forceinline__ i32x2 column(uint32_t col, int i) {
     return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(uintptr_t)(col + i * 256));
 }
 
-// A block's NaN codes as zeros, by one wave. A NaN in a row makes the score, and
-// so the weight, of every row of q that sees it NaN; a row that does not see it
-// has the weight 0, and must not meet 0 * NaN.
-__device__ __forceinline__ void clean(uint8_t* block, int lane) {
+// A block's values that are not finite as zeros, by one wave. Such a value makes the
+// score of every row of q infinite or NaN, and the weight of one that sees it NaN or 0; a
+// row that does not see it has the weight 0, and must not meet 0 * NaN. (Its score tells:
+// the wave looks at the scores before it hides those of positions that are not seen.)
+__device__ __forceinline__ void clean(uint8_t* block, uint32_t scale, int lane) {
+    const bool largest = any_scale(scale) == __uint_as_float(kMaxScale);
     for (int i = 0; i < kC / 64; ++i) {
         u32x4* at = reinterpret_cast<u32x4*>(block + i * 1024 + lane * 16);
         u32x4 v = *at;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = drop_nan(v[j]);
+        for (int j = 0; j < 4; ++j) v[j] = drop_infinite(v[j], largest);
         *at = v;
     }
 }
@@ -366,7 +372,7 @@ __device__ __forceinline__ void attend(const AttendParams& P, FewLds& L, const W
     float m = -INFINITY, ref = -INFINITY, l = 0.f;
     const float slack = kSlack / P.scale;
     f32x4 z, next;              // the scores of the block, and the next step's
-    bool nan = false;           // of the wave
+    bool stray = false;         // a score of the wave is not finite
     float p[4];
     Pages pages{0, 0, 0};
     if (cnt > 0) page_of<kStep>(P, w, pages, off, off + cnt, lane);
@@ -414,7 +420,7 @@ __device__ __forceinline__ void attend(const AttendParams& P, FewLds& L, const W
         const int page = page_of<kStep>(P, w, pages, off + k, off + cnt, lane);
         const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
         const int base = step_of<kStep>(w, off + k) * kStep + blk * kBlock;
-        const bool bad = (z[0] != z[0]) | (z[1] != z[1]) | (z[2] != z[2]) | (z[3] != z[3]);
+        const bool bad = !finite((z[0] + z[1]) + (z[2] + z[3]));
         if (!(ok && common.all(base, kBlock))) {
             asm volatile("");                   // a branch, not twenty instructions every step
             if (!ok && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
@@ -423,17 +429,18 @@ __device__ __forceinline__ void attend(const AttendParams& P, FewLds& L, const W
         }
         weigh(k);
         const float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
-        nan = __ballot(bad) != 0;
+        stray = __ballot(bad) != 0;
         const bool high = __ballot(top > m + slack) != 0;
-        if (lane == 0) L.flag[k & 1][blk] = nan | high;
+        if (lane == 0) L.flag[k & 1][blk] = stray | high;
     };
-    // What is rare: a row's scores beyond its reference, or a NaN, in step k.
+    // What is rare: a row's scores beyond its reference, or one that is not finite, in step k.
     const auto mend = [&](int k) {
         if (weighs) {
             float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
             top = xor32_max(xor16_max(top));
             if (lane < 16) L.top[blk][lane] = top;
-            if (nan) clean(L.tile[k % kRing] + blk * kBlockStep, lane);
+            if (stray)
+                clean(L.tile[k % kRing] + blk * kBlockStep, L.scale[k % kRing][2 * blk], lane);
         }
         barrier();
         const float to = fmaxf(m, fmaxf(L.top[0][n], L.top[1][n]));
@@ -897,7 +904,7 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     const float slack = kSlack / P.scale;
     f32x4 z[2];                                 // the scores of `mine` and the two blocks
     float p0[4], p1[4];
-    bool nan = false;
+    bool stray = false;                         // a score of the wave is not finite
     if (t < 64) L.m[t >> 4][n] = -INFINITY;
     Pages pages{0, 0, 0};
     if (cnt > 0) page_of<kPage>(P, w, pages, off, off + cnt, lane);
@@ -973,9 +980,8 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         const int page = page_of<kPage>(P, w, pages, off + k, off + cnt, lane);
         const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
         const int base = step_of<kPage>(w, off + k) * kPage + bp * 32;
-        bool bad = false;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bad |= (z[0][j] != z[0][j]) | (z[1][j] != z[1][j]);
+        const f32x4 both = z[0] + z[1];
+        const bool bad = !finite((both[0] + both[1]) + (both[2] + both[3]));
         if (!(ok && common.all(base, 32))) {
             asm volatile("");                   // a branch, not forty instructions every step
             if (!ok && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
@@ -988,19 +994,19 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         weigh(k);
         const float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
                                 fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
-        nan = __ballot(bad) != 0;
+        stray = __ballot(bad) != 0;
         const bool high = __ballot(top > m + slack) != 0;
-        if (lane == 0) L.flag[k & 1][wave] = nan | high;
+        if (lane == 0) L.flag[k & 1][wave] = stray | high;
     };
-    // What is rare: a row's scores beyond its reference, or a NaN, in step k.
+    // What is rare: a row's scores beyond its reference, or one that is not finite, in step k.
     const auto mend = [&](int k, int b) {
         float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
                           fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
         top = xor32_max(xor16_max(top));
         if (lane < 16) L.top[mine][bp][lane] = top;
-        if (nan && half == 0 && tp == 0)
+        if (stray && half == 0 && tp == 0)
             for (int j = 0; j < 2; ++j)
-                clean(L.tile[b] + (2 * bp + j) * kBlockStep, lane);
+                clean(L.tile[b] + (2 * bp + j) * kBlockStep, L.scale[b][2 * (2 * bp + j)], lane);
         barrier();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -520,6 +520,40 @@ def test_attention_meets_no_nan_that_it_does_not_see():
     assert np.array_equal(bad, want)
 
 
+@pytest.mark.parametrize("fill", [0x7E, 0xFE, 0x7B, 0x7F, 0x78, 0x80, 0x00])
+@pytest.mark.parametrize("lens, counts", [([5, 100, 17], [1, 1, 1]), ([700], [1]), ([90, 3], [70, 3]),
+                                          ([1500], [5])])
+def test_attention_over_a_pool_that_holds_anything(fill, lens, counts):
+    """Blocks with no position yet, and positions behind the last, of any bytes: the largest
+    codes with the largest scale are infinite, and have weight 0."""
+    b, rng = filled(fill, lens, fill=fill)
+    q = ref.bf16(rng.normal(size=(sum(counts), 16, ref.ROW)) * 0.5)
+    say(f"fill {fill:x} lens {lens} new {counts}")
+    out, lse = b.dev.attend(to_dev(q), starts(counts))
+    compare(b, q, counts, out, lse)
+
+
+@pytest.mark.parametrize("n, new", [(40, 40), (130, 3), (700, 90)])
+def test_attention_meets_no_infinity_that_it_does_not_see(n, new):
+    """Values that the cache holds as infinite (beyond the largest bf16 after rounding),
+    in positions that only the last token sees."""
+    b = Both(16, 1, 16, 1)
+    assert b.grow([n])
+    rng = np.random.default_rng(n)
+    rows = normal(rng, (1, n, ref.ROW))
+    rows[0, n - 1, 3] = -ref.values(np.array([0x7f7f], np.int16))[0]
+    rows[0, n - 1, 200] = ref.values(np.array([0x7f7f], np.int16))[0]
+    b.append([n], rows)
+    assert np.abs(b.ref.values(0)).max() > np.finfo(np.float32).max
+    q = ref.bf16(rng.normal(size=(new, 16, ref.ROW)) * 0.5)
+    out, lse = b.dev.attend(to_dev(q), starts([new]))
+    got = ref.values(out.cpu().numpy())
+    # (the largest scale is the whole block's: its other values are zeros now)
+    want, wl, tol, tl = ref.attend(b.ref.values(0), q[:-1], range(n - new, n - 1), SCALE)
+    assert (np.abs(got[:-1] - want) <= tol).all()
+    assert (np.abs(lse.cpu().numpy()[:-1] - wl) <= tl).all()
+
+
 def test_attention_extreme_scores():
     """Scores far apart and equal ones: one position takes all, or all the same."""
     b, rng = filled(3, [300])
