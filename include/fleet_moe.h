@@ -455,8 +455,8 @@ int fleet_cache_read(const fleet_cache* cache, int32_t layer0, int32_t n_layers,
  * to its own, with window > 0 only those above its own - window and those
  * below sinks. out[token][head][0..511] = sum_p softmax_p(scale * q . row_p)
  * c_p as bf16, lse[token][head] (fp32, may be NULL) = log sum_p exp(scale * q .
- * row_p); a token that sees nothing gets out = 0, lse = -infinity. NaN reaches
- * only the tokens that see it. Products are of bf16 values with fp32 sums; the
+ * row_p); a token that sees nothing gets out = 0, lse = -infinity. NaN and
+ * infinities reach only the tokens that see them. Products are of bf16 values with fp32 sums; the
  * probabilities are rounded to bf16 before the second product. max_len: a bound
  * on lens that the host knows, for the division of the work (longer sequences
  * are still right), or 0. Outputs of tokens before start[0] or behind
