@@ -18,6 +18,8 @@
 // rounded to bf16 (the MFMA's operand; by 2^-8 of a weight at most); its sum, by which
 // the result is divided, is taken of the rounded values, so a common rounding of
 // all weights cancels. lse comes from the unrounded sum.
+#include <atomic>
+
 #include "cache_pages.h"
 
 namespace fleet_moe {
@@ -733,7 +735,8 @@ __device__ __forceinline__ void join(const AttendParams& P, int64_t row_at, int 
     for (int i = 0; i < kJoinAhead; ++i)
         if (part + i * kJoinGroups < count) o += v[i] * factor[part + i * kJoinGroups];
 #pragma unroll 4
-    for (int i = part + kJoinAhead * kJoinGroups; i < count; i += kJoinGroups) o += load(i) * factor[i];
+    for (int i = part + kJoinAhead * kJoinGroups; i < count; i += kJoinGroups)
+        o += load(i) * factor[i];
     sum_o[part][t] = o;
     __syncthreads();
     if (part) return;
@@ -1150,16 +1153,22 @@ int fleet_moe_check_device(int min_cus);
 // the compiler keeps to the registers of two waves on a SIMD, and takes O as an
 // operand of the matrix instructions from them; where it knows that LDS allows one
 // only, it moves O to accumulation registers and back, 400 moves a step.)
-template <class K>
-static int launch(K kernel, int64_t grid, int threads, size_t lds, const AttendParams& P,
+template <auto Kernel>
+static int launch(int64_t grid, int threads, size_t lds, const AttendParams& P,
                   hipStream_t stream) {
     if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)lds);
+        static std::atomic<uint64_t> asked{0};  // once a device
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (e == hipSuccess && !(asked.load() & bit)) {
+            e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e == hipSuccess) asked.fetch_or(bit);
+        }
         if (e != hipSuccess) return (int)e;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, stream, P);
+    hipLaunchKernelGGL(Kernel, dim3((unsigned)grid), dim3(threads), lds, stream, P);
     return (int)hipGetLastError();
 }
 
@@ -1211,12 +1220,12 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
         P.units = (int)few;
         const int64_t steps = few * ((seen + kStep - 1) / kStep);
         P.shares = (int)(steps < kShares ? steps : kShares);
-        if (int e = launch(few_kernel, P.shares, kThreads, sizeof(FewLds), P, stream)) return e;
+        if (int e = launch<few_kernel>(P.shares, kThreads, sizeof(FewLds), P, stream)) return e;
         // A wave a row where the mean is up to 16 parts (64 sequences of 4,000 positions 42
         // to 41 us, of 1,000 25.4 to 23.9; 16 of 1,000 the same), a workgroup a row for more.
         if (P.shares <= kWaveParts * few)
-            return launch(join_few_kernel<true>, few * (kFew / 4), 256, 0, P, stream);
-        return launch(join_few_kernel<false>, few * kFew, kJoinThreads, 0, P, stream);
+            return launch<join_few_kernel<true>>(few * (kFew / 4), 256, 0, P, stream);
+        return launch<join_few_kernel<false>>(few * kFew, kJoinThreads, 0, P, stream);
     }
     P.pad = n_heads % kMany != 0;
     const int64_t units = first_unit(n_tokens, cache->n_seqs, n_heads, kMany, P.pad);
@@ -1230,10 +1239,11 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     if (splits > (n_pages + 3) / 4) splits = (n_pages + 3) / 4;
     if (splits < 1 || n_pages - n_pages / splits < 8) splits = 1;
     P.shares = (int)splits;
-    if (int e = launch(many_kernel, units * P.shares, kManyThreads, sizeof(ManyLds), P, stream)) return e;
+    if (int e = launch<many_kernel>(units * P.shares, kManyThreads, sizeof(ManyLds), P, stream))
+        return e;
     if (P.shares == 1) return 0;
     // (the same to a few percent from 4 parts to 16: 45.7 to 46.5 us of 8,192 positions)
     if (P.shares <= kWaveParts)
-        return launch(join_many_kernel<true>, units * (kMany / 4), 256, 0, P, stream);
-    return launch(join_many_kernel<false>, units * kMany, kJoinThreads, 0, P, stream);
+        return launch<join_many_kernel<true>>(units * (kMany / 4), 256, 0, P, stream);
+    return launch<join_many_kernel<false>>(units * kMany, kJoinThreads, 0, P, stream);
 }
