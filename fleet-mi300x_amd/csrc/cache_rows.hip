@@ -15,13 +15,19 @@ namespace cache {
 constexpr int kRowThreads = kBlock * kChunks;
 static_assert(kRowThreads == 9 * 64, "");
 
+// Layers that a workgroup of read takes, their loads on their way together. (Rows of 27
+// layers, with 1 / 2 / 3 / 7 of them, us: 300 rows 8.1 / 7.9 / 7.9 / 8.1, 1,000 14.7 / 14.2 /
+// 13.8 / 11.7, 1,500 17.8 / 17.2 / 17.9 / 20.7, 8,000 79.8 / 72.8 / 76.0 / 82.6; seven are
+// best only where they make one workgroup a CU. append is fastest with one.)
+constexpr int kRead = 2;
+
 struct RowParams {
     fleet_cache c;
     uint16_t* rows;
     int64_t row_stride, layer_stride;
     const int32_t* start;
     Header* h;
-    int n_rows, layer0;
+    int n_rows, layer0, n_layers;
 };
 
 // The block of positions of a workgroup, and its rows.
@@ -174,27 +180,41 @@ __global__ __launch_bounds__(kRowThreads) void read_kernel(RowParams P) {
     const fleet_cache& c = P.c;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int tok = lane >> 2, chunk = 4 * wave + (lane & 3);
-    const int layer = P.layer0 + (int)blockIdx.y;
-    const uint8_t* page = c.pool + page_offset(b.page, c.n_pages, layer, c.n_layers);
+    const int y0 = (int)blockIdx.y * kRead;
+    const int n = P.n_layers - y0 < kRead ? P.n_layers - y0 : kRead;
+    const uint8_t* page = c.pool + page_offset(b.page, c.n_pages, P.layer0 + y0, c.n_layers);
     const int blk = b.base % kPage / kBlock;
     const int pos = b.base + tok;
-    u32x4 o = ld_stream(reinterpret_cast<const u32x4*>(page + blk * kBlockBytes) +
-                        wave * 4 * kBlock + lane);
-    const float scale = __uint_as_float(
-        ld_global(reinterpret_cast<const uint32_t*>(page + kCodeBytes) + 2 * blk + (wave == 8)));
-    o = to_row_order(o, lane);
-    if (pos < b.first || pos >= b.len) return;
-    u32x4 v[2];
+    u32x4 o[kRead];
+    float scale[kRead];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[i / 2][2 * i % 4] = bf16x2<false>(o[i], scale);
-        v[i / 2][2 * i % 4 + 1] = bf16x2<true>(o[i], scale);
+    for (int j = 0; j < kRead; ++j) {
+        if (j >= n) break;
+        o[j] = ld_stream(reinterpret_cast<const u32x4*>(page + j * kPageBytes + blk * kBlockBytes) +
+                         wave * 4 * kBlock + lane);
+        scale[j] = __uint_as_float(ld_global(
+            reinterpret_cast<const uint32_t*>(page + j * kPageBytes + kCodeBytes) + 2 * blk +
+            (wave == 8)));
     }
-    u32x4* row = reinterpret_cast<u32x4*>(P.rows + blockIdx.y * P.layer_stride +
-                                          (int64_t)(b.row0 + pos - b.first) * P.row_stride +
-                                          chunk * 16);
-    st_global(row, v[0]);
-    st_global(row + 1, v[1]);
+    uint16_t* row = P.rows + y0 * P.layer_stride +
+                    (int64_t)(b.row0 + pos - b.first) * P.row_stride + chunk * 16;
+    const bool there = pos >= b.first && pos < b.len;
+#pragma unroll
+    for (int j = 0; j < kRead; ++j) {
+        if (j >= n) break;
+        const u32x4 w = to_row_order(o[j], lane);
+        if (there) {
+            u32x4 v[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i / 2][2 * i % 4] = bf16x2<false>(w[i], scale[j]);
+                v[i / 2][2 * i % 4 + 1] = bf16x2<true>(w[i], scale[j]);
+            }
+            u32x4* at = reinterpret_cast<u32x4*>(row + j * P.layer_stride);
+            st_global(at, v[0]);
+            st_global(at + 1, v[1]);
+        }
+    }
 }
 
 }  // namespace cache
@@ -235,7 +255,9 @@ static int rows_call(bool append, const fleet_cache* cache, int32_t layer0, int3
     P.n_rows = n_rows;
     P.layer0 = layer0;
     const int64_t units = first_unit(n_rows, cache->n_seqs, 1, kBlock, 2);
-    const dim3 grid((unsigned)units, n_layers);
+    P.n_layers = n_layers;
+    const int each = append ? 1 : kRead;
+    const dim3 grid((unsigned)units, (n_layers + each - 1) / each);
     if (append) hipLaunchKernelGGL(append_kernel, grid, dim3(kRowThreads), 0, stream, P);
     else hipLaunchKernelGGL(read_kernel, grid, dim3(kRowThreads), 0, stream, P);
     return (int)hipGetLastError();
