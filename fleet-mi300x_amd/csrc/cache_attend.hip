@@ -40,7 +40,7 @@ struct AttendParams {
     int4* meta;                 // [unit]: first slot, next workgroup, number of slots
     Header* h;
     int64_t q_stride;
-    uint64_t per_head;          // floor(2^40 / n_heads) + 1
+    uint64_t per_head;          // head_divisor(n_heads)
     int layer, n_tokens, n_heads, window, sinks, pad, units;
     int shares;                 // workgroups, or splits of a unit
     float scale;                // times log2(e)
@@ -51,9 +51,8 @@ constexpr int kThreads = kWaves * 64;
 constexpr float kSlack = 8.f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// row / n_heads: exact for row < 2^33 (n_heads * per_head is over 2^40 by n_heads at most).
 __device__ __forceinline__ int token_of(const AttendParams& P, int row) {
-    return (int)((uint64_t)(uint32_t)row * P.per_head >> 40);
+    return token_of_row(row, P.per_head);
 }
 
 // A unit: up to R rows (token, head) of a sequence, and the steps of S positions
@@ -1179,7 +1178,7 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
                                   size_t workspace_bytes, hipStream_t stream) {
     if (int e = check_cache(cache, workspace, workspace_bytes)) return e;
     if (layer < 0 || layer >= cache->n_layers || n_tokens < 0 || n_heads < 1 ||
-        n_heads > FLEET_CACHE_MAX_HEADS || (int64_t)n_tokens * n_heads > (1 << 26) ||
+        n_heads > FLEET_CACHE_MAX_HEADS || (int64_t)n_tokens * n_heads > kMaxRows ||
         max_len < 0 || window < 0 || sinks < 0 || !(scale > 0.f) || !(scale <= 3.0e38f) ||
         (uintptr_t)start % 4 || (!start && n_tokens != cache->n_seqs))
         return FLEET_MOE_ERR_ARG;
@@ -1203,7 +1202,7 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     P.layer = layer;
     P.n_tokens = n_tokens;
     P.n_heads = n_heads;
-    P.per_head = ((uint64_t)1 << 40) / n_heads + 1;
+    P.per_head = head_divisor(n_heads);
     P.window = window;
     P.sinks = sinks;
     P.scale = scale * 1.4426950408889634f;

@@ -32,6 +32,7 @@ constexpr int kMaxSeqs = 1024;
 constexpr int kMaxLayers = 64;
 constexpr int kMaxPages = 1 << 24;
 constexpr int kMaxRowPages = 1 << 20;
+constexpr int kMaxRows = 1 << 26;             // (token, head) rows of an attention
 
 FLEET_HD int pages_of(int64_t n) { return (int)((n + kPage - 1) / kPage); }
 
@@ -60,6 +61,16 @@ FLEET_HD int64_t first_unit(int start, int s, int mul, int div, int pad) {
 
 // Bounds start entries that are not what the caller promised.
 FLEET_HD int clamp_row(int v, int n_rows) { return v < 0 ? 0 : v > n_rows ? n_rows : v; }
+
+// The token of a (token, head) row: row / n_heads without a division. per = floor(2^36 /
+// n_heads) + 1 is over 2^36 / n_heads by one at most, so row * per is over row * 2^36 /
+// n_heads by less than 2^26, which is less than the 2^36 / 128 to the next token; and
+// row * per <= 2^26 * (2^36 + 1) keeps within 63 bits. So for every row < kMaxRows
+// and n_heads <= 128.
+FLEET_HD uint64_t head_divisor(int n_heads) { return ((uint64_t)1 << 36) / n_heads + 1; }
+FLEET_HD int token_of_row(int row, uint64_t per) {
+    return (int)((uint64_t)(uint32_t)row * per >> 36);
+}
 
 // The range of positions a token at `pos` sees: [0, sink) and [lo, pos].
 struct Seen {
