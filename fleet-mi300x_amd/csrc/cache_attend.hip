@@ -18,6 +18,9 @@
 // rounded to bf16 (the MFMA's operand; by 2^-8 of a weight at most); its sum, by which
 // the result is divided, is taken of the rounded values, so a common rounding of
 // all weights cancels. lse comes from the unrounded sum.
+#include <float.h>
+#include <math.h>
+
 #include <atomic>
 
 #include "cache_pages.h"
@@ -44,12 +47,13 @@ struct AttendParams {
     int layer, n_tokens, n_heads, window, sinks, pad, units;
     int shares;                 // workgroups, or splits of a unit
     float scale;                // times log2(e)
+    float slack;                // kSlack as a score: finite, so that -infinity + slack is too
 };
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr float kSlack = 8.f;
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ int token_of(const AttendParams& P, int row) {
     return token_of_row(row, P.per_head);
@@ -371,7 +375,7 @@ __device__ __forceinline__ void attend(const AttendParams& P, FewLds& L, const W
     // below the maximum, because weights up to 2^kSlack are as exact as those up to 1,
     // and moving it costs a pass over O and a barrier. All waves keep all of them.
     float m = -INFINITY, ref = -INFINITY, l = 0.f;
-    const float slack = kSlack / P.scale;
+    const float slack = P.slack;
     f32x4 z, next;              // the scores of the block, and the next step's
     bool stray = false;         // a score of the wave is not finite
     float p[4];
@@ -903,7 +907,7 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     f32x4 ones{0.f, 0.f, 0.f, 0.f};
     // the references of the wave's tile (see attend())
     float m = -INFINITY, ref = -INFINITY, l = 0.f;
-    const float slack = kSlack / P.scale;
+    const float slack = P.slack;
     f32x4 z[2];                                 // the scores of `mine` and the two blocks
     float p0[4], p1[4];
     bool stray = false;                         // a score of the wave is not finite
@@ -1179,7 +1183,7 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     if (int e = check_cache(cache, workspace, workspace_bytes)) return e;
     if (layer < 0 || layer >= cache->n_layers || n_tokens < 0 || n_heads < 1 ||
         n_heads > FLEET_CACHE_MAX_HEADS || (int64_t)n_tokens * n_heads > kMaxRows ||
-        max_len < 0 || window < 0 || sinks < 0 || !(scale > 0.f) || !(scale <= 3.0e38f) ||
+        max_len < 0 || window < 0 || sinks < 0 || !(scale > 0.f) || !(scale * kLog2e <= FLT_MAX) ||
         (uintptr_t)start % 4 || (!start && n_tokens != cache->n_seqs))
         return FLEET_MOE_ERR_ARG;
     if (n_tokens == 0) return 0;
@@ -1205,7 +1209,8 @@ extern "C" int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const
     P.per_head = head_divisor(n_heads);
     P.window = window;
     P.sinks = sinks;
-    P.scale = scale * 1.4426950408889634f;
+    P.scale = scale * kLog2e;
+    P.slack = fminf(kSlack / P.scale, FLT_MAX);
     // positions that a row may see, as far as the host knows
     int64_t seen = (int64_t)cache->max_pages * kPage;
     if (max_len > 0 && max_len < seen) seen = max_len;

@@ -463,7 +463,7 @@ int fleet_cache_read(const fleet_cache* cache, int32_t layer0, int32_t n_layers,
  * start[n_seqs] are left as they were. A length outside the table sets FLEET_MOE_ABORT_POSITION, and the
  * sequence's tokens see nothing; positions in a page outside the pool are not
  * seen, and set FLEET_MOE_ABORT_BAD_PAGE. 1 <= n_heads <= 128, n_tokens * n_heads
- * <= 2^26, 0 < scale. */
+ * <= 2^26, 0 < scale <= 2.3e38 (scale * log2(e) is an fp32 number). */
 int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const uint16_t* q,
                        int64_t q_stride, const int32_t* start, int32_t n_tokens,
                        int32_t n_heads, int32_t max_len, int32_t window, int32_t sinks,

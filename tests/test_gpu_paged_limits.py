@@ -57,3 +57,27 @@ def test_attention_of_more_than_2_24_rows():
     want, wl, tol, tl = ref.attend(rows, last, range(n), paged.SOFTMAX_SCALE)
     assert (np.abs(ref.values(out[-n:].cpu().numpy()) - want) <= tol).all()
     assert (np.abs(lse[-n:].cpu().numpy() - wl) <= tl).all()
+
+
+@pytest.mark.parametrize("scale", [1e-45, 1e-39, 1e-38, 1.6e-38, 1e-37, 1e30])
+@pytest.mark.parametrize("n, new", [(100, 1), (5000, 1), (100, 40), (1500, 40)])
+def test_attention_with_scales_at_both_ends(scale, n, new):
+    """Few and many rows, whole and in parts. Small scales weigh all positions alike; with
+    the largest the queries are as small."""
+    dev, rows, rng = cache_of(n + new, n)
+    q = ref.bf16(rng.normal(size=(new, 16, ref.ROW)) * (0.5 if scale < 1 else 0.05 / scale))
+    say(f"scale {scale} {n} positions {new} tokens")
+    out, lse = dev.attend(torch.from_numpy(ref.bits(q)).cuda(), i32([0, new]), scale=scale)
+    want, wl, tol, tl = ref.attend(rows, q, range(n - new, n), float(np.float32(scale)))
+    assert (np.abs(ref.values(out.cpu().numpy()) - want) <= tol).all()
+    assert (np.abs(lse.cpu().numpy() - wl) <= tl).all()
+    assert dev.status() == 0
+
+
+def test_attention_with_the_largest_scale():
+    dev, rows, rng = cache_of(5, 70)
+    q = torch.zeros((1, 16, ref.ROW), dtype=torch.int16, device="cuda")
+    out, lse = dev.attend(q, scale=2.35e38)
+    want, wl, tol, tl = ref.attend(rows, np.zeros((1, 16, ref.ROW)), [69], 1.0)
+    assert (np.abs(ref.values(out.cpu().numpy()) - want) <= tol).all()
+    assert (np.abs(lse.cpu().numpy() - wl) <= tl).all()

@@ -1,8 +1,11 @@
 """The ends of the ranges that the paged cache's calls accept, without a GPU."""
 from __future__ import annotations
 
+import ctypes
 import subprocess
 from pathlib import Path
+
+from fleet_moe import _lib
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -36,3 +39,19 @@ def test_the_token_of_every_row(tmp_path):
                     f"-I{ROOT}/fleet-mi300x_amd/csrc", "-o", exe, src], check=True)
     r = subprocess.run([exe], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_scales_that_are_no_number_in_base_2():
+    """scale * log2(e) has to be finite: 2.3586e38 is the largest that is."""
+    lib = _lib.load()
+    n = lib.fleet_cache_workspace_bytes(64, 4)
+    at = 1 << 20                    # a well aligned address that nothing reads
+    cache = _lib.FleetCache(at, at, at, at, 64, 2, 4, 8)
+
+    def call(scale, tokens):
+        return lib.fleet_cache_attend(ctypes.byref(cache), 0, at, 16 * 576, at, tokens, 16, 0, 0, 0,
+                                      scale, at, at, at, n, None)
+    for scale in (2.36e38, 3.0e38, 3.4e38, float("inf"), float("nan"), 0.0, -1e-45):
+        assert call(scale, 6) == _lib.ERR_ARG, scale
+    for scale in (2.35e38, 1.0, 1e-38, 1e-45):
+        assert call(scale, 0) == 0, scale           # (no tokens: nothing is launched)
