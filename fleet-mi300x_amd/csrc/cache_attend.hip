@@ -249,6 +249,16 @@ __device__ __forceinline__ float xor32_max(float v) {
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// A row's reference in the exponent: of a finite score that is infinite times the scale,
+// all weights would be exp2(finite - infinity) = 0, as if nothing were seen.
+__device__ __forceinline__ float reference(float scaled) {
+    return scaled == INFINITY ? __uint_as_float(0x7fc00000u) : scaled;
+}
+// What the sums so far are multiplied by; with the reference -infinity there are none.
+__device__ __forceinline__ float shrink_to(float ref, float was) {
+    return was == -INFINITY ? 1.f : exp2_(was - ref);
+}
+
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -449,8 +459,8 @@ __device__ __forceinline__ void attend(const AttendParams& P, FewLds& L, const W
         }
         barrier();
         const float to = fmaxf(m, fmaxf(L.top[0][n], L.top[1][n]));
-        const float scaled = to * P.scale;
-        const float shrink = to == -INFINITY ? 1.f : exp2_(ref - scaled);
+        const float scaled = reference(to * P.scale);
+        const float shrink = shrink_to(scaled, ref);
         m = to;
         ref = scaled;
         l *= shrink;
@@ -1018,10 +1028,10 @@ __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
         for (int i = 0; i < 4; ++i) {
             const float was = L.m[i][n];
             const float to = fmaxf(was, fmaxf(L.top[i][0][n], L.top[i][1][n]));
-            const float shrink = to == -INFINITY ? 1.f : exp2_(was * P.scale - to * P.scale);
+            const float shrink = shrink_to(to * P.scale, was * P.scale);
             if (i == mine) {
                 m = to;
-                ref = to * P.scale;
+                ref = reference(to * P.scale);
                 l *= shrink;
             }
             if (i == (wave & 3)) ones *= shrink;

@@ -456,7 +456,9 @@ int fleet_cache_read(const fleet_cache* cache, int32_t layer0, int32_t n_layers,
  * below sinks. out[token][head][0..511] = sum_p softmax_p(scale * q . row_p)
  * c_p as bf16, lse[token][head] (fp32, may be NULL) = log sum_p exp(scale * q .
  * row_p); a token that sees nothing gets out = 0, lse = -infinity. NaN and
- * infinities reach only the tokens that see them. Products are of bf16 values with fp32 sums; the
+ * infinities reach only the tokens that see them. A score (scale * q . row) beyond the
+ * range of fp32 is infinite: +infinity makes the outputs of its token and head NaN,
+ * -infinity has the weight 0. Products are of bf16 values with fp32 sums; the
  * probabilities are rounded to bf16 before the second product. max_len: a bound
  * on lens that the host knows, for the division of the work (longer sequences
  * are still right), or 0. Outputs of tokens before start[0] or behind

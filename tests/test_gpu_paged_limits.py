@@ -81,3 +81,51 @@ def test_attention_with_the_largest_scale():
     want, wl, tol, tl = ref.attend(rows, np.zeros((1, 16, ref.ROW)), [69], 1.0)
     assert (np.abs(ref.values(out.cpu().numpy()) - want) <= tol).all()
     assert (np.abs(lse.cpu().numpy() - wl) <= tl).all()
+
+
+@pytest.mark.parametrize("n, new", [(100, 2), (5000, 2), (100, 40), (1500, 40)])
+def test_attention_with_scores_beyond_fp32(n, new):
+    """Finite products q . row that are infinite times the scale: +infinity makes its token
+    and head NaN, and no other."""
+    dev, rows, rng = cache_of(n * new, n)
+    scale = 1e20
+    q = ref.bf16(rng.normal(size=(new, 16, ref.ROW)) * 0.05 / scale)
+    q[0, ::2] = ref.bf16(rng.normal(size=(8, ref.ROW)) * 1e19)
+    say(f"{n} positions {new} tokens")
+    z = q[0, ::2].astype(float) @ rows[:n - new + 1].T
+    top = float(np.finfo(np.float32).max)
+    assert (np.abs(z) < top).all() and (scale * z.max(1) > 2 * top).all()
+    out, lse = dev.attend(torch.from_numpy(ref.bits(q)).cuda(), i32([0, new]), scale=scale)
+    got, gl = ref.values(out.cpu().numpy()), lse.cpu().numpy()
+    assert np.isnan(got[0, ::2]).all() and np.isnan(gl[0, ::2]).all()
+    with np.errstate(invalid="ignore", over="ignore"):
+        want, wl, tol, tl = ref.attend(rows, q, range(n - new, n), scale)
+    for at in (np.s_[0, 1::2], np.s_[1:]):
+        assert (np.abs(got[at] - want[at]) <= tol[at]).all()
+        assert (np.abs(gl[at] - wl[at]) <= tl[at]).all()
+
+
+@pytest.mark.parametrize("n, new", [(1, 1), (64, 1), (200, 1), (5000, 1), (64, 40), (1500, 40)])
+def test_attention_with_scores_of_minus_infinity(n, new):
+    """The first 64 positions have finite products that are -infinity times the scale, the
+    others 0: the first have no weight, and where there is nothing else the output is 0."""
+    rng = np.random.default_rng(n)
+    rows = np.zeros((1, n, ref.ROW), np.float32)
+    rows[0, :64, :256] = ref.bf16(np.abs(rng.normal(size=(min(n, 64), 256))) + 1)
+    rows[0, 64:, 256:512] = ref.bf16(rng.normal(size=(max(n - 64, 0), 256)))
+    pages = -(-n // 64)
+    dev, want = paged.PagedCache.empty(pages, 1, pages, 1), ref.Cache(pages, 1, pages, 1)
+    assert want.grow([n])
+    want.append(rows, [0, n])
+    dev.grow(i32([n]))
+    dev.append(torch.from_numpy(ref.bits(rows)).cuda(), i32([0, n]))
+    q = np.zeros((new, 16, ref.ROW), np.float32)
+    q[..., :256] = -1e19
+    say(f"{n} positions {new} tokens")
+    out, lse = dev.attend(torch.from_numpy(ref.bits(ref.bf16(q))).cuda(), i32([0, new]), scale=1e20)
+    if n <= 64:
+        assert not out.any() and torch.isneginf(lse).all()
+        return
+    o, e, tol, tl = ref.attend(want.values(0)[64:], q, range(n - 64 - new, n - 64), 1.0)
+    assert (np.abs(ref.values(out.cpu().numpy()) - o) <= tol).all()
+    assert (np.abs(lse.cpu().numpy() - e) <= tl).all()
