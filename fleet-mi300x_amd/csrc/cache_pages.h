@@ -99,7 +99,9 @@ struct Header {
     uint32_t unused[2];
     uint32_t status;
     int32_t count;              // pages to copy
-    int32_t pad[60];
+    int32_t used;               // the first page that compact may have moved
+    uint32_t refused;           // why the last grow changed nothing, or 0: append writes only then
+    int32_t pad[58];
 };
 static_assert(sizeof(Header) == 256, "");
 struct Copy {

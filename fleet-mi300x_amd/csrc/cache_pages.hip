@@ -105,7 +105,8 @@ __global__ __launch_bounds__(kBook) void grow_kernel(fleet_cache c, const int32_
                                                      Header* h, Copy* copies, int32_t* list) {
     __shared__ int lastp[kMaxSeqs], first[kMaxSeqs], from[kMaxSeqs];
     __shared__ int scan[kBookWaves + 1];
-    __shared__ int any_shared, stop;
+    __shared__ int any_shared;
+    __shared__ uint32_t stop;
     const int t = threadIdx.x;
     if (t == 0) any_shared = stop = 0;
     __syncthreads();
@@ -130,16 +131,18 @@ __global__ __launch_bounds__(kBook) void grow_kernel(fleet_cache c, const int32_
                 else refs = c.refs[last];
             }
         }
-        if (why) {
-            raise(h, why);
-            stop = 1;
-        }
+        if (why) atomicOr(&stop, why);
         if (refs > 1) any_shared = 1;
         lastp[t] = open ? last : -1;
     }
     __syncthreads();
+    const auto refuse = [&](uint32_t why) {
+        raise(h, why);
+        h->refused = why;
+        h->count = 0;
+    };
     if (stop) {
-        if (t == 0) h->count = 0;
+        if (t == 0) refuse(stop);
         return;
     }
     // Sequences leave a shared page in order, each with a copy, until one holder
@@ -171,10 +174,7 @@ __global__ __launch_bounds__(kBook) void grow_kernel(fleet_cache c, const int32_
     }
     __syncthreads();
     if (found < total) {
-        if (t == 0) {
-            raise(h, FLEET_MOE_ABORT_NO_PAGE);
-            h->count = 0;
-        }
+        if (t == 0) refuse(FLEET_MOE_ABORT_NO_PAGE);
         return;
     }
     if (copy) {
@@ -186,7 +186,10 @@ __global__ __launch_bounds__(kBook) void grow_kernel(fleet_cache c, const int32_
         copies[nth] = k;
         atomicSub(&c.refs[last], 1);
     }
-    if (t == 0) h->count = n_copies;
+    if (t == 0) {
+        h->refused = 0;
+        h->count = n_copies;
+    }
     if (t < c.n_seqs && add > 0) c.lens[t] = len + add;
     // page j of the list goes to the sequence whose share holds j
     for (int j = t; j < total; j += kBook) {
@@ -247,8 +250,7 @@ __global__ __launch_bounds__(kBook) void compact_kernel(fleet_cache c, int32_t* 
     }
     if (t == 0) {
         h->count = movers;
-        // the first page that may have moved, for the table's launch
-        h->pad[0] = used;
+        h->used = used;
         if (n_used) *n_used = used;
     }
 }
@@ -264,7 +266,7 @@ __global__ __launch_bounds__(kCopyThreads) void copy_kernel(fleet_cache c, const
     const int t = threadIdx.x, count = h->count;
     if (count == 0) return;
     if constexpr (kTable) {
-        const int used = h->pad[0];
+        const int used = h->used;
         const int64_t n = (int64_t)c.n_seqs * c.max_pages;
         for (int64_t i = (int64_t)blockIdx.x * kCopyThreads + t; i < n;
              i += (int64_t)gridDim.x * kCopyThreads) {

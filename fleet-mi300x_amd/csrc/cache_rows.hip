@@ -92,8 +92,9 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(RowParams P) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int tok = lane >> 2, chunk = 4 * wave + (lane & 3);
     const int layer = P.layer0 + (int)blockIdx.y;
-    // (the count is read beside the rows: its latency is theirs)
+    // (these are read beside the rows: their latency is the same)
     const int holders = c.refs[b.page];
+    const uint32_t refused = P.h->refused;
     uint8_t* page = c.pool + page_offset(b.page, c.n_pages, layer, c.n_layers);
     const int blk = b.base % kPage / kBlock;
     u32x4* mine = reinterpret_cast<u32x4*>(page + blk * kBlockBytes) + chunk * kBlock + tok;
@@ -129,8 +130,9 @@ __global__ __launch_bounds__(kRowThreads) void append_kernel(RowParams P) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) big = most[i] > big ? most[i] : big;
     }
-    if (holders != 1) {
-        if (t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
+    // without room for the new positions the last ones are older rows
+    if (refused || holders != 1) {
+        if (t == 0) raise(P.h, refused ? refused : (uint32_t)FLEET_MOE_ABORT_BAD_PAGE);
         return;
     }
     int e = scale_exp(big);

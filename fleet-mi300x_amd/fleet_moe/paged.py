@@ -89,7 +89,9 @@ class PagedCache:
 
     def grow(self, n_new: torch.Tensor, stream=None) -> None:
         """Room for n_new[s] (int32 [n_seqs]) more positions of every sequence, all or
-        none (see status()): lens grows by it, append() then writes them."""
+        none (see status()): lens grows by it, append() then writes them. After a
+        refusal append() writes nothing until a grow() succeeds; to go on, free
+        sequences with remap(), clear_status() and grow again."""
         _need(n_new, torch.int32, (self.n_seqs,), "n_new")
         _same_device(self.pool, n_new=n_new)
         self._call("fleet_cache_grow", _ptr(n_new), stream=stream)
@@ -183,3 +185,8 @@ class PagedCache:
                                                         _stream(stream))
         _lib.check(rc, "fleet_moe_workspace_status")
         return int(v.value)
+
+    def clear_status(self, stream=None) -> None:
+        """Forgets the bits that status() collected, on the device."""
+        with _on(self.device), _own(stream):
+            self.workspace[8:12].zero_()

@@ -388,9 +388,11 @@ typedef struct fleet_cache {
     int32_t max_pages;
 } fleet_cache;
 
-/* Workspace bytes of the fleet_cache_* calls (one workspace serves all; about
- * 34 MB). 0 for sizes outside the limits above. Its status word (fleet_moe_workspace_
- * status) collects the FLEET_MOE_ABORT_* bits named below. */
+/* Workspace bytes of the fleet_cache_* calls (one workspace serves all calls on a
+ * cache; about 34 MB). 0 for sizes outside the limits above. Its first 256 bytes are
+ * zero before the first call. Its status word (fleet_moe_workspace_status; the uint32
+ * at byte 8, cleared by writing 0) collects the FLEET_MOE_ABORT_* bits named below.
+ * It also holds whether the last fleet_cache_grow was refused. */
 size_t fleet_cache_workspace_bytes(int32_t n_pages, int32_t n_seqs);
 
 /* Reorders, forks and frees sequences: row i of table and lens becomes what row
@@ -409,7 +411,8 @@ int fleet_cache_remap(const fleet_cache* cache, const int32_t* parents, void* wo
  * call before. All sequences grow or none: too few free pages or a table row
  * that is too short set FLEET_MOE_ABORT_NO_PAGE, a negative count or length
  * FLEET_MOE_ABORT_POSITION, a last page outside the pool
- * FLEET_MOE_ABORT_BAD_PAGE, and nothing changes. */
+ * FLEET_MOE_ABORT_BAD_PAGE, and nothing changes: fleet_cache_append on this workspace
+ * then writes nothing either, until a grow succeeds (one of zeros does). */
 int fleet_cache_grow(const fleet_cache* cache, const int32_t* n_new, void* workspace,
                      size_t workspace_bytes, hipStream_t stream);
 
@@ -430,7 +433,8 @@ int fleet_cache_compact(const fleet_cache* cache, int32_t* n_used, void* workspa
  * within the largest code, 448, and no less than the scale of older positions
  * in the block; where those have a smaller scale they are rounded again to the
  * new one. Rounding is to nearest even; an infinity becomes +-448 times the
- * scale, NaN stays NaN. More rows than positions, or a length outside the
+ * scale, NaN stays NaN. After a grow that was refused, nothing is written, and its
+ * status bits are set again. More rows than positions, or a length outside the
  * table, set FLEET_MOE_ABORT_POSITION, a page outside the pool or one that
  * another sequence holds too FLEET_MOE_ABORT_BAD_PAGE; such rows are not
  * written. */
