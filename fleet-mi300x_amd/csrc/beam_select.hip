@@ -17,8 +17,12 @@
 //
 // Sums: exponentials in fp32 (arguments <= 0, v_exp_f32), 16 of them added in fp32
 // and the rest in 64 bits; scores are compared in 64 bits, because the log sums of
-// beams that compete differ by less than a rounding of fp32.
+// beams that compete differ by less than a rounding of fp32. Where they differ by less than
+// the sums' own error (doubt()), the sums of the beams in question are taken once more in
+// 64 bits, for a subtraction a candidate of the others (the second launch 7.27 and 7.34 us).
 #include <math.h>
+
+#include <type_traits>
 
 #include "moe_common.h"
 
@@ -65,7 +69,7 @@ __device__ __forceinline__ double unorder64(uint64_t k) {
     return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k));
 }
 
-// A beam that offers nothing, or only itself.
+// A beam that offers something; a logit that is offered.
 __device__ __forceinline__ bool has_score(float s) { return s == s && s != -INFINITY; }
 
 // The greatest T that at least k of the N * 64 words in v reach, to as many leading
@@ -258,11 +262,56 @@ struct GroupLds {
     __attribute__((aligned(16))) uint32_t top[kThreads];
     uint64_t rank_score[kHold], key[kHold];
     uint8_t beam[kHold];
+    uint16_t order[kHold];
     Best one[kGroupWaves];
+    double sum[kGroupWaves];
+    uint8_t doubt[kMaxBeams], any_doubt;    // beams whose log sums decide the order
     uint32_t reach;
     int n;
 };
 enum : uint8_t { kNothing, kItself, kTokens };
+
+// How far apart scores of different beams have to be for their order to be certain. A part's
+// sum is off by (2.5 D + 17) 2^-24 of itself at most: 2^-24 |d| from d = x - max, 1.5 *
+// 2^-24 |d| from d * log2(e), 2^-23 from the exponential, 15 roundings of 2^-24 from the
+// addition of 16; and D, the mean of |d| by weight, is log(kPart) at most (the entropy of
+// the weights is D + log of the sum, which is 1 or more). That is 38 * 2^-24, less than
+// 2^-18, for the log sums of each of the two, beside the roundings of the scores themselves.
+__device__ __forceinline__ double doubt(double score) {
+    return 0x1p-17 + fmin(fabs(score), 1.7976931348623157e308) * 0x1p-50;
+}
+
+// The least word of order64 that a score with one of T's word in its doubt can have.
+__device__ __forceinline__ uint32_t below(uint32_t T) {
+    if (T <= 0x00100000u) return T;                       // of the lowest finite score
+    const double s = unorder64((uint64_t)T << 32);
+    return (uint32_t)(order64(s - doubt(s)) >> 32);
+}
+
+// The log sums of the beams in doubt once more, exponentials and sums in 64 bits, from the
+// logits: 40 us for a beam of 102,400, by one workgroup.
+__device__ __forceinline__ void exact_sums(const Params& P, GroupLds& L, int row0) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    for (int b = 0; b < P.n_beams; ++b) {
+        if (!L.doubt[b] || L.kind[b] != kTokens || L.max[b] == -INFINITY) continue;
+        const float* x = P.logits + (int64_t)(row0 + b) * P.ld;
+        const double max = (double)L.max[b];
+        double s = 0.0;
+        for (int i = t; i < P.vocab; i += kGroupThreads) {
+            const float v = ld_global(x + i);
+            if (has_score(v)) s += exp((double)fminf(v, 3.402823466e38f) - max);
+        }
+        s = wave_sum64(s);
+        if (lane == 0) L.sum[wave] = s;
+        __syncthreads();
+        if (t == 0) {
+            double all = 0.0;
+            for (int i = 0; i < kGroupWaves; ++i) all += L.sum[i];
+            L.lse[b] = log(all);
+        }
+        __syncthreads();
+    }
+}
 
 __global__ __launch_bounds__(kGroupThreads) void group_kernel(Params P) {
     __shared__ GroupLds L;
@@ -306,11 +355,10 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Params P) {
             L.max[b] = m;
             L.score[b] = score;
             L.kind[b] = kind;
+            L.doubt[b] = 0;
         }
     }
-    if (t == 0) L.n = 0;
-    if (t < kThreads) L.top[t] = 0;
-    __syncthreads();
+    if (t == 0) L.any_doubt = 0;
     const auto candidate = [&](int i, uint64_t key) {
         Best c;
         c.beam = beam_of(i);
@@ -327,41 +375,6 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Params P) {
         }
         return c;
     };
-    Best held[kGroupPer];
-    uint64_t high = 0;
-#pragma unroll
-    for (int k = 0; k < kGroupPer; ++k) {
-        const int i = t + k * kGroupThreads;
-        held[k] = i < n ? candidate(i, keys[k]) : Best{0, 0, 0};
-        high = held[k].score > high ? held[k].score : high;
-    }
-    constexpr int kHeld = kGroupPer * kGroupThreads;
-    for (int i = t + kHeld; i < n; i += kGroupThreads) {
-        const uint64_t s = candidate(i, ld_global(best + i)).score;
-        high = s > high ? s : high;
-    }
-    // (four threads share a word: reach() takes kThreads of them)
-    atomicMax(&L.top[t % kThreads], (uint32_t)(high >> 32));
-    __syncthreads();
-    if (wave == 0) {
-        const uint32_t T = reach<false>(L.top, P.n_out);
-        if (lane == 0) L.reach = T;
-    }
-    __syncthreads();
-    const uint32_t T = L.reach;
-    const auto hold = [&](const Best& c) {
-        if (c.score == 0 || (uint32_t)(c.score >> 32) < T) return;
-        const int at = atomicAdd(&L.n, 1);
-        if (at < kHold) {
-            L.rank_score[at] = c.score;
-            L.key[at] = c.key;
-            L.beam[at] = (uint8_t)c.beam;
-        }
-    };
-#pragma unroll
-    for (int k = 0; k < kGroupPer; ++k) hold(held[k]);
-    for (int i = t + kHeld; i < n; i += kGroupThreads) hold(candidate(i, ld_global(best + i)));
-    __syncthreads();
     const auto put = [&](int k, const Best& c) {
         const int64_t at = (int64_t)blockIdx.x * P.n_out + k;
         const bool there = c.score != 0;
@@ -373,41 +386,110 @@ __global__ __launch_bounds__(kGroupThreads) void group_kernel(Params P) {
             P.out_finished[at] = there && (L.kind[c.beam] == kItself ||
                                            (P.eos >= 0 && token == P.eos));
     };
-    const int found = L.n;
-    if (found <= kHold) {
-        for (int i = wave; i < found; i += kGroupWaves) {
-            const Best c{L.rank_score[i], L.key[i], L.beam[i]};
-            int rank = 0;
-            for (int j = lane; j - lane < found; j += 64)
-                rank += __popcll(__ballot(
-                    j < found && ahead(Best{L.rank_score[j], L.key[j], L.beam[j]}, c)));
-            if (lane == 0 && rank < P.n_out) put(rank, c);
-        }
-        for (int i = found + t; i < P.n_out; i += kGroupThreads) put(i, Best{0, 0, 0});
-        return;
-    }
-    Best last{~0ull, ~0ull, -1};
-    for (int k = 0; k < P.n_out; ++k) {
-        Best top{0, 0, kMaxBeams};
-        for (int i = t; i < n; i += kGroupThreads) {
-            const Best c = candidate(i, ld_global(best + i));
-            if (c.score != 0 && ahead(last, c) && ahead(c, top)) top = c;
-        }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const Best o{__shfl_xor((unsigned long long)top.score, d),
-                         __shfl_xor((unsigned long long)top.key, d), __shfl_xor(top.beam, d)};
-            if (ahead(o, top)) top = o;
-        }
-        if (lane == 0) L.one[wave] = top;
+    const auto live = [&] {
+        return __popcll(__ballot(lane < P.n_beams && L.kind[lane] != kNothing));
+    };
+    constexpr int kHeld = kGroupPer * kGroupThreads;
+    // Whether the order is in doubt. (Called twice, not a loop: as a loop it takes 128 instead of
+    // 115 registers, and 8.0 us.)
+    const auto choose = [&](auto again) __attribute__((always_inline)) {
+        if (t == 0) L.n = 0;
+        if (t < kThreads) L.top[t] = 0;
         __syncthreads();
-        last = L.one[0];
+        Best held[kGroupPer];
+        uint64_t high = 0;
 #pragma unroll
-        for (int i = 1; i < kGroupWaves; ++i)
-            if (ahead(L.one[i], last)) last = L.one[i];
-        if (last.score == 0) last.beam = 0;
-        if (t == 0) put(k, last);
+        for (int k = 0; k < kGroupPer; ++k) {
+            const int i = t + k * kGroupThreads;
+            held[k] = i < n ? candidate(i, keys[k]) : Best{0, 0, 0};
+            high = held[k].score > high ? held[k].score : high;
+        }
+        for (int i = t + kHeld; i < n; i += kGroupThreads) {
+            const uint64_t s = candidate(i, ld_global(best + i)).score;
+            high = s > high ? s : high;
+        }
+        // (four threads share a word: reach() takes kThreads of them)
+        atomicMax(&L.top[t % kThreads], (uint32_t)(high >> 32));
         __syncthreads();
+        if (wave == 0) {
+            const uint32_t T = reach<false>(L.top, P.n_out);
+            if (lane == 0) L.reach = below(T);
+        }
+        __syncthreads();
+        const uint32_t T = L.reach;
+        const auto hold = [&](const Best& c) {
+            if (c.score == 0 || (uint32_t)(c.score >> 32) < T) return;
+            const int at = atomicAdd(&L.n, 1);
+            if (at < kHold) {
+                L.rank_score[at] = c.score;
+                L.key[at] = c.key;
+                L.beam[at] = (uint8_t)c.beam;
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < kGroupPer; ++k) hold(held[k]);
+        for (int i = t + kHeld; i < n; i += kGroupThreads) hold(candidate(i, ld_global(best + i)));
+        __syncthreads();
+        const int found = L.n;
+        if (found <= kHold) {
+            for (int i = wave; i < found; i += kGroupWaves) {
+                const Best c{L.rank_score[i], L.key[i], L.beam[i]};
+                int rank = 0;
+                for (int j = lane; j - lane < found; j += 64)
+                    rank += __popcll(__ballot(
+                        j < found && ahead(Best{L.rank_score[j], L.key[j], L.beam[j]}, c)));
+                if (lane == 0) {
+                    L.order[rank] = (uint16_t)i;
+                    if (rank < P.n_out) put(rank, c);
+                }
+            }
+            for (int i = found + t; i < P.n_out; i += kGroupThreads) put(i, Best{0, 0, 0});
+        } else if (again || live() < 2) {
+            Best last{~0ull, ~0ull, -1};
+            for (int k = 0; k < P.n_out; ++k) {
+                Best top{0, 0, kMaxBeams};
+                for (int i = t; i < n; i += kGroupThreads) {
+                    const Best c = candidate(i, ld_global(best + i));
+                    if (c.score != 0 && ahead(last, c) && ahead(c, top)) top = c;
+                }
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const Best o{__shfl_xor((unsigned long long)top.score, d),
+                                 __shfl_xor((unsigned long long)top.key, d),
+                                 __shfl_xor(top.beam, d)};
+                    if (ahead(o, top)) top = o;
+                }
+                if (lane == 0) L.one[wave] = top;
+                __syncthreads();
+                last = L.one[0];
+#pragma unroll
+                for (int i = 1; i < kGroupWaves; ++i)
+                    if (ahead(L.one[i], last)) last = L.one[i];
+                if (last.score == 0) last.beam = 0;
+                if (t == 0) put(k, last);
+                __syncthreads();
+            }
+        } else {
+            // more ties than LDS holds, of any beams
+            if (t < P.n_beams) L.doubt[t] = 1;
+            if (t == 0) L.any_doubt = 1;
+        }
+        if constexpr (again) return false;
+        __syncthreads();
+        // neighbours in order, of different beams
+        if (found <= kHold)
+            for (int i = t; i + 1 < found; i += kGroupThreads) {
+                const int a = L.order[i], b = L.order[i + 1];
+                const double score = unorder64(L.rank_score[a]);
+                if (L.beam[a] != L.beam[b] && score - unorder64(L.rank_score[b]) <= doubt(score))
+                    L.doubt[L.beam[a]] = L.doubt[L.beam[b]] = L.any_doubt = 1;
+            }
+        __syncthreads();
+        return L.any_doubt != 0;
+    };
+    if (choose(std::false_type{})) {
+        exact_sums(P, L, row0);
+        choose(std::true_type{});
     }
 }
 
