@@ -364,6 +364,7 @@ struct FewLds {
     float top[2][16], sum[2][16];
 };
 static_assert(sizeof(FewLds) <= 80 * 1024, "two workgroups share a CU");
+static_assert(2 * kShares * kFew <= kPartRows, "a workgroup has two parts at most");
 
 // Steps off .. off + cnt - 1 of a unit, and its results: to `out` and `lse`, or as the
 // partial results of slot `slot` if that is not negative.
@@ -884,6 +885,7 @@ struct ManyLds {
     float m[4][16], top[4][2][16], sum[4][2][16], rounded[4][2][16];
 };
 static_assert(sizeof(ManyLds) <= 160 * 1024, "");
+static_assert(kShares / 2 * kMany <= kPartRows, "units are divided into kShares / 2 parts at most");
 
 __global__ __launch_bounds__(kManyThreads, 1) void many_kernel(AttendParams P) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];

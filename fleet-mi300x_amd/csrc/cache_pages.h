@@ -114,7 +114,7 @@ __device__ __forceinline__ void raise(Header* h, uint32_t bit) { atomicOr(&h->st
 // rows' references and sums, and where a unit's lie.
 constexpr int kShares = 512;           // workgroups: two a CU
 constexpr int kMaxUnits = 4096;
-constexpr int kPartRows = 1024 * 16;   // two parts of 16 rows a workgroup, or one of 32
+constexpr int kPartRows = 1024 * 16;   // two parts of 16 rows a workgroup, or 64 rows of half as many
 constexpr size_t kPartBytes = (size_t)kPartRows * kC * 4;
 constexpr size_t kStatBytes = (size_t)kPartRows * 16;
 constexpr size_t kMetaBytes = (size_t)kMaxUnits * 16;
