@@ -52,6 +52,13 @@ def _need(t: torch.Tensor, dtype, shape, name: str) -> None:
                          f"got {t.dtype} {tuple(t.shape)}")
 
 
+def _int32(v) -> int:
+    """An argument of a call as an int32: what is beyond its range at the range's end (below
+    zero: -1), where ctypes would take the low 32 bits."""
+    v = int(v)
+    return v if -1 <= v < 2**31 else -1 if v < 0 else 2**31 - 1
+
+
 class _Here:
     """The context of a call whose tensors are on the current device: none."""
 
@@ -414,10 +421,10 @@ class BeamSelector:
     def __init__(self, n_groups: int, n_beams: int, n_out: int | None = None,
                  vocab: int | None = None, eos: int = -1, device="cuda"):
         from .layout import VOCAB
-        self.n_groups, self.n_beams = int(n_groups), int(n_beams)
-        self.n_out = self.n_beams if n_out is None else int(n_out)
-        self.vocab = VOCAB if vocab is None else int(vocab)
-        self.eos = int(eos)
+        self.n_groups, self.n_beams = _int32(n_groups), _int32(n_beams)
+        self.n_out = self.n_beams if n_out is None else _int32(n_out)
+        self.vocab = VOCAB if vocab is None else _int32(vocab)
+        self.eos = _int32(eos)
         n = _lib.load().fleet_beam_workspace_bytes(self.n_groups, self.n_beams, self.n_out,
                                                    self.vocab)
         if n == 0 or self.eos >= self.vocab:

@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib
-from .ops import _need, _on, _own, _ptr, _same_device, _stream
+from .ops import _int32, _need, _on, _own, _ptr, _same_device, _stream
 
 ROW = _lib.CACHE_ROW
 LORA = 512
@@ -117,7 +117,7 @@ class PagedCache:
         _same_device(self.pool, rows=rows, start=start)
         row = int(rows.stride(1)) if n > 1 else ROW
         step = int(rows.stride(0)) if layers > 1 else 0
-        self._call(name, int(layer), layers, _ptr(rows), row, step, _ptr(start), n, stream=stream)
+        self._call(name, _int32(layer), layers, _ptr(rows), row, step, _ptr(start), n, stream=stream)
 
     def _check_start(self, start, n: int) -> None:
         if start is not None:
@@ -172,9 +172,9 @@ class PagedCache:
         if n == 0:
             return out, lse
         stride = q.stride(0) if n > 1 else heads * ROW
-        self._call("fleet_cache_attend", int(layer), _ptr(q), stride, _ptr(start), n, heads,
-                   int(max_len), int(window), int(sinks), float(scale), _ptr(out), _ptr(lse),
-                   stream=stream)
+        self._call("fleet_cache_attend", _int32(layer), _ptr(q), stride, _ptr(start), n, heads,
+                   _int32(max_len), _int32(window), _int32(sinks), float(scale), _ptr(out),
+                   _ptr(lse), stream=stream)
         return out, lse
 
     def status(self, stream=None) -> int:

@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 import paged_ref as ref  # noqa: E402
-from fleet_moe import paged  # noqa: E402
+from fleet_moe import _lib, ops, paged  # noqa: E402
 
 
 def say(msg: str) -> None:
@@ -129,3 +129,40 @@ def test_attention_with_scores_of_minus_infinity(n, new):
     o, e, tol, tl = ref.attend(want.values(0)[64:], q, range(n - 64 - new, n - 64), 1.0)
     assert (np.abs(ref.values(out.cpu().numpy()) - o) <= tol).all()
     assert (np.abs(lse.cpu().numpy() - e) <= tl).all()
+
+
+BIG = 2**32                         # whose low 32 bits are zero
+
+
+def test_arguments_beyond_32_bits():
+    """A window, first positions or a bound beyond any length are as good as that; a layer
+    is none."""
+    dev, rows, rng = cache_of(7, 150)
+    q = ref.bf16(rng.normal(size=(1, 16, ref.ROW)) * 0.5)
+    dq = torch.from_numpy(ref.bits(q)).cuda()
+    want, wl, tol, tl = ref.attend(rows, q, [149], paged.SOFTMAX_SCALE)
+    for kw in (dict(window=BIG + 5), dict(window=5, sinks=BIG), dict(max_len=BIG + 1)):
+        out, lse = dev.attend(dq, **kw)
+        assert (np.abs(ref.values(out.cpu().numpy()) - want) <= tol).all(), kw
+        assert (np.abs(lse.cpu().numpy() - wl) <= tl).all(), kw
+    row = torch.zeros((1, ref.ROW), dtype=torch.int16, device="cuda")
+    for f in (lambda: dev.attend(dq, layer=BIG), lambda: dev.attend(dq, layer=-BIG),
+              lambda: dev.attend(dq, window=-BIG), lambda: dev.attend(dq, sinks=-BIG),
+              lambda: dev.attend(dq, max_len=-BIG), lambda: dev.append(row, layer=BIG),
+              lambda: dev.append(row, layer=-BIG), lambda: dev.read(row, layer=BIG)):
+        with pytest.raises(_lib.FleetMoeError):
+            f()
+
+
+def test_beam_arguments_beyond_32_bits():
+    for bad in ((BIG + 1, 2, 2, 100), (1, BIG + 2, 2, 100), (1, 2, BIG + 2, 100), (1, 2, 2, BIG + 100)):
+        with pytest.raises(ValueError):
+            ops.BeamSelector(*bad)
+    with pytest.raises(ValueError):
+        ops.BeamSelector(1, 2, 2, 100, eos=BIG)
+    select = ops.BeamSelector(1, 2, 2, 100, eos=3 - BIG)            # no such token
+    logits = torch.zeros((2, 100), device="cuda")
+    logits[1, 3] = 20.0
+    got = select.select(logits, torch.tensor([[-1.0, -2.0]], device="cuda"),
+                        torch.tensor([[1, 0]], dtype=torch.uint8, device="cuda"))
+    assert got["tokens"].tolist() == [[-1, 3]] and got["finished"].tolist() == [[1, 0]]
