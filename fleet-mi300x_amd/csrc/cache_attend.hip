@@ -14,10 +14,15 @@
 // each widened to bf16 with its block's scale, exactly (4 significant bits and a
 // power of two).
 //
-// Roundings: q and the cache are exact in bf16, products and sums fp32. P is
-// rounded to bf16 (the MFMA's operand; by 2^-8 of a weight at most); its sum, by which
-// the result is divided, is taken of the rounded values, so a common rounding of
-// all weights cancels. lse comes from the unrounded sum.
+// Roundings: q and the cache are exact in bf16, products and sums fp32. P is the MFMA's
+// operand in bf16. With few rows it is two operands, P rounded and what that leaves, so its
+// weights are good to 2^-16: the bytes of the pages bound that kernel, and the second
+// product of the same widened K costs 0.1 of 55.7 us. With many rows the matrix instructions
+// and their issue bound it, and P is rounded (by 2^-8 of a weight at most): the second operand
+// took 250 to 349 us there, for an error against 64 bits of 1.7e-3 instead of 2.1e-3, of which
+// the result's own rounding to bf16 is 1.7e-3. The sum by which the result is divided is
+// taken of the same operands, so a common rounding of all weights cancels. lse comes from the
+// unrounded sum.
 #include <float.h>
 #include <math.h>
 
@@ -302,6 +307,13 @@ __device__ __forceinline__ void clean(uint8_t* block, uint32_t scale, int lane) 
     }
 }
 
+// What their rounding leaves of them, as bf16.
+__device__ __forceinline__ uint2 rest(const float (&p)[4], uint2 w) {
+    const float r[4] = {p[0] - bf_lo(w.x), p[1] - bf_hi(w.x), p[2] - bf_lo(w.y),
+                        p[3] - bf_hi(w.y)};
+    return weights(r);
+}
+
 __device__ __forceinline__ uint32_t bf16x2_bits(float a, float b) {
     return bf16_bits(a) | bf16_bits(b) << 16;
 }
@@ -359,7 +371,7 @@ struct FewLds {
     __attribute__((aligned(16))) uint8_t tile[kRing][2 * kBlockStep];
     uint32_t scale[kRing][4];   // c and k_pe of either block
     f32x4 half[2][64];          // half of the scores of a block, for the wave that weighs
-    u32x4 p[2][64];             // [step parity][lane]
+    u32x4 p[2][2][64];          // [step parity][weights, their rests][lane]
     int flag[2][2];             // [step parity][block]
     float top[2][16], sum[2][16];
 };
@@ -429,7 +441,9 @@ __device__ __forceinline__ void attend(const AttendParams& P, FewLds& L, const W
         const float down = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
         for (int j = 0; j < 4; ++j) p[j] = exp2_(fmaf(z[j], P.scale, -down));
-        reinterpret_cast<uint2*>(&L.p[k & 1][lane])[blk] = weights(p);
+        const uint2 w = weights(p);
+        reinterpret_cast<uint2*>(&L.p[k & 1][0][lane])[blk] = w;
+        reinterpret_cast<uint2*>(&L.p[k & 1][1][lane])[blk] = rest(p, w);
     };
     const auto finish = [&](int k) {
         z = next + L.half[blk][lane];
@@ -474,15 +488,20 @@ __device__ __forceinline__ void attend(const AttendParams& P, FewLds& L, const W
     // O over step k
     const auto add = [&](int k) {
         const int b = k % kRing;
-        const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[k & 1][lane]);
+        const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[k & 1][0][lane]);
+        const bf16x8 pr = __builtin_bit_cast(bf16x8, L.p[k & 1][1][lane]);
         const float sa = any_scale(L.scale[b][0]), sb = any_scale(L.scale[b][2]);
         const uint32_t col = lds_addr(L.tile[b]) + wave * kCols * 256 + column_at(lane);
 #pragma unroll
         for (int i = 0; i < kCols; ++i) {
             const i32x2 v = column(col, i);
-            acc[i] = mfma(widen((uint32_t)v.x, (uint32_t)v.y, sa, sb), pb, acc[i]);
+            const bf16x8 a = widen((uint32_t)v.x, (uint32_t)v.y, sa, sb);
+            acc[i] = mfma(a, pb, acc[i]);
+            acc[i] = mfma(a, pr, acc[i]);
         }
-        ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}), pb, ones);
+        const bf16x8 one = __builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes});
+        ones = mfma(one, pb, ones);
+        ones = mfma(one, pr, ones);
     };
 
     // The first step's copies are waited for here, the others' kRing - 2 steps after

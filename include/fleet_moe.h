@@ -462,8 +462,9 @@ int fleet_cache_read(const fleet_cache* cache, int32_t layer0, int32_t n_layers,
  * row_p); a token that sees nothing gets out = 0, lse = -infinity. NaN and
  * infinities reach only the tokens that see them. A score (scale * q . row) beyond the
  * range of fp32 is infinite: +infinity makes the outputs of its token and head NaN,
- * -infinity has the weight 0. Products are of bf16 values with fp32 sums; the
- * probabilities are rounded to bf16 before the second product. max_len: a bound
+ * -infinity has the weight 0. Products are of bf16 values with fp32 sums;
+ * before the second product the probabilities are rounded to 16 bits where a call has 32
+ * (token, head) rows a sequence or fewer, to bf16's 8 where it has more. max_len: a bound
  * on lens that the host knows, for the division of the work (longer sequences
  * are still right), or 0. Outputs of tokens before start[0] or behind
  * start[n_seqs] are left as they were. A length outside the table sets FLEET_MOE_ABORT_POSITION, and the
