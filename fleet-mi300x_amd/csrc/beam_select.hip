@@ -6,7 +6,7 @@
 // kept. Reading the logits bounds it (HBM for many beams; for few, the two
 // launches' latency). Measured, 102,400 logits a beam: 32 groups of 8 beams, 16
 // outputs each, 20 + 7 us (105 MB; the loads by themselves take 15.5); 4 beams,
-// 5.2 + 4.8. (With 32 logits a thread 22.8 + 6.1 us where 16 took 22.0 + 7.)
+// 4.9 + 5.2. (With 32 logits a thread 22.8 + 6.1 us where 16 took 22.0 + 7.)
 //
 // The best of many without sorting them: let T be a value that at least n_out of
 // the threads' maxima reach. Every one of the n_out best is then >= T, and few

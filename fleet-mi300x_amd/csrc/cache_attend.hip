@@ -564,9 +564,9 @@ __device__ __forceinline__ void attend(const AttendParams& P, FewLds& L, const W
 // concatenated steps, across units where it has to. A unit that several have a part
 // in leaves partial results, which join_few_kernel adds in order.
 //
-// Measured, both launches: one sequence of 1,024 positions 12 us, of 65,536 29; 64 of
-// 5,120 to 8,192 56 us, 4.4 TB/s of pages (the copies alone reach 5.8, the 16 rows'
-// products and the widening are the rest).
+// Measured, both launches: one sequence of 1,024 positions 12.6 us, of 65,536 29; 64 of
+// 5,120 to 8,192 55 us, 4.5 TB/s of pages (the copies alone reach 5.8; the waves wait 42% of
+// their time, and the matrix units are busy 22%).
 // The steps of all units of a sequence, an empty unit as one.
 __device__ __forceinline__ int seq_steps(const AttendParams& P, Work& w) {
     int n = 0;
@@ -602,8 +602,8 @@ struct Shares {
 
 // A unit counts kSetup steps besides its own where shares are long: beginning one in
 // the middle of a share takes as long (queries, page numbers and the first copies
-// one after the other: 7 us of 64 sequences' 45, which the workgroups that had two
-// units ended later).
+// one after the other), so that workgroups with two units ended later than the
+// others. 64 sequences of 5,120 to 8,192: 55.6 us, without it 59.5.
 constexpr int kSetup = 6;
 
 // How many shares. A share of few steps is short, but each is a part to join: n steps
@@ -881,13 +881,17 @@ __global__ __launch_bounds__(kWave ? 256 : kJoinThreads) void join_few_kernel(At
 // tiles. 72 registers of q, 64 of O: two waves a SIMD.
 //
 // A workgroup per unit, or several with a share of the unit's steps where there are
-// few units. The last units come first: a causal prompt's are the longest.
+// few units. A sequence's last units come before its first ones: a causal prompt's are
+// the longest. The last sequence's come first, whatever its length; of several sequences that
+// is not the longest first, and ends later (the case below after 110 pages' time, where
+// longest first would end after 103 and the mean is 93).
 //
-// Measured: the last 500 tokens of four sequences of up to 4,096 positions 251 us, 837
+// Measured: the last 500 tokens of four sequences of up to 4,096 positions 250 us, 840
 // TFLOP/s of the 1,212 that a library product of 8,192 cubed reaches. A step takes
-// 5,000 cycles, 2,300 of them matrix instructions; two waves a SIMD issue the others
-// (widening, softmax, reads of LDS: some 500 a wave) at one in three to four cycles, and
-// the second round of 455 units leaves a tenth of the chip idle. Tried: 32 rows and four
+// 5,350 cycles with its part of a unit's begin and end, 2,210 of them matrix instructions;
+// two waves a SIMD issue 494 instructions each (308 vector ones with the 69 matrix, 100
+// scalar, 40 of LDS), and a wave is ready without being issued 39% of its time. The second round
+// of 455 units leaves 15% of the chip idle. Tried: 32 rows and four
 // waves, two workgroups a CU 363 us (the copies of 32 rows take a third of the time), 64
 // rows and four waves 288, two groups of four waves half a step apart 305 where this took
 // 280. A prompt of 384: 26 us.

@@ -371,7 +371,7 @@ int fleet_lm_head_argmax(const float* x, const uint16_t* final_norm, const uint1
  * positions, each [36 chunks][16 positions][16 bytes] of e4m3 codes (value
  * 16 * chunk + byte of a row), then fp32 scales [4 blocks][2], of c and of
  * k_pe, powers of two in [2^-110, 2^120], and 96 unused bytes. A row's value is
- * code * scale. Sequence s holds positions 0 .. lens[s] - 1 in the pages
+ * code * scale as a bf16 (beyond its range, with the scale 2^120 only: infinity). Sequence s holds positions 0 .. lens[s] - 1 in the pages
  * table[s][0 ..]; table[s][j] = -1 from page ceil(lens[s] / 64) on. refs[p] is
  * the number of table entries that name page p, 0 for a free page. All
  * sequences empty: table all -1, lens and refs zero (the pool may hold
