@@ -40,6 +40,7 @@ struct BlockAt {
     int page;
 };
 
+template <bool kAppend>
 __device__ __forceinline__ bool block_at(const RowParams& P, BlockAt& b) {
     const fleet_cache& c = P.c;
     const int64_t u = blockIdx.x;
@@ -54,7 +55,11 @@ __device__ __forceinline__ bool block_at(const RowParams& P, BlockAt& b) {
     const bool lead = threadIdx.x == 0 && blockIdx.y == 0 &&
                       u == first_unit(a, b.seq, 1, kBlock, 2);
     if (b.len < 0 || b.first < 0) {
-        if (lead) raise(P.h, FLEET_MOE_ABORT_POSITION);
+        if (lead) {
+            // (without the room that a grow refused, there may be fewer positions than rows)
+            const uint32_t refused = kAppend ? P.h->refused : 0;
+            raise(P.h, refused ? refused : (uint32_t)FLEET_MOE_ABORT_POSITION);
+        }
         if (b.len < 0) return false;
     }
     const int lo = b.first < 0 ? 0 : b.first;
@@ -90,7 +95,7 @@ __device__ __forceinline__ uint32_t bf16x2(uint32_t codes, float scale) {
 __global__ __launch_bounds__(kRowThreads) void append_kernel(RowParams P) {
     __shared__ unsigned most[8];
     BlockAt b;
-    if (!block_at(P, b)) return;
+    if (!block_at<true>(P, b)) return;
     const fleet_cache& c = P.c;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int tok = lane >> 2, chunk = 4 * wave + (lane & 3);
@@ -181,7 +186,7 @@ __device__ __forceinline__ u32x4 to_row_order(const u32x4& v, int lane) {
 
 __global__ __launch_bounds__(kRowThreads) void read_kernel(RowParams P) {
     BlockAt b;
-    if (!block_at(P, b)) return;
+    if (!block_at<false>(P, b)) return;
     const fleet_cache& c = P.c;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int tok = lane >> 2, chunk = 4 * wave + (lane & 3);

@@ -59,7 +59,7 @@ class PagedCache:
         if n == 0:
             raise ValueError(f"unsupported cache sizes: {self.n_pages} pages, "
                              f"{self.n_seqs} sequences")
-        # only the status word has to start as zero
+        # only the header (status word, the last grow's refusal) has to start as zero
         self.workspace = torch.empty(n, dtype=torch.uint8, device=self.device)
         self.workspace[:256].zero_()
         self._ws = (self.workspace.data_ptr(), n)

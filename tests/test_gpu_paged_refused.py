@@ -155,3 +155,16 @@ def test_a_captured_step_without_room_and_again_with_it():
         assert dev.status() == 0
         want.remap([0, 1, 2])
         check(dev, want)
+
+
+def test_more_rows_than_positions_after_a_refusal():
+    """An empty sequence whose prompt finds no room: the refusal is what is reported."""
+    dev, want, rng = full_pool(5, (64, 10, 0))
+    before = state(dev)
+    rows = dev_rows(normal(rng, (2, 70, ref.ROW)))
+    dev.grow(i32([0, 0, 70]))
+    dev.clear_status()
+    dev.append(rows, i32([0, 0, 0, 70]))
+    assert dev.status() == _lib.ABORT_NO_PAGE and same(dev, before)
+    dev.append(rows, i32([0, 0, 20, 70]))
+    assert dev.status() == _lib.ABORT_NO_PAGE and same(dev, before)
