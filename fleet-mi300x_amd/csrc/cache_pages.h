@@ -101,7 +101,8 @@ struct Header {
     int32_t count;              // pages to copy
     int32_t used;               // the first page that compact may have moved
     uint32_t refused;           // why the last grow changed nothing, or 0: append writes only then
-    int32_t pad[58];
+    uint32_t remaps;            // calls of remap: what was found of the table before is stale
+    int32_t pad[57];
 };
 static_assert(sizeof(Header) == 256, "");
 struct Copy {

@@ -92,6 +92,7 @@ __global__ __launch_bounds__(kRemapThreads) void remap_kernel(fleet_cache c,
         if (p != s) c.table[(int64_t)s * c.max_pages + col0 + k] = p < 0 ? -1 : slab[p * kCols + k];
     }
     if (blockIdx.x != 0) return;
+    if (t == 0) h->remaps += 1;
     __syncthreads();
     for (int i = t; i < c.n_seqs; i += kRemapThreads) slab[i] = c.lens[i];
     __syncthreads();

@@ -1,0 +1,839 @@
+// Attention of sequences that share their first pages: fleet_cache_share and
+// fleet_cache_attend_shared (declarations in fleet_moe.h).
+//
+// Sequences of a group (a request's beams, requests behind one prompt) name the same pages
+// first. The softmax of a row over its positions splits into parts of positions, each with a
+// reference m, a sum l and a sum O of weighted rows, which are added as
+//   O = sum_i 2^(m_i - m) O_i,  l = sum_i 2^(m_i - m) l_i,
+// so the common pages are one part, in which the rows of all the group's sequences stand
+// together: each page is read, widened and multiplied once for 64 rows, where
+// fleet_cache_attend does it for every sequence's 16. What is a sequence's own is another part.
+//
+// A unit is up to 64 (token, head) rows and a range of pages: a group's rows over its
+// common pages, or a sequence's rows over the pages behind them. The steps (a page each) of all
+// units follow each other, and a workgroup a CU takes an equal share of them, across units
+// where it has to, so that neither the groups' sizes nor the lengths leave a CU idle. The
+// parts go to the caller's plan, and a second launch adds those of a row, in order.
+#include "attend_tile.h"
+
+namespace fleet_moe {
+namespace cache {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 64;               // rows of a unit
+constexpr int kGrid = kShares / 2;      // workgroups
+constexpr int kGridWaves = 8;
+constexpr int kGridThreads = kGridWaves * 64;
+constexpr int kPageRing = 3;
+
+// The plan: what share found, and the parts of an attention.
+struct PlanHeader {
+    uint32_t remaps;            // the cache's when share was called
+    uint32_t ok;                // the attention's starts were in order
+    int32_t pad[62];
+};
+static_assert(sizeof(PlanHeader) == 256, "");
+struct Group {
+    int32_t first, end;         // sequences
+    int32_t pages;              // common to those that hold anything
+    int32_t lead;               // one of these
+};
+struct Parts {                  // of a row and kind: part 0, part 1, part 1 + kStep, ..
+    int32_t at, next, count;
+    int32_t front;              // there are parts over common pages, too
+};
+constexpr int kPartStep = 2 * kTile;    // a workgroup has two slots
+constexpr int64_t kMaxPlanRows = 1 << 20;
+
+struct Plan {
+    PlanHeader* h;
+    Group* groups;              // [n_seqs]: a sequence's
+    Parts* meta;                // [2][rows]: over the common pages, over its own
+    f32x4* stat;                // [2 rows + slots]
+    float* part;                // [2 rows + slots][512]
+};
+__host__ __device__ inline int64_t plan_parts(int64_t rows) {
+    return 2 * rows + (int64_t)kGrid * kPartStep;
+}
+inline size_t plan_size(int n_seqs, int64_t rows) {
+    return sizeof(PlanHeader) + up256((size_t)n_seqs * sizeof(Group)) +
+           up256((size_t)rows * 2 * sizeof(Parts)) + (size_t)plan_parts(rows) * (16 + 4 * kC);
+}
+inline Plan plan_at(void* p, int n_seqs, int64_t rows) {
+    char* c = static_cast<char*>(p);
+    Plan r;
+    r.h = reinterpret_cast<PlanHeader*>(c);
+    c += sizeof(PlanHeader);
+    r.groups = reinterpret_cast<Group*>(c);
+    c += up256((size_t)n_seqs * sizeof(Group));
+    r.meta = reinterpret_cast<Parts*>(c);
+    c += up256((size_t)rows * 2 * sizeof(Parts));
+    r.stat = reinterpret_cast<f32x4*>(c);
+    r.part = reinterpret_cast<float*>(c + (size_t)plan_parts(rows) * 16);
+    return r;
+}
+
+// ---------------------------------------------------------------- share
+
+// A workgroup a group: the leading pages that all its sequences with positions name, as far as
+// all of them have filled them. (An append writes no such page, so the number stays right
+// until sequences move.)
+constexpr int kShareThreads = 1024;
+__global__ __launch_bounds__(kShareThreads) void share_kernel(fleet_cache c, const int32_t* groups,
+                                                              int n_groups, int32_t* pages_out,
+                                                              Plan plan, Header* h) {
+    __shared__ int pages, lead;
+    const int t = threadIdx.x;
+    // offsets that do not increase from 0 to the sequences at most: no groups at all
+    bool bad = false;
+    for (int i = t; i <= n_groups; i += kShareThreads) {
+        const int at = groups[i];
+        bad |= at < 0 || at > c.n_seqs || (i > 0 && at < groups[i - 1]);
+    }
+    const bool none = __syncthreads_or(bad);
+    const int first = none ? 0 : groups[blockIdx.x], end = none ? 0 : groups[blockIdx.x + 1];
+    if (blockIdx.x == 0) {
+        if (t == 0) plan.h->remaps = h->remaps;
+        if (t == 0 && none) raise(h, FLEET_MOE_ABORT_POSITION);
+        const int lo = none ? 0 : groups[0], hi = none ? 0 : groups[n_groups];
+        for (int s = t; s < c.n_seqs; s += kShareThreads)
+            if (s < lo || s >= hi) plan.groups[s] = Group{s, s + 1, 0, s};
+    }
+    if (t == 0) {
+        pages = 0x7fffffff;
+        lead = 0x7fffffff;
+    }
+    __syncthreads();
+    int held = 0;
+    for (int s = first + t; s < end; s += kShareThreads) {
+        const int len = checked_len(c.lens[s], c.max_pages);
+        if (len > 0) {
+            ++held;
+            atomicMin(&pages, len / kPage);
+            atomicMin(&lead, s);
+        }
+    }
+    held = __syncthreads_count(held > 0);     // 0, 1, or more (not how many more)
+    int most = pages;
+    const int from = lead;
+    if (held == 0 || end - first < 2) most = 0;
+    __syncthreads();
+    // columns 64 at a time, a row a wave, until one differs
+    const int lane = t & 63, wave = t >> 6;
+    const int32_t* row = c.table + (int64_t)from * c.max_pages;
+    for (int j0 = 0; j0 < most; j0 += 64) {
+        const int j = j0 + lane;
+        const int mine = j < most ? row[j] : -1;
+        bool same = j >= most || (unsigned)mine < (unsigned)c.n_pages;
+        for (int s = first + wave; s < end && __ballot(same) == ~0ull; s += kShareThreads / 64) {
+            if (checked_len(c.lens[s], c.max_pages) <= 0) continue;
+            same = j >= most || c.table[(int64_t)s * c.max_pages + j] == mine;
+        }
+        const uint64_t all = __ballot(same);
+        if (all != ~0ull && lane == 0) atomicMin(&pages, j0 + __ffsll((long long)~all) - 1);
+        __syncthreads();
+        const int now = pages;
+        __syncthreads();
+        if (now < most) {
+            most = now;
+            break;
+        }
+    }
+    for (int s = first + t; s < end; s += kShareThreads)
+        plan.groups[s] = Group{first, end, most, from};
+    if (pages_out && t == 0) pages_out[blockIdx.x] = most;
+}
+
+// ---------------------------------------------------------------- the work
+
+struct SharedParams {
+    fleet_cache c;
+    const uint16_t* q;
+    const int32_t* start;
+    uint16_t* out;
+    float* lse;
+    Plan plan;
+    Header* h;
+    int64_t q_stride;
+    uint64_t per_head;          // head_divisor(n_heads)
+    int layer, n_tokens, n_heads;
+    float scale;                // times log2(e)
+    float slack;                // kSlack as a score: finite
+};
+
+__device__ __forceinline__ int start_of(const SharedParams& P, int s) {
+    return P.start ? clamp_row(ld_global(P.start + s), P.n_tokens) : s;
+}
+
+// What a sequence adds to the steps: its group's rows over their common pages, if it is the
+// group's first, and its own rows over what is behind them.
+struct Item {
+    int seq, tok0, n_new, len;
+    int first, end, pages, lead;        // its group
+    int units0, steps0, units1, steps1; // a unit's steps, whether they see anything or not
+    __device__ __forceinline__ int total() const { return units0 * steps0 + units1 * steps1; }
+};
+__device__ __forceinline__ Item item_of(const SharedParams& P, int seq, bool stale) {
+    Item w;
+    w.seq = seq;
+    w.first = seq;
+    w.end = seq + 1;
+    w.pages = 0;
+    w.lead = seq;
+    if (!stale) {
+        const i32x4 g = ld_global(reinterpret_cast<const i32x4*>(P.plan.groups + seq));
+        w.first = g.x;
+        w.end = g.y;
+        w.pages = g.z;
+        w.lead = g.w;
+    }
+    w.tok0 = start_of(P, seq);
+    w.n_new = start_of(P, seq + 1) - w.tok0;              // (negative: not in order)
+    w.len = checked_len(ld_global(P.c.lens + seq), P.c.max_pages);
+    w.units0 = w.steps0 = 0;
+    if (w.pages > 0 && seq == w.first) {
+        const int last = start_of(P, w.end);
+        w.units0 = last > w.tok0 ? ((last - w.tok0) * P.n_heads + kTile - 1) / kTile : 0;
+        w.steps0 = w.pages;
+    }
+    w.units1 = w.n_new > 0 ? (w.n_new * P.n_heads + kTile - 1) / kTile : 0;
+    const int own = w.len < 0 ? 0 : pages_of(w.len) - w.pages;
+    w.steps1 = own > 1 ? own : 1;
+    return w;
+}
+
+// A range of n things in `shares` parts that differ by one at most.
+struct Split {
+    int each, more;             // the first `more` have each + 1
+    __device__ Split(int n, int shares) : each(n / shares), more(n % shares) {}
+    __device__ int first(int i) const { return i * each + (i < more ? i : more); }
+    __device__ int holder(int at) const {
+        const int big = more * (each + 1);
+        return at < big ? at / (each + 1) : more + (at - big) / each;
+    }
+};
+
+// How many workgroups take part: a share of few pages is short, but each is a part to join.
+__device__ __forceinline__ int shares_of(int total) {
+    return total < kGrid ? total : kGrid;
+}
+
+// The sequence in whose steps workgroup wg begins, and where. Every wave for itself, a lane
+// a sequence, or several.
+struct Place {
+    int seq, off, total, shares;
+};
+__device__ __forceinline__ bool locate(const SharedParams& P, int wg, bool stale, Place& at) {
+    const int lane = threadIdx.x & 63;
+    const int each = (P.c.n_seqs + 63) / 64;
+    int n = 0;
+    bool bad = false;
+    for (int i = 0; i < each; ++i) {
+        const int s = lane * each + i;
+        if (s < P.c.n_seqs) {
+            const Item w = item_of(P, s, stale);
+            bad |= w.n_new < 0;
+            n += w.total();
+        }
+    }
+    bad = __ballot(bad) != 0;
+    if (wg == 0 && threadIdx.x == 0) {
+        P.plan.h->ok = !bad;
+        if (bad) raise(P.h, FLEET_MOE_ABORT_POSITION);
+    }
+    if (bad) return false;
+    int incl = wave_incl_scan(n);
+    at.total = __builtin_amdgcn_readlane(incl, 63);
+    at.shares = shares_of(at.total);
+    if (wg >= at.shares) return false;
+    int off = Split(at.total, at.shares).first(wg);
+    int owner = __popcll(__ballot(incl <= off));
+    off -= __builtin_amdgcn_readlane(incl - n, owner);
+    at.seq = owner;
+    if (each > 1) {
+        const int s = owner * each + lane;
+        n = lane < each && s < P.c.n_seqs ? item_of(P, s, stale).total() : 0;
+        incl = wave_incl_scan(n);
+        const int k = __popcll(__ballot(incl <= off));
+        off -= __builtin_amdgcn_readlane(incl - n, k);
+        at.seq = owner * each + k;
+    }
+    at.off = off;
+    return true;
+}
+
+// Up to 64 rows and the pages of a table row that they see.
+struct Unit {
+    int row0, rows;             // rows row0 .. of the sequence's or group's `rows`
+    int tok0;                   // the token of row 0
+    int base;                   // own pages: the position of that token
+    int first, end;             // common pages: the group
+    bool common;
+    const int32_t* table;       // from the first page on
+    int page0;
+    int n;                      // pages that some row may see
+};
+
+// The position of token `tok` (a lane's) of the sequences [first, end).
+__device__ __forceinline__ int position_of(const SharedParams& P, int first, int end, int tok) {
+    int s = tok;
+    if (P.start) {
+        const int lane = threadIdx.x & 63;
+        s = first;              // and how many sequences end at tok or before
+        for (int s0 = first; s0 < end; s0 += 64) {
+            const int z = s0 + lane < end ? start_of(P, s0 + lane + 1) : 0x7fffffff;
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) n += __builtin_amdgcn_readlane(z, j) <= tok;
+            s += n;
+            if (!__ballot(n == 64)) break;
+        }
+    }
+    if (s >= end) return -1;
+    const int len = checked_len(ld_global(P.c.lens + s), P.c.max_pages);
+    return len < 0 ? -1 : len - (start_of(P, s + 1) - tok);
+}
+
+// A lane's row.
+struct TileRow {
+    bool live;
+    int tok, head, pos;         // dead rows: the unit's first
+};
+__device__ __forceinline__ TileRow tile_row(const SharedParams& P, const Unit& u, int row) {
+    TileRow r;
+    r.live = row < u.rows;
+    if (!r.live) row = u.row0;
+    const int t = token_of_row(row, P.per_head);
+    r.tok = u.tok0 + t;
+    r.head = row - t * P.n_heads;
+    r.pos = -1;
+    return r;
+}
+
+struct PageLds {
+    __attribute__((aligned(16))) uint8_t tile[kPageRing][4 * kBlockStep];
+    uint32_t scale[kPageRing][8];
+    f32x4 half[kGridWaves][2][64];  // half of the scores of a tile and two blocks
+    u32x4 p[2][4][2][64];       // [step parity][tile][half of the page][lane]
+    int flag[2][kGridWaves];
+    float m[4][16], top[4][2][16], sum[4][2][16], rounded[4][2][16];
+    Item item;                  // what follows a unit, out of the registers meanwhile
+    int at, off;
+};
+static_assert(sizeof(PageLds) <= 160 * 1024, "");
+
+// Pages of 64 steps, one per lane.
+struct PageList {
+    int held, from, page;
+};
+__device__ __forceinline__ int page_of(const Unit& u, PageList& h, int i, int end, int lane) {
+    if (i >= h.held) {
+        h.from = i - 4;         // (the steps whose scores are not finished yet)
+        h.held = h.from + 64;
+        const int mine = h.from + lane;
+        h.page = mine >= 0 && mine < end ? ld_global(u.table + mine) : 0;
+        // here, not at the use: there the compiler would wait, every step, for
+        // whatever copies are in flight
+        __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0)
+    }
+    return __builtin_amdgcn_readlane(h.page, i - h.from);
+}
+
+constexpr int kTileHalf = kChunks / 4;          // steps of a wave
+__device__ __forceinline__ void load_q(const SharedParams& P, const TileRow& r, int g, int half,
+                                       bf16x8 (&q)[kTileHalf]) {
+    const uint16_t* src = P.q + (int64_t)r.tok * P.q_stride + r.head * kRow + g * 16;
+    const auto at = [&](int v) {
+        return __builtin_bit_cast(bf16x8, ld_global(reinterpret_cast<const u32x4*>(src + v)));
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        q[2 * i] = at((2 * i + half) * 64);
+        q[2 * i + 1] = at((2 * i + half) * 64 + 8);
+    }
+    q[8] = at(8 * 64 + half * 8);
+}
+
+// Pages off .. off + cnt - 1 of a unit; its results to `out` and `lse` if `at` is negative,
+// else as the parts at + row.
+//
+// Eight waves: wave (tile pair, half, block pair) takes half of the 576 products of 32 rows
+// with 32 positions, so that a widened K operand serves two tiles; it exchanges halves with
+// its partner, makes the weights of one tile and 32 positions, and adds its 64 columns of O
+// for all rows over the whole page, where a widened V operand serves four tiles.
+__device__ __forceinline__ void attend(const SharedParams& P, PageLds& L, const Unit& u, int off,
+                                       int cnt, int64_t to_part) {
+    constexpr int kCols = kC / 16 / kGridWaves; // of 16
+    // (fm_tid: no lane's index is kept in a register from one unit to the next)
+    const int t = fm_tid(), lane = t & 63, wave = wave_bcast(t >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int bp = wave & 1, half = wave >> 1 & 1, tp = wave >> 2;
+    const int mine = 2 * tp + half;             // the tile whose weights this wave makes
+
+    TileRow r = tile_row(P, u, u.row0 + mine * 16 + n);
+    bf16x8 q[2][kTileHalf];                     // of `mine` and of the pair's other tile
+    load_q(P, r, g, half, q[0]);
+    load_q(P, tile_row(P, u, u.row0 + (mine ^ 1) * 16 + n), g, half, q[1]);
+    if (u.common) {
+        const int pos = position_of(P, u.first, u.end, r.tok);
+        r.pos = r.live ? pos : -1;
+    } else {
+        r.pos = r.live ? u.base + r.tok - u.tok0 : -1;
+    }
+    // the position that all rows of the wave see, apart from the dead ones
+    int common = r.live ? r.pos : 0x7fffffff;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        const int o = __shfl_xor(common, d);
+        common = o < common ? o : common;
+    }
+    common = wave_bcast(common);
+    f32x4 acc[4][kCols];
+#pragma unroll
+    for (auto& a : acc)
+#pragma unroll
+        for (auto& b : a) b = f32x4{0.f, 0.f, 0.f, 0.f};
+    // the sum of the rounded weights of tile wave & 3 and half of the page wave >> 2
+    f32x4 ones{0.f, 0.f, 0.f, 0.f};
+    // Every row's reference, as a score and as it is in the exponent: any score not far below
+    // the maximum, because weights up to 2^kSlack are as exact as those up to 1, and moving
+    // it costs a pass over O and two barriers.
+    float m = -INFINITY, ref = -INFINITY, l = 0.f;
+    const float slack = P.slack;
+    f32x4 z[2];                                 // the scores of `mine` and the two blocks
+    float p0[4], p1[4];
+    bool stray = false;                         // a score of the wave is not finite
+    if (t < 64) L.m[t >> 4][n] = -INFINITY;
+    PageList pages{0, 0, 0};
+    if (cnt > 0) page_of(u, pages, off, off + cnt, lane);
+    // q is there before a copy is issued, also as far as the compiler counts
+    __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0)
+
+    // (b is k % kPageRing, counted)
+    const auto issue = [&](int k, int b) {
+        const int page = page_of(u, pages, off + k, off + cnt, lane);
+        const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
+        const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
+        // a wave a block; the first the scales too
+        const uint8_t* from = src + wave * kBlockBytes + lane * 16;
+        const uint32_t to = lds_addr(L.tile[b]) + wave * kBlockStep;
+        copy_kb<4, false>(from, to);
+        copy_kb<4, false>(from + 4096, to + 4096);
+        copy_kb<1, false>(from + 8192, to + 8192);
+        if (wave == 0 && lane < 2)
+            copy_kb<1, false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[b]));
+    };
+    const auto score = [&](int b) {
+        u32x4 c[2][4];
+        uint2 e[2];
+        uint32_t f[2][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint8_t* block = L.tile[b] + (2 * bp + j) * kBlockStep + lane * 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                c[j][i] = *reinterpret_cast<const u32x4*>(block + (2 * i + half) * 1024);
+            e[j] = *reinterpret_cast<const uint2*>(block + 8 * 1024 + half * 8);
+            f[j][0] = L.scale[b][2 * (2 * bp + j)];
+            f[j][1] = L.scale[b][2 * (2 * bp + j) + 1];
+        }
+        __builtin_amdgcn_sched_barrier(0);      // every read on its way
+        f32x4 y[2][2];                          // [tile][block]
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float sc = any_scale(f[j][0]), sp = any_scale(f[j][1]);
+            y[0][j] = y[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u32x4 a = c[j][i];
+                const bf16x8 lo = widen(a.x, a.y, sc, sc), hi = widen(a.z, a.w, sc, sc);
+                y[0][j] = mfma(lo, q[0][2 * i], y[0][j]);
+                y[1][j] = mfma(lo, q[1][2 * i], y[1][j]);
+                y[0][j] = mfma(hi, q[0][2 * i + 1], y[0][j]);
+                y[1][j] = mfma(hi, q[1][2 * i + 1], y[1][j]);
+            }
+            const bf16x8 pe = widen(e[j].x, e[j].y, sp, sp);
+            y[0][j] = mfma(pe, q[0][8], y[0][j]);
+            y[1][j] = mfma(pe, q[1][8], y[1][j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            z[j] = y[0][j];
+            L.half[wave][j][lane] = y[1][j];
+        }
+    };
+    const auto weigh = [&](int k) {
+        const float down = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            p0[j] = exp2_(fmaf(z[0][j], P.scale, -down));
+            p1[j] = exp2_(fmaf(z[1][j], P.scale, -down));
+        }
+        const uint2 a = weights(p0), b = weights(p1);
+        L.p[k & 1][mine][bp][lane] = u32x4{a.x, a.y, b.x, b.y};
+    };
+    const auto finish = [&](int k) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) z[j] += L.half[wave ^ 2][j][lane];
+        const int page = page_of(u, pages, off + k, off + cnt, lane);
+        const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
+        const int base = (u.page0 + off + k) * kPage + bp * 32;
+        const f32x4 both = z[0] + z[1];
+        const bool bad = !finite((both[0] + both[1]) + (both[2] + both[3]));
+        if (!(ok && base + 31 <= common)) {
+            asm volatile("");                   // a branch, not forty instructions every step
+            if (!ok && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    z[j][i] = (ok & (base + kBlock * j + 4 * g + i <= r.pos)) ? z[j][i] : -INFINITY;
+        }
+        weigh(k);
+        const float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
+                                fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
+        stray = __ballot(bad) != 0;
+        const bool high = __ballot(top > m + slack) != 0;
+        if (lane == 0) L.flag[k & 1][wave] = stray | high;
+    };
+    // What is rare: a row's scores beyond its reference, or one that is not finite, in step k.
+    const auto mend = [&](int k, int b) {
+        float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
+                          fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
+        top = xor32_max(xor16_max(top));
+        if (lane < 16) L.top[mine][bp][lane] = top;
+        if (stray && half == 0 && tp == 0)
+            for (int j = 0; j < 2; ++j)
+                clean(L.tile[b] + (2 * bp + j) * kBlockStep, L.scale[b][2 * (2 * bp + j)], lane);
+        barrier();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float was = L.m[i][n];
+            const float to = fmaxf(was, fmaxf(L.top[i][0][n], L.top[i][1][n]));
+            const float shrink = shrink_to(to * P.scale, was * P.scale);
+            if (i == mine) {
+                m = to;
+                ref = reference(to * P.scale);
+                l *= shrink;
+            }
+            if (i == (wave & 3)) ones *= shrink;
+#pragma unroll
+            for (auto& a : acc[i]) a *= shrink;
+        }
+        weigh(k);
+        barrier();
+        if (bp == 0 && lane < 16) L.m[mine][lane] = m;
+    };
+    // O over step k
+    const auto add = [&](int k, int b) {
+        uint32_t first = lds_addr(L.tile[b]) + wave * kCols * 256 + column_at(lane);
+        asm("" : "+v"(first));                // one address, the rest is offsets
+        bf16x8 pb[2][4];
+        i32x2 v[2][kCols];
+        uint32_t f[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t col = first + 2 * h * kBlockStep;
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) v[h][i] = column(col, i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pb[h][j] = __builtin_bit_cast(bf16x8, L.p[k & 1][j][h][lane]);
+            f[h][0] = L.scale[b][4 * h];
+            f[h][1] = L.scale[b][4 * h + 2];
+        }
+        __builtin_amdgcn_sched_barrier(0);      // every read on its way
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float sa = any_scale(f[h][0]), sb = any_scale(f[h][1]);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) {
+                const bf16x8 a = widen((uint32_t)v[h][i].x, (uint32_t)v[h][i].y, sa, sb);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j][i] = mfma(a, pb[h][j], acc[j][i]);
+            }
+        }
+        ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}),
+                    __builtin_bit_cast(bf16x8, L.p[k & 1][wave & 3][wave >> 2][lane]), ones);
+    };
+
+    if (tp == 0)
+        for (int k = 0; k < kPageRing - 1 && k < cnt; ++k) issue(k, k);
+    wait_copies<0>();
+    barrier();
+    if (cnt > 0) {
+        score(0);
+        barrier();
+        finish(0);
+    }
+    // Step k: behind barrier A the weights of k and the rows of k + 1 are there, behind
+    // B both halves of the scores of k + 1.
+    int b = 0;                                  // of step k
+    for (int k = 0; k < cnt; ++k) {
+        const int b1 = b == kPageRing - 1 ? 0 : b + 1, b2 = b1 == kPageRing - 1 ? 0 : b1 + 1;
+        wait_copies<0>();                       // step k + 1
+        barrier();                              // A
+        const int* f = L.flag[k & 1];
+        const int flags = ((f[0] | f[1]) | (f[2] | f[3])) | ((f[4] | f[5]) | (f[6] | f[7]));
+        if (tp == 0 && k + kPageRing - 1 < cnt) issue(k + kPageRing - 1, b2);  // where step k - 1 was
+        if (wave_bcast(flags)) mend(k, b);
+        l += ((p0[0] + p0[1]) + (p0[2] + p0[3])) + ((p1[0] + p1[1]) + (p1[2] + p1[3]));
+        if (k + 1 < cnt) {
+            score(b1);
+            barrier();                          // B
+            finish(k + 1);
+        }
+        add(k, b);
+        b = b1;
+        asm("" : "+s"(b));
+    }
+    // the sums of the blocks, and of the page's halves
+    l = xor32_sum(xor16_sum(l));
+    if (lane < 16) {
+        L.sum[mine][bp][lane] = l;
+        L.rounded[wave & 3][wave >> 2][lane] = ones[0];
+        if (bp == 0) L.m[mine][lane] = m;
+    }
+    barrier();
+    const int column0 = wave * kCols * 16 + 4 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 16 + n;
+        if (u.row0 + row >= u.rows) continue;
+        const float sum = L.sum[i][0][n] + L.sum[i][1][n];
+        const float rounded = L.rounded[i][0][n] + L.rounded[i][1][n];
+        const float scaled = L.m[i][n] * P.scale;
+        if (to_part < 0) {
+            const int64_t to = (int64_t)u.tok0 * P.n_heads + u.row0 + row;
+            const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+                put(P.out + to * kC + column0 + j * 16, acc[i][j], inv);
+            if (P.lse && wave == 0 && g == 0) P.lse[to] = lse_of(scaled, sum);
+        } else {
+            const int64_t to = to_part + row;
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+                st_global(reinterpret_cast<f32x4*>(P.plan.part + to * kC + column0 + j * 16), acc[i][j]);
+            if (wave == 0 && g == 0) st_global(P.plan.stat + to, f32x4{scaled, sum, rounded, 0.f});
+        }
+    }
+}
+
+__global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    PageLds& L = *reinterpret_cast<PageLds*>(lds);
+    const int t = threadIdx.x, wg = blockIdx.x;
+    // sequences have moved since share: every one by itself
+    const bool stale = ld_global(&P.plan.h->remaps) != ld_global(&P.h->remaps);
+    Place place;
+    if (!locate(P, wg, stale, place)) return;
+    const Split share(place.total, place.shares);
+    const int64_t all_rows = (int64_t)P.n_tokens * P.n_heads;
+    int at = share.first(wg), off = place.off;
+    Item w = item_of(P, place.seq, stale);
+    for (;;) {
+        // the unit of the item's step `off`
+        Unit u;
+        const int n0 = w.units0 * w.steps0;
+        u.common = off < n0;
+        const int steps = u.common ? w.steps0 : w.steps1, o = u.common ? off : off - n0;
+        const int k = o / steps, from = o - k * steps;
+        u.row0 = k * kTile;
+        u.tok0 = w.tok0;
+        u.first = w.first;
+        u.end = w.end;
+        if (u.common) {
+            u.rows = (start_of(P, w.end) - w.tok0) * P.n_heads;
+            u.base = 0;
+            u.page0 = 0;
+            u.n = steps;
+            u.table = P.c.table + (int64_t)w.lead * P.c.max_pages;
+        } else {
+            u.rows = w.n_new * P.n_heads;
+            u.base = w.len - w.n_new;
+            u.page0 = w.pages;
+            u.table = P.c.table + (int64_t)w.seq * P.c.max_pages + w.pages;
+            // up to the position of the unit's last token
+            const int last = u.row0 + kTile - 1 < u.rows ? u.row0 + kTile - 1 : u.rows - 1;
+            const int p = u.base + token_of_row(last, P.per_head);
+            u.n = w.len < 0 || p < 0 ? 0 : pages_of((int64_t)p + 1) - w.pages;
+            if (w.len < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
+        }
+        const int left = share.first(wg + 1) - at;
+        const int take = steps - from < left ? steps - from : left;
+        const int to = from + take < u.n ? from + take : u.n;
+        // where the part goes: a whole unit's to its rows, or to one of two slots
+        const bool whole = take == steps;
+        const int64_t row = (int64_t)u.tok0 * P.n_heads + u.row0;
+        const int64_t slots = 2 * all_rows;
+        const int64_t part =
+            whole ? (u.common ? row : w.pages > 0 ? all_rows + row : -1)
+                  : slots + (int64_t)(2 * wg + (from == 0 ? 1 : 0)) * kTile;
+        if (from == 0 && t < kTile && u.row0 + t < u.rows) {
+            const int last = share.holder(at + steps - 1);
+            Parts m;
+            m.at = (int)(part + t);
+            m.next = (int)(slots + (int64_t)(wg + 1) * kPartStep + t);
+            m.count = part < 0 ? 0 : whole ? 1 : last - wg + 1;
+            m.front = !u.common && w.pages > 0;
+            P.plan.meta[(u.common ? 0 : all_rows) + row + t] = m;
+        }
+        if (t == 0) {
+            L.item = w;
+            L.at = at + take;
+            L.off = off + take;
+        }
+        attend(P, L, u, from, to > from ? to - from : 0, part);
+        barrier();                              // LDS is free again
+        at = L.at;
+        if (at >= share.first(wg + 1)) return;
+        w = L.item;
+        off = L.off;
+        while (off >= w.total()) {
+            if (w.seq + 1 >= P.c.n_seqs) return;
+            w = item_of(P, w.seq + 1, stale);
+            off = 0;
+        }
+        barrier();
+    }
+}
+
+// Adds the parts of a row, those over common pages first: a wave a row, 16 parts at a time.
+constexpr int kJoinRows = 4, kJoinParts = 16;
+__global__ __launch_bounds__(64 * kJoinRows) void join_kernel(SharedParams P) {
+    const int lane = threadIdx.x & 63;
+    const int64_t all_rows = (int64_t)P.n_tokens * P.n_heads;
+    const int64_t row = (int64_t)blockIdx.x * kJoinRows + wave_bcast(threadIdx.x >> 6);
+    if (row >= all_rows) return;
+    const i32x4 own = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + all_rows + row));
+    const i32x4 front = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + row));
+    // (rows that are nobody's have no parts of this call)
+    if (row < (int64_t)start_of(P, 0) * P.n_heads ||
+        row >= (int64_t)start_of(P, P.c.n_seqs) * P.n_heads || !ld_global(&P.plan.h->ok) ||
+        own.z == 0)
+        return;
+    const int n0 = own.w ? front.z : 0, count = n0 + own.z;
+    const auto slot = [&](int i) -> int64_t {
+        const bool mine = i >= n0;
+        const int j = mine ? i - n0 : i;
+        const int first = mine ? own.x : front.x, next = mine ? own.y : front.y;
+        return j == 0 ? first : next + (int64_t)(j - 1) * kPartStep;
+    };
+    f32x4 v[kJoinParts][2];
+    const auto load = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < kJoinParts; ++i) {
+            if (i0 + i >= count) break;
+            const f32x4* at =
+                reinterpret_cast<const f32x4*>(P.plan.part + slot(i0 + i) * kC) + lane;
+            v[i][0] = ld_global(at);
+            v[i][1] = ld_global(at + 64);
+        }
+    };
+    load(0);
+    float top = -INFINITY;
+    for (int i = lane; i < count; i += 64) top = fmaxf(top, ld_global(P.plan.stat + slot(i))[0]);
+    top = wave_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float f = 0.f, sum = 0.f, rounded = 0.f;
+    f32x4 o[2]{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int i0 = 0;;) {
+        if (i0 % 64 == 0) {                     // the weights of 64 parts, a lane each
+            f32x4 st{-INFINITY, 0.f, 0.f, 0.f};
+            if (i0 + lane < count) st = ld_global(P.plan.stat + slot(i0 + lane));
+            f = exp2_(st[0] - ref);
+            sum += f * st[1];
+            rounded += f * st[2];
+        }
+#pragma unroll
+        for (int i = 0; i < kJoinParts; ++i) {
+            if (i0 + i >= count) break;
+            const float weight = __builtin_bit_cast(
+                float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i0 % 64 + i));
+            o[0] += v[i][0] * weight;
+            o[1] += v[i][1] * weight;
+        }
+        i0 += kJoinParts;
+        if (i0 >= count) break;
+        load(i0);
+    }
+    static_assert(64 % kJoinParts == 0, "");
+    sum = wave_sum(sum);
+    rounded = wave_sum(rounded);
+    const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
+    put(P.out + row * kC + 4 * lane, o[0], inv);
+    put(P.out + row * kC + 4 * lane + 256, o[1], inv);
+    if (P.lse && lane == 0) P.lse[row] = lse_of(top, sum);
+}
+
+}  // namespace cache
+}  // namespace fleet_moe
+
+using namespace fleet_moe;
+using namespace fleet_moe::cache;
+
+int fleet_moe_check_device(int min_cus);
+
+extern "C" size_t fleet_cache_plan_bytes(int32_t n_seqs, int32_t max_tokens, int32_t n_heads) {
+    if (n_seqs < 1 || n_seqs > kMaxSeqs || max_tokens < 1 || n_heads < 1 ||
+        n_heads > FLEET_CACHE_MAX_HEADS || (int64_t)max_tokens * n_heads > kMaxPlanRows)
+        return 0;
+    return plan_size(n_seqs, (int64_t)max_tokens * n_heads);
+}
+
+extern "C" int fleet_cache_share(const fleet_cache* cache, const int32_t* groups,
+                                 int32_t n_groups, int32_t* pages, void* plan, size_t plan_bytes,
+                                 void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (int e = check_cache(cache, workspace, workspace_bytes)) return e;
+    if (!groups || (uintptr_t)groups % 4 || (uintptr_t)pages % 4 || n_groups < 1 ||
+        n_groups > cache->n_seqs || !plan || (uintptr_t)plan % 256)
+        return FLEET_MOE_ERR_ARG;
+    if (plan_bytes < plan_size(cache->n_seqs, 0)) return FLEET_MOE_ERR_WORKSPACE;
+    if (int e = fleet_moe_check_device(1)) return e;
+    hipLaunchKernelGGL(share_kernel, dim3(n_groups), dim3(kShareThreads), 0, stream, *cache, groups,
+                       n_groups, pages, plan_at(plan, cache->n_seqs, 0),
+                       static_cast<Header*>(workspace));
+    return (int)hipGetLastError();
+}
+
+extern "C" int fleet_cache_attend_shared(const fleet_cache* cache, int32_t layer,
+                                         const uint16_t* q, int64_t q_stride,
+                                         const int32_t* start, int32_t n_tokens, int32_t n_heads,
+                                         float scale, uint16_t* out, float* lse, void* plan,
+                                         size_t plan_bytes, void* workspace,
+                                         size_t workspace_bytes, hipStream_t stream) {
+    if (int e = check_cache(cache, workspace, workspace_bytes)) return e;
+    const int64_t rows = (int64_t)n_tokens * n_heads;
+    if (layer < 0 || layer >= cache->n_layers || n_tokens < 0 || n_heads < 1 ||
+        n_heads > FLEET_CACHE_MAX_HEADS || rows > kMaxPlanRows || !(scale > 0.f) ||
+        !(scale * kLog2e <= FLT_MAX) || (uintptr_t)start % 4 ||
+        (!start && n_tokens != cache->n_seqs) || !plan || (uintptr_t)plan % 256)
+        return FLEET_MOE_ERR_ARG;
+    if (n_tokens == 0) return 0;
+    if (!q || !out || (uintptr_t)q % 16 || (uintptr_t)out % 8 || (uintptr_t)lse % 4 ||
+        q_stride < (int64_t)n_heads * kRow || q_stride % 8 || q_stride > ((int64_t)1 << 32))
+        return FLEET_MOE_ERR_ARG;
+    // the steps of all units are counted in 32 bits
+    if ((2 * (rows / kTile) + 2 * (int64_t)cache->n_seqs) * cache->max_pages > 0x7fffffff)
+        return FLEET_MOE_ERR_ARG;
+    if (plan_bytes < plan_size(cache->n_seqs, rows)) return FLEET_MOE_ERR_WORKSPACE;
+    if (int e = fleet_moe_check_device(1)) return e;
+    SharedParams P{};
+    P.c = *cache;
+    P.q = q;
+    P.start = start;
+    P.out = out;
+    P.lse = lse;
+    P.plan = plan_at(plan, cache->n_seqs, rows);
+    P.h = static_cast<Header*>(workspace);
+    P.q_stride = q_stride;
+    P.per_head = head_divisor(n_heads);
+    P.layer = layer;
+    P.n_tokens = n_tokens;
+    P.n_heads = n_heads;
+    P.scale = scale * kLog2e;
+    P.slack = fminf(kSlack / P.scale, FLT_MAX);
+    if (int e = launch<shared_kernel>(kGrid, kGridThreads, sizeof(PageLds), P, stream)) return e;
+    return launch<join_kernel>((rows + kJoinRows - 1) / kJoinRows, 64 * kJoinRows, 0, P, stream);
+}

@@ -1,0 +1,281 @@
+// Rotary positions: fleet_rope_rotate and fleet_cache_rotate (declarations in
+// fleet_moe.h).
+//
+// A pair (a, b) of a head's values becomes (a cos - b sin, b cos + a sin), with the angle
+// of its position and frequency; the bytes of x and out bound many tokens, a launch's
+// latency few. An angle costs some sixty instructions and serves all heads of its token, so
+// a thread takes the same four pairs of several heads where there are enough tokens.
+#include <math.h>
+
+#include "cache_pages.h"
+#include "rope.h"
+
+namespace fleet_moe {
+namespace rope {
+
+struct Params {
+    fleet_rope r;
+    const void* x;
+    void* out;
+    int64_t x_token, x_head, o_token, o_head;
+    const int32_t* positions;   // or from the cache:
+    const int32_t* lens;
+    const int32_t* start;
+    cache::Header* h;
+    int n_seqs, max_pages;
+    int n_tokens, n_heads, width, at;
+    int items;                  // of a head: four pairs or four other values each (or one)
+    int pairs;                  // items that are pairs
+    int parts;                  // groups of heads
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+template <class T, int kN>
+struct Few {                    // kN neighbouring values
+    float v[kN];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kN == 4 && sizeof(T) == 4) {
+            const f32x4 w = ld_global(reinterpret_cast<const f32x4*>(p));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = w[i];
+        } else if constexpr (kN == 4) {
+            const uint64_t w = ld_global(reinterpret_cast<const uint64_t*>(p));
+            v[0] = bf_lo((uint32_t)w);
+            v[1] = bf_hi((uint32_t)w);
+            v[2] = bf_lo((uint32_t)(w >> 32));
+            v[3] = bf_hi((uint32_t)(w >> 32));
+        } else if constexpr (sizeof(T) == 4) {
+            v[0] = ld_global(p);
+        } else {
+            v[0] = __uint_as_float((uint32_t)ld_global(p) << 16);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kN == 4 && sizeof(T) == 4) {
+            st_global(reinterpret_cast<f32x4*>(p), f32x4{v[0], v[1], v[2], v[3]});
+        } else if constexpr (kN == 4) {
+            bf16x4 b;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = (__bf16)v[i];
+            st_global(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, b));
+        } else if constexpr (sizeof(T) == 4) {
+            st_global(p, v[0]);
+        } else {
+            st_global(p, __builtin_bit_cast(uint16_t, (__bf16)v[0]));
+        }
+    }
+};
+
+// The position of a token, from the sequences' lengths, if it has one.
+__device__ __forceinline__ bool cache_position(const Params& P, const int* start, int token,
+                                               bool lead, int& pos) {
+    int s = token, a = token, z = token + 1;
+    if (P.start) {
+        int lo = 0, hi = P.n_seqs;                        // the last s with start[s] <= token
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (start[mid] <= token) lo = mid;
+            else hi = mid - 1;
+        }
+        if (lo >= P.n_seqs) return false;
+        s = lo;
+        a = start[s];
+        z = start[s + 1];
+        if (token < a || token >= z) return false;        // nobody's
+    }
+    const int len = cache::checked_len(ld_global(P.lens + s), P.max_pages);
+    pos = len - (z - token);
+    if (len >= 0 && pos >= 0) return true;
+    if (lead) cache::raise(P.h, FLEET_MOE_ABORT_POSITION);
+    return false;
+}
+
+constexpr int kThreads = 256;
+
+// Thread (slot, item) of a workgroup; a slot is a token and kHeads of its heads. kN is 4
+// where everything lies in groups of four values.
+template <class T, int kN, int kHeads>
+__global__ __launch_bounds__(kThreads) void rope_kernel(Params P) {
+    __shared__ int starts[cache::kMaxSeqs + 1];
+    if (!P.positions && P.start) {
+        for (int i = threadIdx.x; i <= P.n_seqs; i += kThreads)
+            starts[i] = cache::clamp_row(ld_global(P.start + i), P.n_tokens);
+        __syncthreads();
+    }
+    const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t slot = id / P.items;
+    const int item = (int)(id - slot * P.items);
+    const int64_t tok = slot / P.parts;
+    if (tok >= P.n_tokens) return;
+    const int token = (int)tok, head0 = (int)(slot - tok * P.parts) * kHeads;
+    int pos = 0;
+    if (P.positions) pos = ld_global(P.positions + token);
+    else if (!cache_position(P, starts, token, item == 0 && head0 == 0, pos)) return;
+    const T* x = static_cast<const T*>(P.x) + token * P.x_token;
+    T* out = static_cast<T*>(P.out) + token * P.o_token;
+    const int half = P.r.dim / 2;
+    if (item < P.pairs) {
+        const int p = item * kN;
+        // (the first values of the pairs and their second ones, or pairs as they are)
+        const int xa = P.at + (P.r.halves_in ? p : 2 * p), xb = P.r.halves_in ? xa + half : xa + kN;
+        const int oa = P.at + (P.r.halves_out ? p : 2 * p);
+        const int ob = P.r.halves_out ? oa + half : oa + kN;
+        float2 cs[kN];
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            cs[i] = angle(ld_global(P.r.turns + p + i), pos, P.r.magnitude);
+        Few<T, kN> a[kHeads], b[kHeads];
+#pragma unroll
+        for (int j = 0; j < kHeads; ++j)
+            if (head0 + j < P.n_heads) {
+                a[j].load(x + (head0 + j) * P.x_head + xa);
+                b[j].load(x + (head0 + j) * P.x_head + xb);
+            }
+#pragma unroll
+        for (int j = 0; j < kHeads; ++j) {
+            if (head0 + j >= P.n_heads) break;
+            const auto at = [&](int k) { return k < kN ? a[j].v[k] : b[j].v[k - kN]; };
+            Few<T, kN> first, second;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                const float u = P.r.halves_in ? a[j].v[i] : at(2 * i);
+                const float v = P.r.halves_in ? b[j].v[i] : at(2 * i + 1);
+                first.v[i] = fmaf(u, cs[i].x, -(v * cs[i].y));
+                second.v[i] = fmaf(v, cs[i].x, u * cs[i].y);
+            }
+            if (!P.r.halves_out) {
+                const Few<T, kN> f = first, s = second;
+#pragma unroll
+                for (int k = 0; k < 2 * kN; ++k)
+                    (k < kN ? first.v[k] : second.v[k - kN]) = k % 2 ? s.v[k / 2] : f.v[k / 2];
+            }
+            first.store(out + (head0 + j) * P.o_head + oa);
+            second.store(out + (head0 + j) * P.o_head + ob);
+        }
+    } else {
+        // what is beside the rotated part
+        int at = (item - P.pairs) * kN;
+        if (at >= P.at) at += P.r.dim;
+        Few<T, kN> a[kHeads];
+#pragma unroll
+        for (int j = 0; j < kHeads; ++j)
+            if (head0 + j < P.n_heads) a[j].load(x + (head0 + j) * P.x_head + at);
+#pragma unroll
+        for (int j = 0; j < kHeads; ++j)
+            if (head0 + j < P.n_heads) a[j].store(out + (head0 + j) * P.o_head + at);
+    }
+}
+
+}  // namespace rope
+}  // namespace fleet_moe
+
+using namespace fleet_moe;
+using namespace fleet_moe::rope;
+
+int fleet_moe_check_device(int min_cus);
+
+int fleet_moe_check_rope(const fleet_rope* r) {
+    if (!r || !r->turns || (uintptr_t)r->turns % 8 || r->dim < 2 || r->dim > FLEET_ROPE_MAX_DIM ||
+        r->dim % 2 || (r->halves_in | 1) != 1 || (r->halves_out | 1) != 1 ||
+        !(fabsf(r->magnitude) <= 3.402823466e38f))
+        return FLEET_MOE_ERR_ARG;
+    return 0;
+}
+
+template <class T, int kN>
+static int launch_rope(Params& P, hipStream_t stream) {
+    const bool same = P.out == P.x;               // then what is not rotated is there
+    P.pairs = P.r.dim / 2 / kN;
+    P.items = P.pairs + (same ? 0 : (P.width - P.r.dim) / kN);
+    // Four heads a thread where that still leaves two workgroups a CU.
+    const bool many = (int64_t)P.n_tokens * ((P.n_heads + 3) / 4) * P.items >= 512 * kThreads;
+    P.parts = many ? (P.n_heads + 3) / 4 : P.n_heads;
+    const int64_t n = (int64_t)P.n_tokens * P.parts * P.items;
+    const int64_t grid = (n + kThreads - 1) / kThreads;
+    if (grid > 0x7fffffff) return FLEET_MOE_ERR_ARG;
+    if (many)
+        hipLaunchKernelGGL((rope_kernel<T, kN, 4>), dim3((unsigned)grid), dim3(kThreads), 0, stream, P);
+    else
+        hipLaunchKernelGGL((rope_kernel<T, kN, 1>), dim3((unsigned)grid), dim3(kThreads), 0, stream, P);
+    return (int)hipGetLastError();
+}
+
+static int rotate(Params& P, bool f32, hipStream_t stream) {
+    const int64_t most = (int64_t)1 << 32, w = P.width, t = P.n_tokens, n = P.n_heads;
+    if (int e = fleet_moe_check_rope(&P.r)) return e;
+    if (P.n_tokens < 0 || P.n_tokens > (1 << 28) || P.n_heads < 1 || P.n_heads > (1 << 16) ||
+        P.at < 0 || P.width < P.r.dim || P.at > P.width - P.r.dim ||
+        P.width > FLEET_ROPE_MAX_WIDTH)
+        return FLEET_MOE_ERR_ARG;
+    if (P.n_tokens == 0) return 0;
+    const int size = f32 ? 4 : 2;
+    if (!P.x || !P.out || (uintptr_t)P.x % size || (uintptr_t)P.out % size || P.x_token < 0 ||
+        P.x_token > most || P.x_head < 0 || P.x_head > most || P.o_token < 0 || P.o_token > most ||
+        P.o_head < 0 || P.o_head > most)
+        return FLEET_MOE_ERR_ARG;
+    // no two heads are written to one place
+    if ((n > 1 && P.o_head < w) || (t > 1 && P.o_token < w) ||
+        (n > 1 && t > 1 && P.o_token < (n - 1) * P.o_head + w &&
+         P.o_head < (t - 1) * P.o_token + w))
+        return FLEET_MOE_ERR_ARG;
+    // in place, a head's values stay with the thread that reads them
+    if (P.out == P.x && (P.r.halves_in != P.r.halves_out || (n > 1 && P.x_head != P.o_head) ||
+                         (t > 1 && P.x_token != P.o_token)))
+        return FLEET_MOE_ERR_ARG;
+    if (int e = fleet_moe_check_device(1)) return e;
+    const bool wide = (P.r.dim / 2 | P.at | P.width) % 4 == 0 &&
+                      ((P.x_token | P.x_head | P.o_token | P.o_head) % 4 == 0) &&
+                      ((uintptr_t)P.x | (uintptr_t)P.out) % (4 * size) == 0;
+    if (f32) return wide ? launch_rope<float, 4>(P, stream) : launch_rope<float, 1>(P, stream);
+    return wide ? launch_rope<uint16_t, 4>(P, stream) : launch_rope<uint16_t, 1>(P, stream);
+}
+
+static Params rope_params(const fleet_rope* rope, const void* x, int64_t x_token, int64_t x_head,
+                          void* out, int64_t out_token, int64_t out_head, int32_t n_tokens,
+                          int32_t n_heads, int32_t width, int32_t at) {
+    Params P{};
+    if (rope) P.r = *rope;
+    P.x = x;
+    P.out = out;
+    P.x_token = x_token;
+    P.x_head = x_head;
+    P.o_token = out_token;
+    P.o_head = out_head;
+    P.n_tokens = n_tokens;
+    P.n_heads = n_heads;
+    P.width = width;
+    P.at = at;
+    return P;
+}
+
+extern "C" int fleet_rope_rotate(const fleet_rope* rope, const void* x, int32_t f32,
+                                 int64_t x_token, int64_t x_head, void* out, int64_t out_token,
+                                 int64_t out_head, const int32_t* positions, int32_t n_tokens,
+                                 int32_t n_heads, int32_t width, int32_t at, hipStream_t stream) {
+    if ((f32 | 1) != 1 || (uintptr_t)positions % 4 || (n_tokens > 0 && !positions))
+        return FLEET_MOE_ERR_ARG;
+    Params P = rope_params(rope, x, x_token, x_head, out, out_token, out_head, n_tokens, n_heads,
+                           width, at);
+    P.positions = positions;
+    return rotate(P, f32, stream);
+}
+
+extern "C" int fleet_cache_rotate(const fleet_cache* cache, const fleet_rope* rope, const void* x,
+                                  int32_t f32, int64_t x_token, int64_t x_head, void* out,
+                                  int64_t out_token, int64_t out_head, const int32_t* start,
+                                  int32_t n_tokens, int32_t n_heads, int32_t width, int32_t at,
+                                  void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (int e = cache::check_cache(cache, workspace, workspace_bytes)) return e;
+    if ((f32 | 1) != 1 || (uintptr_t)start % 4 || (!start && n_tokens != cache->n_seqs))
+        return FLEET_MOE_ERR_ARG;
+    Params P = rope_params(rope, x, x_token, x_head, out, out_token, out_head, n_tokens, n_heads,
+                           width, at);
+    P.lens = cache->lens;
+    P.start = start;
+    P.h = static_cast<cache::Header*>(workspace);
+    P.n_seqs = cache->n_seqs;
+    P.max_pages = cache->max_pages;
+    return rotate(P, f32, stream);
+}

@@ -76,6 +76,12 @@ class FleetCache(ctypes.Structure):
                 ("max_pages", c_int32)]
 
 
+class FleetRope(ctypes.Structure):
+    """struct fleet_rope (turns: a device pointer)."""
+    _fields_ = [("turns", c_void_p), ("dim", c_int32), ("halves_in", c_int32),
+                ("halves_out", c_int32), ("magnitude", c_float)]
+
+
 # (name, restype, argtypes) of every symbol the header declares.
 SYMBOLS = [
     ("fleet_moe_router_topk", c_int,
@@ -134,6 +140,26 @@ SYMBOLS = [
     ("fleet_cache_attend", c_int,
      [POINTER(FleetCache), c_int32, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32,
       c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    ("fleet_residual_norm", c_int,
+     [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_int64, c_float,
+      c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
+    ("fleet_rope_rotate", c_int,
+     [POINTER(FleetRope), c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int64, c_int64,
+      c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p]),
+    ("fleet_cache_rotate", c_int,
+     [POINTER(FleetCache), POINTER(FleetRope), c_void_p, c_int32, c_int64, c_int64, c_void_p,
+      c_int64, c_int64, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_size_t,
+      c_void_p]),
+    ("fleet_cache_append_latent", c_int,
+     [POINTER(FleetCache), c_int32, c_void_p, c_int64, c_void_p, c_float, POINTER(FleetRope),
+      c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
+    ("fleet_cache_plan_bytes", c_size_t, [c_int32, c_int32, c_int32]),
+    ("fleet_cache_share", c_int,
+     [POINTER(FleetCache), c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t,
+      c_void_p]),
+    ("fleet_cache_attend_shared", c_int,
+     [POINTER(FleetCache), c_int32, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_float,
+      c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_size_t, c_void_p]),
     ("fleet_beam_workspace_bytes", c_size_t, [c_int32, c_int32, c_int32, c_int32]),
     ("fleet_beam_select", c_int,
      [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32,

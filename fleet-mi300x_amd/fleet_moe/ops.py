@@ -274,6 +274,131 @@ def moe(layer: DeviceLayer, x_norm: torch.Tensor, runner: GroupedRunner, stream=
     return {"logits": logits, "ids": ids, "weights": ws, "out": out}
 
 
+def _rows_of(t: torch.Tensor, shape, name: str) -> int:
+    """The row stride of int16 (bf16 bits) or fp32 rows of `shape`."""
+    if (not t.is_cuda or t.dtype not in (torch.int16, torch.float32) or t.shape != shape
+            or (t.numel() and shape[-1] > 1 and t.stride(-1) != 1)):
+        raise ValueError(f"{name}: expected device int16 (bf16 bits) or fp32 {tuple(shape)} with "
+                         f"unit column stride, got {t.dtype} {tuple(t.shape)}")
+    return t.stride(0) if shape[0] > 1 else shape[-1]
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None,
+                  norm: torch.Tensor | None = None, post_norm: torch.Tensor | None = None,
+                  gate: torch.Tensor | None = None, scale: float = 1.0, eps: float = 1e-6,
+                  x_out: torch.Tensor | None = None, h: torch.Tensor | None = None,
+                  h_f32: torch.Tensor | None = None, stream=None):
+    """The end of a block and the norm before the next (fleet_residual_norm) of T tokens: from
+    the residual x and the block's output y, each int16 (bf16 bits) or fp32 [T, W],
+        x' = x + scale * gate * y (or * y / rms(y) * post_norm),  h = x' / rms(x') * norm,
+    in one pass. norm and post_norm int16 [W] (None: unit weight; no norm of y); gate
+    int16 [W] or [T, W]. Without y, h is x's norm. Returns (x' as x, h int16 [T, W]), the given
+    tensors or new ones (x' is x without y); x_out may be x. h_f32 fp32 [T, W] takes h's values, as
+    route() and moe() take them."""
+    if x.dim() != 2:
+        raise ValueError(f"x: expected [tokens, width], got {tuple(x.shape)}")
+    shape = x.shape
+    rows, width = shape
+    x_stride, y_stride, gate_stride = _rows_of(x, shape, "x"), 0, 0
+    if y is not None:
+        y_stride = _rows_of(y, shape, "y")
+    elif post_norm is not None or gate is not None or x_out is not None:
+        raise ValueError("post_norm, gate and x_out come with y")
+    if gate is not None:
+        if gate.dtype != torch.int16:
+            raise ValueError(f"gate: expected int16 (bf16 bits), got {gate.dtype}")
+        if gate.dim() == 1:
+            _need(gate, torch.int16, (width,), "gate")
+        else:
+            gate_stride = _rows_of(gate, shape, "gate")
+    if norm is not None:
+        _need(norm, torch.int16, (width,), "norm")
+    if post_norm is not None:
+        _need(post_norm, torch.int16, (width,), "post_norm")
+    if x_out is not None:
+        _need(x_out, x.dtype, shape, "x_out")
+    if h is not None:
+        _need(h, torch.int16, shape, "h")
+    if h_f32 is not None:
+        _need(h_f32, torch.float32, shape, "h_f32")
+    _same_device(x, y=y, norm=norm, post_norm=post_norm, gate=gate, x_out=x_out, h=h, h_f32=h_f32)
+    if h is None or (x_out is None and y is not None):
+        with _on(x.device), _own(stream):
+            if h is None:
+                h = torch.empty(shape, dtype=torch.int16, device=x.device)
+            if x_out is None and y is not None:
+                x_out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    if x.numel():
+        with _on(x.device):
+            rc = _lib.load().fleet_residual_norm(
+                x.data_ptr(), x.dtype == torch.float32, x_stride, _ptr(y),
+                y is not None and y.dtype == torch.float32, y_stride, _ptr(post_norm), _ptr(gate),
+                gate_stride, scale, _ptr(norm), eps, _ptr(x_out), h.data_ptr(), _ptr(h_f32),
+                rows, width, _stream(stream))
+        if rc:
+            _lib.check(rc, "fleet_residual_norm")
+    return (x if x_out is None else x_out), h
+
+
+class Rotary:
+    """A rotation of queries and keys by their positions (fleet_rope_rotate): `freqs`
+    [dim / 2] radians a position, kept on the device in 64 bits (rope.frequencies() gives
+    DeepSeek-V2-Lite's, scaled for its context), values times `magnitude`. Pairs are
+    neighbours, or the values i and i + dim / 2 where halves_in (of what is read) or
+    halves_out (of what is written) is set; the cache has halves."""
+
+    def __init__(self, freqs, magnitude: float = 1.0, halves_in: bool = False,
+                 halves_out: bool = True, device="cuda"):
+        if isinstance(freqs, torch.Tensor) and freqs.is_cuda:
+            device = freqs.device
+        f = torch.as_tensor(freqs, dtype=torch.float64, device=device)
+        if f.dim() != 1 or f.numel() < 1:
+            raise ValueError(f"freqs: expected [dim / 2], got {tuple(f.shape)}")
+        self.turns = (f / (2.0 * math.pi)).contiguous()
+        self.dim = 2 * f.numel()
+        self._c = _lib.FleetRope(self.turns.data_ptr(), self.dim, bool(halves_in),
+                                 bool(halves_out), float(magnitude))
+        self._ref = ctypes.byref(self._c)
+
+    def _heads(self, x: torch.Tensor, out: torch.Tensor | None, at: int, stream):
+        """out, and what the calls take of x and out."""
+        for name, t in (("x", x), ("out", out)):
+            if t is not None and (not t.is_cuda or t.dtype not in (torch.int16, torch.float32)
+                                  or t.dim() != 3 or (t.numel() and t.shape[2] > 1
+                                                      and t.stride(2) != 1)):
+                raise ValueError(f"{name}: expected device int16 (bf16 bits) or fp32 [tokens]"
+                                 f"[heads][width] with unit column stride, got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+        n, heads, width = x.shape
+        if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
+            raise ValueError(f"out: expected {x.dtype} {tuple(x.shape)}, got {out.dtype} "
+                             f"{tuple(out.shape)}")
+        _same_device(self.turns, x=x, out=out)
+        if out is None:
+            with _on(x.device), _own(stream):
+                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        place = (x.data_ptr(), x.dtype == torch.float32, *x.stride()[:2], out.data_ptr(),
+                 *out.stride()[:2])
+        return out, place, (n, heads, width, _int32(at))
+
+    def rotate(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor | None = None,
+               at: int = 0, stream=None) -> torch.Tensor:
+        """x int16 (bf16 bits) or fp32 [tokens][heads][width], any token and head strides, with
+        the values at .. at + dim - 1 of each head rotated by the token's position
+        (int32 [tokens]). Returns out: the given tensor (x itself where pairs are written
+        as they are read), which may be part of wider heads, or a new one."""
+        out, place, sizes = self._heads(x, out, at, stream)
+        _need(positions, torch.int32, (x.shape[0],), "positions")
+        _same_device(self.turns, positions=positions)
+        if x.numel():
+            with _on(x.device):
+                rc = _lib.load().fleet_rope_rotate(self._ref, *place, _ptr(positions), *sizes,
+                                                   _stream(stream))
+            if rc:
+                _lib.check(rc, "fleet_rope_rotate")
+        return out
+
+
 class DenseDecoder:
     """Batch-1 dense SwiGLU layer (fleet_moe_dense_decode) with its own
     workspace: x_out = bf16(x + mlp(rms_norm(x)))."""

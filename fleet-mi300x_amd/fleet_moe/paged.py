@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib
-from .ops import _int32, _need, _on, _own, _ptr, _same_device, _stream
+from .ops import Rotary, _int32, _need, _on, _own, _ptr, _same_device, _stream
 
 ROW = _lib.CACHE_ROW
 LORA = 512
@@ -140,17 +140,8 @@ class PagedCache:
         """The reverse of append(): fills rows with the values the pages hold."""
         self._rows("fleet_cache_read", rows, start, layer, stream)
 
-    def attend(self, q: torch.Tensor, start: torch.Tensor | None = None, layer: int = 0,
-               max_len: int = 0, window: int = 0, sinks: int = 0,
-               scale: float = SOFTMAX_SCALE, out: torch.Tensor | None = None,
-               lse: torch.Tensor | None = None, stream=None):
-        """Attention of q int16 (bf16 bits) [n][heads][576] over the cache's layer:
-        tokens start[s] .. start[s + 1] - 1 stand at the last positions of sequence
-        s (None: one token each). A token sees the positions up to its own; with
-        window > 0 the last `window` of them and the first `sinks`. max_len: a
-        bound on lens known to the caller, for the division of the work.
-        Returns (out int16 [n][heads][512], lse fp32 [n][heads]), the given
-        tensors or new ones."""
+    def _attend_args(self, q, start, out, lse, stream):
+        """Tokens, heads and stride of q, and the outputs, after their checks."""
         if (not q.is_cuda or q.dtype != torch.int16 or q.dim() != 3 or q.shape[2] != ROW
                 or (q.numel() and (q.stride(2) != 1 or (q.shape[1] > 1 and q.stride(1) != ROW)))):
             raise ValueError(f"q: expected device int16 (bf16 bits) [tokens][heads][{ROW}] with "
@@ -169,13 +160,61 @@ class PagedCache:
                     out = torch.empty((n, heads, LORA), dtype=torch.int16, device=self.device)
                 if lse is None:
                     lse = torch.empty((n, heads), dtype=torch.float32, device=self.device)
+        return n, heads, q.stride(0) if n > 1 else heads * ROW, out, lse
+
+    def attend(self, q: torch.Tensor, start: torch.Tensor | None = None, layer: int = 0,
+               max_len: int = 0, window: int = 0, sinks: int = 0,
+               scale: float = SOFTMAX_SCALE, out: torch.Tensor | None = None,
+               lse: torch.Tensor | None = None, stream=None):
+        """Attention of q int16 (bf16 bits) [n][heads][576] over the cache's layer:
+        tokens start[s] .. start[s + 1] - 1 stand at the last positions of sequence
+        s (None: one token each). A token sees the positions up to its own; with
+        window > 0 the last `window` of them and the first `sinks`. max_len: a
+        bound on lens known to the caller, for the division of the work.
+        Returns (out int16 [n][heads][512], lse fp32 [n][heads]), the given
+        tensors or new ones."""
+        n, heads, stride, out, lse = self._attend_args(q, start, out, lse, stream)
         if n == 0:
             return out, lse
-        stride = q.stride(0) if n > 1 else heads * ROW
         self._call("fleet_cache_attend", _int32(layer), _ptr(q), stride, _ptr(start), n, heads,
                    _int32(max_len), _int32(window), _int32(sinks), float(scale), _ptr(out),
                    _ptr(lse), stream=stream)
         return out, lse
+
+    def append_latent(self, rows: torch.Tensor, rope: Rotary, norm: torch.Tensor | None = None,
+                      start: torch.Tensor | None = None, layer: int = 0, eps: float = 1e-6,
+                      stream=None) -> None:
+        """append() of one layer's rows as kv_a_proj leaves them: int16 (bf16 bits) [n][576],
+        c (512) and k_pe (64), any row stride that is a multiple of 8 (so they may be
+        part of a fused projection's). c is normed, times norm int16 [512] (None: unit
+        weight), k_pe rotated by the row's position with `rope` (dim 64, halves out), and both
+        are rounded once, to the pages' 8 bits."""
+        if (not rows.is_cuda or rows.dtype != torch.int16 or rows.dim() != 2
+                or rows.shape[1] != ROW or (rows.numel() and rows.stride(1) != 1)):
+            raise ValueError(f"rows: expected device int16 (bf16 bits) [rows][{ROW}] with unit "
+                             f"column stride, got {rows.dtype} {tuple(rows.shape)}")
+        if norm is not None:
+            _need(norm, torch.int16, (LORA,), "norm")
+        n = rows.shape[0]
+        if n == 0:
+            return
+        self._check_start(start, n)
+        _same_device(self.pool, rows=rows, norm=norm, start=start, rope=rope.turns)
+        self._call("fleet_cache_append_latent", _int32(layer), _ptr(rows),
+                   rows.stride(0) if n > 1 else ROW, _ptr(norm), float(eps), rope._ref,
+                   _ptr(start), n, stream=stream)
+
+    def rotate(self, rope: Rotary, x: torch.Tensor, start: torch.Tensor | None = None,
+               out: torch.Tensor | None = None, at: int = 0, stream=None) -> torch.Tensor:
+        """rope.rotate(x, ..) at the positions that attend() gives the tokens: start[s] ..
+        start[s + 1] - 1 stand at the last positions of sequence s (None: one token
+        each). Tokens without a position are left as they were."""
+        out, place, sizes = rope._heads(x, out, at, stream)
+        if x.numel():
+            self._check_start(start, x.shape[0])
+            _same_device(self.pool, x=x, start=start)
+            self._call("fleet_cache_rotate", rope._ref, *place, _ptr(start), *sizes, stream=stream)
+        return out
 
     def status(self, stream=None) -> int:
         """The FLEET_MOE_ABORT_* bits the calls left; synchronises."""
@@ -190,3 +229,54 @@ class PagedCache:
         """Forgets the bits that status() collected, on the device."""
         with _on(self.device), _own(stream):
             self.workspace[8:12].zero_()
+
+
+class SharedPrefix:
+    """attend() for sequences that share their first pages: a request's beams, or requests
+    behind one prompt. `groups` int32 [n + 1] on the device: sequences groups[g] ..
+    groups[g + 1] - 1 are group g, others are by themselves. The pages that all of a group
+    name first are read once for all its rows.
+
+    update() finds them (`pages` int32 [n], how many), and is called before the first
+    attend(), after remap(), and after changes of table or lens by other means; grow() and
+    append() need none, so once a step serves all layers. (After a remap() without it
+    attend() is right, but takes every sequence by itself.) Holds the plan of up to max_tokens
+    tokens of n_heads heads, 67 MB and 4,144 bytes a token and head. Calls are ordered on
+    one stream, as the cache's."""
+
+    def __init__(self, cache: PagedCache, groups: torch.Tensor, max_tokens: int, n_heads: int):
+        if groups.dim() != 1 or groups.numel() < 2:
+            raise ValueError(f"groups: expected int32 [n + 1], got {tuple(groups.shape)}")
+        _need(groups, torch.int32, groups.shape, "groups")
+        _same_device(cache.pool, groups=groups)
+        self.cache, self.groups = cache, groups
+        self.max_tokens, self.n_heads = _int32(max_tokens), _int32(n_heads)
+        n = _lib.load().fleet_cache_plan_bytes(cache.n_seqs, self.max_tokens, self.n_heads)
+        if n == 0 or groups.numel() - 1 > cache.n_seqs:
+            raise ValueError(f"unsupported sizes: {groups.numel() - 1} groups of "
+                             f"{cache.n_seqs} sequences, {max_tokens} tokens, {n_heads} heads")
+        self.plan = torch.empty(n, dtype=torch.uint8, device=cache.device)
+        self.plan[:256].fill_(255)              # of no state of the cache: nothing is shared yet
+        self.pages = torch.zeros(groups.numel() - 1, dtype=torch.int32, device=cache.device)
+        self._plan = (self.plan.data_ptr(), n)
+
+    def update(self, stream=None) -> torch.Tensor:
+        """Finds the groups' common pages, on the device; returns `pages`."""
+        self.cache._call("fleet_cache_share", _ptr(self.groups), self.pages.numel(),
+                         _ptr(self.pages), *self._plan, stream=stream)
+        return self.pages
+
+    def attend(self, q: torch.Tensor, start: torch.Tensor | None = None, layer: int = 0,
+               scale: float = SOFTMAX_SCALE, out: torch.Tensor | None = None,
+               lse: torch.Tensor | None = None, stream=None):
+        """PagedCache.attend() without a window: q int16 (bf16 bits) [n][heads][576], n * heads
+        up to max_tokens * n_heads. Returns (out int16 [n][heads][512], lse fp32 [n][heads])."""
+        cache = self.cache
+        n, heads, stride, out, lse = cache._attend_args(q, start, out, lse, stream)
+        if n:
+            if n * heads > self.max_tokens * self.n_heads:
+                raise ValueError(f"{n} tokens of {heads} heads are more than the plan's "
+                                 f"{self.max_tokens} of {self.n_heads}")
+            cache._call("fleet_cache_attend_shared", _int32(layer), _ptr(q), stride, _ptr(start), n,
+                        heads, float(scale), _ptr(out), _ptr(lse), *self._plan, stream=stream)
+        return out, lse

@@ -58,16 +58,25 @@ def _correction_range(p: RopeParams) -> tuple[float, float]:
     return float(low), float(high) + (0.001 if low == high else 0.0)
 
 
-def yarn_tables(max_pos: int, p: RopeParams = RopeParams()) -> tuple[np.ndarray, np.ndarray]:
-    """(cos, sin), fp32 [max_pos][dim]."""
+def frequencies(p: RopeParams = RopeParams()) -> np.ndarray:
+    """Radians a position of each pair, fp32 [dim / 2]: the model's inv_freq."""
     exps = np.arange(0, p.dim, 2, dtype=np.float32) / p.dim
     extra = 1.0 / (p.base ** exps)
     inter = 1.0 / (p.factor * p.base ** exps)
     low, high = _correction_range(p)
     ramp = np.clip((np.arange(p.dim // 2, dtype=np.float32) - low) / (high - low), 0, 1)
     keep = 1.0 - ramp
-    inv_freq = inter * (1 - keep) + extra * keep
-    ang = np.outer(np.arange(max_pos, dtype=np.float32), inv_freq)
+    return inter * (1 - keep) + extra * keep
+
+
+def magnitude(p: RopeParams = RopeParams()) -> float:
+    """The factor of cos and sin."""
+    return get_mscale(p.factor, p.mscale) / get_mscale(p.factor, p.mscale_all_dim)
+
+
+def yarn_tables(max_pos: int, p: RopeParams = RopeParams()) -> tuple[np.ndarray, np.ndarray]:
+    """(cos, sin), fp32 [max_pos][dim]."""
+    ang = np.outer(np.arange(max_pos, dtype=np.float32), frequencies(p))
     ang = np.concatenate([ang, ang], axis=-1)
-    m = get_mscale(p.factor, p.mscale) / get_mscale(p.factor, p.mscale_all_dim)
+    m = magnitude(p)
     return ((np.cos(ang) * m).astype(np.float32), (np.sin(ang) * m).astype(np.float32))

@@ -477,6 +477,113 @@ int fleet_cache_attend(const fleet_cache* cache, int32_t layer, const uint16_t* 
                        float scale, uint16_t* out, float* lse, void* workspace,
                        size_t workspace_bytes, hipStream_t stream);
 
+/* ------------------------------------------------------------------------
+ * The way of several sequences' tokens through a layer, between its matrix
+ * products: the norms around a block with its residual, the rotation of
+ * queries, and the rows of kv_a_proj into the pages (no counterpart in the
+ * reference, whose task bodies do it for one token). */
+
+#define FLEET_NORM_MAX_WIDTH 32768
+#define FLEET_NORM_MAX_ROWS 268435456    /* 2^28 */
+
+/* The end of a block and the norm before the next, n_rows rows of width values:
+ *   u = y, or y / rms(y) * post_norm; x' = x + scale * gate * u;
+ *   h = x' / rms(x') * norm; rms(v) = sqrt(mean(v^2) + eps).
+ * x and y: bf16 bits, or fp32 where x_f32 / y_f32 is 1; post_norm, norm: bf16[width],
+ * NULL for no norm of y and for the unit weight; gate: bf16, a value a channel
+ * (gate_stride 0) or rows of width, or NULL for 1. y NULL: h is the norm of x, and
+ * post_norm, gate and x_out are NULL. Strides are in elements, from 0 (one row for all) to
+ * 2^32; x_out (as x; NULL: not wanted; may be x itself with x_stride == width), h
+ * (bf16) and h_f32 (the same values, as fleet_moe_router_topk takes them, or NULL) are
+ * contiguous and overlap nothing else. Arithmetic is fp32; x' and h are rounded once each, h taken
+ * from x' before its rounding. A row is its own: infinities and NaN stay in it.
+ * 1e-30 <= eps <= 1e30, scale finite. One launch. */
+int fleet_residual_norm(const void* x, int32_t x_f32, int64_t x_stride, const void* y,
+                        int32_t y_f32, int64_t y_stride, const uint16_t* post_norm,
+                        const uint16_t* gate, int64_t gate_stride, float scale,
+                        const uint16_t* norm, float eps, void* x_out, uint16_t* h, float* h_f32,
+                        int32_t n_rows, int32_t width, hipStream_t stream);
+
+#define FLEET_ROPE_MAX_DIM 1024
+#define FLEET_ROPE_MAX_WIDTH 65536
+
+/* A rotation: pair i of dim / 2 pairs (a, b) becomes (a cos - b sin, b cos + a sin) *
+ * magnitude at the angle 2 pi * turns[i] * position. turns: device fp64[dim / 2],
+ * frequencies in turns a position, scaled for long contexts as the model has it. Pairs are
+ * neighbours (2i, 2i + 1), or with halves_in / halves_out 1 (i, i + dim / 2) in what
+ * is read / written; DeepSeek-V2's projections have neighbours, its cache and the
+ * queries that meet it halves. */
+typedef struct fleet_rope {
+    const double* turns;
+    int32_t dim;            /* even, 2 .. FLEET_ROPE_MAX_DIM */
+    int32_t halves_in;
+    int32_t halves_out;
+    float magnitude;        /* finite */
+} fleet_rope;
+
+/* out = x with the values at .. at + dim - 1 of each head rotated by its token's
+ * position, the others of the head's `width` as they are. x, out: bf16 bits, or fp32 where f32
+ * is 1, heads x_head / out_head and tokens x_token / out_token elements apart (0 to 2^32;
+ * no two heads of out overlap), so both may be parts of wider heads and rows. out may be x
+ * itself, with the same strides and halves_in == halves_out; else they share no element.
+ * positions: device int32[n_tokens], any. Angles are reduced in 64 bits: good to 2^-24 for
+ * positions up to 2^27 radians. n_heads <= 65536, n_tokens <= 2^28. */
+int fleet_rope_rotate(const fleet_rope* rope, const void* x, int32_t f32, int64_t x_token,
+                      int64_t x_head, void* out, int64_t out_token, int64_t out_head,
+                      const int32_t* positions, int32_t n_tokens, int32_t n_heads, int32_t width,
+                      int32_t at, hipStream_t stream);
+
+/* The same at the positions that fleet_cache_attend gives the tokens: those start[s] ..
+ * start[s + 1] - 1 are the last of the lens[s] positions of sequence s (NULL: one
+ * each). Tokens that name no position or follow a length outside the table
+ * (FLEET_MOE_ABORT_POSITION), and those of no sequence, are left as they were. */
+int fleet_cache_rotate(const fleet_cache* cache, const fleet_rope* rope, const void* x,
+                       int32_t f32, int64_t x_token, int64_t x_head, void* out,
+                       int64_t out_token, int64_t out_head, const int32_t* start,
+                       int32_t n_tokens, int32_t n_heads, int32_t width, int32_t at,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* fleet_cache_append for one layer's rows as kv_a_proj leaves them, bf16 [n_rows]
+ * [c (512) | k_pe (64)], row_stride elements apart (a multiple of 8): c / sqrt(mean(c^2) +
+ * eps) * norm (bf16[512], 16-byte aligned, or NULL for the unit weight) and k_pe
+ * rotated by the row's position go into the pages, rounded once, to the block's 8
+ * bits (fleet_cache_append's rows were rounded to bf16 before). rope: dim 64,
+ * halves_out 1. 1e-30 <= eps <= 1e30. Everything else as in fleet_cache_append. */
+int fleet_cache_append_latent(const fleet_cache* cache, int32_t layer, const uint16_t* rows,
+                              int64_t row_stride, const uint16_t* norm, float eps,
+                              const fleet_rope* rope, const int32_t* start, int32_t n_rows,
+                              void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Bytes of a plan for attentions of up to max_tokens tokens of n_heads heads
+ * (67 MB and 4,144 bytes a token and head; max_tokens * n_heads <= 2^20). 0: outside the
+ * limits. It needs no clearing, and serves the calls on one cache that are ordered
+ * on one stream. */
+size_t fleet_cache_plan_bytes(int32_t n_seqs, int32_t max_tokens, int32_t n_heads);
+
+/* Finds what sequences share: group g is groups[g] .. groups[g + 1] - 1 (device
+ * int32[n_groups + 1], not decreasing, within the cache's sequences; those
+ * outside are groups of one), and pages[g] (device int32[n_groups] or NULL) becomes the number
+ * of leading table entries that all its sequences with positions have in common and
+ * have filled. Kept in the plan; it stays right while the sequences grow and pages are
+ * compacted. After a remap the plan is stale: fleet_cache_attend_shared then takes every
+ * sequence by itself until the next call. A caller that changes table or lens by other
+ * means calls this again. Offsets out of order set FLEET_MOE_ABORT_POSITION, and nothing is shared.
+ * 1 <= n_groups <= n_seqs. */
+int fleet_cache_share(const fleet_cache* cache, const int32_t* groups, int32_t n_groups,
+                      int32_t* pages, void* plan, size_t plan_bytes, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream);
+
+/* fleet_cache_attend without a window, the pages that a group shares read once for all
+ * its rows: what it takes, sees and leaves is as there. (The probabilities are
+ * rounded to bf16's 8 bits before the second product, whatever the number of rows.) plan: as
+ * fleet_cache_share left it, for at least as many tokens and heads. n_tokens *
+ * n_heads <= 2^20, (n_tokens * n_heads / 32 + 2 * n_seqs) * max_pages < 2^31. */
+int fleet_cache_attend_shared(const fleet_cache* cache, int32_t layer, const uint16_t* q,
+                              int64_t q_stride, const int32_t* start, int32_t n_tokens,
+                              int32_t n_heads, float scale, uint16_t* out, float* lse, void* plan,
+                              size_t plan_bytes, void* workspace, size_t workspace_bytes,
+                              hipStream_t stream);
+
 #define FLEET_BEAM_MAX_BEAMS 64
 #define FLEET_BEAM_MAX_OUT 64
 
