@@ -170,38 +170,66 @@ __device__ __forceinline__ int start_of(const SharedParams& P, int s) {
 // group's first, and its own rows over what is behind them.
 struct Item {
     int seq, tok0, n_new, len;
-    int first, end, pages, lead;        // its group
-    int units0, steps0, units1, steps1; // a unit's steps, whether they see anything or not
-    __device__ __forceinline__ int total() const { return units0 * steps0 + units1 * steps1; }
+    int pages, lead;                    // its group's, and
+    int first, end, last;               // the sequences, and the token behind them
+    int steps0, steps1;                 // of a unit, whether they see anything or not
 };
 __device__ __forceinline__ Item item_of(const SharedParams& P, int seq, bool stale) {
     Item w;
+    const i32x4 g = ld_global(reinterpret_cast<const i32x4*>(P.plan.groups + seq));
     w.seq = seq;
-    w.first = seq;
-    w.end = seq + 1;
-    w.pages = 0;
-    w.lead = seq;
-    if (!stale) {
-        const i32x4 g = ld_global(reinterpret_cast<const i32x4*>(P.plan.groups + seq));
-        w.first = g.x;
-        w.end = g.y;
-        w.pages = g.z;
-        w.lead = g.w;
-    }
     w.tok0 = start_of(P, seq);
     w.n_new = start_of(P, seq + 1) - w.tok0;              // (negative: not in order)
     w.len = checked_len(ld_global(P.c.lens + seq), P.c.max_pages);
-    w.units0 = w.steps0 = 0;
-    if (w.pages > 0 && seq == w.first) {
-        const int last = start_of(P, w.end);
-        w.units0 = last > w.tok0 ? ((last - w.tok0) * P.n_heads + kTile - 1) / kTile : 0;
-        w.steps0 = w.pages;
-    }
-    w.units1 = w.n_new > 0 ? (w.n_new * P.n_heads + kTile - 1) / kTile : 0;
+    w.first = stale ? seq : g.x;
+    w.end = stale ? seq + 1 : g.y;
+    w.pages = stale ? 0 : g.z;
+    w.lead = stale ? seq : g.w;
+    w.last = w.pages > 0 && seq == w.first ? start_of(P, w.end) : w.tok0;
+    w.steps0 = w.pages;
     const int own = w.len < 0 ? 0 : pages_of(w.len) - w.pages;
     w.steps1 = own > 1 ? own : 1;
     return w;
 }
+__device__ __forceinline__ Item lane_of(const Item& v, int lane) {
+    static_assert(sizeof(Item) == 44, "");
+    struct Words {
+        int w[sizeof(Item) / 4];
+    } x = __builtin_bit_cast(Words, v);
+#pragma unroll
+    for (int& i : x.w) i = __builtin_amdgcn_readlane(i, lane);
+    return __builtin_bit_cast(Item, x);
+}
+
+// What the work is divided by: the time of a unit's beginning and end, and of a page, for units
+// of up to 16 rows and of more (measured, in 1,200 cycles: 11,000 and 3,650, 20,000 and 4,750).
+// A workgroup does the pages whose time begins in its share.
+struct Cost {
+    int setup, page;
+};
+constexpr Cost kCost16{9, 3}, kCost64{17, 4};
+struct Sizes {
+    int rows0, units0, rows1, units1;
+    __device__ __forceinline__ Sizes(const SharedParams& P, const Item& w) {
+        rows0 = (w.last - w.tok0) * P.n_heads;
+        rows1 = w.n_new > 0 ? w.n_new * P.n_heads : 0;
+        units0 = (rows0 + kTile - 1) / kTile;
+        units1 = (rows1 + kTile - 1) / kTile;
+    }
+    // The time of unit k of either kind.
+    __device__ __forceinline__ static Cost cost(int rows, int k) {
+        return rows - k * kTile <= 16 ? kCost16 : kCost64;
+    }
+    __device__ __forceinline__ static int time(int rows, int units, int pages) {
+        if (units == 0) return 0;
+        const Cost z = cost(rows, units - 1);
+        return (units - 1) * (kCost64.setup + kCost64.page * pages) + z.setup + z.page * pages;
+    }
+    __device__ __forceinline__ int front(const Item& w) const { return time(rows0, units0, w.steps0); }
+    __device__ __forceinline__ int total(const Item& w) const {
+        return front(w) + time(rows1, units1, w.steps1);
+    }
+};
 
 // A range of n things in `shares` parts that differ by one at most.
 struct Split {
@@ -214,53 +242,14 @@ struct Split {
     }
 };
 
-// How many workgroups take part: a share of few pages is short, but each is a part to join.
+constexpr int kLeast = 8;
+static_assert(kLeast >= kCost64.page && kLeast >= kCost16.page, "");
+// How many workgroups take part. No share is shorter than a page's time (so that every one
+// between a unit's first and last has a part of it), and few pages are left to many only as
+// far as the parts are joined in less time than that saves.
 __device__ __forceinline__ int shares_of(int total) {
-    return total < kGrid ? total : kGrid;
-}
-
-// The sequence in whose steps workgroup wg begins, and where. Every wave for itself, a lane
-// a sequence, or several.
-struct Place {
-    int seq, off, total, shares;
-};
-__device__ __forceinline__ bool locate(const SharedParams& P, int wg, bool stale, Place& at) {
-    const int lane = threadIdx.x & 63;
-    const int each = (P.c.n_seqs + 63) / 64;
-    int n = 0;
-    bool bad = false;
-    for (int i = 0; i < each; ++i) {
-        const int s = lane * each + i;
-        if (s < P.c.n_seqs) {
-            const Item w = item_of(P, s, stale);
-            bad |= w.n_new < 0;
-            n += w.total();
-        }
-    }
-    bad = __ballot(bad) != 0;
-    if (wg == 0 && threadIdx.x == 0) {
-        P.plan.h->ok = !bad;
-        if (bad) raise(P.h, FLEET_MOE_ABORT_POSITION);
-    }
-    if (bad) return false;
-    int incl = wave_incl_scan(n);
-    at.total = __builtin_amdgcn_readlane(incl, 63);
-    at.shares = shares_of(at.total);
-    if (wg >= at.shares) return false;
-    int off = Split(at.total, at.shares).first(wg);
-    int owner = __popcll(__ballot(incl <= off));
-    off -= __builtin_amdgcn_readlane(incl - n, owner);
-    at.seq = owner;
-    if (each > 1) {
-        const int s = owner * each + lane;
-        n = lane < each && s < P.c.n_seqs ? item_of(P, s, stale).total() : 0;
-        incl = wave_incl_scan(n);
-        const int k = __popcll(__ballot(incl <= off));
-        off -= __builtin_amdgcn_readlane(incl - n, k);
-        at.seq = owner * each + k;
-    }
-    at.off = off;
-    return true;
+    const int n = total / kLeast;
+    return n < 1 ? total > 0 : n < kGrid ? n : kGrid;
 }
 
 // Up to 64 rows and the pages of a table row that they see.
@@ -269,7 +258,7 @@ struct Unit {
     int tok0;                   // the token of row 0
     int base;                   // own pages: the position of that token
     int first, end;             // common pages: the group
-    bool common;
+    bool common, inside;
     const int32_t* table;       // from the first page on
     int page0;
     int n;                      // pages that some row may see
@@ -311,17 +300,88 @@ __device__ __forceinline__ TileRow tile_row(const SharedParams& P, const Unit& u
     return r;
 }
 
+// The position that all rows of a wave see, apart from the dead ones.
+__device__ __forceinline__ int common_position(const TileRow& r) {
+    int v = r.live ? r.pos : 0x7fffffff;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        const int o = __shfl_xor(v, d);
+        v = o < v ? o : v;
+    }
+    return wave_bcast(v);
+}
+
 struct PageLds {
     __attribute__((aligned(16))) uint8_t tile[kPageRing][4 * kBlockStep];
-    uint32_t scale[kPageRing][8];
+    u32x4 p[2][4][2][64];       // [step parity][tile][half of the page][lane] (first: the last
+                                // of the queries, read before a weight is written)
     f32x4 half[kGridWaves][2][64];  // half of the scores of a tile and two blocks
-    u32x4 p[2][4][2][64];       // [step parity][tile][half of the page][lane]
+    uint32_t scale[kPageRing][8];
     int flag[2][kGridWaves];
     float m[4][16], top[4][2][16], sum[4][2][16], rounded[4][2][16];
     Item item;                  // what follows a unit, out of the registers meanwhile
     int at, off;
 };
 static_assert(sizeof(PageLds) <= 160 * 1024, "");
+static_assert(kTile * (2 * kRow + 16) <= 2 * 4 * kBlockStep + 16 * 1024, "");
+
+// The sequence in whose steps workgroup wg begins, and where, into L: a thread a sequence, or
+// two.
+struct Place {
+    int total, shares;
+    bool inside;                // some token stands within its group's common pages
+};
+__device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg, bool stale,
+                                       Place& at) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int each = P.c.n_seqs > kGridThreads ? 2 : 1;
+    static_assert(kMaxSeqs <= 2 * kGridThreads, "");
+    int n = 0, first = 0;
+    bool bad = false, inside = false;
+    Item w{}, w1{};
+    if (t * each < P.c.n_seqs) {
+        w = item_of(P, t * each, stale);
+        if (each > 1 && t * each + 1 < P.c.n_seqs) w1 = item_of(P, t * each + 1, stale);
+        first = Sizes(P, w).total(w);
+        n = first + Sizes(P, w1).total(w1);
+        bad = (w.n_new | w1.n_new) < 0;
+        inside = (w.n_new > 0 && w.len - w.n_new < w.pages * kPage) ||
+                 (w1.n_new > 0 && w1.len - w1.n_new < w1.pages * kPage);
+    }
+    const int incl = wave_incl_scan(n);
+    const int flags = (__ballot(bad) ? 1 : 0) | (__ballot(inside) ? 2 : 0);
+    if (lane == 63) {
+        L.flag[0][wave] = incl;
+        L.flag[1][wave] = flags;
+    }
+    barrier();
+    int before = 0, any = 0;
+    at.total = 0;
+#pragma unroll
+    for (int i = 0; i < kGridWaves; ++i) {
+        if (i < wave) before += L.flag[0][i];
+        at.total += L.flag[0][i];
+        any |= L.flag[1][i];
+    }
+    at.total = wave_bcast(at.total);
+    any = wave_bcast(any);
+    at.inside = any & 2;
+    if (wg == 0 && t == 0) {
+        P.plan.h->ok = !(any & 1);
+        if (any & 1) raise(P.h, FLEET_MOE_ABORT_POSITION);
+    }
+    if (any & 1) return false;
+    at.shares = shares_of(at.total);
+    if (wg >= at.shares) return false;
+    const int off = Split(at.total, at.shares).first(wg) - (before + incl - n);
+    if (off >= 0 && off < n) {
+        const bool second = off >= first;
+        L.item = second ? w1 : w;
+        L.off = second ? off - first : off;
+    }
+    barrier();
+    return true;
+}
 
 // Pages of 64 steps, one per lane.
 struct PageList {
@@ -340,12 +400,37 @@ __device__ __forceinline__ int page_of(const Unit& u, PageList& h, int i, int en
     return __builtin_amdgcn_readlane(h.page, i - h.from);
 }
 
+// The queries of a unit go through the ring before its pages: a lane's own loads of them, 16
+// bytes of 16 rows at a time, took 12,000 cycles for 64 rows (a page's step takes 4,800). Rows
+// lie 16 bytes further apart than they are long, so that the operands of 16 rows fall into
+// different banks.
+constexpr int kQueryStep = 2 * kRow + 16;
+__device__ __forceinline__ uint8_t* query_at(PageLds& L, int place, int row) {
+    return L.tile[place] + row * kQueryStep;
+}
+// A wave's rows; of dead ones the unit's first.
+__device__ __forceinline__ void copy_q(const SharedParams& P, PageLds& L, const Unit& u, int place,
+                                       int rows, int wave, int lane) {
+    for (int i = 0; i < rows; ++i) {
+        const int at = wave * rows + i;
+        const int row = u.row0 + at < u.rows ? u.row0 + at : u.row0;
+        const int tok = token_of_row(row, P.per_head);
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(
+            P.q + (int64_t)(u.tok0 + tok) * P.q_stride + (row - tok * P.n_heads) * kRow);
+        const uint32_t to = lds_addr(query_at(L, place, at));
+        copy_kb<1, false>(src + lane * 16, to);
+        if (lane < (2 * kRow - 1024) / 16) copy_kb<1, false>(src + 1024 + lane * 16, to + 1024);
+    }
+}
+// A lane's row as the right operand. The k order of the products is that of the bytes a lane of
+// group g takes of a cache row: its chunks 4i + g, 16 values each, i = 0 .. 8, make two of 18
+// steps. Wave `half` has those of i = half, 2 + half, 4 + half, 6 + half, and one of i = 8.
 constexpr int kTileHalf = kChunks / 4;          // steps of a wave
-__device__ __forceinline__ void load_q(const SharedParams& P, const TileRow& r, int g, int half,
+__device__ __forceinline__ void read_q(PageLds& L, int place, int row, int g, int half,
                                        bf16x8 (&q)[kTileHalf]) {
-    const uint16_t* src = P.q + (int64_t)r.tok * P.q_stride + r.head * kRow + g * 16;
+    const uint8_t* src = query_at(L, place, row) + g * 32;
     const auto at = [&](int v) {
-        return __builtin_bit_cast(bf16x8, ld_global(reinterpret_cast<const u32x4*>(src + v)));
+        return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(src + 2 * v));
     };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -355,6 +440,27 @@ __device__ __forceinline__ void load_q(const SharedParams& P, const TileRow& r, 
     q[8] = at(8 * 64 + half * 8);
 }
 
+__device__ __forceinline__ void set_position(const SharedParams& P, const Unit& u, TileRow& r) {
+    int pos = 0x7fffffff;                       // common pages, in front of every token
+    if (!u.common) pos = u.base + r.tok - u.tok0;
+    else if (u.inside) pos = position_of(P, u.first, u.end, r.tok);
+    r.pos = r.live ? pos : -1;
+}
+
+// The copies of a page to place b of the ring: a wave of four a block, the first the scales too.
+__device__ __forceinline__ void issue_page(const SharedParams& P, PageLds& L, int page, int b,
+                                           int wave, int lane) {
+    const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
+    const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
+    const uint8_t* from = src + wave * kBlockBytes + lane * 16;
+    const uint32_t to = lds_addr(L.tile[b]) + wave * kBlockStep;
+    copy_kb<4, false>(from, to);
+    copy_kb<4, false>(from + 4096, to + 4096);
+    copy_kb<1, false>(from + 8192, to + 8192);
+    if (wave == 0 && lane < 2)
+        copy_kb<1, false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[b]));
+}
+
 // Pages off .. off + cnt - 1 of a unit; its results to `out` and `lse` if `at` is negative,
 // else as the parts at + row.
 //
@@ -362,8 +468,8 @@ __device__ __forceinline__ void load_q(const SharedParams& P, const TileRow& r, 
 // with 32 positions, so that a widened K operand serves two tiles; it exchanges halves with
 // its partner, makes the weights of one tile and 32 positions, and adds its 64 columns of O
 // for all rows over the whole page, where a widened V operand serves four tiles.
-__device__ __forceinline__ void attend(const SharedParams& P, PageLds& L, const Unit& u, int off,
-                                       int cnt, int64_t to_part) {
+__device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, const Unit& u, int off,
+                                         int cnt, int64_t to_part) {
     constexpr int kCols = kC / 16 / kGridWaves; // of 16
     // (fm_tid: no lane's index is kept in a register from one unit to the next)
     const int t = fm_tid(), lane = t & 63, wave = wave_bcast(t >> 6);
@@ -371,24 +477,20 @@ __device__ __forceinline__ void attend(const SharedParams& P, PageLds& L, const 
     const int bp = wave & 1, half = wave >> 1 & 1, tp = wave >> 2;
     const int mine = 2 * tp + half;             // the tile whose weights this wave makes
 
+    // (b is k % kPageRing, counted)
+    PageList pages{0, 0, 0};
+    const auto issue = [&](int k, int b) {
+        issue_page(P, L, page_of(u, pages, off + k, off + cnt, lane), b, wave, lane);
+    };
+    // the first page's copies, and the queries'
+    if (cnt > 0) {
+        page_of(u, pages, off, off + cnt, lane);
+        if (tp == 0) issue(0, 0);
+        copy_q(P, L, u, 1, kTile / kGridWaves, wave, lane);
+    }
     TileRow r = tile_row(P, u, u.row0 + mine * 16 + n);
-    bf16x8 q[2][kTileHalf];                     // of `mine` and of the pair's other tile
-    load_q(P, r, g, half, q[0]);
-    load_q(P, tile_row(P, u, u.row0 + (mine ^ 1) * 16 + n), g, half, q[1]);
-    if (u.common) {
-        const int pos = position_of(P, u.first, u.end, r.tok);
-        r.pos = r.live ? pos : -1;
-    } else {
-        r.pos = r.live ? u.base + r.tok - u.tok0 : -1;
-    }
-    // the position that all rows of the wave see, apart from the dead ones
-    int common = r.live ? r.pos : 0x7fffffff;
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
-        const int o = __shfl_xor(common, d);
-        common = o < common ? o : common;
-    }
-    common = wave_bcast(common);
+    set_position(P, u, r);
+    const int common = common_position(r);
     f32x4 acc[4][kCols];
 #pragma unroll
     for (auto& a : acc)
@@ -405,25 +507,12 @@ __device__ __forceinline__ void attend(const SharedParams& P, PageLds& L, const 
     float p0[4], p1[4];
     bool stray = false;                         // a score of the wave is not finite
     if (t < 64) L.m[t >> 4][n] = -INFINITY;
-    PageList pages{0, 0, 0};
-    if (cnt > 0) page_of(u, pages, off, off + cnt, lane);
-    // q is there before a copy is issued, also as far as the compiler counts
-    __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0)
+    wait_copies<0>();
+    barrier();
+    bf16x8 q[2][kTileHalf];                     // of `mine` and of the pair's other tile
+    read_q(L, 1, mine * 16 + n, g, half, q[0]);
+    read_q(L, 1, (mine ^ 1) * 16 + n, g, half, q[1]);
 
-    // (b is k % kPageRing, counted)
-    const auto issue = [&](int k, int b) {
-        const int page = page_of(u, pages, off + k, off + cnt, lane);
-        const int64_t base = page_offset(page, P.c.n_pages, P.layer, P.c.n_layers);
-        const uint8_t* src = P.c.pool + (base < 0 ? 0 : base);
-        // a wave a block; the first the scales too
-        const uint8_t* from = src + wave * kBlockBytes + lane * 16;
-        const uint32_t to = lds_addr(L.tile[b]) + wave * kBlockStep;
-        copy_kb<4, false>(from, to);
-        copy_kb<4, false>(from + 4096, to + 4096);
-        copy_kb<1, false>(from + 8192, to + 8192);
-        if (wave == 0 && lane < 2)
-            copy_kb<1, false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[b]));
-    };
     const auto score = [&](int b) {
         u32x4 c[2][4];
         uint2 e[2];
@@ -557,13 +646,11 @@ __device__ __forceinline__ void attend(const SharedParams& P, PageLds& L, const 
                     __builtin_bit_cast(bf16x8, L.p[k & 1][wave & 3][wave >> 2][lane]), ones);
     };
 
-    if (tp == 0)
-        for (int k = 0; k < kPageRing - 1 && k < cnt; ++k) issue(k, k);
-    wait_copies<0>();
-    barrier();
     if (cnt > 0) {
         score(0);
-        barrier();
+        barrier();                              // (and q has been read: its place is free)
+        if (tp == 0)
+            for (int k = 1; k < kPageRing - 1 && k < cnt; ++k) issue(k, k);
         finish(0);
     }
     // Step k: behind barrier A the weights of k and the rows of k + 1 are there, behind
@@ -573,8 +660,8 @@ __device__ __forceinline__ void attend(const SharedParams& P, PageLds& L, const 
         const int b1 = b == kPageRing - 1 ? 0 : b + 1, b2 = b1 == kPageRing - 1 ? 0 : b1 + 1;
         wait_copies<0>();                       // step k + 1
         barrier();                              // A
-        const int* f = L.flag[k & 1];
-        const int flags = ((f[0] | f[1]) | (f[2] | f[3])) | ((f[4] | f[5]) | (f[6] | f[7]));
+        const int* fl = L.flag[k & 1];
+        const int flags = ((fl[0] | fl[1]) | (fl[2] | fl[3])) | ((fl[4] | fl[5]) | (fl[6] | fl[7]));
         if (tp == 0 && k + kPageRing - 1 < cnt) issue(k + kPageRing - 1, b2);  // where step k - 1 was
         if (wave_bcast(flags)) mend(k, b);
         l += ((p0[0] + p0[1]) + (p0[2] + p0[3])) + ((p1[0] + p1[1]) + (p1[2] + p1[3]));
@@ -620,6 +707,170 @@ __device__ __forceinline__ void attend(const SharedParams& P, PageLds& L, const 
     }
 }
 
+// The same for a unit of 16 rows or fewer, a sequence's one token: wave (block, half) takes half
+// of the 576 products of the rows with 16 positions, half 0 makes the weights, and every wave
+// adds 64 columns of O. Here a page's bytes bound a step, not its products, so the weights are
+// two operands, bf16 and what that leaves: 16 bits.
+__device__ __forceinline__ void attend16(const SharedParams& P, PageLds& L, const Unit& u, int off,
+                                         int cnt, int64_t to_part) {
+    constexpr int kCols = kC / 16 / kGridWaves;
+    const int t = fm_tid(), lane = t & 63, wave = wave_bcast(t >> 6);
+    const int g = lane >> 4, n = lane & 15, blk = wave & 3, half = wave >> 2;
+    const bool weighs = half == 1;              // the others copy
+
+    PageList pages{0, 0, 0};
+    const auto issue = [&](int k, int b) {
+        issue_page(P, L, page_of(u, pages, off + k, off + cnt, lane), b, wave, lane);
+    };
+    if (cnt > 0) {
+        page_of(u, pages, off, off + cnt, lane);
+        if (!weighs)
+            for (int k = 0; k < kPageRing - 1 && k < cnt; ++k) issue(k, k);
+        copy_q(P, L, u, kPageRing - 1, 16 / kGridWaves, wave, lane);
+    }
+    TileRow r = tile_row(P, u, u.row0 + n);
+    set_position(P, u, r);
+    const int common = common_position(r);
+    f32x4 acc[kCols], ones{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (auto& a : acc) a = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, ref = -INFINITY, l = 0.f;
+    const float slack = P.slack;
+    f32x4 z, next;
+    bool stray = false;
+    float p[4]{0.f, 0.f, 0.f, 0.f};
+    wait_copies<0>();
+    barrier();
+    bf16x8 q[kTileHalf];
+    read_q(L, kPageRing - 1, n, g, half, q);
+
+    const auto score = [&](int b) {
+        const uint8_t* block = L.tile[b] + blk * kBlockStep + lane * 16;
+        const float sc = any_scale(L.scale[b][2 * blk]), sp = any_scale(L.scale[b][2 * blk + 1]);
+        f32x4 y0{0.f, 0.f, 0.f, 0.f}, y1{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const u32x4 a = *reinterpret_cast<const u32x4*>(block + (2 * i + half) * 1024);
+            y0 = mfma(widen(a.x, a.y, sc, sc), q[2 * i], y0);
+            y1 = mfma(widen(a.z, a.w, sc, sc), q[2 * i + 1], y1);
+        }
+        const uint2 a = *reinterpret_cast<const uint2*>(block + 8 * 1024 + half * 8);
+        y0 = mfma(widen(a.x, a.y, sp, sp), q[8], y0);
+        next = y0 + y1;
+        if (!weighs) L.half[blk][0][lane] = next;
+    };
+    const auto weigh = [&](int k) {
+        const float down = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = exp2_(fmaf(z[j], P.scale, -down));
+        const uint2 w = weights(p);
+        reinterpret_cast<uint2*>(&L.p[k & 1][0][blk >> 1][lane])[blk & 1] = w;
+        reinterpret_cast<uint2*>(&L.p[k & 1][1][blk >> 1][lane])[blk & 1] = rest(p, w);
+    };
+    const auto finish = [&](int k) {
+        z = next + L.half[blk][0][lane];
+        const int page = page_of(u, pages, off + k, off + cnt, lane);
+        const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
+        const int base = (u.page0 + off + k) * kPage + blk * kBlock;
+        const bool bad = !finite((z[0] + z[1]) + (z[2] + z[3]));
+        if (!(ok && base + kBlock - 1 <= common)) {
+            asm volatile("");                   // a branch, not twenty instructions every step
+            if (!ok && lane == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] = (ok & (base + 4 * g + i <= r.pos)) ? z[i] : -INFINITY;
+        }
+        weigh(k);
+        const float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+        stray = __ballot(bad) != 0;
+        const bool high = __ballot(top > m + slack) != 0;
+        if (lane == 0) L.flag[k & 1][blk] = stray | high;
+    };
+    const auto mend = [&](int k, int b) {
+        if (weighs) {
+            float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+            top = xor32_max(xor16_max(top));
+            if (lane < 16) L.top[blk][0][lane] = top;
+            if (stray) clean(L.tile[b] + blk * kBlockStep, L.scale[b][2 * blk], lane);
+        }
+        barrier();
+        const float to = fmaxf(m, fmaxf(fmaxf(L.top[0][0][n], L.top[1][0][n]),
+                                        fmaxf(L.top[2][0][n], L.top[3][0][n])));
+        const float scaled = reference(to * P.scale);
+        const float shrink = shrink_to(scaled, ref);
+        m = to;
+        ref = scaled;
+        l *= shrink;
+        ones *= shrink;
+#pragma unroll
+        for (auto& a : acc) a *= shrink;
+        if (weighs) weigh(k);
+        barrier();
+    };
+    const auto add = [&](int k, int b) {
+        const uint32_t first = lds_addr(L.tile[b]) + wave * kCols * 256 + column_at(lane);
+        const bf16x8 one = __builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes});
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bf16x8 pb = __builtin_bit_cast(bf16x8, L.p[k & 1][0][h][lane]);
+            const bf16x8 pr = __builtin_bit_cast(bf16x8, L.p[k & 1][1][h][lane]);
+            const float sa = any_scale(L.scale[b][4 * h]), sb = any_scale(L.scale[b][4 * h + 2]);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) {
+                const i32x2 v = column(first + 2 * h * kBlockStep, i);
+                const bf16x8 a = widen((uint32_t)v.x, (uint32_t)v.y, sa, sb);
+                acc[i] = mfma(a, pb, acc[i]);
+                acc[i] = mfma(a, pr, acc[i]);
+            }
+            ones = mfma(one, pb, ones);
+            ones = mfma(one, pr, ones);
+        }
+    };
+
+    if (cnt > 0) {
+        score(0);
+        barrier();
+        if (weighs) finish(0);
+    }
+    int b = 0;                                  // of step k; the barriers as in attend64()
+    for (int k = 0; k < cnt; ++k) {
+        const int b1 = b == kPageRing - 1 ? 0 : b + 1, b2 = b1 == kPageRing - 1 ? 0 : b1 + 1;
+        wait_copies<0>();
+        barrier();                              // A
+        const int* f = L.flag[k & 1];
+        const int flags = (f[0] | f[1]) | (f[2] | f[3]);
+        if (!weighs && k + kPageRing - 1 < cnt) issue(k + kPageRing - 1, b2);
+        if (wave_bcast(flags)) mend(k, b);
+        if (weighs) l += (p[0] + p[1]) + (p[2] + p[3]);
+        if (k + 1 < cnt) {
+            score(b1);
+            barrier();                          // B
+            if (weighs) finish(k + 1);
+        }
+        add(k, b);
+        b = b1;
+        asm("" : "+s"(b));
+    }
+    l = xor32_sum(xor16_sum(l));
+    if (weighs && lane < 16) L.sum[blk][0][lane] = l;
+    barrier();
+    if (u.row0 + n >= u.rows) return;
+    const int column0 = wave * kCols * 16 + 4 * g;
+    const float sum = (L.sum[0][0][n] + L.sum[1][0][n]) + (L.sum[2][0][n] + L.sum[3][0][n]);
+    if (to_part < 0) {
+        const int64_t to = (int64_t)u.tok0 * P.n_heads + u.row0 + n;
+        const float inv = ones[0] == 0.f ? 0.f : 1.f / ones[0];
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) put(P.out + to * kC + column0 + j * 16, acc[j], inv);
+        if (P.lse && wave == 0 && g == 0) P.lse[to] = lse_of(ref, sum);
+    } else {
+        const int64_t to = to_part + n;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+            st_global(reinterpret_cast<f32x4*>(P.plan.part + to * kC + column0 + j * 16), acc[j]);
+        if (wave == 0 && g == 0) st_global(P.plan.stat + to, f32x4{ref, sum, ones[0], 0.f});
+    }
+}
+
 __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     PageLds& L = *reinterpret_cast<PageLds*>(lds);
@@ -627,30 +878,37 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
     // sequences have moved since share: every one by itself
     const bool stale = ld_global(&P.plan.h->remaps) != ld_global(&P.h->remaps);
     Place place;
-    if (!locate(P, wg, stale, place)) return;
+    if (!locate(P, L, wg, stale, place)) return;
     const Split share(place.total, place.shares);
     const int64_t all_rows = (int64_t)P.n_tokens * P.n_heads;
-    int at = share.first(wg), off = place.off;
-    Item w = item_of(P, place.seq, stale);
-    for (;;) {
-        // the unit of the item's step `off`
+    const int end = share.first(wg + 1);
+    for (int at = share.first(wg);;) {
+        const Item w = lane_of(L.item, 0);
+        const int off = wave_bcast(L.off);
+        barrier();                              // they are read
+        // the unit at time `off` of the item
+        const Sizes z(P, w);
+        const int front = z.front(w);
         Unit u;
-        const int n0 = w.units0 * w.steps0;
-        u.common = off < n0;
-        const int steps = u.common ? w.steps0 : w.steps1, o = u.common ? off : off - n0;
-        const int k = o / steps, from = o - k * steps;
+        u.common = off < front;
+        const int rows = u.common ? z.rows0 : z.rows1, steps = u.common ? w.steps0 : w.steps1;
+        const int o = u.common ? off : off - front, whole64 = kCost64.setup + kCost64.page * steps;
+        const int units = u.common ? z.units0 : z.units1;
+        const int k = o / whole64 < units ? o / whole64 : units - 1;
+        const Cost cost = Sizes::cost(rows, k);
+        const int from = o - k * whole64, all = cost.setup + cost.page * steps;
         u.row0 = k * kTile;
+        u.rows = rows;
         u.tok0 = w.tok0;
         u.first = w.first;
         u.end = w.end;
+        u.inside = place.inside;
         if (u.common) {
-            u.rows = (start_of(P, w.end) - w.tok0) * P.n_heads;
             u.base = 0;
             u.page0 = 0;
-            u.n = steps;
+            u.n = w.steps0;
             u.table = P.c.table + (int64_t)w.lead * P.c.max_pages;
         } else {
-            u.rows = w.n_new * P.n_heads;
             u.base = w.len - w.n_new;
             u.page0 = w.pages;
             u.table = P.c.table + (int64_t)w.seq * P.c.max_pages + w.pages;
@@ -660,42 +918,50 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
             u.n = w.len < 0 || p < 0 ? 0 : pages_of((int64_t)p + 1) - w.pages;
             if (w.len < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
         }
-        const int left = share.first(wg + 1) - at;
-        const int take = steps - from < left ? steps - from : left;
-        const int to = from + take < u.n ? from + take : u.n;
-        // where the part goes: a whole unit's to its rows, or to one of two slots
-        const bool whole = take == steps;
-        const int64_t row = (int64_t)u.tok0 * P.n_heads + u.row0;
-        const int64_t slots = 2 * all_rows;
-        const int64_t part =
-            whole ? (u.common ? row : w.pages > 0 ? all_rows + row : -1)
-                  : slots + (int64_t)(2 * wg + (from == 0 ? 1 : 0)) * kTile;
-        if (from == 0 && t < kTile && u.row0 + t < u.rows) {
-            const int last = share.holder(at + steps - 1);
-            Parts m;
-            m.at = (int)(part + t);
-            m.next = (int)(slots + (int64_t)(wg + 1) * kPartStep + t);
-            m.count = part < 0 ? 0 : whole ? 1 : last - wg + 1;
-            m.front = !u.common && w.pages > 0;
-            P.plan.meta[(u.common ? 0 : all_rows) + row + t] = m;
-        }
-        if (t == 0) {
-            L.item = w;
+        // the steps that begin from here to the share's end
+        const int take = all - from < end - at ? all - from : end - at;
+        const auto step_at = [&](int time) {
+            const int i = time <= cost.setup ? 0 : (time - cost.setup + cost.page - 1) / cost.page;
+            return i < steps ? i : steps;
+        };
+        const int lo = step_at(from), hi = step_at(from + take);
+        // what comes next, out of the registers meanwhile
+        if (t == kGridThreads - 64) {
+            int o2 = off + take;
+            Item next = w;
+            if (end - at > take)
+                while (o2 >= Sizes(P, next).total(next) && next.seq + 1 < P.c.n_seqs) {
+                    next = item_of(P, next.seq + 1, stale);
+                    o2 = 0;
+                }
+            L.item = next;
+            L.off = o2;
             L.at = at + take;
-            L.off = off + take;
         }
-        attend(P, L, u, from, to > from ? to - from : 0, part);
+        if (hi > lo) {
+            // where the part goes: a whole unit's to its rows, or to one of two slots
+            const bool whole = lo == 0 && hi == steps;
+            const int64_t row = (int64_t)u.tok0 * P.n_heads + u.row0;
+            const int64_t slots = 2 * all_rows;
+            const int64_t part =
+                whole ? (u.common ? row : w.pages > 0 ? all_rows + row : -1)
+                      : slots + (int64_t)(2 * wg + (lo == 0 ? 1 : 0)) * kTile;
+            if (lo == 0 && t < kTile && u.row0 + t < u.rows) {
+                const int last = at - from + cost.setup + (steps - 1) * cost.page;
+                Parts m;
+                m.at = (int)(part + t);
+                m.next = (int)(slots + (int64_t)(wg + 1) * kPartStep + t);
+                m.count = part < 0 ? 0 : whole ? 1 : share.holder(last) - wg + 1;
+                m.front = !u.common && w.pages > 0;
+                P.plan.meta[(u.common ? 0 : all_rows) + row + t] = m;
+            }
+            const int n = hi < u.n ? hi : u.n;
+            if (u.rows - u.row0 <= 16) attend16(P, L, u, lo, n > lo ? n - lo : 0, part);
+            else attend64(P, L, u, lo, n > lo ? n - lo : 0, part);
+        }
         barrier();                              // LDS is free again
-        at = L.at;
-        if (at >= share.first(wg + 1)) return;
-        w = L.item;
-        off = L.off;
-        while (off >= w.total()) {
-            if (w.seq + 1 >= P.c.n_seqs) return;
-            w = item_of(P, w.seq + 1, stale);
-            off = 0;
-        }
-        barrier();
+        at = wave_bcast(L.at);
+        if (at >= end) return;
     }
 }
 
@@ -814,8 +1080,9 @@ extern "C" int fleet_cache_attend_shared(const fleet_cache* cache, int32_t layer
     if (!q || !out || (uintptr_t)q % 16 || (uintptr_t)out % 8 || (uintptr_t)lse % 4 ||
         q_stride < (int64_t)n_heads * kRow || q_stride % 8 || q_stride > ((int64_t)1 << 32))
         return FLEET_MOE_ERR_ARG;
-    // the steps of all units are counted in 32 bits
-    if ((2 * (rows / kTile) + 2 * (int64_t)cache->n_seqs) * cache->max_pages > 0x7fffffff)
+    // the time of all units is counted in 32 bits
+    if ((2 * (rows / kTile) + 2 * (int64_t)cache->n_seqs) *
+            (kCost64.setup + kCost64.page * (int64_t)cache->max_pages) > 0x7fffffff)
         return FLEET_MOE_ERR_ARG;
     if (plan_bytes < plan_size(cache->n_seqs, rows)) return FLEET_MOE_ERR_WORKSPACE;
     if (int e = fleet_moe_check_device(1)) return e;
