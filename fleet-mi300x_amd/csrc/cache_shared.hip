@@ -26,6 +26,7 @@ constexpr int kGrid = kShares / 2;      // workgroups
 constexpr int kGridWaves = 8;
 constexpr int kGridThreads = kGridWaves * 64;
 constexpr int kPageRing = 3;
+constexpr float kRise = 12.f;           // (8: 186 us where this takes 184)
 
 // The plan: what share found, and the parts of an attention.
 struct PlanHeader {
@@ -159,7 +160,7 @@ struct SharedParams {
     uint64_t per_head;          // head_divisor(n_heads)
     int layer, n_tokens, n_heads;
     float scale;                // times log2(e)
-    float slack;                // kSlack as a score: finite
+    float slack;                // kRise as a score: finite
 };
 
 __device__ __forceinline__ int start_of(const SharedParams& P, int s) {
@@ -202,12 +203,12 @@ __device__ __forceinline__ Item lane_of(const Item& v, int lane) {
 }
 
 // What the work is divided by: the time of a unit's beginning and end, and of a page, for units
-// of up to 16 rows and of more (measured, in 1,200 cycles: 11,000 and 3,650, 20,000 and 4,750).
+// of up to 16 rows and of more (measured, in 400 cycles: 12,000 and 3,250, 24,000 and 4,450).
 // A workgroup does the pages whose time begins in its share.
 struct Cost {
     int setup, page;
 };
-constexpr Cost kCost16{9, 3}, kCost64{17, 4};
+constexpr Cost kCost16{30, 8}, kCost64{60, 11};
 struct Sizes {
     int rows0, units0, rows1, units1;
     __device__ __forceinline__ Sizes(const SharedParams& P, const Item& w) {
@@ -242,7 +243,7 @@ struct Split {
     }
 };
 
-constexpr int kLeast = 8;
+constexpr int kLeast = 20;
 static_assert(kLeast >= kCost64.page && kLeast >= kCost16.page, "");
 // How many workgroups take part. No share is shorter than a page's time (so that every one
 // between a unit's first and last has a part of it), and few pages are left to many only as
@@ -315,9 +316,12 @@ struct PageLds {
     __attribute__((aligned(16))) uint8_t tile[kPageRing][4 * kBlockStep];
     u32x4 p[2][4][2][64];       // [step parity][tile][half of the page][lane] (first: the last
                                 // of the queries, read before a weight is written)
-    f32x4 half[kGridWaves][2][64];  // half of the scores of a tile and two blocks
+    f32x4 half[2][kGridWaves][2][64];   // [step parity] half of the scores of a tile and two
+                                        // blocks
     uint32_t scale[kPageRing][8];
     int flag[2][kGridWaves];
+    __attribute__((aligned(8))) uint8_t flags[2][kGridWaves];   // (64 rows) 1: a row's reference
+                                // rises, 2: a score is not finite
     float m[4][16], top[4][2][16], sum[4][2][16], rounded[4][2][16];
     Item item;                  // what follows a unit, out of the registers meanwhile
     int at, off;
@@ -383,21 +387,29 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
     return true;
 }
 
-// Pages of 64 steps, one per lane.
+// Pages of 64 steps, one per lane, and which of them are not of the pool.
 struct PageList {
     int held, from, page;
+    uint64_t bad;
 };
-__device__ __forceinline__ int page_of(const Unit& u, PageList& h, int i, int end, int lane) {
-    if (i >= h.held) {
-        h.from = i - 4;         // (the steps whose scores are not finished yet)
-        h.held = h.from + 64;
-        const int mine = h.from + lane;
-        h.page = mine >= 0 && mine < end ? ld_global(u.table + mine) : 0;
-        // here, not at the use: there the compiler would wait, every step, for
-        // whatever copies are in flight
-        __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0)
-    }
+__device__ __forceinline__ void turn_to(const SharedParams& P, const Unit& u, PageList& h, int i,
+                                        int end, int lane) {
+    if (i < h.held) return;
+    h.from = i - 4;             // (the steps whose scores are not finished yet)
+    h.held = h.from + 64;
+    const int mine = h.from + lane;
+    const bool there = mine >= 0 && mine < end;
+    h.page = there ? ld_global(u.table + mine) : 0;
+    // here, not at the use: there the compiler would wait, every step, for
+    // whatever copies are in flight
+    __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0)
+    h.bad = __ballot(there && (unsigned)h.page >= (unsigned)P.c.n_pages);
+}
+__device__ __forceinline__ int page_of(const PageList& h, int i) {
     return __builtin_amdgcn_readlane(h.page, i - h.from);
+}
+__device__ __forceinline__ bool valid(const PageList& h, int i) {
+    return !(h.bad >> (i - h.from) & 1);
 }
 
 // The queries of a unit go through the ring before its pages: a lane's own loads of them, 16
@@ -461,13 +473,18 @@ __device__ __forceinline__ void issue_page(const SharedParams& P, PageLds& L, in
         copy_kb<1, false>(src + kCodeBytes + lane * 16, lds_addr(L.scale[b]));
 }
 
-// Pages off .. off + cnt - 1 of a unit; its results to `out` and `lse` if `at` is negative,
-// else as the parts at + row.
+// Pages off .. off + cnt - 1 of a unit; its results to `out` and `lse` if `to_part` is negative,
+// else as the parts to_part + row.
 //
 // Eight waves: wave (tile pair, half, block pair) takes half of the 576 products of 32 rows
 // with 32 positions, so that a widened K operand serves two tiles; it exchanges halves with
 // its partner, makes the weights of one tile and 32 positions, and adds its 64 columns of O
 // for all rows over the whole page, where a widened V operand serves four tiles.
+//
+// Three pages are in work between two barriers: the scores of page k + 2, the weights of page
+// k + 1 and the products of page k, none of which needs another, so that matrix and vector
+// instructions and reads of LDS run beside each other. The codes of V are read a page ahead, so
+// that three places of the ring suffice.
 __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, const Unit& u, int off,
                                          int cnt, int64_t to_part) {
     constexpr int kCols = kC / 16 / kGridWaves; // of 16
@@ -478,13 +495,14 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
     const int mine = 2 * tp + half;             // the tile whose weights this wave makes
 
     // (b is k % kPageRing, counted)
-    PageList pages{0, 0, 0};
+    PageList pages{0, 0, 0, 0};
     const auto issue = [&](int k, int b) {
-        issue_page(P, L, page_of(u, pages, off + k, off + cnt, lane), b, wave, lane);
+        turn_to(P, u, pages, off + k, off + cnt, lane);
+        issue_page(P, L, page_of(pages, off + k), b, wave, lane);
     };
     // the first page's copies, and the queries'
     if (cnt > 0) {
-        page_of(u, pages, off, off + cnt, lane);
+        turn_to(P, u, pages, off, off + cnt, lane);
         if (tp == 0) issue(0, 0);
         copy_q(P, L, u, 1, kTile / kGridWaves, wave, lane);
     }
@@ -499,21 +517,21 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
     // the sum of the rounded weights of tile wave & 3 and half of the page wave >> 2
     f32x4 ones{0.f, 0.f, 0.f, 0.f};
     // Every row's reference, as a score and as it is in the exponent: any score not far below
-    // the maximum, because weights up to 2^kSlack are as exact as those up to 1, and moving
+    // the maximum, because weights up to 2^kRise are as exact as those up to 1, and moving
     // it costs a pass over O and two barriers.
-    float m = -INFINITY, ref = -INFINITY, l = 0.f;
+    float m = -INFINITY, ref = -INFINITY, l = 0.f, sum = 0.f;
     const float slack = P.slack;
     f32x4 z[2];                                 // the scores of `mine` and the two blocks
-    float p0[4], p1[4];
-    bool stray = false;                         // a score of the wave is not finite
+    f32x4 own[2];                               // the wave's half of the next ones
     if (t < 64) L.m[t >> 4][n] = -INFINITY;
+    // q is there, also as far as the compiler counts, and the pages are
     wait_copies<0>();
     barrier();
     bf16x8 q[2][kTileHalf];                     // of `mine` and of the pair's other tile
     read_q(L, 1, mine * 16 + n, g, half, q[0]);
     read_q(L, 1, (mine ^ 1) * 16 + n, g, half, q[1]);
 
-    const auto score = [&](int b) {
+    const auto score = [&](int k, int b) {
         u32x4 c[2][4];
         uint2 e[2];
         uint32_t f[2][2];
@@ -527,7 +545,6 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
             f[j][0] = L.scale[b][2 * (2 * bp + j)];
             f[j][1] = L.scale[b][2 * (2 * bp + j) + 1];
         }
-        __builtin_amdgcn_sched_barrier(0);      // every read on its way
         f32x4 y[2][2];                          // [tile][block]
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -548,12 +565,13 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            z[j] = y[0][j];
-            L.half[wave][j][lane] = y[1][j];
+            own[j] = y[0][j];
+            L.half[k & 1][wave][j][lane] = y[1][j];
         }
     };
     const auto weigh = [&](int k) {
         const float down = ref == -INFINITY ? 0.f : ref;
+        float p0[4], p1[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             p0[j] = exp2_(fmaf(z[0][j], P.scale, -down));
@@ -561,15 +579,18 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
         }
         const uint2 a = weights(p0), b = weights(p1);
         L.p[k & 1][mine][bp][lane] = u32x4{a.x, a.y, b.x, b.y};
+        sum = ((p0[0] + p0[1]) + (p0[2] + p0[3])) + ((p1[0] + p1[1]) + (p1[2] + p1[3]));
     };
-    const auto finish = [&](int k) {
+    // The scores of step k whole, hidden where they are not seen, and whether some are not finite.
+    bool stray = false;
+    const auto join = [&](int k) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) z[j] += L.half[wave ^ 2][j][lane];
-        const int page = page_of(u, pages, off + k, off + cnt, lane);
-        const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
+        for (int j = 0; j < 2; ++j) z[j] = own[j] + L.half[k & 1][wave ^ 2][j][lane];
+        turn_to(P, u, pages, off + k, off + cnt, lane);
+        const bool ok = valid(pages, off + k);
         const int base = (u.page0 + off + k) * kPage + bp * 32;
         const f32x4 both = z[0] + z[1];
-        const bool bad = !finite((both[0] + both[1]) + (both[2] + both[3]));
+        stray = __ballot(!finite((both[0] + both[1]) + (both[2] + both[3]))) != 0;
         if (!(ok && base + 31 <= common)) {
             asm volatile("");                   // a branch, not forty instructions every step
             if (!ok && t == 0) raise(P.h, FLEET_MOE_ABORT_BAD_PAGE);
@@ -579,22 +600,49 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
                 for (int i = 0; i < 4; ++i)
                     z[j][i] = (ok & (base + kBlock * j + 4 * g + i <= r.pos)) ? z[j][i] : -INFINITY;
         }
+    };
+    const auto finish = [&](int k) {
         weigh(k);
         const float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
                                 fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
-        stray = __ballot(bad) != 0;
         const bool high = __ballot(top > m + slack) != 0;
-        if (lane == 0) L.flag[k & 1][wave] = stray | high;
+        if (lane == 0) L.flags[k & 1][wave] = (stray ? 2 : 0) | (high ? 1 : 0);
+    };
+    // The codes of V of a page, and their scales
+    i32x2 v[2][kCols];
+    uint32_t f[2][2];
+    const auto fetch = [&](int b) {
+        uint32_t first = lds_addr(L.tile[b]) + wave * kCols * 256 + column_at(lane);
+        asm("" : "+v"(first));                // one address, the rest is offsets
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) v[h][i] = column(first + 2 * h * kBlockStep, i);
+            f[h][0] = L.scale[b][4 * h];
+            f[h][1] = L.scale[b][4 * h + 2];
+        }
     };
     // What is rare: a row's scores beyond its reference, or one that is not finite, in step k.
-    const auto mend = [&](int k, int b) {
+    const auto mend = [&](int k, bool strays) {
+        // (its addresses are made here, not kept in registers through all steps)
+        const int lane = fm_tid() & 63, n = lane & 15;
         float top = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
                           fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
         top = xor32_max(xor16_max(top));
         if (lane < 16) L.top[mine][bp][lane] = top;
-        if (stray && half == 0 && tp == 0)
-            for (int j = 0; j < 2; ++j)
-                clean(L.tile[b] + (2 * bp + j) * kBlockStep, L.scale[b][2 * (2 * bp + j)], lane);
+        if (strays) {
+            // Such a value makes the score of every row infinite or NaN, and the weight of one
+            // that sees it NaN or 0; a row that does not see it has the weight 0, and must not
+            // meet 0 * NaN.
+            const float most = __uint_as_float(kMaxScale);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) {
+                    v[h][i].x = (int)drop_infinite((uint32_t)v[h][i].x, any_scale(f[h][0]) == most);
+                    v[h][i].y = (int)drop_infinite((uint32_t)v[h][i].y, any_scale(f[h][1]) == most);
+                }
+        }
         barrier();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -615,23 +663,12 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
         if (bp == 0 && lane < 16) L.m[mine][lane] = m;
     };
     // O over step k
-    const auto add = [&](int k, int b) {
-        uint32_t first = lds_addr(L.tile[b]) + wave * kCols * 256 + column_at(lane);
-        asm("" : "+v"(first));                // one address, the rest is offsets
+    const auto add = [&](int k) {
         bf16x8 pb[2][4];
-        i32x2 v[2][kCols];
-        uint32_t f[2][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t col = first + 2 * h * kBlockStep;
-#pragma unroll
-            for (int i = 0; i < kCols; ++i) v[h][i] = column(col, i);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < 4; ++j) pb[h][j] = __builtin_bit_cast(bf16x8, L.p[k & 1][j][h][lane]);
-            f[h][0] = L.scale[b][4 * h];
-            f[h][1] = L.scale[b][4 * h + 2];
-        }
-        __builtin_amdgcn_sched_barrier(0);      // every read on its way
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const float sa = any_scale(f[h][0]), sb = any_scale(f[h][1]);
@@ -647,30 +684,47 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
     };
 
     if (cnt > 0) {
-        score(0);
+        score(0, 0);
         barrier();                              // (and q has been read: its place is free)
         if (tp == 0)
-            for (int k = 1; k < kPageRing - 1 && k < cnt; ++k) issue(k, k);
+            for (int k = 1; k < kPageRing && k < cnt; ++k) issue(k, k);
+        join(0);
         finish(0);
+        fetch(0);
+        wait_copies<0>();
+        barrier();
+        if (cnt > 1) score(1, 1);
     }
-    // Step k: behind barrier A the weights of k and the rows of k + 1 are there, behind
-    // B both halves of the scores of k + 1.
+    // Step k: behind the barrier the weights of k, both halves of the scores of k + 1 and the
+    // rows of k + 2 are there.
     int b = 0;                                  // of step k
     for (int k = 0; k < cnt; ++k) {
         const int b1 = b == kPageRing - 1 ? 0 : b + 1, b2 = b1 == kPageRing - 1 ? 0 : b1 + 1;
-        wait_copies<0>();                       // step k + 1
-        barrier();                              // A
-        const int* fl = L.flag[k & 1];
-        const int flags = ((fl[0] | fl[1]) | (fl[2] | fl[3])) | ((fl[4] | fl[5]) | (fl[6] | fl[7]));
-        if (tp == 0 && k + kPageRing - 1 < cnt) issue(k + kPageRing - 1, b2);  // where step k - 1 was
-        if (wave_bcast(flags)) mend(k, b);
-        l += ((p0[0] + p0[1]) + (p0[2] + p0[3])) + ((p1[0] + p1[1]) + (p1[2] + p1[3]));
+        wait_copies<0>();
+        barrier();
+        const uint2 fl = *reinterpret_cast<const uint2*>(L.flags[k & 1]);
+        const int flags = wave_bcast((int)(fl.x | fl.y));
+        if (flags) mend(k, flags & 0x02020202);
+        l += sum;
+        if (tp == 0 && k + kPageRing < cnt) issue(k + kPageRing, b);    // where step k was
+        // Of a SIMD's two waves (w and w + 4) one makes its weights while the other multiplies.
+        // (The asm keeps each in its place: the compiler would fetch both's operands before.)
+        if (tp != 0) {
+            asm volatile("; products first" ::: "memory");
+            add(k);
+            asm volatile("; products made" ::: "memory");
+        }
         if (k + 1 < cnt) {
-            score(b1);
-            barrier();                          // B
+            join(k + 1);
             finish(k + 1);
         }
-        add(k, b);
+        if (tp == 0) {
+            asm volatile("; products last" ::: "memory");
+            add(k);
+            asm volatile("; products made, too" ::: "memory");
+        }
+        if (k + 2 < cnt) score(k + 2, b2);
+        if (k + 1 < cnt) fetch(b1);
         b = b1;
         asm("" : "+s"(b));
     }
@@ -718,12 +772,13 @@ __device__ __forceinline__ void attend16(const SharedParams& P, PageLds& L, cons
     const int g = lane >> 4, n = lane & 15, blk = wave & 3, half = wave >> 2;
     const bool weighs = half == 1;              // the others copy
 
-    PageList pages{0, 0, 0};
+    PageList pages{0, 0, 0, 0};
     const auto issue = [&](int k, int b) {
-        issue_page(P, L, page_of(u, pages, off + k, off + cnt, lane), b, wave, lane);
+        turn_to(P, u, pages, off + k, off + cnt, lane);
+        issue_page(P, L, page_of(pages, off + k), b, wave, lane);
     };
     if (cnt > 0) {
-        page_of(u, pages, off, off + cnt, lane);
+        turn_to(P, u, pages, off, off + cnt, lane);
         if (!weighs)
             for (int k = 0; k < kPageRing - 1 && k < cnt; ++k) issue(k, k);
         copy_q(P, L, u, kPageRing - 1, 16 / kGridWaves, wave, lane);
@@ -757,7 +812,7 @@ __device__ __forceinline__ void attend16(const SharedParams& P, PageLds& L, cons
         const uint2 a = *reinterpret_cast<const uint2*>(block + 8 * 1024 + half * 8);
         y0 = mfma(widen(a.x, a.y, sp, sp), q[8], y0);
         next = y0 + y1;
-        if (!weighs) L.half[blk][0][lane] = next;
+        if (!weighs) L.half[0][blk][0][lane] = next;
     };
     const auto weigh = [&](int k) {
         const float down = ref == -INFINITY ? 0.f : ref;
@@ -768,9 +823,9 @@ __device__ __forceinline__ void attend16(const SharedParams& P, PageLds& L, cons
         reinterpret_cast<uint2*>(&L.p[k & 1][1][blk >> 1][lane])[blk & 1] = rest(p, w);
     };
     const auto finish = [&](int k) {
-        z = next + L.half[blk][0][lane];
-        const int page = page_of(u, pages, off + k, off + cnt, lane);
-        const bool ok = (unsigned)page < (unsigned)P.c.n_pages;
+        z = next + L.half[0][blk][0][lane];
+        turn_to(P, u, pages, off + k, off + cnt, lane);
+        const bool ok = valid(pages, off + k);
         const int base = (u.page0 + off + k) * kPage + blk * kBlock;
         const bool bad = !finite((z[0] + z[1]) + (z[2] + z[3]));
         if (!(ok && base + kBlock - 1 <= common)) {
@@ -1100,7 +1155,7 @@ extern "C" int fleet_cache_attend_shared(const fleet_cache* cache, int32_t layer
     P.n_tokens = n_tokens;
     P.n_heads = n_heads;
     P.scale = scale * kLog2e;
-    P.slack = fminf(kSlack / P.scale, FLT_MAX);
+    P.slack = fminf(kRise / P.scale, FLT_MAX);
     if (int e = launch<shared_kernel>(kGrid, kGridThreads, sizeof(PageLds), P, stream)) return e;
     return launch<join_kernel>((rows + kJoinRows - 1) / kJoinRows, 64 * kJoinRows, 0, P, stream);
 }
