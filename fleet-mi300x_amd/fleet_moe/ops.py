@@ -25,12 +25,15 @@ from .layout import DSV2_LITE, Layout, MoeDims
 # The current stream's handle without a Stream object (0.1 us instead of 2.8,
 # of the 13 a routing call spent on the host); None where torch has no GPU.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# The current device's index without the check that torch has a GPU (0.1 us of 0.4): for
+# calls that have a device tensor in hand.
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream(stream=None) -> int:
     if stream is None:
         if _raw_stream is not None:
-            return _raw_stream(torch.cuda.current_device())
+            return _raw_stream(_device())
         stream = torch.cuda.current_stream()
     return int(stream.cuda_stream)
 
@@ -47,7 +50,7 @@ def _ptr(t) -> int | None:
 def _need(t: torch.Tensor, dtype, shape, name: str) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor")
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != tuple(shape) or not t.is_contiguous():
         raise ValueError(f"{name}: expected contiguous {dtype} {tuple(shape)}, "
                          f"got {t.dtype} {tuple(t.shape)}")
 
@@ -75,7 +78,7 @@ _HERE = _Here()
 def _on(device: torch.device):
     """A context in which `device` is the current one: launches go there, and a
     call without a stream takes that device's current one."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == _device():
         return _HERE
     return torch.cuda.device(device)
 
@@ -274,13 +277,23 @@ def moe(layer: DeviceLayer, x_norm: torch.Tensor, runner: GroupedRunner, stream=
     return {"logits": logits, "ids": ids, "weights": ws, "out": out}
 
 
+_F32, _BITS = torch.float32, torch.int16
+
+
 def _rows_of(t: torch.Tensor, shape, name: str) -> int:
     """The row stride of int16 (bf16 bits) or fp32 rows of `shape`."""
-    if (not t.is_cuda or t.dtype not in (torch.int16, torch.float32) or t.shape != shape
-            or (t.numel() and shape[-1] > 1 and t.stride(-1) != 1)):
+    if (not t.is_cuda or (t.dtype != _BITS and t.dtype != _F32) or t.shape != shape
+            or (shape[-1] > 1 and shape[0] and t.stride(-1) != 1)):
         raise ValueError(f"{name}: expected device int16 (bf16 bits) or fp32 {tuple(shape)} with "
                          f"unit column stride, got {t.dtype} {tuple(t.shape)}")
     return t.stride(0) if shape[0] > 1 else shape[-1]
+
+
+def _like(t: torch.Tensor, dtype) -> torch.Tensor:
+    """An output of t's shape, contiguous. (empty_like takes half of empty's time.)"""
+    if t.dtype == dtype and t.is_contiguous():
+        return torch.empty_like(t)
+    return t.new_empty(t.shape, dtype=dtype)
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None,
@@ -297,7 +310,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None,
     route() and moe() take them."""
     if x.dim() != 2:
         raise ValueError(f"x: expected [tokens, width], got {tuple(x.shape)}")
-    shape = x.shape
+    shape, dev = x.shape, x.device
     rows, width = shape
     x_stride, y_stride, gate_stride = _rows_of(x, shape, "x"), 0, 0
     if y is not None:
@@ -305,38 +318,36 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None,
     elif post_norm is not None or gate is not None or x_out is not None:
         raise ValueError("post_norm, gate and x_out come with y")
     if gate is not None:
-        if gate.dtype != torch.int16:
+        if gate.dtype != _BITS:
             raise ValueError(f"gate: expected int16 (bf16 bits), got {gate.dtype}")
         if gate.dim() == 1:
-            _need(gate, torch.int16, (width,), "gate")
+            _need(gate, _BITS, (width,), "gate")
         else:
             gate_stride = _rows_of(gate, shape, "gate")
-    if norm is not None:
-        _need(norm, torch.int16, (width,), "norm")
-    if post_norm is not None:
-        _need(post_norm, torch.int16, (width,), "post_norm")
-    if x_out is not None:
-        _need(x_out, x.dtype, shape, "x_out")
-    if h is not None:
-        _need(h, torch.int16, shape, "h")
-    if h_f32 is not None:
-        _need(h_f32, torch.float32, shape, "h_f32")
-    _same_device(x, y=y, norm=norm, post_norm=post_norm, gate=gate, x_out=x_out, h=h, h_f32=h_f32)
-    if h is None or (x_out is None and y is not None):
-        with _on(x.device), _own(stream):
-            if h is None:
-                h = torch.empty(shape, dtype=torch.int16, device=x.device)
-            if x_out is None and y is not None:
-                x_out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    if x.numel():
-        with _on(x.device):
+    for name, t, dtype, want in (("norm", norm, _BITS, (width,)),
+                                 ("post_norm", post_norm, _BITS, (width,)),
+                                 ("x_out", x_out, x.dtype, shape), ("h", h, _BITS, shape),
+                                 ("h_f32", h_f32, _F32, shape)):
+        if t is not None:
+            _need(t, dtype, want, name)
+            if t.device != dev:
+                raise ValueError(f"{name} is on {t.device}, not on {dev}")
+    _same_device(x, y=y, gate=gate)
+    with _on(dev):
+        if h is None or (x_out is None and y is not None):
+            with _own(stream):
+                if h is None:
+                    h = _like(x, _BITS) if y is None or x.dtype == _BITS else _like(y, _BITS)
+                if x_out is None and y is not None:
+                    x_out = _like(x, x.dtype)
+        if rows and width:
             rc = _lib.load().fleet_residual_norm(
-                x.data_ptr(), x.dtype == torch.float32, x_stride, _ptr(y),
-                y is not None and y.dtype == torch.float32, y_stride, _ptr(post_norm), _ptr(gate),
+                x.data_ptr(), x.dtype == _F32, x_stride, _ptr(y),
+                y is not None and y.dtype == _F32, y_stride, _ptr(post_norm), _ptr(gate),
                 gate_stride, scale, _ptr(norm), eps, _ptr(x_out), h.data_ptr(), _ptr(h_f32),
                 rows, width, _stream(stream))
-        if rc:
-            _lib.check(rc, "fleet_residual_norm")
+            if rc:
+                _lib.check(rc, "fleet_residual_norm")
     return (x if x_out is None else x_out), h
 
 
@@ -362,24 +373,21 @@ class Rotary:
 
     def _heads(self, x: torch.Tensor, out: torch.Tensor | None, at: int, stream):
         """out, and what the calls take of x and out."""
-        for name, t in (("x", x), ("out", out)):
-            if t is not None and (not t.is_cuda or t.dtype not in (torch.int16, torch.float32)
-                                  or t.dim() != 3 or (t.numel() and t.shape[2] > 1
-                                                      and t.stride(2) != 1)):
-                raise ValueError(f"{name}: expected device int16 (bf16 bits) or fp32 [tokens]"
-                                 f"[heads][width] with unit column stride, got {t.dtype} "
-                                 f"{tuple(t.shape)}")
-        n, heads, width = x.shape
-        if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
-            raise ValueError(f"out: expected {x.dtype} {tuple(x.shape)}, got {out.dtype} "
-                             f"{tuple(out.shape)}")
-        _same_device(self.turns, x=x, out=out)
+        dtype, shape, dev = x.dtype, x.shape, self.turns.device
         if out is None:
-            with _on(x.device), _own(stream):
-                out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        place = (x.data_ptr(), x.dtype == torch.float32, *x.stride()[:2], out.data_ptr(),
-                 *out.stride()[:2])
-        return out, place, (n, heads, width, _int32(at))
+            with _on(dev), _own(stream):
+                out = x.new_empty(shape)
+        for name, t in (("x", x), ("out", out)):
+            if (t.device != dev or (dtype != _BITS and dtype != _F32) or t.dtype != dtype
+                    or len(shape) != 3 or t.shape != shape
+                    or (shape[2] > 1 and t.stride(2) != 1 and t.numel())):
+                raise ValueError(f"{name}: expected int16 (bf16 bits) or fp32 [tokens][heads]"
+                                 f"[width] on {dev} with unit column stride, got {t.dtype} "
+                                 f"{tuple(t.shape)} on {t.device}")
+        x0, x1, _ = x.stride()
+        o0, o1, _ = out.stride()
+        return (out, (x.data_ptr(), dtype == _F32, x0, x1, out.data_ptr(), o0, o1),
+                (shape[0], shape[1], shape[2], _int32(at)))
 
     def rotate(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor | None = None,
                at: int = 0, stream=None) -> torch.Tensor:

@@ -157,9 +157,9 @@ class PagedCache:
         if out is None or lse is None:
             with _own(stream):
                 if out is None:
-                    out = torch.empty((n, heads, LORA), dtype=torch.int16, device=self.device)
+                    out = q.new_empty((n, heads, LORA))
                 if lse is None:
-                    lse = torch.empty((n, heads), dtype=torch.float32, device=self.device)
+                    lse = q.new_empty((n, heads), dtype=torch.float32)
         return n, heads, q.stride(0) if n > 1 else heads * ROW, out, lse
 
     def attend(self, q: torch.Tensor, start: torch.Tensor | None = None, layer: int = 0,
@@ -212,7 +212,7 @@ class PagedCache:
         out, place, sizes = rope._heads(x, out, at, stream)
         if x.numel():
             self._check_start(start, x.shape[0])
-            _same_device(self.pool, x=x, start=start)
+            _same_device(self.pool, x=x, start=start)      # (rope's tensors are where x is)
             self._call("fleet_cache_rotate", rope._ref, *place, _ptr(start), *sizes, stream=stream)
         return out
 
