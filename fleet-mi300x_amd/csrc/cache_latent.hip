@@ -7,6 +7,13 @@
 // 16 positions as fleet_cache_append does; beside it the 8 waves of c share their rows' sums of
 // squares, and all waves compute an angle a thread (16 positions of 32 pairs) while the
 // rows are on their way.
+//
+// One row for each of 17 sequences: 5.0 us, the latency of the loads before the rows (start,
+// length, table), the angle and two barriers. 11,004 rows: 9.7 us (19 MB, 2 TB/s; a copy of as
+// much takes 4): that latency once, with every workgroup of the call on the chip (70
+// registers; with 83 only two workgroups a CU, 13.5), and some 450 vector instructions a wave.
+#include <math.h>
+
 #include "cache_rows.h"
 #include "rope.h"
 
@@ -31,11 +38,18 @@ __global__ __launch_bounds__(kRowThreads) void latent_kernel(LatentParams P) {
     __shared__ float2 cs[kBlock][kPairs + 1];
     __shared__ double squares[8][kBlock];
     __shared__ uint32_t most[8];
+    const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
+    const int tok = lane >> 2, part = lane & 3, chunk = 4 * wave + part;
+    // what depends on no position is on its way first
+    const double turns = ld_global(P.rope.turns + t % kPairs);
+    u32x4 w[2];
+    if (P.norm && wave < 8) {
+        w[0] = ld_global(reinterpret_cast<const u32x4*>(P.norm + chunk * 16));
+        w[1] = ld_global(reinterpret_cast<const u32x4*>(P.norm + chunk * 16) + 1);
+    }
     BlockAt b;
     if (!block_at<true>(P.r, b)) return;
     const fleet_cache& c = P.r.c;
-    const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
-    const int tok = lane >> 2, part = lane & 3, chunk = 4 * wave + part;
     const int holders = c.refs[b.page];
     const uint32_t refused = P.r.h->refused;
     uint8_t* page = c.pool + page_offset(b.page, c.n_pages, P.r.layer0, c.n_layers);
@@ -47,7 +61,6 @@ __global__ __launch_bounds__(kRowThreads) void latent_kernel(LatentParams P) {
     const bool aged = b.base < b.first;                   // older positions in the block
     // c: a lane's 16 values; k_pe: the 16 pairs of which it makes the first or second values
     u32x4 in[4] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-    u32x4 w[2];
     if (fresh) {
         const uint16_t* row = P.r.rows + (int64_t)(b.row0 + pos - b.first) * P.r.row_stride;
         if (wave < 8) {
@@ -64,14 +77,9 @@ __global__ __launch_bounds__(kRowThreads) void latent_kernel(LatentParams P) {
             in[3] = ld_global(at + second + 1);
         }
     }
-    if (P.norm && wave < 8) {
-        w[0] = ld_global(reinterpret_cast<const u32x4*>(P.norm + chunk * 16));
-        w[1] = ld_global(reinterpret_cast<const u32x4*>(P.norm + chunk * 16) + 1);
-    }
     const uint32_t was = aged ? ld_global(scale) : 0;
     if (t < kBlock * kPairs)
-        cs[t / kPairs][t % kPairs] = rope::angle(ld_global(P.rope.turns + t % kPairs),
-                                                 b.base + t / kPairs, P.rope.magnitude);
+        cs[t / kPairs][t % kPairs] = rope::angle(turns, b.base + t / kPairs, P.rope.magnitude);
     float v[16];
     if (wave < 8) {
         // (64 bits: the squares of any finite bf16 fit, and cost what 32 cost)
@@ -96,10 +104,15 @@ __global__ __launch_bounds__(kRowThreads) void latent_kernel(LatentParams P) {
         s = s * (1.0 / kC) + (double)P.eps;
         // (good to 2^-24; where it is below the least fp32, the values take part of it)
         const double inv = __builtin_amdgcn_rsq(s);
-        const bool huge = s > 0x1p200;
-        const float pre = huge ? 0x1p-64f : 1.f, rms = (float)(huge ? inv * 0x1p64 : inv);
+        if (s > 0x1p200) {
+            const float rms = (float)(inv * 0x1p64);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = v[i] * pre * rms;
+            for (float& x : v) x = x * 0x1p-64f * rms;
+        } else {
+            const float rms = (float)inv;
+#pragma unroll
+            for (float& x : v) x *= rms;
+        }
         if (P.norm)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -107,27 +120,29 @@ __global__ __launch_bounds__(kRowThreads) void latent_kernel(LatentParams P) {
                 v[2 * i + 1] *= bf_hi(w[i / 4][i % 4]);
             }
     } else {
-        const bool halves = P.rope.halves_in;
-        float x[32];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            x[2 * i] = bf_lo(in[i / 4][i % 4]);
-            x[2 * i + 1] = bf_hi(in[i / 4][i % 4]);
-        }
+        // first values (parts 0, 1) are p cos - q sin, second ones q cos + p sin
+        const bool halves = P.rope.halves_in, second = part >= 2;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float2 a = cs[tok][(part & 1) * 16 + i];
-            const float p = halves ? x[i] : x[2 * i], q = halves ? x[16 + i] : x[2 * i + 1];
-            v[i] = part < 2 ? fmaf(p, a.x, -(q * a.y)) : fmaf(q, a.x, p * a.y);
+            const uint32_t w0 = in[i / 8][i / 2 % 4], w1 = in[2 + i / 8][i / 2 % 4];
+            const uint32_t both = in[i / 4][i % 4];
+            const float p = halves ? (i % 2 ? bf_hi(w0) : bf_lo(w0)) : bf_lo(both);
+            const float q = halves ? (i % 2 ? bf_hi(w1) : bf_lo(w1)) : bf_hi(both);
+            v[i] = fmaf(second ? q : p, a.x, (second ? p : -q) * a.y);
         }
     }
-    // the largest finite magnitude, as bits: they order as the values do
-    uint32_t big = 0;
+    // the largest finite magnitude, as bits: they order as the values do (rows that are not new
+    // are zeros here; a maximum leaves NaN out, and the infinities are rare)
+    float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const uint32_t x = __float_as_uint(v[i]) & 0x7fffffff;
-        big = fresh && x < 0x7f800000 && x > big ? x : big;
+    for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, fabsf(v[i])), fabsf(v[i + 1]));
+    if (!(top < INFINITY)) {
+        top = 0.f;
+#pragma unroll
+        for (const float& x : v) top = fabsf(x) < INFINITY ? fmaxf(top, fabsf(x)) : top;
     }
+    uint32_t big = __float_as_uint(top);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const uint32_t o = __shfl_xor(big, d);

@@ -50,6 +50,20 @@ __device__ __forceinline__ void st_global(T* p, T v) {
     *(__attribute__((address_space(1))) T*)p = v;
 }
 
+// The same where the value lies at a multiple of kAlign bytes only: one load or store, too.
+template <int kAlign, class T>
+struct __attribute__((packed, aligned(kAlign))) AlignedTo {
+    T v;
+};
+template <int kAlign, class T>
+__device__ __forceinline__ T ld_global_at(const void* p) {
+    return ((gmem_ptr<AlignedTo<kAlign, T>>)p)->v;
+}
+template <int kAlign, class T>
+__device__ __forceinline__ void st_global_at(void* p, const T& v) {
+    ((__attribute__((address_space(1))) AlignedTo<kAlign, T>*)p)->v = v;
+}
+
 // DeepSeek-V2-Lite MoE shape (reference/dsv2lite_config.json).
 constexpr int kHidden = 2048;
 constexpr int kInter = 1408;          // routed expert intermediate

@@ -41,83 +41,75 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
-// A thread's values of a row: kN chunks of 8, chunk i from value 8 * (t + i * kThreads)
-// on, in 16-byte loads; or, where a row's values do not lie in such chunks, one by one, value
-// t + j * kThreads. What is behind the row is 0.
-template <int kThreads, int kN, bool kWide>
+// A thread's values of a row: kN chunks of 8, chunk i from value 8 * (t + i * kThreads) on.
+// A row's last chunk may be short; what is behind the row is 0. (A row may begin anywhere a
+// value may: odd widths take 70 us where one value at a time took 200, of 3,000 rows of 8,191.)
+template <int kThreads, int kN>
 struct Row {
     static constexpr int kValues = 8 * kN;
     float v[kValues];
 
-    __device__ __forceinline__ static int chunk(int t, int i) { return 8 * (t + i * kThreads); }
-    template <class F>
-    __device__ __forceinline__ static void each_chunk(int t, int width, F f) {
+    // whole(i, at) for a chunk of v[i ..] at value `at`, one(i, at) for a value of a short one
+    template <class F, class G>
+    __device__ __forceinline__ static void each(int t, int width, F whole, G one) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i)
-            if (chunk(t, i) < width) f(8 * i, chunk(t, i));
-    }
-    template <class F>
-    __device__ __forceinline__ static void each_value(int t, int width, F f) {
+        for (int i = 0; i < kN; ++i) {
+            const int at = 8 * (t + i * kThreads);
+            if (at + 8 <= width) {
+                whole(8 * i, at);
+            } else if (at < width) {
 #pragma unroll
-        for (int j = 0; j < kValues; ++j)
-            if (t + j * kThreads < width) f(j, t + j * kThreads);
+                for (int k = 0; k < 7; ++k)
+                    if (at + k < width) one(8 * i + k, at + k);
+            }
+        }
     }
-
     __device__ __forceinline__ void load(const uint16_t* p, int t, int width) {
 #pragma unroll
         for (auto& e : v) e = 0.f;
-        if constexpr (kWide)
-            each_chunk(t, width, [&](int i, int at) {
-                const u32x4 w = ld_global(reinterpret_cast<const u32x4*>(p + at));
+        each(t, width,
+             [&](int i, int at) {
+                 const u32x4 w = ld_global_at<2, u32x4>(p + at);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[i + 2 * k] = bf_lo(w[k]);
-                    v[i + 2 * k + 1] = bf_hi(w[k]);
-                }
-            });
-        else
-            each_value(t, width, [&](int j, int at) {
-                v[j] = __uint_as_float((uint32_t)ld_global(p + at) << 16);
-            });
+                 for (int k = 0; k < 4; ++k) {
+                     v[i + 2 * k] = bf_lo(w[k]);
+                     v[i + 2 * k + 1] = bf_hi(w[k]);
+                 }
+             },
+             [&](int i, int at) { v[i] = __uint_as_float((uint32_t)ld_global(p + at) << 16); });
     }
     __device__ __forceinline__ void load(const float* p, int t, int width) {
 #pragma unroll
         for (auto& e : v) e = 0.f;
-        if constexpr (kWide)
-            each_chunk(t, width, [&](int i, int at) {
-                const f32x4 a = ld_global(reinterpret_cast<const f32x4*>(p + at));
-                const f32x4 b = ld_global(reinterpret_cast<const f32x4*>(p + at) + 1);
+        each(t, width,
+             [&](int i, int at) {
+                 const f32x4 a = ld_global_at<4, f32x4>(p + at);
+                 const f32x4 b = ld_global_at<4, f32x4>(p + at + 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[i + k] = a[k];
-                    v[i + 4 + k] = b[k];
-                }
-            });
-        else
-            each_value(t, width, [&](int j, int at) { v[j] = ld_global(p + at); });
+                 for (int k = 0; k < 4; ++k) {
+                     v[i + k] = a[k];
+                     v[i + 4 + k] = b[k];
+                 }
+             },
+             [&](int i, int at) { v[i] = ld_global(p + at); });
     }
     __device__ __forceinline__ void store(uint16_t* p, int t, int width) const {
-        if constexpr (kWide)
-            each_chunk(t, width, [&](int i, int at) {
-                u32x4 w;
+        each(t, width,
+             [&](int i, int at) {
+                 u32x4 w;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = pack(v[i + 2 * k], v[i + 2 * k + 1]);
-                st_global(reinterpret_cast<u32x4*>(p + at), w);
-            });
-        else
-            each_value(t, width, [&](int j, int at) {
-                st_global(p + at, (uint16_t)pack(v[j], 0.f));
-            });
+                 for (int k = 0; k < 4; ++k) w[k] = pack(v[i + 2 * k], v[i + 2 * k + 1]);
+                 st_global_at<2>(p + at, w);
+             },
+             [&](int i, int at) { st_global(p + at, (uint16_t)pack(v[i], 0.f)); });
     }
     __device__ __forceinline__ void store(float* p, int t, int width) const {
-        if constexpr (kWide)
-            each_chunk(t, width, [&](int i, int at) {
-                f32x4* to = reinterpret_cast<f32x4*>(p + at);
-                st_global(to, f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]});
-                st_global(to + 1, f32x4{v[i + 4], v[i + 5], v[i + 6], v[i + 7]});
-            });
-        else
-            each_value(t, width, [&](int j, int at) { st_global(p + at, v[j]); });
+        each(t, width,
+             [&](int i, int at) {
+                 st_global_at<4>(p + at, f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]});
+                 st_global_at<4>(p + at + 4, f32x4{v[i + 4], v[i + 5], v[i + 6], v[i + 7]});
+             },
+             [&](int i, int at) { st_global(p + at, v[i]); });
     }
     __device__ __forceinline__ void load(const void* p, bool f32, int64_t at, int t, int width) {
         if (f32) load(static_cast<const float*>(p) + at, t, width);
@@ -170,9 +162,9 @@ __device__ __forceinline__ void unit(R& r, int width, float eps, float* lds) {
     for (float& e : r.v) e *= inv;
 }
 
-// kThreads threads a row, 64 for rows of which there are enough to fill the chip: no
-// barrier, and four rows a workgroup.
-template <int kThreads, int kN, bool kWide>
+// kThreads threads a row, with 8 kN values each; a wave for narrow rows, four a workgroup and
+// no barrier.
+template <int kThreads, int kN>
 __global__ __launch_bounds__(kThreads > 256 ? kThreads : 256) void norm_kernel(Params P) {
     __shared__ float lds[16];
     constexpr int kRows = kThreads > 256 ? 1 : 256 / kThreads;
@@ -180,7 +172,7 @@ __global__ __launch_bounds__(kThreads > 256 ? kThreads : 256) void norm_kernel(P
     const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kThreads;
     if (row >= P.rows) return;
     const int w = P.width;
-    Row<kThreads, kN, kWide> x, u, f;
+    Row<kThreads, kN> x, u, f;
     x.load(P.x, P.x_f32, row * P.x_stride, t, w);
     if (P.y) {
         u.load(P.y, P.y_f32, row * P.y_stride, t, w);
@@ -225,11 +217,10 @@ using namespace fleet_moe::norm;
 int fleet_moe_check_device(int min_cus);
 
 template <int kThreads, int kN>
-static int launch_norm(const Params& P, bool wide, hipStream_t stream) {
+static int launch_norm(const Params& P, hipStream_t stream) {
     constexpr int kBlock = kThreads > 256 ? kThreads : 256, kRows = kBlock / kThreads;
-    const dim3 grid((unsigned)((P.rows + kRows - 1) / kRows)), block(kBlock);
-    if (wide) hipLaunchKernelGGL((norm_kernel<kThreads, kN, true>), grid, block, 0, stream, P);
-    else hipLaunchKernelGGL((norm_kernel<kThreads, kN, false>), grid, block, 0, stream, P);
+    hipLaunchKernelGGL((norm_kernel<kThreads, kN>), dim3((unsigned)((P.rows + kRows - 1) / kRows)),
+                       dim3(kBlock), 0, stream, P);
     return (int)hipGetLastError();
 }
 
@@ -273,12 +264,8 @@ extern "C" int fleet_residual_norm(const void* x, int32_t x_f32, int64_t x_strid
     P.width = width;
     P.x_f32 = x_f32;
     P.y_f32 = y_f32;
-    const uintptr_t all = (uintptr_t)x | (uintptr_t)y | (uintptr_t)post_norm | (uintptr_t)gate |
-                          (uintptr_t)norm | (uintptr_t)x_out | (uintptr_t)h | (uintptr_t)h_f32;
-    const bool wide = all % 16 == 0 && (width | x_stride | y_stride | gate_stride) % 8 == 0;
-    // Few rows take more threads a row: a wave's 32 values a lane would be its latency.
-    if (width <= 2048 && n_rows > 1024) return launch_norm<64, 4>(P, wide, stream);
-    if (width <= 2048) return launch_norm<256, 1>(P, wide, stream);
-    if (width <= 8192) return launch_norm<256, 4>(P, wide, stream);
-    return launch_norm<1024, 4>(P, wide, stream);
+    if (width <= 512) return launch_norm<64, 1>(P, stream);
+    if (width <= 2048) return launch_norm<256, 1>(P, stream);
+    if (width <= 8192) return launch_norm<512, 2>(P, stream);
+    return launch_norm<1024, 4>(P, stream);
 }
