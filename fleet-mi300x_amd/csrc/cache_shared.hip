@@ -120,19 +120,41 @@ __global__ __launch_bounds__(kShareThreads) void share_kernel(fleet_cache c, con
     const int from = lead;
     if (held == 0 || end - first < 2) most = 0;
     __syncthreads();
-    // columns 64 at a time, a row a wave, until one differs
+    // 256 columns at a time, a row a wave, until one differs; 16 loads of a lane on their way
     const int lane = t & 63, wave = t >> 6;
     const int32_t* row = c.table + (int64_t)from * c.max_pages;
-    for (int j0 = 0; j0 < most; j0 += 64) {
-        const int j = j0 + lane;
-        const int mine = j < most ? row[j] : -1;
-        bool same = j >= most || (unsigned)mine < (unsigned)c.n_pages;
-        for (int s = first + wave; s < end && __ballot(same) == ~0ull; s += kShareThreads / 64) {
-            if (checked_len(c.lens[s], c.max_pages) <= 0) continue;
-            same = j >= most || c.table[(int64_t)s * c.max_pages + j] == mine;
+    constexpr int kCols = 4, kRows = 4, kWaves = kShareThreads / 64;
+    for (int j0 = 0; j0 < most; j0 += 64 * kCols) {
+        int mine[kCols];
+        int differs = 0x7fffffff;
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) {
+            const int j = j0 + 64 * k + lane;
+            mine[k] = j < most ? row[j] : 0;
+            if (j < most && (unsigned)mine[k] >= (unsigned)c.n_pages) differs = j < differs ? j : differs;
         }
-        const uint64_t all = __ballot(same);
-        if (all != ~0ull && lane == 0) atomicMin(&pages, j0 + __ffsll((long long)~all) - 1);
+        for (int s0 = first + wave; s0 < end; s0 += kRows * kWaves) {
+            int there[kRows][kCols], lens[kRows];
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                const int s = s0 + r * kWaves;
+                lens[r] = s < end ? c.lens[s] : 0;
+#pragma unroll
+                for (int k = 0; k < kCols; ++k) {
+                    const int j = j0 + 64 * k + lane;
+                    there[r][k] = s < end && j < most ? c.table[(int64_t)s * c.max_pages + j] : mine[k];
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+                if (checked_len(lens[r], c.max_pages) > 0)
+#pragma unroll
+                    for (int k = 0; k < kCols; ++k) {
+                        const int j = j0 + 64 * k + lane;
+                        if (there[r][k] != mine[k] && j < differs) differs = j;
+                    }
+        }
+        if (differs < most) atomicMin(&pages, differs);
         __syncthreads();
         const int now = pages;
         __syncthreads();
@@ -175,6 +197,7 @@ struct Item {
     int first, end, last;               // the sequences, and the token behind them
     int steps0, steps1;                 // of a unit, whether they see anything or not
 };
+// All but `last`, which needs the group's end.
 __device__ __forceinline__ Item item_of(const SharedParams& P, int seq, bool stale) {
     Item w;
     const i32x4 g = ld_global(reinterpret_cast<const i32x4*>(P.plan.groups + seq));
@@ -186,12 +209,13 @@ __device__ __forceinline__ Item item_of(const SharedParams& P, int seq, bool sta
     w.end = stale ? seq + 1 : g.y;
     w.pages = stale ? 0 : g.z;
     w.lead = stale ? seq : g.w;
-    w.last = w.pages > 0 && seq == w.first ? start_of(P, w.end) : w.tok0;
+    w.last = w.tok0;
     w.steps0 = w.pages;
     const int own = w.len < 0 ? 0 : pages_of(w.len) - w.pages;
     w.steps1 = own > 1 ? own : 1;
     return w;
 }
+__device__ __forceinline__ bool leads(const Item& w) { return w.pages > 0 && w.seq == w.first; }
 __device__ __forceinline__ Item lane_of(const Item& v, int lane) {
     static_assert(sizeof(Item) == 44, "");
     struct Words {
@@ -207,8 +231,15 @@ __device__ __forceinline__ Item lane_of(const Item& v, int lane) {
 // A workgroup does the pages whose time begins in its share.
 struct Cost {
     int setup, page;
+    // How many pages begin before `time`.
+    __device__ __forceinline__ int begun(int time) const;
 };
 constexpr Cost kCost16{30, 8}, kCost64{60, 11};
+__device__ __forceinline__ int Cost::begun(int time) const {
+    const int t = time > setup ? time - setup : 0;        // (divided by constants)
+    return page == kCost16.page ? (t + kCost16.page - 1) / kCost16.page
+                                : (t + kCost64.page - 1) / kCost64.page;
+}
 struct Sizes {
     int rows0, units0, rows1, units1;
     __device__ __forceinline__ Sizes(const SharedParams& P, const Item& w) {
@@ -235,7 +266,7 @@ struct Sizes {
 // A range of n things in `shares` parts that differ by one at most.
 struct Split {
     int each, more;             // the first `more` have each + 1
-    __device__ Split(int n, int shares) : each(n / shares), more(n % shares) {}
+    __device__ Split(int n, int shares) : each(n / shares), more(n - each * shares) {}
     __device__ int first(int i) const { return i * each + (i < more ? i : more); }
     __device__ int holder(int at) const {
         const int big = more * (each + 1);
@@ -243,7 +274,7 @@ struct Split {
     }
 };
 
-constexpr int kLeast = 20;
+constexpr int kLeast = 11;
 static_assert(kLeast >= kCost64.page && kLeast >= kCost16.page, "");
 // How many workgroups take part. No share is shorter than a page's time (so that every one
 // between a unit's first and last has a part of it), and few pages are left to many only as
@@ -343,9 +374,19 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
     int n = 0, first = 0;
     bool bad = false, inside = false;
     Item w{}, w1{};
+    int* starts = reinterpret_cast<int*>(L.tile);         // [n_seqs + 1]
     if (t * each < P.c.n_seqs) {
         w = item_of(P, t * each, stale);
-        if (each > 1 && t * each + 1 < P.c.n_seqs) w1 = item_of(P, t * each + 1, stale);
+        starts[t * each + 1] = w.tok0 + w.n_new;
+        if (each > 1 && t * each + 1 < P.c.n_seqs) {
+            w1 = item_of(P, t * each + 1, stale);
+            starts[t * each + 2] = w1.tok0 + w1.n_new;
+        }
+    }
+    barrier();
+    if (t * each < P.c.n_seqs) {
+        if (leads(w)) w.last = starts[w.end];
+        if (leads(w1)) w1.last = starts[w1.end];
         first = Sizes(P, w).total(w);
         n = first + Sizes(P, w1).total(w1);
         bad = (w.n_new | w1.n_new) < 0;
@@ -420,18 +461,23 @@ constexpr int kQueryStep = 2 * kRow + 16;
 __device__ __forceinline__ uint8_t* query_at(PageLds& L, int place, int row) {
     return L.tile[place] + row * kQueryStep;
 }
-// A wave's rows; of dead ones the unit's first.
+// A wave's rows; of dead ones the unit's first. (A lane a row's address.)
+template <int kRows>
 __device__ __forceinline__ void copy_q(const SharedParams& P, PageLds& L, const Unit& u, int place,
-                                       int rows, int wave, int lane) {
-    for (int i = 0; i < rows; ++i) {
-        const int at = wave * rows + i;
-        const int row = u.row0 + at < u.rows ? u.row0 + at : u.row0;
-        const int tok = token_of_row(row, P.per_head);
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(
-            P.q + (int64_t)(u.tok0 + tok) * P.q_stride + (row - tok * P.n_heads) * kRow);
-        const uint32_t to = lds_addr(query_at(L, place, at));
-        copy_kb<1, false>(src + lane * 16, to);
-        if (lane < (2 * kRow - 1024) / 16) copy_kb<1, false>(src + 1024 + lane * 16, to + 1024);
+                                       int wave, int lane) {
+    const int mine = u.row0 + wave * kRows + lane % kRows, row = mine < u.rows ? mine : u.row0;
+    const int tok = token_of_row(row, P.per_head);
+    const uint64_t from = (uint64_t)(uintptr_t)(P.q + (int64_t)(u.tok0 + tok) * P.q_stride +
+                                                (row - tok * P.n_heads) * kRow);
+    const uint32_t to = lds_addr(query_at(L, place, wave * kRows));
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)from, i);
+        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(from >> 32), i);
+        const uint8_t* src = reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo) + lane * 16;
+        copy_kb<1, false>(src, to + i * kQueryStep);
+        if (lane < (2 * kRow - 1024) / 16)
+            copy_kb<1, false>(src + 1024, to + i * kQueryStep + 1024);
     }
 }
 // A lane's row as the right operand. The k order of the products is that of the bytes a lane of
@@ -504,7 +550,7 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
     if (cnt > 0) {
         turn_to(P, u, pages, off, off + cnt, lane);
         if (tp == 0) issue(0, 0);
-        copy_q(P, L, u, 1, kTile / kGridWaves, wave, lane);
+        copy_q<kTile / kGridWaves>(P, L, u, 1, wave, lane);
     }
     TileRow r = tile_row(P, u, u.row0 + mine * 16 + n);
     set_position(P, u, r);
@@ -781,7 +827,7 @@ __device__ __forceinline__ void attend16(const SharedParams& P, PageLds& L, cons
         turn_to(P, u, pages, off, off + cnt, lane);
         if (!weighs)
             for (int k = 0; k < kPageRing - 1 && k < cnt; ++k) issue(k, k);
-        copy_q(P, L, u, kPageRing - 1, 16 / kGridWaves, wave, lane);
+        copy_q<16 / kGridWaves>(P, L, u, kPageRing - 1, wave, lane);
     }
     TileRow r = tile_row(P, u, u.row0 + n);
     set_position(P, u, r);
@@ -949,7 +995,7 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
         const int rows = u.common ? z.rows0 : z.rows1, steps = u.common ? w.steps0 : w.steps1;
         const int o = u.common ? off : off - front, whole64 = kCost64.setup + kCost64.page * steps;
         const int units = u.common ? z.units0 : z.units1;
-        const int k = o / whole64 < units ? o / whole64 : units - 1;
+        const int k64 = o / whole64, k = k64 < units ? k64 : units - 1;
         const Cost cost = Sizes::cost(rows, k);
         const int from = o - k * whole64, all = cost.setup + cost.page * steps;
         u.row0 = k * kTile;
@@ -976,7 +1022,7 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
         // the steps that begin from here to the share's end
         const int take = all - from < end - at ? all - from : end - at;
         const auto step_at = [&](int time) {
-            const int i = time <= cost.setup ? 0 : (time - cost.setup + cost.page - 1) / cost.page;
+            const int i = cost.begun(time);
             return i < steps ? i : steps;
         };
         const int lo = step_at(from), hi = step_at(from + take);
@@ -987,6 +1033,7 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
             if (end - at > take)
                 while (o2 >= Sizes(P, next).total(next) && next.seq + 1 < P.c.n_seqs) {
                     next = item_of(P, next.seq + 1, stale);
+                    if (leads(next)) next.last = start_of(P, next.end);
                     o2 = 0;
                 }
             L.item = next;

@@ -233,7 +233,9 @@ def test_a_prompt_like_the_decoders_attention():
     s.step(x, i32([0, n]), keep)
     assert dec.status() == 0 and s.cache.status() == 0
     got, y = ops.bf16_bits_to_f32(keep["x1"]), want - ops.bf16_bits_to_f32(x)
-    # cos of the angle between the two updates: an error of 2^-5 in the mean of the rows' values
+    # Rounding to 8 bits is off by 2^-4 of a value at most, 2^-4 / sqrt(3) in the mean square: the
+    # outputs by no more of their length than that, their scores' share of it again, and the
+    # roundings to bf16 (2^-8). A sine of 2^-3, three times as much, is a cosine of 1 - 2^-7.
     g = got - ops.bf16_bits_to_f32(x)
     cosine = (g * y).sum(1) / (g.norm(dim=1) * y.norm(dim=1))
     assert (cosine > 1 - 2.0**-7).all(), cosine.min()
