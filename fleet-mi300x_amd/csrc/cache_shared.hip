@@ -40,26 +40,38 @@ struct Group {
     int32_t pages;              // common to those that hold anything
     int32_t lead;               // one of these
 };
-struct Parts {                  // of a row and kind: part 0, part 1, part 1 + kStep, ..
+struct Parts {                  // of a row and kind: part 0, part 1, part 1 + kPartStep, ..
     int32_t at, next, count;
     int32_t front;              // there are parts over common pages, too
 };
 constexpr int kPartStep = 2 * kTile;    // a workgroup has two slots
 constexpr int64_t kMaxPlanRows = 1 << 20;
 
+// Partial results lie in tiles of 16 rows as the matrix instructions leave them: [wave (64
+// columns)][16 columns][lane (4 columns, row)], 32 KB, so that a wave's store is 1 KB of
+// consecutive bytes (rows of 512 columns: 64 bytes of 16 rows each, 6,300 cycles a unit where
+// this takes 3,100). Part `at` is row at % 16 of tile at / 16. Whole units have a tile for every 16
+// rows of a sequence (or group, by its first sequence), split ones the slots behind those.
 struct Plan {
     PlanHeader* h;
     Group* groups;              // [n_seqs]: a sequence's
     Parts* meta;                // [2][rows]: over the common pages, over its own
-    f32x4* stat;                // [2 rows + slots]
-    float* part;                // [2 rows + slots][512]
+    f32x4* stat;                // [parts]
+    f32x4* part;                // [parts / 16][8][4][64]
 };
-__host__ __device__ inline int64_t plan_parts(int64_t rows) {
-    return 2 * rows + (int64_t)kGrid * kPartStep;
+__host__ __device__ inline int64_t whole_parts(int n_seqs, int64_t rows) {
+    return 16 * (rows / 16 + n_seqs + 1);
+}
+__host__ __device__ inline int64_t whole_part(int seq, int64_t first_row) {
+    return 16 * (first_row / 16 + seq);
+}
+inline int64_t plan_parts(int n_seqs, int64_t rows) {
+    return 2 * whole_parts(n_seqs, rows) + (int64_t)kGrid * kPartStep;
 }
 inline size_t plan_size(int n_seqs, int64_t rows) {
     return sizeof(PlanHeader) + up256((size_t)n_seqs * sizeof(Group)) +
-           up256((size_t)rows * 2 * sizeof(Parts)) + (size_t)plan_parts(rows) * (16 + 4 * kC);
+           up256((size_t)rows * 2 * sizeof(Parts)) +
+           (size_t)plan_parts(n_seqs, rows) * (16 + 4 * kC);
 }
 inline Plan plan_at(void* p, int n_seqs, int64_t rows) {
     char* c = static_cast<char*>(p);
@@ -71,8 +83,12 @@ inline Plan plan_at(void* p, int n_seqs, int64_t rows) {
     r.meta = reinterpret_cast<Parts*>(c);
     c += up256((size_t)rows * 2 * sizeof(Parts));
     r.stat = reinterpret_cast<f32x4*>(c);
-    r.part = reinterpret_cast<float*>(c + (size_t)plan_parts(rows) * 16);
+    r.part = reinterpret_cast<f32x4*>(c + (size_t)plan_parts(n_seqs, rows) * 16);
     return r;
+}
+// Where lane `lane`'s four of columns 64 wave + 16 j .. lie.
+__device__ __forceinline__ f32x4* part_at(const Plan& p, int64_t tile, int wave, int j, int lane) {
+    return p.part + ((tile * kGridWaves + wave) * 4 + j) * 64 + lane;
 }
 
 // ---------------------------------------------------------------- share
@@ -240,28 +256,42 @@ __device__ __forceinline__ int Cost::begun(int time) const {
     return page == kCost16.page ? (t + kCost16.page - 1) / kCost16.page
                                 : (t + kCost64.page - 1) / kCost64.page;
 }
+// Units have 64 rows, or 16 where there are few pages: up to eight a workgroup of 16 rows take
+// less time than the two of 64 rows, with a unit's beginning and the parts to be joined (16
+// sequences of 4,100 positions 24.0 us, in 64 rows 28.6; with eleven, 32 in eight groups 32.8 us,
+// in 64 rows 31.6).
+constexpr int kFewSteps = 8 * kGrid;
 struct Sizes {
     int rows0, units0, rows1, units1;
-    __device__ __forceinline__ Sizes(const SharedParams& P, const Item& w) {
+    int tile;
+    __device__ __forceinline__ Sizes(const SharedParams& P, const Item& w, int rows) {
+        tile = rows;
         rows0 = (w.last - w.tok0) * P.n_heads;
         rows1 = w.n_new > 0 ? w.n_new * P.n_heads : 0;
-        units0 = (rows0 + kTile - 1) / kTile;
-        units1 = (rows1 + kTile - 1) / kTile;
+        const int shift = tile == kTile ? 6 : 4;
+        units0 = (rows0 + tile - 1) >> shift;
+        units1 = (rows1 + tile - 1) >> shift;
     }
+    __device__ __forceinline__ Cost full() const { return tile == kTile ? kCost64 : kCost16; }
     // The time of unit k of either kind.
-    __device__ __forceinline__ static Cost cost(int rows, int k) {
-        return rows - k * kTile <= 16 ? kCost16 : kCost64;
+    __device__ __forceinline__ Cost cost(int rows, int k) const {
+        return rows - k * tile <= 16 ? kCost16 : full();
     }
-    __device__ __forceinline__ static int time(int rows, int units, int pages) {
+    __device__ __forceinline__ int time(int rows, int units, int pages) const {
         if (units == 0) return 0;
         const Cost z = cost(rows, units - 1);
-        return (units - 1) * (kCost64.setup + kCost64.page * pages) + z.setup + z.page * pages;
+        return (units - 1) * (full().setup + full().page * pages) + z.setup + z.page * pages;
     }
     __device__ __forceinline__ int front(const Item& w) const { return time(rows0, units0, w.steps0); }
     __device__ __forceinline__ int total(const Item& w) const {
         return front(w) + time(rows1, units1, w.steps1);
     }
+    __device__ __forceinline__ int units() const { return units0 + units1; }
+    __device__ __forceinline__ int steps(const Item& w) const {
+        return units0 * w.steps0 + units1 * w.steps1;
+    }
 };
+static_assert(kTile == 64, "");
 
 // A range of n things in `shares` parts that differ by one at most.
 struct Split {
@@ -350,7 +380,7 @@ struct PageLds {
     f32x4 half[2][kGridWaves][2][64];   // [step parity] half of the scores of a tile and two
                                         // blocks
     uint32_t scale[kPageRing][8];
-    int flag[2][kGridWaves];
+    int flag[2][kGridWaves], units[2][kGridWaves];
     __attribute__((aligned(8))) uint8_t flags[2][kGridWaves];   // (64 rows) 1: a row's reference
                                 // rises, 2: a score is not finite
     float m[4][16], top[4][2][16], sum[4][2][16], rounded[4][2][16];
@@ -364,6 +394,7 @@ static_assert(kTile * (2 * kRow + 16) <= 2 * 4 * kBlockStep + 16 * 1024, "");
 // two.
 struct Place {
     int total, shares;
+    int tile;                   // rows of a unit
     bool inside;                // some token stands within its group's common pages
 };
 __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg, bool stale,
@@ -371,7 +402,7 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int each = P.c.n_seqs > kGridThreads ? 2 : 1;
     static_assert(kMaxSeqs <= 2 * kGridThreads, "");
-    int n = 0, first = 0;
+    int n = 0, first = 0, units = 0, steps = 0, first16 = 0;
     bool bad = false, inside = false;
     Item w{}, w1{};
     int* starts = reinterpret_cast<int*>(L.tile);         // [n_seqs + 1]
@@ -387,26 +418,50 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
     if (t * each < P.c.n_seqs) {
         if (leads(w)) w.last = starts[w.end];
         if (leads(w1)) w1.last = starts[w1.end];
-        first = Sizes(P, w).total(w);
-        n = first + Sizes(P, w1).total(w1);
+        first = Sizes(P, w, kTile).total(w);
+        n = first + Sizes(P, w1, kTile).total(w1);
+        const Sizes a(P, w, 16), b(P, w1, 16);
+        first16 = a.units() * kCost16.setup + a.steps(w) * kCost16.page;
+        units = a.units() + b.units();
+        steps = a.steps(w) + b.steps(w1);
         bad = (w.n_new | w1.n_new) < 0;
         inside = (w.n_new > 0 && w.len - w.n_new < w.pages * kPage) ||
                  (w1.n_new > 0 && w1.len - w1.n_new < w1.pages * kPage);
     }
-    const int incl = wave_incl_scan(n);
+    int incl = wave_incl_scan(n);
+    const int units_incl = wave_incl_scan(units), steps_incl = wave_incl_scan(steps);
     const int flags = (__ballot(bad) ? 1 : 0) | (__ballot(inside) ? 2 : 0);
     if (lane == 63) {
         L.flag[0][wave] = incl;
         L.flag[1][wave] = flags;
+        L.units[0][wave] = units_incl;
+        L.units[1][wave] = steps_incl;
     }
     barrier();
-    int before = 0, any = 0;
+    int before = 0, any = 0, all_units = 0, all_steps = 0, units_before = 0, steps_before = 0;
     at.total = 0;
 #pragma unroll
     for (int i = 0; i < kGridWaves; ++i) {
-        if (i < wave) before += L.flag[0][i];
+        if (i < wave) {
+            before += L.flag[0][i];
+            units_before += L.units[0][i];
+            steps_before += L.units[1][i];
+        }
         at.total += L.flag[0][i];
+        all_units += L.units[0][i];
+        all_steps += L.units[1][i];
         any |= L.flag[1][i];
+    }
+    at.tile = kTile;
+    if (wave_bcast(all_steps) <= kFewSteps) {
+        // (a unit has a page at least: the times are small)
+        const auto time = [](int u, int s) { return u * kCost16.setup + s * kCost16.page; };
+        at.tile = 16;
+        at.total = time(all_units, all_steps);
+        before = time(units_before, steps_before);
+        incl = time(units_incl, steps_incl);
+        n = time(units, steps);
+        first = first16;
     }
     at.total = wave_bcast(at.total);
     any = wave_bcast(any);
@@ -454,7 +509,7 @@ __device__ __forceinline__ bool valid(const PageList& h, int i) {
 }
 
 // The queries of a unit go through the ring before its pages: a lane's own loads of them, 16
-// bytes of 16 rows at a time, took 12,000 cycles for 64 rows (a page's step takes 4,800). Rows
+// bytes of 16 rows at a time, took 12,000 cycles for 64 rows (a page's step takes 4,450). Rows
 // lie 16 bytes further apart than they are long, so that the operands of 16 rows fall into
 // different banks.
 constexpr int kQueryStep = 2 * kRow + 16;
@@ -785,24 +840,24 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
     const int column0 = wave * kCols * 16 + 4 * g;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+        if (u.row0 + i * 16 >= u.rows) break;
         const int row = i * 16 + n;
-        if (u.row0 + row >= u.rows) continue;
         const float sum = L.sum[i][0][n] + L.sum[i][1][n];
         const float rounded = L.rounded[i][0][n] + L.rounded[i][1][n];
         const float scaled = L.m[i][n] * P.scale;
-        if (to_part < 0) {
+        if (to_part >= 0) {
+#pragma unroll
+            for (int j = 0; j < kCols; ++j)
+                st_global(part_at(P.plan, to_part / 16 + i, wave, j, lane), acc[i][j]);
+            if (wave == 0 && g == 0)
+                st_global(P.plan.stat + to_part + row, f32x4{scaled, sum, rounded, 0.f});
+        } else if (u.row0 + row < u.rows) {
             const int64_t to = (int64_t)u.tok0 * P.n_heads + u.row0 + row;
             const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
 #pragma unroll
             for (int j = 0; j < kCols; ++j)
                 put(P.out + to * kC + column0 + j * 16, acc[i][j], inv);
             if (P.lse && wave == 0 && g == 0) P.lse[to] = lse_of(scaled, sum);
-        } else {
-            const int64_t to = to_part + row;
-#pragma unroll
-            for (int j = 0; j < kCols; ++j)
-                st_global(reinterpret_cast<f32x4*>(P.plan.part + to * kC + column0 + j * 16), acc[i][j]);
-            if (wave == 0 && g == 0) st_global(P.plan.stat + to, f32x4{scaled, sum, rounded, 0.f});
         }
     }
 }
@@ -954,21 +1009,20 @@ __device__ __forceinline__ void attend16(const SharedParams& P, PageLds& L, cons
     l = xor32_sum(xor16_sum(l));
     if (weighs && lane < 16) L.sum[blk][0][lane] = l;
     barrier();
-    if (u.row0 + n >= u.rows) return;
-    const int column0 = wave * kCols * 16 + 4 * g;
     const float sum = (L.sum[0][0][n] + L.sum[1][0][n]) + (L.sum[2][0][n] + L.sum[3][0][n]);
-    if (to_part < 0) {
+    if (to_part >= 0) {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+            st_global(part_at(P.plan, to_part / 16, wave, j, lane), acc[j]);
+        if (wave == 0 && g == 0)
+            st_global(P.plan.stat + to_part + n, f32x4{ref, sum, ones[0], 0.f});
+    } else if (u.row0 + n < u.rows) {
         const int64_t to = (int64_t)u.tok0 * P.n_heads + u.row0 + n;
         const float inv = ones[0] == 0.f ? 0.f : 1.f / ones[0];
+        const int column0 = wave * kCols * 16 + 4 * g;
 #pragma unroll
         for (int j = 0; j < kCols; ++j) put(P.out + to * kC + column0 + j * 16, acc[j], inv);
         if (P.lse && wave == 0 && g == 0) P.lse[to] = lse_of(ref, sum);
-    } else {
-        const int64_t to = to_part + n;
-#pragma unroll
-        for (int j = 0; j < kCols; ++j)
-            st_global(reinterpret_cast<f32x4*>(P.plan.part + to * kC + column0 + j * 16), acc[j]);
-        if (wave == 0 && g == 0) st_global(P.plan.stat + to, f32x4{ref, sum, ones[0], 0.f});
     }
 }
 
@@ -988,17 +1042,17 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
         const int off = wave_bcast(L.off);
         barrier();                              // they are read
         // the unit at time `off` of the item
-        const Sizes z(P, w);
+        const Sizes z(P, w, place.tile);
         const int front = z.front(w);
         Unit u;
         u.common = off < front;
         const int rows = u.common ? z.rows0 : z.rows1, steps = u.common ? w.steps0 : w.steps1;
-        const int o = u.common ? off : off - front, whole64 = kCost64.setup + kCost64.page * steps;
+        const int o = u.common ? off : off - front, whole_unit = z.full().setup + z.full().page * steps;
         const int units = u.common ? z.units0 : z.units1;
-        const int k64 = o / whole64, k = k64 < units ? k64 : units - 1;
-        const Cost cost = Sizes::cost(rows, k);
-        const int from = o - k * whole64, all = cost.setup + cost.page * steps;
-        u.row0 = k * kTile;
+        const int k0 = o / whole_unit, k = k0 < units ? k0 : units - 1;
+        const Cost cost = z.cost(rows, k);
+        const int from = o - k * whole_unit, all = cost.setup + cost.page * steps;
+        u.row0 = k * z.tile;
         u.rows = rows;
         u.tok0 = w.tok0;
         u.first = w.first;
@@ -1014,7 +1068,7 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
             u.page0 = w.pages;
             u.table = P.c.table + (int64_t)w.seq * P.c.max_pages + w.pages;
             // up to the position of the unit's last token
-            const int last = u.row0 + kTile - 1 < u.rows ? u.row0 + kTile - 1 : u.rows - 1;
+            const int last = u.row0 + z.tile - 1 < u.rows ? u.row0 + z.tile - 1 : u.rows - 1;
             const int p = u.base + token_of_row(last, P.per_head);
             u.n = w.len < 0 || p < 0 ? 0 : pages_of((int64_t)p + 1) - w.pages;
             if (w.len < 0 && t == 0) raise(P.h, FLEET_MOE_ABORT_POSITION);
@@ -1031,7 +1085,7 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
             int o2 = off + take;
             Item next = w;
             if (end - at > take)
-                while (o2 >= Sizes(P, next).total(next) && next.seq + 1 < P.c.n_seqs) {
+                while (o2 >= Sizes(P, next, place.tile).total(next) && next.seq + 1 < P.c.n_seqs) {
                     next = item_of(P, next.seq + 1, stale);
                     if (leads(next)) next.last = start_of(P, next.end);
                     o2 = 0;
@@ -1044,11 +1098,12 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
             // where the part goes: a whole unit's to its rows, or to one of two slots
             const bool whole = lo == 0 && hi == steps;
             const int64_t row = (int64_t)u.tok0 * P.n_heads + u.row0;
-            const int64_t slots = 2 * all_rows;
+            const int64_t wholes = whole_parts(P.c.n_seqs, all_rows), slots = 2 * wholes;
+            const int64_t mine = whole_part(w.seq, (int64_t)u.tok0 * P.n_heads) + u.row0;
             const int64_t part =
-                whole ? (u.common ? row : w.pages > 0 ? all_rows + row : -1)
+                whole ? (u.common ? mine : w.pages > 0 ? wholes + mine : -1)
                       : slots + (int64_t)(2 * wg + (lo == 0 ? 1 : 0)) * kTile;
-            if (lo == 0 && t < kTile && u.row0 + t < u.rows) {
+            if (lo == 0 && t < z.tile && u.row0 + t < u.rows) {
                 const int last = at - from + cost.setup + (steps - 1) * cost.page;
                 Parts m;
                 m.at = (int)(part + t);
@@ -1058,7 +1113,7 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
                 P.plan.meta[(u.common ? 0 : all_rows) + row + t] = m;
             }
             const int n = hi < u.n ? hi : u.n;
-            if (u.rows - u.row0 <= 16) attend16(P, L, u, lo, n > lo ? n - lo : 0, part);
+            if (z.tile == 16 || u.rows - u.row0 <= 16) attend16(P, L, u, lo, n > lo ? n - lo : 0, part);
             else attend64(P, L, u, lo, n > lo ? n - lo : 0, part);
         }
         barrier();                              // LDS is free again
@@ -1067,72 +1122,103 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
     }
 }
 
-// Adds the parts of a row, those over common pages first: a wave a row, 16 parts at a time.
-constexpr int kJoinRows = 4, kJoinParts = 16;
-__global__ __launch_bounds__(64 * kJoinRows) void join_kernel(SharedParams P) {
-    const int lane = threadIdx.x & 63;
+// Adds the parts of 16 rows, those over common pages first: lane (g, n) has four columns of row
+// n. A wave 64 columns and all parts of their rows, or, where there are few rows of many parts, an
+// eighth of the parts, and the workgroup's eight waves their sum.
+constexpr int kJoinParts = 4;                   // on their way together
+constexpr int64_t kManyRows = 2048;
+template <bool kSplit>
+__global__ __launch_bounds__(kGridThreads) void join_kernel(SharedParams P) {
+    const int t = threadIdx.x, lane = t & 63, wave = wave_bcast(t >> 6);
+    const int g = lane >> 4, n = lane & 15;
     const int64_t all_rows = (int64_t)P.n_tokens * P.n_heads;
-    const int64_t row = (int64_t)blockIdx.x * kJoinRows + wave_bcast(threadIdx.x >> 6);
-    if (row >= all_rows) return;
-    const i32x4 own = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + all_rows + row));
-    const i32x4 front = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + row));
+    const int64_t block = kSplit ? blockIdx.x / kGridWaves : blockIdx.x;
+    const int column = kSplit ? blockIdx.x % kGridWaves : wave;         // of 64
+    const int64_t row = block * 16 + n;
+    i32x4 own{0, 0, 0, 0}, front{0, 0, 0, 0};
     // (rows that are nobody's have no parts of this call)
-    if (row < (int64_t)start_of(P, 0) * P.n_heads ||
-        row >= (int64_t)start_of(P, P.c.n_seqs) * P.n_heads || !ld_global(&P.plan.h->ok) ||
-        own.z == 0)
-        return;
-    const int n0 = own.w ? front.z : 0, count = n0 + own.z;
-    const auto slot = [&](int i) -> int64_t {
+    const int64_t lo = (int64_t)start_of(P, 0) * P.n_heads;
+    const int64_t hi = (int64_t)start_of(P, P.c.n_seqs) * P.n_heads;
+    if (row < all_rows && row >= lo && row < hi && ld_global(&P.plan.h->ok)) {
+        own = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + all_rows + row));
+        front = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + row));
+    }
+    const int n0 = own.z > 0 && own.w ? front.z : 0, count = n0 + own.z;
+    const auto part = [&](int i) -> int64_t {
         const bool mine = i >= n0;
         const int j = mine ? i - n0 : i;
         const int first = mine ? own.x : front.x, next = mine ? own.y : front.y;
         return j == 0 ? first : next + (int64_t)(j - 1) * kPartStep;
     };
-    f32x4 v[kJoinParts][2];
-    const auto load = [&](int i0) {
+    constexpr int kEach = kSplit ? kGridWaves : 1;
+    float top = -INFINITY, sum = 0.f, rounded = 0.f;
+    f32x4 o[4];
 #pragma unroll
-        for (int i = 0; i < kJoinParts; ++i) {
-            if (i0 + i >= count) break;
-            const f32x4* at =
-                reinterpret_cast<const f32x4*>(P.plan.part + slot(i0 + i) * kC) + lane;
-            v[i][0] = ld_global(at);
-            v[i][1] = ld_global(at + 64);
-        }
-    };
-    load(0);
-    float top = -INFINITY;
-    for (int i = lane; i < count; i += 64) top = fmaxf(top, ld_global(P.plan.stat + slot(i))[0]);
-    top = wave_max(top);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float f = 0.f, sum = 0.f, rounded = 0.f;
-    f32x4 o[2]{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    for (int i0 = 0;;) {
-        if (i0 % 64 == 0) {                     // the weights of 64 parts, a lane each
-            f32x4 st{-INFINITY, 0.f, 0.f, 0.f};
-            if (i0 + lane < count) st = ld_global(P.plan.stat + slot(i0 + lane));
-            f = exp2_(st[0] - ref);
-            sum += f * st[1];
-            rounded += f * st[2];
-        }
+    for (auto& e : o) e = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i0 = kSplit ? wave : 0; __ballot(i0 < count); i0 += kJoinParts * kEach) {
+        f32x4 st[kJoinParts], v[kJoinParts][4];
 #pragma unroll
-        for (int i = 0; i < kJoinParts; ++i) {
-            if (i0 + i >= count) break;
-            const float weight = __builtin_bit_cast(
-                float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i0 % 64 + i));
-            o[0] += v[i][0] * weight;
-            o[1] += v[i][1] * weight;
+        for (int k = 0; k < kJoinParts; ++k) {
+            const int i = i0 + k * kEach;
+            st[k] = f32x4{-INFINITY, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (auto& e : v[k]) e = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (i < count) {
+                const int64_t at = part(i);
+                st[k] = ld_global(P.plan.stat + at);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[k][j] = ld_global(part_at(P.plan, at / 16, column, j, g * 16 + (int)(at & 15)));
+            }
         }
-        i0 += kJoinParts;
-        if (i0 >= count) break;
-        load(i0);
+        float to = top;
+#pragma unroll
+        for (const f32x4& s : st) to = fmaxf(to, s[0]);
+        const float ref = to == -INFINITY ? 0.f : to, shrink = exp2_(top - ref);
+        top = to;
+        sum *= shrink;
+        rounded *= shrink;
+#pragma unroll
+        for (auto& e : o) e *= shrink;
+#pragma unroll
+        for (int k = 0; k < kJoinParts; ++k) {
+            const float f = exp2_(st[k][0] - ref);
+            sum += f * st[k][1];
+            rounded += f * st[k][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += v[k][j] * f;
+        }
     }
-    static_assert(64 % kJoinParts == 0, "");
-    sum = wave_sum(sum);
-    rounded = wave_sum(rounded);
-    const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
-    put(P.out + row * kC + 4 * lane, o[0], inv);
-    put(P.out + row * kC + 4 * lane + 256, o[1], inv);
-    if (P.lse && lane == 0) P.lse[row] = lse_of(top, sum);
+    const auto finish = [&](int j, const f32x4& e) {
+        if (count == 0) return;
+        put(P.out + row * kC + column * 64 + j * 16 + 4 * g, e, rounded == 0.f ? 0.f : 1.f / rounded);
+        if (P.lse && column == 0 && j == 0 && g == 0) P.lse[row] = lse_of(top, sum);
+    };
+    if constexpr (kSplit) {
+        __shared__ f32x4 all[kGridWaves][4][64], stats[kGridWaves][16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) all[wave][j][lane] = o[j];
+        if (g == 0) stats[wave][n] = f32x4{top, sum, rounded, 0.f};
+        __syncthreads();
+        if (wave >= 4) return;
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kGridWaves; ++i) top = fmaxf(top, stats[i][n][0]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        sum = rounded = 0.f;
+        f32x4 e{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kGridWaves; ++i) {
+            const float f = exp2_(stats[i][n][0] - ref);
+            sum += f * stats[i][n][1];
+            rounded += f * stats[i][n][2];
+            e += all[i][wave][lane] * f;
+        }
+        finish(wave, e);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) finish(j, o[j]);
+    }
 }
 
 }  // namespace cache
@@ -1204,5 +1290,7 @@ extern "C" int fleet_cache_attend_shared(const fleet_cache* cache, int32_t layer
     P.scale = scale * kLog2e;
     P.slack = fminf(kRise / P.scale, FLT_MAX);
     if (int e = launch<shared_kernel>(kGrid, kGridThreads, sizeof(PageLds), P, stream)) return e;
-    return launch<join_kernel>((rows + kJoinRows - 1) / kJoinRows, 64 * kJoinRows, 0, P, stream);
+    // (a call of many rows has few parts a row: a unit's share of the workgroups)
+    if (rows >= kManyRows) return launch<join_kernel<false>>((rows + 15) / 16, kGridThreads, 0, P, stream);
+    return launch<join_kernel<true>>((rows + 15) / 16 * kGridWaves, kGridThreads, 0, P, stream);
 }

@@ -20,10 +20,18 @@ def gpu():
         pytest.skip("no GPU")
 
 
-def forked(seed, prefixes, own, layers=1, fill=0xFF, extra=(), room=0):
+LONG = 9000
+FEW = 16                # sequences behind LONG positions: pages for more than 2,048 units of 16 rows
+both_heights = pytest.mark.parametrize("tall", [False, True])
+
+
+def forked(seed, prefixes, own, layers=1, fill=0xFF, extra=(), room=0, tall=0):
     """Groups of sequences: group g has len(own[g]) of them behind prefixes[g] common positions,
-    with own[g][i] positions of its own; then the sequences `extra` by themselves; `room` pages
+    with own[g][i] positions of its own; then, with `tall`, that many behind LONG positions, so
+    that units have 64 rows and not 16; then the sequences `extra` by themselves; `room` pages
     more for each."""
+    if tall:
+        prefixes, own = [*prefixes, LONG], [*own, [1] * tall]
     rng = np.random.default_rng(seed)
     n = sum(len(o) for o in own) + len(extra)
     top = max([p + max(o) for p, o in zip(prefixes, own)] + [*extra, 1])
@@ -72,11 +80,21 @@ CASES = [
 ]
 
 
+def compare_first(b, q, counts, out, lse, n, layer=0):
+    """The first n sequences' rows."""
+    r = sum(counts[:n])
+    compare(b, q[:r], counts[:n] + [0] * (len(counts) - n), out[:r], lse[:r], layer)
+
+
+@both_heights
 @pytest.mark.parametrize("case", range(len(CASES)))
-def test_against_every_sequence(case):
+def test_against_every_sequence(case, tall):
     prefixes, own, new, heads, extra = CASES[case]
-    say(f"case {CASES[case]}")
-    b, rng, groups = forked(case, prefixes, own, extra=extra)
+    say(f"case {CASES[case]} {tall}")
+    b, rng, groups = forked(case, prefixes, own, extra=extra,
+                            tall=-(-16 * 16 // (new * heads)) if tall else 0)
+    if tall:
+        prefixes = [*prefixes, LONG]
     n = len(b.ref.lens)
     counts = [min(new, x) for x in b.ref.lens]
     q = query(rng, sum(counts), heads)
@@ -85,7 +103,7 @@ def test_against_every_sequence(case):
     want = [min(w, pre // 64) for w, pre in zip(want, prefixes)]
     assert p.pages.tolist() == want
     out, lse = p.attend(to_dev(q), starts(counts))
-    compare(b, q, counts, out, lse)
+    compare_first(b, q, counts, out, lse, sum(map(len, own)) + 1 if tall else n)
     if new == 1 and all(c == 1 for c in counts):
         o2, l2 = p.attend(to_dev(q))
         assert torch.equal(o2, out) and torch.equal(l2, lse)
@@ -112,45 +130,51 @@ def test_many_sequences_and_few():
         compare(b, q, counts, out, lse)
 
 
-def test_tokens_inside_the_common_pages():
+@both_heights
+def test_tokens_inside_the_common_pages(tall):
     """Sequences that agree to the end: tokens stand in common pages and see them up to their own
     position; more tokens than positions see nothing."""
-    b, rng, groups = forked(52, [256], [[0, 0, 0]])
+    more = [1] * FEW * tall
+    b, rng, groups = forked(52, [256], [[0, 0, 0]], tall=len(more))
     p = plan(b, groups, 400)
-    assert p.pages.tolist() == [4]
+    assert p.pages.tolist() == [4, LONG // 64][: 1 + tall]
     for counts in ([1, 1, 1], [1, 200, 70], [256, 10, 0], [3, 260, 1]):
         say(f"counts {counts}")
+        counts = counts + more
         q = query(rng, sum(counts))
         out, lse = p.attend(to_dev(q), starts(counts))
-        compare(b, q, counts, out, lse)
+        compare_first(b, q, counts, out, lse, 3)
     assert b.dev.status() == 0
 
 
-def test_steps_of_beams():
+@both_heights
+def test_steps_of_beams(tall):
     """remap, update, grow, append, attend over several steps; a plan that a remap has made stale
     is right too, and so is one that was never updated."""
-    b, rng, groups = forked(53, [200, 70], [[3] * 4, [5] * 3], layers=2, room=4)
-    p = plan(b, groups, 7)
-    old = plan(b, groups, 7)
-    new = paged.SharedPrefix(b.dev, i32(groups), 7, 16)
+    b, rng, groups = forked(53, [200, 70], [[3] * 4, [5] * 3], layers=2, room=4, tall=FEW * tall)
+    n = 7 + FEW * tall
+    more = list(range(7, n))
+    p = plan(b, groups, n)
+    old = plan(b, groups, n)
+    new = paged.SharedPrefix(b.dev, i32(groups), n, 16)
     for step in range(6):
         parents = [*rng.integers(0, 4, 4), *(4 + rng.integers(0, 3, 3))]
         if step == 3:                           # the groups' sequences change places
             parents = [4, 5, 6, 0, 0, 1, 2]
-        b.remap([int(x) for x in parents])
-        b.remap(list(range(7)))
+        b.remap([int(x) for x in parents] + more)
+        b.remap(list(range(n)))
         p.update()
-        assert b.grow([1 + step * 9] * 7)
-        b.append([1 + step * 9] * 7, normal(rng, (2, 7 * (1 + step * 9), ref.ROW)))
-        q = query(rng, 7)
+        assert b.grow([1 + step * 9] * n)
+        b.append([1 + step * 9] * n, normal(rng, (2, n * (1 + step * 9), ref.ROW)))
+        q = query(rng, n)
         for layer in range(2):
             for x in (p, old, new):
                 out, lse = x.attend(to_dev(q), layer=layer)
-                compare(b, q, [1] * 7, out, lse, layer)
+                compare_first(b, q, [1] * n, out, lse, 7, layer)
     if step:
         b.compact()                             # moves pages, for all rows alike
         out, lse = p.attend(to_dev(q))
-        compare(b, q, [1] * 7, out, lse)
+        compare_first(b, q, [1] * n, out, lse, 7)
     assert b.dev.status() == 0
 
 
@@ -176,17 +200,19 @@ def test_groups_out_of_order_and_starts_that_decrease():
     compare(b, q[1:2], [0, 1, 0], out[1:2], lse[1:2])
 
 
-def test_bad_tables():
+@both_heights
+def test_bad_tables(tall):
     """A page outside the pool ends what is shared, and is not seen; a length outside the table
     sees nothing."""
-    b, rng, groups = forked(55, [400], [[3, 9, 5]])
-    q = query(rng, 3)
-    good, gl = plan(b, groups, 3).attend(to_dev(q))
+    b, rng, groups = forked(55, [400], [[3, 9, 5]], tall=FEW * tall)
+    n = 3 + FEW * tall
+    q = query(rng, n)
+    good, gl = plan(b, groups, n).attend(to_dev(q))
     table = b.dev.table.clone()
     for page in (b.ref.n_pages, -1, 2**31 - 1):
-        b.dev.table[:, 2] = page
-        p = plan(b, groups, 3)
-        assert p.pages.tolist() == [2]
+        b.dev.table[:3, 2] = page
+        p = plan(b, groups, n)
+        assert p.pages[0] == 2
         out, lse = p.attend(to_dev(q))
         assert b.dev.status() == _lib.ABORT_BAD_PAGE
         b.dev.clear_status()
@@ -198,53 +224,60 @@ def test_bad_tables():
             assert (np.abs(lse[s: s + 1].cpu().numpy() - wl) <= tl).all()
     b.dev.table.copy_(table)
     b.dev.table[1, 1] = b.dev.table[1, 0]       # one differs in the second page
-    p = plan(b, groups, 3)
-    assert p.pages.tolist() == [1]
+    p = plan(b, groups, n)
+    assert p.pages[0] == 1
     b.dev.table.copy_(table)
-    p = plan(b, groups, 3)
+    p = plan(b, groups, n)
     b.dev.lens[1] = 64 * b.dev.max_pages + 1
     out, lse = p.attend(to_dev(q))
     assert b.dev.status() == _lib.ABORT_POSITION
     assert (out[1] == 0).all() and torch.isneginf(lse[1]).all()
     # (the parts are other ones now, so are the sums' last bits)
-    compare(b, q[:1], [1], out[:1], lse[:1])
+    compare_first(b, q, [1] * n, out, lse, 1)
     b.dev.clear_status()
     b.dev.lens[1] = -1
     p.update()
-    assert p.pages.tolist() == [6]              # of those that hold anything
+    assert p.pages[0] == 6                      # of those that hold anything
 
 
 @pytest.mark.parametrize("fill", [0x7E, 0x7F, 0xFF, 0x78])
-def test_a_pool_that_holds_anything(fill):
-    b, rng, groups = forked(56, [130, 700], [[1, 40, 64], [9, 9]], fill=fill)
-    q = query(rng, 5)
-    out, lse = plan(b, groups, 5).attend(to_dev(q))
-    compare(b, q, [1] * 5, out, lse)
+@both_heights
+def test_a_pool_that_holds_anything(fill, tall):
+    b, rng, groups = forked(56, [130, 700], [[1, 40, 64], [9, 9]], fill=fill, tall=FEW * tall)
+    n = 5 + FEW * tall
+    q = query(rng, n)
+    out, lse = plan(b, groups, n).attend(to_dev(q))
+    compare_first(b, q, [1] * n, out, lse, 5)
 
 
-def test_what_is_not_finite_and_extreme_scores():
+@both_heights
+def test_what_is_not_finite_and_extreme_scores(tall):
     """A NaN in the common pages reaches all, one in a sequence's own that alone; scores far apart
     and equal ones."""
-    b, rng, groups = forked(57, [200], [[30, 40, 50]])
-    q = query(rng, 3)
-    p = plan(b, groups, 3)
+    b, rng, groups = forked(57, [200], [[30, 40, 50]], tall=FEW * tall)
+    n = 3 + FEW * tall
+    q = query(rng, n)
+    p = plan(b, groups, n)
     for mag in (60.0, 0.0):
         out, lse = p.attend(to_dev(ref.bf16(q * mag)))
-        compare(b, ref.bf16(q * mag), [1] * 3, out, lse)
+        compare_first(b, ref.bf16(q * mag), [1] * n, out, lse, 3)
     good, gl = p.attend(to_dev(q))
     last = int(b.dev.table[1, 3])
     b.dev.pool[last, 0, 9216 + 5 * 16] = 0x7F               # sequence 1, positions 208 on
     out, lse = p.attend(to_dev(q))
-    assert torch.equal(out[[0, 2]], good[[0, 2]]) and torch.equal(lse[[0, 2]], gl[[0, 2]])
+    assert torch.equal(out[0], good[0]) and torch.equal(lse[0], gl[0])
+    assert torch.equal(out[2:], good[2:]) and torch.equal(lse[2:], gl[2:])
     assert np.isnan(ref.values(out[1].cpu().numpy())).all()
-    bad = query(rng, 3)
+    bad = query(rng, n)
     bad[2, 5, 100] = np.nan
     out, _ = p.attend(to_dev(bad))
     nan = np.isnan(ref.values(out.cpu().numpy()))
     assert nan[1].all() and nan[2, 5].all() and not nan[0].any() and not np.delete(nan[2], 5, 0).any()
+    assert not nan[3:].any()
     b.dev.pool[int(b.dev.table[0, 1]), 0, 3] = 0xFF          # common
     out, _ = p.attend(to_dev(q))
-    assert np.isnan(ref.values(out.cpu().numpy())).all()
+    nan = np.isnan(ref.values(out.cpu().numpy()))
+    assert nan[:3].all() and not nan[3:].any()
 
 
 def test_strides_and_given_outputs():
