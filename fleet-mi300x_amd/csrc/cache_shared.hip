@@ -36,9 +36,9 @@ struct PlanHeader {
 };
 static_assert(sizeof(PlanHeader) == 256, "");
 struct Group {
-    int32_t first, end;         // sequences
-    int32_t pages;              // common to those that hold anything
-    int32_t lead;               // one of these
+    int32_t first, end;         // sequences, from the first that holds anything
+    int32_t pages;              // common to those that do
+    int32_t pad;
 };
 struct Parts {                  // of a row and kind: part 0, part 1, part 1 + kPartStep, ..
     int32_t at, next, count;
@@ -95,7 +95,8 @@ __device__ __forceinline__ f32x4* part_at(const Plan& p, int64_t tile, int wave,
 
 // A workgroup a group: the leading pages that all its sequences with positions name, as far as
 // all of them have filled them. (An append writes no such page, so the number stays right
-// until sequences move.)
+// until sequences move.) One without positions is by itself, whatever pages it gets later; where
+// its tokens are between the group's, their rows are computed and not used.
 constexpr int kShareThreads = 1024;
 __global__ __launch_bounds__(kShareThreads) void share_kernel(fleet_cache c, const int32_t* groups,
                                                               int n_groups, int32_t* pages_out,
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(kShareThreads) void share_kernel(fleet_cache c, con
         if (t == 0 && none) raise(h, FLEET_MOE_ABORT_POSITION);
         const int lo = none ? 0 : groups[0], hi = none ? 0 : groups[n_groups];
         for (int s = t; s < c.n_seqs; s += kShareThreads)
-            if (s < lo || s >= hi) plan.groups[s] = Group{s, s + 1, 0, s};
+            if (s < lo || s >= hi) plan.groups[s] = Group{s, s + 1, 0, 0};
     }
     if (t == 0) {
         pages = 0x7fffffff;
@@ -180,7 +181,8 @@ __global__ __launch_bounds__(kShareThreads) void share_kernel(fleet_cache c, con
         }
     }
     for (int s = first + t; s < end; s += kShareThreads)
-        plan.groups[s] = Group{first, end, most, from};
+        plan.groups[s] = checked_len(c.lens[s], c.max_pages) > 0 ? Group{from, end, most, 0}
+                                                                 : Group{s, s + 1, 0, 0};
     if (pages_out && t == 0) pages_out[blockIdx.x] = most;
 }
 
@@ -209,7 +211,7 @@ __device__ __forceinline__ int start_of(const SharedParams& P, int s) {
 // group's first, and its own rows over what is behind them.
 struct Item {
     int seq, tok0, n_new, len;
-    int pages, lead;                    // its group's, and
+    int pages;                          // its group's, and
     int first, end, last;               // the sequences, and the token behind them
     int steps0, steps1;                 // of a unit, whether they see anything or not
 };
@@ -224,7 +226,6 @@ __device__ __forceinline__ Item item_of(const SharedParams& P, int seq, bool sta
     w.first = stale ? seq : g.x;
     w.end = stale ? seq + 1 : g.y;
     w.pages = stale ? 0 : g.z;
-    w.lead = stale ? seq : g.w;
     w.last = w.tok0;
     w.steps0 = w.pages;
     const int own = w.len < 0 ? 0 : pages_of(w.len) - w.pages;
@@ -233,7 +234,7 @@ __device__ __forceinline__ Item item_of(const SharedParams& P, int seq, bool sta
 }
 __device__ __forceinline__ bool leads(const Item& w) { return w.pages > 0 && w.seq == w.first; }
 __device__ __forceinline__ Item lane_of(const Item& v, int lane) {
-    static_assert(sizeof(Item) == 44, "");
+    static_assert(sizeof(Item) == 40, "");
     struct Words {
         int w[sizeof(Item) / 4];
     } x = __builtin_bit_cast(Words, v);
@@ -1062,7 +1063,7 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
             u.base = 0;
             u.page0 = 0;
             u.n = w.steps0;
-            u.table = P.c.table + (int64_t)w.lead * P.c.max_pages;
+            u.table = P.c.table + (int64_t)w.first * P.c.max_pages;
         } else {
             u.base = w.len - w.n_new;
             u.page0 = w.pages;
@@ -1124,8 +1125,10 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
 
 // Adds the parts of 16 rows, those over common pages first: lane (g, n) has four columns of row
 // n. A wave 64 columns and all parts of their rows, or, where there are few rows of many parts, an
-// eighth of the parts, and the workgroup's eight waves their sum.
-constexpr int kJoinParts = 4;                   // on their way together
+// eighth of the parts, and the workgroup's eight waves their sum (shared and joined, 64 sequences
+// of 16 heads 47.0 us and 48.2 in one wave each; 256 sequences 182 us and 180).
+constexpr int kJoinParts = 2;                   // on their way together (four: more registers,
+                                                // 8,192 rows 109.1 us where this takes 108.3)
 constexpr int64_t kManyRows = 2048;
 template <bool kSplit>
 __global__ __launch_bounds__(kGridThreads) void join_kernel(SharedParams P) {

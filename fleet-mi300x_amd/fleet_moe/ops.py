@@ -344,8 +344,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None,
             rc = _lib.load().fleet_residual_norm(
                 x.data_ptr(), x.dtype == _F32, x_stride, _ptr(y),
                 y is not None and y.dtype == _F32, y_stride, _ptr(post_norm), _ptr(gate),
-                gate_stride, scale, _ptr(norm), eps, _ptr(x_out), h.data_ptr(), _ptr(h_f32),
-                rows, width, _stream(stream))
+                gate_stride, float(scale), _ptr(norm), float(eps), _ptr(x_out), h.data_ptr(),
+                _ptr(h_f32), _int32(rows), _int32(width), _stream(stream))
             if rc:
                 _lib.check(rc, "fleet_residual_norm")
     return (x if x_out is None else x_out), h
@@ -387,7 +387,7 @@ class Rotary:
         x0, x1, _ = x.stride()
         o0, o1, _ = out.stride()
         return (out, (x.data_ptr(), dtype == _F32, x0, x1, out.data_ptr(), o0, o1),
-                (shape[0], shape[1], shape[2], _int32(at)))
+                (_int32(shape[0]), _int32(shape[1]), _int32(shape[2]), _int32(at)))
 
     def rotate(self, x: torch.Tensor, positions: torch.Tensor, out: torch.Tensor | None = None,
                at: int = 0, stream=None) -> torch.Tensor:

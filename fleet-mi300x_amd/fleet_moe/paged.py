@@ -241,8 +241,8 @@ class SharedPrefix:
     attend(), after remap(), and after changes of table or lens by other means; grow() and
     append() need none, so once a step serves all layers. (After a remap() without it
     attend() is right, but takes every sequence by itself.) Holds the plan of up to max_tokens
-    tokens of n_heads heads, 67 MB and 4,144 bytes a token and head. Calls are ordered on
-    one stream, as the cache's."""
+    tokens of n_heads heads: 68 MB, 66 KB a sequence and 4,160 bytes a token and head. Calls are
+    ordered on one stream, as the cache's."""
 
     def __init__(self, cache: PagedCache, groups: torch.Tensor, max_tokens: int, n_heads: int):
         if groups.dim() != 1 or groups.numel() < 2:

@@ -555,8 +555,8 @@ int fleet_cache_append_latent(const fleet_cache* cache, int32_t layer, const uin
                               void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* Bytes of a plan for attentions of up to max_tokens tokens of n_heads heads
- * (67 MB and 4,144 bytes a token and head; max_tokens * n_heads <= 2^20). 0: outside the
- * limits. It needs no clearing, and serves the calls on one cache that are ordered
+ * (68 MB, 66 KB a sequence and 4,160 bytes a token and head; max_tokens * n_heads <= 2^20). 0:
+ * outside the limits. It needs no clearing, and serves the calls on one cache that are ordered
  * on one stream. */
 size_t fleet_cache_plan_bytes(int32_t n_seqs, int32_t max_tokens, int32_t n_heads);
 
@@ -575,7 +575,8 @@ int fleet_cache_share(const fleet_cache* cache, const int32_t* groups, int32_t n
 
 /* fleet_cache_attend without a window, the pages that a group shares read once for all
  * its rows: what it takes, sees and leaves is as there. (The probabilities are
- * rounded to bf16's 8 bits before the second product, whatever the number of rows.) plan: as
+ * rounded to bf16's 8 bits before the second product, or to 16 bits where the call has few
+ * pages: what that is follows from starts, lengths and groups.) plan: as
  * fleet_cache_share left it, for at least as many tokens and heads. n_tokens *
  * n_heads <= 2^20, (n_tokens * n_heads / 32 + 2 * n_seqs) * (11 * max_pages + 60) < 2^31. */
 int fleet_cache_attend_shared(const fleet_cache* cache, int32_t layer, const uint16_t* q,

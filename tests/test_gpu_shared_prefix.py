@@ -148,6 +148,25 @@ def test_tokens_inside_the_common_pages(tall):
 
 
 @both_heights
+@pytest.mark.parametrize("empty", [[0], [1], [3], [0, 1], [1, 2], [0, 1, 2, 3]])
+def test_sequences_that_begin_after_the_update(empty, tall):
+    """Sequences of a group that hold nothing at update() grow later, into pages of their own."""
+    b, rng, groups = forked(61, [200], [[3, 9, 5, 70]], room=2, tall=FEW * tall)
+    n = 4 + FEW * tall
+    b.remap([-1 if s in empty else s for s in range(n)])
+    p = plan(b, groups, 3 * n)
+    assert p.pages[0] == (3 if len(empty) < 4 else 0)
+    for new in (1, 2):
+        counts = [new if s in empty else 1 for s in range(n)]
+        assert b.grow(counts)
+        b.append(counts, normal(rng, (1, sum(counts), ref.ROW)))
+        q = query(rng, sum(counts))
+        out, lse = p.attend(to_dev(q), starts(counts))
+        compare_first(b, q, counts, out, lse, 4)
+    assert b.dev.status() == 0
+
+
+@both_heights
 def test_steps_of_beams(tall):
     """remap, update, grow, append, attend over several steps; a plan that a remap has made stale
     is right too, and so is one that was never updated."""
