@@ -64,6 +64,15 @@ __device__ __forceinline__ void st_global_at(void* p, const T& v) {
     ((__attribute__((address_space(1))) AlignedTo<kAlign, T>*)p)->v = v;
 }
 
+// A grid of n workgroups, in rows of 2^20: a launch takes fewer than 2^32 threads in a row.
+constexpr int64_t kGridRow = 1 << 20;
+inline dim3 wide_grid(int64_t n) {
+    return n <= kGridRow ? dim3((unsigned)n) : dim3(kGridRow, (unsigned)((n + kGridRow - 1) / kGridRow));
+}
+__device__ __forceinline__ int64_t wide_block() {
+    return (int64_t)blockIdx.y * kGridRow + blockIdx.x;
+}
+
 // DeepSeek-V2-Lite MoE shape (reference/dsv2lite_config.json).
 constexpr int kHidden = 2048;
 constexpr int kInter = 1408;          // routed expert intermediate

@@ -117,7 +117,7 @@ void rope_kernel(Params P) {
             starts[i] = cache::clamp_row(ld_global(P.start + i), P.n_tokens);
         __syncthreads();
     }
-    const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t id = wide_block() * kThreads + threadIdx.x;
     const int64_t slot = id / P.items;
     const int item = (int)(id - slot * P.items);
     const int64_t tok = slot / P.parts;
@@ -208,9 +208,9 @@ static int launch_rope(Params& P, hipStream_t stream) {
     P.parts = many ? (P.n_heads + 3) / 4 : P.n_heads;
     const int64_t n = (int64_t)P.n_tokens * P.parts * P.items;
     const int64_t grid = (n + kThreads - 1) / kThreads;
-    if (grid > 0x7fffffff) return FLEET_MOE_ERR_ARG;
+    if (grid > 65535 * kGridRow) return FLEET_MOE_ERR_ARG;
     const auto launch = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, stream, P);
+        hipLaunchKernelGGL(kernel, wide_grid(grid), dim3(kThreads), 0, stream, P);
         return (int)hipGetLastError();
     };
     if ((P.r.dim / 2 | P.at | P.width) % 4 == 0)

@@ -138,8 +138,7 @@ def test_values_far_out(dtype):
 
 
 def test_a_row_is_the_same_in_any_batch():
-    """Results do not depend on the rows beside a row (they do on the number of rows: from 1,025 on
-    a wave takes a row)."""
+    """Results depend neither on the rows beside a row nor on their number."""
     rng = np.random.default_rng(5)
     x, y = dev(rng.normal(size=(700, 2048)), BITS), dev(rng.normal(size=(700, 2048)), BITS)
     a, h = ops.residual_norm(x, y)
