@@ -63,6 +63,17 @@ template <int kAlign, class T>
 __device__ __forceinline__ void st_global_at(void* p, const T& v) {
     ((__attribute__((address_space(1))) AlignedTo<kAlign, T>*)p)->v = v;
 }
+// The same of memory that nobody is to find in L2 again.
+template <int kAlign, class T>
+__device__ __forceinline__ T ld_stream_at(const void* p) {
+    typedef T V __attribute__((aligned(kAlign)));
+    return __builtin_nontemporal_load((gmem_ptr<V>)p);
+}
+template <int kAlign, class T>
+__device__ __forceinline__ void st_stream_at(void* p, const T& v) {
+    typedef T V __attribute__((aligned(kAlign)));
+    __builtin_nontemporal_store(v, (__attribute__((address_space(1))) V*)p);
+}
 
 // A grid of n workgroups, in rows of 2^20: a launch takes fewer than 2^32 threads in a row.
 constexpr int64_t kGridRow = 1 << 20;

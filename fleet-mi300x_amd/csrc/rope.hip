@@ -5,8 +5,8 @@
 // of its position and frequency; the bytes of x and out bound many tokens, a launch's
 // latency few. An angle costs some sixty instructions and serves all heads of its token, so
 // a thread takes the same four pairs of several heads where there are enough tokens. Measured: one
-// token of 16 heads 3.1 us, 2,000 5.0; 8,001 whole heads of 192 fp32 values (197 MB) 44 us, 4.5
-// TB/s, a large copy's 5.1.
+// token of 16 heads 2.6 us, 2,000 5.4; 8,001 whole heads of 192 fp32 values (197 MB) 39 us, a
+// large copy's 5.1 TB/s.
 #include <math.h>
 
 #include "cache_pages.h"
@@ -35,18 +35,21 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 // Up to four neighbouring values, anywhere a value may lie: four are one load or store.
+template <bool kStream>
 __device__ __forceinline__ f32x4 load4(const float* p, int n) {
-    if (n >= 4) return ld_global_at<4, f32x4>(p);
+    if (n >= 4) return kStream ? ld_stream_at<4, f32x4>(p) : ld_global_at<4, f32x4>(p);
     f32x4 v{0.f, 0.f, 0.f, 0.f};
     if (n > 0) v[0] = ld_global(p);
     if (n > 1) v[1] = ld_global(p + 1);
     if (n > 2) v[2] = ld_global(p + 2);
     return v;
 }
+template <bool kStream>
 __device__ __forceinline__ f32x4 load4(const uint16_t* p, int n) {
     const auto one = [&](int i) { return __uint_as_float((uint32_t)ld_global(p + i) << 16); };
     if (n >= 4) {
-        const uint64_t w = ld_global_at<2, uint64_t>(p);
+        const uint64_t w =
+            kStream ? ld_stream_at<2, uint64_t>(p) : ld_global_at<2, uint64_t>(p);
         const uint32_t lo = (uint32_t)w, hi = (uint32_t)(w >> 32);
         return f32x4{bf_lo(lo), bf_hi(lo), bf_lo(hi), bf_hi(hi)};
     }
@@ -56,22 +59,26 @@ __device__ __forceinline__ f32x4 load4(const uint16_t* p, int n) {
     if (n > 2) v[2] = one(2);
     return v;
 }
+template <bool kStream>
 __device__ __forceinline__ void store4(float* p, const f32x4& v, int n) {
     if (n >= 4) {
-        st_global_at<4>(p, v);
+        if (kStream) st_stream_at<4>(p, v);
+        else st_global_at<4>(p, v);
         return;
     }
     if (n > 0) st_global(p, v[0]);
     if (n > 1) st_global(p + 1, v[1]);
     if (n > 2) st_global(p + 2, v[2]);
 }
+template <bool kStream>
 __device__ __forceinline__ void store4(uint16_t* p, const f32x4& v, int n) {
     bf16x4 b;
 #pragma unroll
     for (int i = 0; i < 4; ++i) b[i] = (__bf16)v[i];
     const uint64_t w = __builtin_bit_cast(uint64_t, b);
     if (n >= 4) {
-        st_global_at<2>(p, w);
+        if (kStream) st_stream_at<2>(p, w);
+        else st_global_at<2>(p, w);
         return;
     }
     if (n > 0) st_global(p, (uint16_t)w);
@@ -108,7 +115,7 @@ constexpr int kThreads = 256;
 // Thread (slot, item); a slot is a token and kHeads of its heads, an item up to four pairs or
 // four of the other values, always four with kFours.
 // (Seven waves a SIMD: with the 90 registers the compiler takes otherwise, five, 49 us.)
-template <class T, int kHeads, bool kFours>
+template <class T, int kHeads, bool kFours, bool kStream>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(7)))
 void rope_kernel(Params P) {
     __shared__ int starts[cache::kMaxSeqs + 1];
@@ -145,8 +152,8 @@ void rope_kernel(Params P) {
 #pragma unroll
         for (int j = 0; j < kHeads; ++j)
             if (head0 + j < P.n_heads) {
-                a[j] = load4(x + (head0 + j) * P.x_head + xa, xn);
-                b[j] = load4(x + (head0 + j) * P.x_head + xb, xm);
+                a[j] = load4<kStream>(x + (head0 + j) * P.x_head + xa, xn);
+                b[j] = load4<kStream>(x + (head0 + j) * P.x_head + xb, xm);
             }
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) {
@@ -161,8 +168,8 @@ void rope_kernel(Params P) {
                     g[i] = fmaf(v[i], cs[i].x, u[i] * cs[i].y);
                 }
                 T* to = out + (head0 + j) * P.o_head;
-                store4(to + oa, hout ? f : f32x4{f[0], g[0], f[1], g[1]}, on);
-                store4(to + ob, hout ? g : f32x4{f[2], g[2], f[3], g[3]}, om);
+                store4<kStream>(to + oa, hout ? f : f32x4{f[0], g[0], f[1], g[1]}, on);
+                store4<kStream>(to + ob, hout ? g : f32x4{f[2], g[2], f[3], g[3]}, om);
             }
         }
     } else {
@@ -174,10 +181,10 @@ void rope_kernel(Params P) {
         f32x4 a[kHeads];
 #pragma unroll
         for (int j = 0; j < kHeads; ++j)
-            if (head0 + j < P.n_heads) a[j] = load4(x + (head0 + j) * P.x_head + at, n);
+            if (head0 + j < P.n_heads) a[j] = load4<kStream>(x + (head0 + j) * P.x_head + at, n);
 #pragma unroll
         for (int j = 0; j < kHeads; ++j)
-            if (head0 + j < P.n_heads) store4(out + (head0 + j) * P.o_head + at, a[j], n);
+            if (head0 + j < P.n_heads) store4<kStream>(out + (head0 + j) * P.o_head + at, a[j], n);
     }
 }
 
@@ -197,6 +204,10 @@ int fleet_moe_check_rope(const fleet_rope* r) {
     return 0;
 }
 
+// Results of that many bytes go by L2, and so do the values: what reads them next finds little of
+// them there (with a copy of the result behind it, 98 MB 72.7 us, through L2 79.6; 49 MB 41.0
+// and 39.4, the rotation alone 21.5 and 24.3).
+constexpr int64_t kStreamed = 64 << 20;
 template <class T>
 static int launch_rope(Params& P, hipStream_t stream) {
     P.pairs = (P.r.dim / 2 + 3) / 4;
@@ -213,9 +224,14 @@ static int launch_rope(Params& P, hipStream_t stream) {
         hipLaunchKernelGGL(kernel, wide_grid(grid), dim3(kThreads), 0, stream, P);
         return (int)hipGetLastError();
     };
-    if ((P.r.dim / 2 | P.at | P.width) % 4 == 0)
-        return many ? launch(rope_kernel<T, 4, true>) : launch(rope_kernel<T, 1, true>);
-    return many ? launch(rope_kernel<T, 4, false>) : launch(rope_kernel<T, 1, false>);
+    const int64_t values = (int64_t)P.n_tokens * P.n_heads * P.width;
+    const bool large = many && values >= kStreamed / (int64_t)sizeof(T);
+    if ((P.r.dim / 2 | P.at | P.width) % 4 == 0) {
+        if (large) return launch(rope_kernel<T, 4, true, true>);
+        return many ? launch(rope_kernel<T, 4, true, false>) : launch(rope_kernel<T, 1, true, false>);
+    }
+    if (large) return launch(rope_kernel<T, 4, false, true>);
+    return many ? launch(rope_kernel<T, 4, false, false>) : launch(rope_kernel<T, 1, false, false>);
 }
 
 static int rotate(Params& P, bool f32, hipStream_t stream) {

@@ -143,6 +143,21 @@ def test_parts_of_wider_rows():
     check(r.rotate(one, i32(pos)), want, both, False)
 
 
+@pytest.mark.parametrize("dtype, tokens, width, at", [(F32, 5500, 192, 128), (BITS, 11_000, 193, 3)])
+def test_more_than_the_caches_hold(dtype, tokens, width, at):
+    """Results of 64 MB and more, of 16 heads, and in place."""
+    rng = np.random.default_rng(9)
+    f = rope.frequencies().astype(np.float64)
+    x = dev(rng.normal(size=(tokens, 16, width)).astype(np.float32), dtype)
+    pos = rng.integers(0, 1 << 20, tokens)
+    want, both = turned(host(x), pos, f, at, False, False)
+    r = ops.Rotary(f, halves_out=False)
+    got = r.rotate(x, i32(pos), at=at)
+    check(got, want, both, dtype == F32)
+    assert torch.equal(got[..., :at], x[..., :at]) and torch.equal(got[..., at + 64:], x[..., at + 64:])
+    assert r.rotate(x, i32(pos), out=x, at=at) is x and torch.equal(x, got)
+
+
 @pytest.mark.parametrize("tokens", [3, 900])
 def test_positions_of_the_cache(tokens):
     rng = np.random.default_rng(tokens)
