@@ -215,17 +215,30 @@ struct Item {
     int first, end, last;               // the sequences, and the token behind them
     int steps0, steps1;                 // of a unit, whether they see anything or not
 };
+// What is loaded for a sequence, all on its way together.
+struct RawItem {
+    i32x4 group;
+    int at, behind, len;
+};
+__device__ __forceinline__ RawItem raw_of(const SharedParams& P, int seq) {
+    RawItem r;
+    const int32_t* starts = P.start ? P.start : P.c.lens;     // (any, where tokens are sequences)
+    r.group = ld_global(reinterpret_cast<const i32x4*>(P.plan.groups + seq));
+    r.at = ld_global(starts + seq);
+    r.behind = ld_global(starts + seq + (P.start ? 1 : 0));
+    r.len = ld_global(P.c.lens + seq);
+    return r;
+}
 // All but `last`, which needs the group's end.
-__device__ __forceinline__ Item item_of(const SharedParams& P, int seq, bool stale) {
+__device__ __forceinline__ Item item_of(const SharedParams& P, int seq, const RawItem& r, bool stale) {
     Item w;
-    const i32x4 g = ld_global(reinterpret_cast<const i32x4*>(P.plan.groups + seq));
     w.seq = seq;
-    w.tok0 = start_of(P, seq);
-    w.n_new = start_of(P, seq + 1) - w.tok0;              // (negative: not in order)
-    w.len = checked_len(ld_global(P.c.lens + seq), P.c.max_pages);
-    w.first = stale ? seq : g.x;
-    w.end = stale ? seq + 1 : g.y;
-    w.pages = stale ? 0 : g.z;
+    w.tok0 = P.start ? clamp_row(r.at, P.n_tokens) : seq;
+    w.n_new = (P.start ? clamp_row(r.behind, P.n_tokens) : seq + 1) - w.tok0;  // (< 0: out of order)
+    w.len = checked_len(r.len, P.c.max_pages);
+    w.first = stale ? seq : r.group.x;
+    w.end = stale ? seq + 1 : r.group.y;
+    w.pages = stale ? 0 : r.group.z;
     w.last = w.tok0;
     w.steps0 = w.pages;
     const int own = w.len < 0 ? 0 : pages_of(w.len) - w.pages;
@@ -396,10 +409,10 @@ static_assert(kTile * (2 * kRow + 16) <= 2 * 4 * kBlockStep + 16 * 1024, "");
 struct Place {
     int total, shares;
     int tile;                   // rows of a unit
+    bool stale;                 // sequences have moved since share: every one by itself
     bool inside;                // some token stands within its group's common pages
 };
-__device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg, bool stale,
-                                       Place& at) {
+__device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg, Place& at) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int each = P.c.n_seqs > kGridThreads ? 2 : 1;
     static_assert(kMaxSeqs <= 2 * kGridThreads, "");
@@ -407,16 +420,21 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
     bool bad = false, inside = false;
     Item w{}, w1{};
     int* starts = reinterpret_cast<int*>(L.tile);         // [n_seqs + 1]
-    if (t * each < P.c.n_seqs) {
-        w = item_of(P, t * each, stale);
-        starts[t * each + 1] = w.tok0 + w.n_new;
-        if (each > 1 && t * each + 1 < P.c.n_seqs) {
-            w1 = item_of(P, t * each + 1, stale);
-            starts[t * each + 2] = w1.tok0 + w1.n_new;
+    const int seq = t * each, top = P.c.n_seqs - 1;
+    RawItem r = raw_of(P, seq < top ? seq : top), r1{};
+    if (each > 1) r1 = raw_of(P, seq + 1 < top ? seq + 1 : top);
+    asm volatile("" ::: "memory");              // (the loads above first)
+    at.stale = ld_global(&P.plan.h->remaps) != ld_global(&P.h->remaps);
+    if (seq <= top) {
+        w = item_of(P, seq, r, at.stale);
+        starts[seq + 1] = w.tok0 + w.n_new;
+        if (each > 1 && seq < top) {
+            w1 = item_of(P, seq + 1, r1, at.stale);
+            starts[seq + 2] = w1.tok0 + w1.n_new;
         }
     }
     barrier();
-    if (t * each < P.c.n_seqs) {
+    if (seq <= top) {
         if (leads(w)) w.last = starts[w.end];
         if (leads(w1)) w1.last = starts[w1.end];
         first = Sizes(P, w, kTile).total(w);
@@ -475,10 +493,12 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
     at.shares = shares_of(at.total);
     if (wg >= at.shares) return false;
     const int off = Split(at.total, at.shares).first(wg) - (before + incl - n);
-    if (off >= 0 && off < n) {
-        const bool second = off >= first;
-        L.item = second ? w1 : w;
-        L.off = second ? off - first : off;
+    if (off >= 0 && off < first) {
+        L.item = w;
+        L.off = off;
+    } else if (off >= first && off < n) {
+        L.item = w1;
+        L.off = off - first;
     }
     barrier();
     return true;
@@ -1031,10 +1051,8 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     PageLds& L = *reinterpret_cast<PageLds*>(lds);
     const int t = threadIdx.x, wg = blockIdx.x;
-    // sequences have moved since share: every one by itself
-    const bool stale = ld_global(&P.plan.h->remaps) != ld_global(&P.h->remaps);
     Place place;
-    if (!locate(P, L, wg, stale, place)) return;
+    if (!locate(P, L, wg, place)) return;
     const Split share(place.total, place.shares);
     const int64_t all_rows = (int64_t)P.n_tokens * P.n_heads;
     const int end = share.first(wg + 1);
@@ -1087,7 +1105,7 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
             Item next = w;
             if (end - at > take)
                 while (o2 >= Sizes(P, next, place.tile).total(next) && next.seq + 1 < P.c.n_seqs) {
-                    next = item_of(P, next.seq + 1, stale);
+                    next = item_of(P, next.seq + 1, raw_of(P, next.seq + 1), place.stale);
                     if (leads(next)) next.last = start_of(P, next.end);
                     o2 = 0;
                 }
