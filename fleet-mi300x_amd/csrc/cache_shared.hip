@@ -31,8 +31,9 @@ constexpr float kRise = 12.f;           // (8: 186 us where this takes 184)
 // The plan: what share found, and the parts of an attention.
 struct PlanHeader {
     uint32_t remaps;            // the cache's when share was called
-    uint32_t ok;                // the attention's starts were in order
-    int32_t pad[62];
+    int32_t pad;
+    int32_t first, end;         // the attention's rows: none if its starts are not in order
+    int32_t pads[60];
 };
 static_assert(sizeof(PlanHeader) == 256, "");
 struct Group {
@@ -486,7 +487,8 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
     any = wave_bcast(any);
     at.inside = any & 2;
     if (wg == 0 && t == 0) {
-        P.plan.h->ok = !(any & 1);
+        P.plan.h->first = any & 1 ? 0 : w.tok0 * P.n_heads;
+        P.plan.h->end = any & 1 ? 0 : starts[P.c.n_seqs] * P.n_heads;
         if (any & 1) raise(P.h, FLEET_MOE_ABORT_POSITION);
     }
     if (any & 1) return false;
@@ -1156,14 +1158,12 @@ __global__ __launch_bounds__(kGridThreads) void join_kernel(SharedParams P) {
     const int64_t block = kSplit ? blockIdx.x / kGridWaves : blockIdx.x;
     const int column = kSplit ? blockIdx.x % kGridWaves : wave;         // of 64
     const int64_t row = block * 16 + n;
-    i32x4 own{0, 0, 0, 0}, front{0, 0, 0, 0};
-    // (rows that are nobody's have no parts of this call)
-    const int64_t lo = (int64_t)start_of(P, 0) * P.n_heads;
-    const int64_t hi = (int64_t)start_of(P, P.c.n_seqs) * P.n_heads;
-    if (row < all_rows && row >= lo && row < hi && ld_global(&P.plan.h->ok)) {
-        own = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + all_rows + row));
-        front = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + row));
-    }
+    // all on its way together; rows that are nobody's have no parts of this call
+    const int64_t safe = row < all_rows ? row : 0;
+    i32x4 own = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + all_rows + safe));
+    const i32x4 front = ld_global(reinterpret_cast<const i32x4*>(P.plan.meta + safe));
+    const i32x2 rows = ld_global(reinterpret_cast<const i32x2*>(&P.plan.h->first));
+    if (row < rows.x || row >= rows.y) own.z = 0;
     const int n0 = own.z > 0 && own.w ? front.z : 0, count = n0 + own.z;
     const auto part = [&](int i) -> int64_t {
         const bool mine = i >= n0;
