@@ -578,7 +578,7 @@ int fleet_cache_share(const fleet_cache* cache, const int32_t* groups, int32_t n
  * rounded to bf16's 8 bits before the second product, or to 16 bits where the call has few
  * pages: what that is follows from starts, lengths and groups.) plan: as
  * fleet_cache_share left it, for at least as many tokens and heads. n_tokens *
- * n_heads <= 2^20, (n_tokens * n_heads / 32 + 2 * n_seqs) * (11 * max_pages + 60) < 2^31. */
+ * n_heads <= 2^20, (n_tokens * n_heads / 32 + 2 * n_seqs) * (11 * max_pages + 40) < 2^31. */
 int fleet_cache_attend_shared(const fleet_cache* cache, int32_t layer, const uint16_t* q,
                               int64_t q_stride, const int32_t* start, int32_t n_tokens,
                               int32_t n_heads, float scale, uint16_t* out, float* lse, void* plan,
