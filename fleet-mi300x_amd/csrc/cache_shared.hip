@@ -397,7 +397,7 @@ struct PageLds {
     f32x4 half[2][kGridWaves][2][64];   // [step parity] half of the scores of a tile and two
                                         // blocks
     uint32_t scale[kPageRing][8];
-    int flag[2][kGridWaves], units[2][kGridWaves];
+    int flag[2][kGridWaves], units[2][kGridWaves], front[2];
     __attribute__((aligned(8))) uint8_t flags[2][kGridWaves];   // (64 rows) 1: a row's reference
                                 // rises, 2: a score is not finite
     float m[4][16], top[4][2][16], sum[4][2][16], rounded[4][2][16];
@@ -412,6 +412,7 @@ static_assert(kTile * (2 * kRow + 16) <= 2 * 4 * kBlockStep + 16 * 1024, "");
 struct Place {
     int total, shares;
     int tile;                   // rows of a unit
+    int wg;                     // the share of the workgroup
     bool stale;                 // sequences have moved since share: every one by itself
     bool inside;                // some token stands within its group's common pages
 };
@@ -460,6 +461,10 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
         L.units[0][wave] = units_incl;
         L.units[1][wave] = steps_incl;
     }
+    if (t == 0) {
+        L.front[0] = first;
+        L.front[1] = first16;
+    }
     barrier();
     int before = 0, any = 0, all_units = 0, all_steps = 0, units_before = 0, steps_before = 0;
     at.total = 0;
@@ -475,11 +480,13 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
         all_steps += L.units[1][i];
         any |= L.flag[1][i];
     }
+    int most = wave_bcast(L.front[0]);          // (the first group's, which is the one as a rule)
     at.tile = kTile;
     if (wave_bcast(all_steps) <= kFewSteps) {
         // (a unit has a page at least: the times are small)
         const auto time = [](int u, int s) { return u * kCost16.setup + s * kCost16.page; };
         at.tile = 16;
+        most = wave_bcast(L.front[1]);
         at.total = time(all_units, all_steps);
         before = time(units_before, steps_before);
         incl = time(units_incl, steps_incl);
@@ -497,7 +504,13 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
     if (any & 1) return false;
     at.shares = shares_of(at.total);
     if (wg >= at.shares) return false;
-    const int off = Split(at.total, at.shares).first(wg) - (before + incl - n);
+    // Workgroups that are one die's take shares that follow each other, so that they meet a
+    // group's pages in one L2 (eight groups of 16 sequences with 4 tokens fetch 76 MB where they
+    // took 239, 101 us and 103); not where a group has most of the work: the eight dies come to its
+    // pages in turn then, unit after unit (16 sequences of 4,100 21.8 us, and 22.4).
+    const bool spread = at.shares < kGrid || 2 * (int64_t)most > at.total;
+    at.wg = spread ? wg : (wg & 7) * (kGrid / 8) + (wg >> 3);
+    const int off = Split(at.total, at.shares).first(at.wg) - (before + incl - n);
     if (off >= 0 && off < first) {
         L.item = w;
         L.off = off;
@@ -1055,9 +1068,10 @@ __device__ __forceinline__ void attend16(const SharedParams& P, PageLds& L, cons
 __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     PageLds& L = *reinterpret_cast<PageLds*>(lds);
-    const int t = threadIdx.x, wg = blockIdx.x;
+    const int t = threadIdx.x;
     Place place;
-    if (!locate(P, L, wg, place)) return;
+    if (!locate(P, L, blockIdx.x, place)) return;
+    const int wg = place.wg;
     const Split share(place.total, place.shares);
     const int64_t all_rows = (int64_t)P.n_tokens * P.n_heads;
     const int end = share.first(wg + 1);
