@@ -14,6 +14,13 @@
 // units follow each other, and a workgroup a CU takes an equal share of them, across units
 // where it has to, so that neither the groups' sizes nor the lengths leave a CU idle. The
 // parts go to the caller's plan, and a second launch adds those of a row, in order.
+//
+// Measured, a layer, 16 heads, both launches in a graph: 4 sequences of 1,000 + 40 positions 13.5 us
+// (latency: the unit, its queries and first page, the join); 64 behind 8,192, 500 own, 44.6
+// (19 GFLOP, 15 us at a library's rate: eight pages a workgroup after a beginning of 8 us); 8
+// groups of 16 behind 4,000, 300 own, 4 tokens each, 101 (76 GFLOP, 58 us); 2 of 128 behind
+// 16,300, 1,000 own, 180 (153 GFLOP, 117 us). The large ones are bound by the instructions of a
+// page: the matrix unit has 39% of the time, other vector instructions 45%.
 #include "attend_tile.h"
 
 namespace fleet_moe {
@@ -620,6 +627,9 @@ __device__ __forceinline__ void issue_page(const SharedParams& P, PageLds& L, in
 // with 32 positions, so that a widened K operand serves two tiles; it exchanges halves with
 // its partner, makes the weights of one tile and 32 positions, and adds its 64 columns of O
 // for all rows over the whole page, where a widened V operand serves four tiles.
+//
+// A page takes 4,450 cycles, of which the matrix unit has 2,235 (69 instructions of 16 cycles of
+// each of a SIMD's two waves).
 //
 // Three pages are in work between two barriers: the scores of page k + 2, the weights of page
 // k + 1 and the products of page k, none of which needs another, so that matrix and vector

@@ -392,7 +392,8 @@ typedef struct fleet_cache {
  * cache; about 34 MB). 0 for sizes outside the limits above. Its first 256 bytes are
  * zero before the first call. Its status word (fleet_moe_workspace_status; the uint32
  * at byte 8, cleared by writing 0) collects the FLEET_MOE_ABORT_* bits named below.
- * It also holds whether the last fleet_cache_grow was refused. */
+ * It also holds whether the last fleet_cache_grow was refused, and how often sequences
+ * were moved. */
 size_t fleet_cache_workspace_bytes(int32_t n_pages, int32_t n_seqs);
 
 /* Reorders, forks and frees sequences: row i of table and lens becomes what row
@@ -574,7 +575,9 @@ int fleet_cache_share(const fleet_cache* cache, const int32_t* groups, int32_t n
                       size_t workspace_bytes, hipStream_t stream);
 
 /* fleet_cache_attend without a window, the pages that a group shares read once for all
- * its rows: what it takes, sees and leaves is as there. (The probabilities are
+ * its rows: what it takes, sees and leaves is as there, for less time the more sequences
+ * share and the more of their positions (DeepSeek-V2-Lite's 16 heads, one layer: 4 sequences
+ * of 1,040 13 us as there, 64 behind 8,192 45 for 62, 256 behind two times 16,300 180 for 382). (The probabilities are
  * rounded to bf16's 8 bits before the second product, or to 16 bits where the call has few
  * pages: what that is follows from starts, lengths and groups.) plan: as
  * fleet_cache_share left it, for at least as many tokens and heads. n_tokens *
