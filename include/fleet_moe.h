@@ -576,10 +576,10 @@ int fleet_cache_share(const fleet_cache* cache, const int32_t* groups, int32_t n
 
 /* fleet_cache_attend without a window, the pages that a group shares read once for all
  * its rows: what it takes, sees and leaves is as there, for less time the more sequences
- * share and the more of their positions (DeepSeek-V2-Lite's 16 heads, one layer: 4 sequences
- * of 1,040 13 us as there, 64 behind 8,192 45 for 62, 256 behind two times 16,300 180 for 382). (The probabilities are
- * rounded to bf16's 8 bits before the second product, or to 16 bits where the call has few
- * pages: what that is follows from starts, lengths and groups.) plan: as
+ * share and the more of their positions (16 heads, one layer: 4 sequences of 1,040
+ * 13 us as there; 64 behind 8,192 45 for 62; 256 behind two times 16,300 180 for 382). The
+ * probabilities are rounded to bf16's 8 bits before the second product, or, for a sequence's
+ * 16 rows or fewer and in calls of few pages, to 16 bits. plan: as
  * fleet_cache_share left it, for at least as many tokens and heads. n_tokens *
  * n_heads <= 2^20, (n_tokens * n_heads / 32 + 2 * n_seqs) * (11 * max_pages + 40) < 2^31. */
 int fleet_cache_attend_shared(const fleet_cache* cache, int32_t layer, const uint16_t* q,
