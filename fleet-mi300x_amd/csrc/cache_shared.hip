@@ -853,10 +853,11 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
         wait_copies<0>();
         barrier();
         const uint2 fl = *reinterpret_cast<const uint2*>(L.flags[k & 1]);
+        asm volatile("" ::: "memory");          // (the copies' addresses while it is on its way)
+        if (tp == 0 && k + kPageRing < cnt) issue(k + kPageRing, b);    // where step k was
         const int flags = wave_bcast((int)(fl.x | fl.y));
         if (flags) mend(k, flags & 0x02020202);
         l += sum;
-        if (tp == 0 && k + kPageRing < cnt) issue(k + kPageRing, b);    // where step k was
         // Of a SIMD's two waves (w and w + 4) one makes its weights while the other multiplies.
         // (The asm keeps each in its place: the compiler would fetch both's operands before.)
         if (tp != 0) {
