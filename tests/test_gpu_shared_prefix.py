@@ -130,6 +130,28 @@ def test_many_sequences_and_few():
         compare(b, q, counts, out, lse)
 
 
+@pytest.mark.parametrize("heads", [1, 16])
+def test_more_sequences_than_threads(heads):
+    """700 sequences in three groups and by themselves, units of 16 rows and of 64; a thread
+    finds the work of two of them."""
+    sizes, extra = [300, 200, 170], [500] * 30
+    b, rng, groups = forked(62, [700, 129, 64], [[5 + i % 90 for i in range(n)] for n in sizes],
+                            extra=extra)
+    n = sum(sizes) + len(extra)
+    counts = [1 + (i % 50 == 0) for i in range(n)]
+    at = np.concatenate([[0], np.cumsum(counts)])
+    q = query(rng, sum(counts), heads)
+    p = plan(b, groups, sum(counts), heads)
+    assert p.pages.tolist() == [10, 2, 1]
+    out, lse = p.attend(to_dev(q), starts(counts))
+    got, gl = ref.values(out.cpu().numpy()), lse.cpu().numpy()
+    for s in [0, 1, 50, 298, 299, 300, 301, 499, 500, 511, 512, 513, 669, 670, 671, 698, 699]:
+        total, rows = b.ref.lens[s], slice(at[s], at[s + 1])
+        want, wl, tol, tl = ref.attend(b.ref.values(s), q[rows], range(total - counts[s], total), SCALE)
+        assert (np.abs(got[rows] - want) <= tol).all() and (np.abs(gl[rows] - wl) <= tl).all(), s
+    assert b.dev.status() == 0
+
+
 @both_heights
 def test_tokens_inside_the_common_pages(tall):
     """Sequences that agree to the end: tokens stand in common pages and see them up to their own
