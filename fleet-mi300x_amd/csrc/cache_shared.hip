@@ -21,6 +21,8 @@
 // groups of 16 behind 4,000, 300 own, 4 tokens each, 101 (76 GFLOP, 58 us); 2 of 128 behind
 // 16,300, 1,000 own, 180 (153 GFLOP, 117 us). The large ones are bound by the instructions of a
 // page: the matrix unit has 39% of the time, other vector instructions 45%.
+#include <stddef.h>
+
 #include "attend_tile.h"
 
 namespace fleet_moe {
@@ -399,8 +401,8 @@ __device__ __forceinline__ int common_position(const TileRow& r) {
 
 struct PageLds {
     __attribute__((aligned(16))) uint8_t tile[kPageRing][4 * kBlockStep];
-    u32x4 p[2][4][2][64];       // [step parity][tile][half of the page][lane] (first: the last
-                                // of the queries, read before a weight is written)
+    u32x4 p[2][4][2][64];       // [step parity][tile][half of the page][lane] (p and `half` hold
+                                // the rest of the queries first)
     f32x4 half[2][kGridWaves][2][64];   // [step parity] half of the scores of a tile and two
                                         // blocks
     uint32_t scale[kPageRing][8];
@@ -412,7 +414,11 @@ struct PageLds {
     int at, off;
 };
 static_assert(sizeof(PageLds) <= 160 * 1024, "");
-static_assert(kTile * (2 * kRow + 16) <= 2 * 4 * kBlockStep + 16 * 1024, "");
+static_assert(kPageRing == 3 && offsetof(PageLds, p) == sizeof(PageLds::tile) &&
+                  offsetof(PageLds, half) == offsetof(PageLds, p) + sizeof(PageLds::p) &&
+                  kTile * (2 * kRow + 16) <=
+                      4 * kBlockStep + sizeof(PageLds::p) + sizeof(PageLds::half),
+              "");
 
 // The sequence in whose steps workgroup wg begins, and where, into L: a thread a sequence, or
 // two.
@@ -554,7 +560,7 @@ __device__ __forceinline__ bool valid(const PageList& h, int i) {
     return !(h.bad >> (i - h.from) & 1);
 }
 
-// The queries of a unit go through the ring before its pages: a lane's own loads of them, 16
+// The queries of a unit go through LDS, where its later pages come: a lane's own loads of them, 16
 // bytes of 16 rows at a time, took 12,000 cycles for 64 rows (a page's step takes 4,450). Rows
 // lie 16 bytes further apart than they are long, so that the operands of 16 rows fall into
 // different banks.
@@ -650,11 +656,11 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
         turn_to(P, u, pages, off + k, off + cnt, lane);
         issue_page(P, L, page_of(pages, off + k), b, wave, lane);
     };
-    // the first page's copies, and the queries'
+    // the copies of the first two pages, a wave of four a block, and the queries', behind them
     if (cnt > 0) {
         turn_to(P, u, pages, off, off + cnt, lane);
-        if (tp == 0) issue(0, 0);
-        copy_q<kTile / kGridWaves>(P, L, u, 1, wave, lane);
+        if (tp < cnt) issue_page(P, L, page_of(pages, off + tp), tp, wave & 3, lane);
+        copy_q<kTile / kGridWaves>(P, L, u, kPageRing - 1, wave, lane);
     }
     TileRow r = tile_row(P, u, u.row0 + mine * 16 + n);
     set_position(P, u, r);
@@ -678,8 +684,8 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
     wait_copies<0>();
     barrier();
     bf16x8 q[2][kTileHalf];                     // of `mine` and of the pair's other tile
-    read_q(L, 1, mine * 16 + n, g, half, q[0]);
-    read_q(L, 1, (mine ^ 1) * 16 + n, g, half, q[1]);
+    read_q(L, kPageRing - 1, mine * 16 + n, g, half, q[0]);
+    read_q(L, kPageRing - 1, (mine ^ 1) * 16 + n, g, half, q[1]);
 
     const auto score = [&](int k, int b) {
         u32x4 c[2][4];
@@ -834,15 +840,13 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
     };
 
     if (cnt > 0) {
+        barrier();                              // q has been read: its place is free
+        if (tp == 0 && kPageRing - 1 < cnt) issue(kPageRing - 1, kPageRing - 1);
         score(0, 0);
-        barrier();                              // (and q has been read: its place is free)
-        if (tp == 0)
-            for (int k = 1; k < kPageRing && k < cnt; ++k) issue(k, k);
+        barrier();
         join(0);
         finish(0);
         fetch(0);
-        wait_copies<0>();
-        barrier();
         if (cnt > 1) score(1, 1);
     }
     // Step k: behind the barrier the weights of k, both halves of the scores of k + 1 and the
