@@ -68,6 +68,8 @@ def check(x, y=None, norm=None, post=None, gate=None, scale=1.0, eps=1e-6, got=N
 
 SIZES = [(1, 2048), (3, 2048), (1100, 2048), (5, 1), (2, 7), (4, 8), (3, 577), (1030, 577), (2, 2056),
          (3, 4100), (2, 8192), (2, 8200), (1, 32768), (1, 12345)]
+# the ends of what a number of threads holds
+SIZES += [(3, w) for w in (512, 513, 1024, 1025, 1536, 1537, 2049, 4096, 4097, 16384, 16385, 24576, 24577)]
 
 
 @pytest.mark.parametrize("rows, width", SIZES)
