@@ -143,6 +143,21 @@ def test_parts_of_wider_rows():
     check(r.rotate(one, i32(pos)), want, both, False)
 
 
+@pytest.mark.parametrize("dtype", [BITS, F32])
+@pytest.mark.parametrize("tokens", [2, 3000])
+@pytest.mark.parametrize("width, at", [(192, 128), (83, 7), (100, 31), (64 + 12, 0)])
+def test_other_values_keep_their_bits(dtype, tokens, width, at):
+    """What is not rotated is copied, whatever its bits are."""
+    ints = torch.int16 if dtype == BITS else torch.int32
+    info = torch.iinfo(ints)
+    x = torch.randint(info.min, info.max + 1, (tokens, 5, width), device="cuda", dtype=ints)
+    rest = torch.ones(width, dtype=torch.bool, device="cuda")
+    rest[at: at + 64] = False
+    r, p = ops.Rotary(rope.frequencies()), i32(np.arange(tokens))
+    got = r.rotate(x.view(dtype), p, at=at).view(ints)
+    assert torch.equal(got[..., rest], x[..., rest])
+
+
 @pytest.mark.parametrize("dtype, tokens, width, at", [(F32, 5500, 192, 128), (BITS, 11_000, 193, 3)])
 def test_more_than_the_caches_hold(dtype, tokens, width, at):
     """Results of 64 MB and more, of 16 heads, and in place."""
