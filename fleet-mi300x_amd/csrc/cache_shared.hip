@@ -15,12 +15,12 @@
 // where it has to, so that neither the groups' sizes nor the lengths leave a CU idle. The
 // parts go to the caller's plan, and a second launch adds those of a row, in order.
 //
-// Measured, a layer, 16 heads, both launches in a graph: 4 sequences of 1,000 + 40 positions 13.5 us
-// (latency: the unit, its queries and first page, the join); 64 behind 8,192, 500 own, 44.6
+// Measured, a layer, 16 heads, both launches in a graph: 4 sequences of 1,000 + 40 positions 13.4 us
+// (latency: the unit, its queries and first page, the join); 64 behind 8,192, 500 own, 44.3
 // (19 GFLOP, 15 us at a library's rate: eight pages a workgroup after a beginning of 8 us); 8
 // groups of 16 behind 4,000, 300 own, 4 tokens each, 101 (76 GFLOP, 58 us); 2 of 128 behind
-// 16,300, 1,000 own, 180 (153 GFLOP, 117 us). The large ones are bound by the instructions of a
-// page: the matrix unit has 39% of the time, other vector instructions 45%.
+// 16,300, 1,000 own, 177 (153 GFLOP, 117 us). The large ones are bound by the instructions of a
+// page: the matrix unit has 40% of the time, other vector instructions 45%.
 #include <stddef.h>
 
 #include "attend_tile.h"
