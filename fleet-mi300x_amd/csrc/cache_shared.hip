@@ -15,12 +15,12 @@
 // where it has to, so that neither the groups' sizes nor the lengths leave a CU idle. The
 // parts go to the caller's plan, and a second launch adds those of a row, in order.
 //
-// Measured, a layer, 16 heads, both launches in a graph: 4 sequences of 1,000 + 40 positions 13.4 us
-// (latency: the unit, its queries and first page, the join); 64 behind 8,192, 500 own, 44.3
+// Measured, a layer, 16 heads, both launches in a graph: 4 sequences of 1,000 + 40 positions 13.5 us
+// (latency: the unit, its queries and first page, the join); 64 behind 8,192, 500 own, 48.3
 // (19 GFLOP, 15 us at a library's rate: eight pages a workgroup after a beginning of 8 us); 8
-// groups of 16 behind 4,000, 300 own, 4 tokens each, 101 (76 GFLOP, 58 us); 2 of 128 behind
-// 16,300, 1,000 own, 177 (153 GFLOP, 117 us). The large ones are bound by the instructions of a
-// page: the matrix unit has 40% of the time, other vector instructions 45%.
+// groups of 16 behind 4,000, 300 own, 4 tokens each, 118 (76 GFLOP, 58 us); 2 of 128 behind
+// 16,300, 1,000 own, 209 (153 GFLOP, 117 us). The large ones are bound by the instructions of a
+// page, half as many matrix instructions again as the formula has: weights are two operands.
 #include <stddef.h>
 
 #include "attend_tile.h"
@@ -267,15 +267,15 @@ __device__ __forceinline__ Item lane_of(const Item& v, int lane) {
 }
 
 // What the work is divided by: the time of a unit's beginning and end, and of a page, for units
-// of up to 16 rows and of more, in 400 cycles (a page takes 3,250 and 4,450; with beginnings of
-// 18 and 40, or 30 and 60, 13 calls of 13 to 185 us take 1 to 1.5% longer, their mean).
+// of up to 16 rows and of more, in 500 cycles (a page takes 3,250 and 5,500; with 24, 8 and 40, 11
+// twelve calls of 13 to 290 us take 1.4% longer, their mean, with 20, 7 and 33, 11 1.5%).
 // A workgroup does the pages whose time begins in its share.
 struct Cost {
     int setup, page;
     // How many pages begin before `time`.
     __device__ __forceinline__ int begun(int time) const;
 };
-constexpr Cost kCost16{24, 8}, kCost64{40, 11};
+constexpr Cost kCost16{18, 6}, kCost64{36, 11};
 __device__ __forceinline__ int Cost::begun(int time) const {
     const int t = time > setup ? time - setup : 0;        // (divided by constants)
     return page == kCost16.page ? (t + kCost16.page - 1) / kCost16.page
@@ -283,8 +283,8 @@ __device__ __forceinline__ int Cost::begun(int time) const {
 }
 // Units have 64 rows, or 16 where there are few pages: up to eight a workgroup of 16 rows take
 // less time than the two of 64 rows, with a unit's beginning and the parts to be joined (16
-// sequences of 4,100 positions 24.0 us, in 64 rows 28.6; with eleven, 32 in eight groups 32.8 us,
-// in 64 rows 31.6).
+// sequences of 4,100 positions 20.9 us, in 64 rows 30.0; up to eleven, 32 in eight groups would
+// take 28.2 for 30.5).
 constexpr int kFewSteps = 8 * kGrid;
 struct Sizes {
     int rows0, units0, rows1, units1;
@@ -401,10 +401,10 @@ __device__ __forceinline__ int common_position(const TileRow& r) {
 
 struct PageLds {
     __attribute__((aligned(16))) uint8_t tile[kPageRing][4 * kBlockStep];
-    u32x4 p[2][4][2][64];       // [step parity][tile][half of the page][lane] (p and `half` hold
-                                // the rest of the queries first)
-    f32x4 half[2][kGridWaves][2][64];   // [step parity] half of the scores of a tile and two
-                                        // blocks
+    u32x4 p[2][4][2][64];       // [step parity][tile][half of the page][lane], and what the
+    u32x4 left[2][4][2][64];    // weights' rounding leaves (p, this and `half` hold the rest of
+                                // the queries first)
+    f32x4 half[kGridWaves][2][64];      // half of the scores of a tile and two blocks
     uint32_t scale[kPageRing][8];
     int flag[2][kGridWaves], units[2][kGridWaves], front[2];
     __attribute__((aligned(8))) uint8_t flags[2][kGridWaves];   // (64 rows) 1: a row's reference
@@ -415,9 +415,10 @@ struct PageLds {
 };
 static_assert(sizeof(PageLds) <= 160 * 1024, "");
 static_assert(kPageRing == 3 && offsetof(PageLds, p) == sizeof(PageLds::tile) &&
-                  offsetof(PageLds, half) == offsetof(PageLds, p) + sizeof(PageLds::p) &&
-                  kTile * (2 * kRow + 16) <=
-                      4 * kBlockStep + sizeof(PageLds::p) + sizeof(PageLds::half),
+                  offsetof(PageLds, left) == offsetof(PageLds, p) + sizeof(PageLds::p) &&
+                  offsetof(PageLds, half) == offsetof(PageLds, left) + sizeof(PageLds::left) &&
+                  kTile * (2 * kRow + 16) <= 4 * kBlockStep + sizeof(PageLds::p) +
+                                                 sizeof(PageLds::left) + sizeof(PageLds::half),
               "");
 
 // The sequence in whose steps workgroup wg begins, and where, into L: a thread a sequence, or
@@ -561,7 +562,7 @@ __device__ __forceinline__ bool valid(const PageList& h, int i) {
 }
 
 // The queries of a unit go through LDS, where its later pages come: a lane's own loads of them, 16
-// bytes of 16 rows at a time, took 12,000 cycles for 64 rows (a page's step takes 4,450). Rows
+// bytes of 16 rows at a time, took 12,000 cycles for 64 rows (a page's step takes 5,500). Rows
 // lie 16 bytes further apart than they are long, so that the operands of 16 rows fall into
 // different banks.
 constexpr int kQueryStep = 2 * kRow + 16;
@@ -634,13 +635,19 @@ __device__ __forceinline__ void issue_page(const SharedParams& P, PageLds& L, in
 // its partner, makes the weights of one tile and 32 positions, and adds its 64 columns of O
 // for all rows over the whole page, where a widened V operand serves four tiles.
 //
-// A page takes 4,450 cycles, of which the matrix unit has 2,235 (69 instructions of 16 cycles of
+// The weights are two operands, bf16 and what that leaves: 16 bits, as in attend16, so that what
+// a sequence gets does not lose bits when other requests make the units higher. (With the first
+// alone a page takes 4,450 cycles, 64 sequences 44 us for 48, 256 176 for 209, and sums of weights
+// that nearly cancel are lost.)
+//
+// A page takes 5,500 cycles, of which the matrix unit has 3,264 (102 instructions of 16 cycles of
 // each of a SIMD's two waves).
 //
-// Three pages are in work between two barriers: the scores of page k + 2, the weights of page
-// k + 1 and the products of page k, none of which needs another, so that matrix and vector
-// instructions and reads of LDS run beside each other. The codes of V are read a page ahead, so
-// that three places of the ring suffice.
+// Three pages are in work in a step: the scores of page k + 2, the weights of page k + 1 and the
+// products of page k, none of which needs another, so that matrix and vector instructions and
+// reads of LDS run beside each other. The codes of V are read a page ahead, so that three places
+// of the ring suffice. The LDS has room for one page's halves of scores: those of page k + 2 come
+// behind a second barrier.
 __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, const Unit& u, int off,
                                          int cnt, int64_t to_part) {
     constexpr int kCols = kC / 16 / kGridWaves; // of 16
@@ -687,7 +694,7 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
     read_q(L, kPageRing - 1, mine * 16 + n, g, half, q[0]);
     read_q(L, kPageRing - 1, (mine ^ 1) * 16 + n, g, half, q[1]);
 
-    const auto score = [&](int k, int b) {
+    const auto score = [&](int b) {
         u32x4 c[2][4];
         uint2 e[2];
         uint32_t f[2][2];
@@ -722,7 +729,7 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             own[j] = y[0][j];
-            L.half[k & 1][wave][j][lane] = y[1][j];
+            L.half[wave][j][lane] = y[1][j];
         }
     };
     const auto weigh = [&](int k) {
@@ -733,15 +740,16 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
             p0[j] = exp2_(fmaf(z[0][j], P.scale, -down));
             p1[j] = exp2_(fmaf(z[1][j], P.scale, -down));
         }
-        const uint2 a = weights(p0), b = weights(p1);
+        const uint2 a = weights(p0), b = weights(p1), c = rest(p0, a), d = rest(p1, b);
         L.p[k & 1][mine][bp][lane] = u32x4{a.x, a.y, b.x, b.y};
+        L.left[k & 1][mine][bp][lane] = u32x4{c.x, c.y, d.x, d.y};
         sum = ((p0[0] + p0[1]) + (p0[2] + p0[3])) + ((p1[0] + p1[1]) + (p1[2] + p1[3]));
     };
     // The scores of step k whole, hidden where they are not seen, and whether some are not finite.
     bool stray = false;
     const auto join = [&](int k) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) z[j] = own[j] + L.half[k & 1][wave ^ 2][j][lane];
+        for (int j = 0; j < 2; ++j) z[j] = own[j] + L.half[wave ^ 2][j][lane];
         turn_to(P, u, pages, off + k, off + cnt, lane);
         const bool ok = valid(pages, off + k);
         const int base = (u.page0 + off + k) * kPage + bp * 32;
@@ -820,34 +828,41 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
     };
     // O over step k
     const auto add = [&](int k) {
-        bf16x8 pb[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) pb[h][j] = __builtin_bit_cast(bf16x8, L.p[k & 1][j][h][lane]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            bf16x8 pb[4], pr[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                pb[j] = __builtin_bit_cast(bf16x8, L.p[k & 1][j][h][lane]);
+                pr[j] = __builtin_bit_cast(bf16x8, L.left[k & 1][j][h][lane]);
+            }
             const float sa = any_scale(f[h][0]), sb = any_scale(f[h][1]);
 #pragma unroll
             for (int i = 0; i < kCols; ++i) {
                 const bf16x8 a = widen((uint32_t)v[h][i].x, (uint32_t)v[h][i].y, sa, sb);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j][i] = mfma(a, pb[h][j], acc[j][i]);
+                for (int j = 0; j < 4; ++j) acc[j][i] = mfma(a, pb[j], acc[j][i]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j][i] = mfma(a, pr[j], acc[j][i]);
             }
         }
-        ones = mfma(__builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes}),
-                    __builtin_bit_cast(bf16x8, L.p[k & 1][wave & 3][wave >> 2][lane]), ones);
+        const bf16x8 one = __builtin_bit_cast(bf16x8, u32x4{kOnes, kOnes, kOnes, kOnes});
+        ones = mfma(one, __builtin_bit_cast(bf16x8, L.p[k & 1][wave & 3][wave >> 2][lane]), ones);
+        ones = mfma(one, __builtin_bit_cast(bf16x8, L.left[k & 1][wave & 3][wave >> 2][lane]), ones);
     };
 
     if (cnt > 0) {
         barrier();                              // q has been read: its place is free
         if (tp == 0 && kPageRing - 1 < cnt) issue(kPageRing - 1, kPageRing - 1);
-        score(0, 0);
+        score(0);
         barrier();
         join(0);
         finish(0);
         fetch(0);
-        if (cnt > 1) score(1, 1);
+        if (cnt > 1) {
+            barrier();                          // the halves of step 0 have been read
+            score(1);
+        }
     }
     // Step k: behind the barrier the weights of k, both halves of the scores of k + 1 and the
     // rows of k + 2 are there.
@@ -878,7 +893,10 @@ __device__ __forceinline__ void attend64(const SharedParams& P, PageLds& L, cons
             add(k);
             asm volatile("; products made, too" ::: "memory");
         }
-        if (k + 2 < cnt) score(k + 2, b2);
+        if (k + 2 < cnt) {
+            barrier();                          // the halves of step k + 1 have been read
+            score(b2);
+        }
         if (k + 1 < cnt) fetch(b1);
         b = b1;
         asm("" : "+s"(b));
@@ -967,7 +985,7 @@ __device__ __forceinline__ void attend16(const SharedParams& P, PageLds& L, cons
         const uint2 a = *reinterpret_cast<const uint2*>(block + 8 * 1024 + half * 8);
         y0 = mfma(widen(a.x, a.y, sp, sp), q[8], y0);
         next = y0 + y1;
-        if (!weighs) L.half[0][blk][0][lane] = next;
+        if (!weighs) L.half[blk][0][lane] = next;
     };
     const auto weigh = [&](int k) {
         const float down = ref == -INFINITY ? 0.f : ref;
@@ -978,7 +996,7 @@ __device__ __forceinline__ void attend16(const SharedParams& P, PageLds& L, cons
         reinterpret_cast<uint2*>(&L.p[k & 1][1][blk >> 1][lane])[blk & 1] = rest(p, w);
     };
     const auto finish = [&](int k) {
-        z = next + L.half[0][blk][0][lane];
+        z = next + L.half[blk][0][lane];
         turn_to(P, u, pages, off + k, off + cnt, lane);
         const bool ok = valid(pages, off + k);
         const int base = (u.page0 + off + k) * kPage + blk * kBlock;

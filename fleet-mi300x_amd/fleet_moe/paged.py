@@ -235,8 +235,8 @@ class SharedPrefix:
     """attend() for sequences that share their first pages: a request's beams, or requests
     behind one prompt. `groups` int32 [n + 1] on the device: sequences groups[g] ..
     groups[g + 1] - 1 are group g, others are by themselves. The pages that all of a group
-    name first are read once for all its rows: 64 sequences behind 8,192 positions take 45 us
-    for 62, 256 behind two times 16,300 180 for 382, four of 1,000 as long as with attend().
+    name first are read once for all its rows: 64 sequences behind 8,192 positions take 48 us
+    for 62, 256 behind two times 16,300 210 for 382, four of 1,000 as long as with attend().
 
     update() finds them (`pages` int32 [n], how many), and is called before the first
     attend(), after remap(), and after changes of table or lens by other means; grow() and
