@@ -134,8 +134,9 @@ __device__ __forceinline__ float row_sum(float v, float* lds) {
 }
 
 // Divides a row by rms(row). Squares beyond fp32 are taken again of 2^-75 of the values: then
-// the sum of 32,768 of the largest is below 2^122, and eps is nothing beside it. (A row with
-// an infinity gets NaN there and zeros elsewhere, as the formula says.)
+// the sum of 32,768 of the largest is below 2^122, and eps has the same 2^-150 (1e30 is 2% of the
+// mean of 32,768 squares of 2^105). (A row with an infinity gets NaN there and zeros elsewhere, as
+// the formula says.)
 template <int kThreads, class R>
 __device__ __forceinline__ void unit(R& r, int width, float eps, float* lds) {
     float s = 0.f;
@@ -151,7 +152,7 @@ __device__ __forceinline__ void unit(R& r, int width, float eps, float* lds) {
             s = fmaf(d, d, s);
         }
         s = row_sum<kThreads>(s, lds);
-        eps = 0.f;
+        eps = eps * 0x1p-75f * 0x1p-75f;
     }
     float inv = 1.f / sqrtf(s / (float)width + eps);
     if (large) {                                          // (2^-75 in two steps: in range)
