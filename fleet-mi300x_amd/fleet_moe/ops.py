@@ -89,6 +89,13 @@ def _own(stream):
     return _HERE if stream is None else torch.cuda.stream(stream)
 
 
+def _settle(t: torch.Tensor) -> None:
+    """The end of a constructor: waits for what it left on the current stream, so that the
+    first call may be on any. (In a capture that order is the graph's.)"""
+    if t.is_cuda and not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(t.device).synchronize()
+
+
 def _same_device(owner: torch.Tensor, **tensors) -> None:
     dev = owner.device
     for name, t in tensors.items():
@@ -365,10 +372,11 @@ class Rotary:
                  halves_out: bool = True, device="cuda"):
         if isinstance(freqs, torch.Tensor) and freqs.is_cuda:
             device = freqs.device
-        f = torch.as_tensor(freqs, dtype=torch.float64, device=device)
+        f = torch.as_tensor(freqs, dtype=torch.float64)
         if f.dim() != 1 or f.numel() < 1:
             raise ValueError(f"freqs: expected [dim / 2], got {tuple(f.shape)}")
-        self.turns = (f / (2.0 * math.pi)).contiguous()
+        self.turns = (f / (2.0 * math.pi)).contiguous().to(device)
+        _settle(self.turns)
         self.dim = 2 * f.numel()
         self._c = _lib.FleetRope(self.turns.data_ptr(), self.dim, bool(halves_in),
                                  bool(halves_out), float(magnitude))

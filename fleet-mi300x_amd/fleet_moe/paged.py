@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib
-from .ops import Rotary, _int32, _need, _on, _own, _ptr, _same_device, _stream
+from .ops import Rotary, _int32, _need, _on, _own, _ptr, _same_device, _settle, _stream
 
 ROW = _lib.CACHE_ROW
 LORA = 512
@@ -62,6 +62,7 @@ class PagedCache:
         # only the header (status word, the last grow's refusal) has to start as zero
         self.workspace = torch.empty(n, dtype=torch.uint8, device=self.device)
         self.workspace[:256].zero_()
+        _settle(self.workspace)
         self._ws = (self.workspace.data_ptr(), n)
         self._fn = {name: getattr(_lib.load(), name) for name, *_ in _lib.SYMBOLS
                     if name.startswith("fleet_cache_")}
@@ -259,6 +260,7 @@ class SharedPrefix:
         self.plan = torch.empty(n, dtype=torch.uint8, device=cache.device)
         self.plan[:256].fill_(255)              # of no state of the cache: nothing is shared yet
         self.pages = torch.zeros(groups.numel() - 1, dtype=torch.int32, device=cache.device)
+        _settle(self.plan)
         self._plan = (self.plan.data_ptr(), n)
 
     def update(self, stream=None) -> torch.Tensor:
