@@ -8,10 +8,10 @@
 // squares, and all waves compute an angle a thread (16 positions of 32 pairs) while the
 // rows are on their way.
 //
-// One row for each of 17 sequences: 5.0 us, the latency of the loads before the rows (start,
-// length, table), the angle and two barriers. 11,004 rows: 9.7 us (19 MB, 2 TB/s; a copy of as
+// One row for each of 17 sequences: 5.3 us, the latency of the loads before the rows (start,
+// length, table), the angle and two barriers. 11,004 rows: 10.8 us (19 MB, 1.8 TB/s; a copy of as
 // much takes 4): that latency once, with every workgroup of the call on the chip (70
-// registers; with 83 only two workgroups a CU, 13.5), and some 450 vector instructions a wave.
+// registers; with 83 only two workgroups a CU, 13.5), and 424 vector instructions a wave.
 #include <math.h>
 
 #include "cache_rows.h"

@@ -19,8 +19,9 @@
 // (latency: the unit, its queries and first page, the join); 64 behind 8,192, 500 own, 48.3
 // (19 GFLOP, 15 us at a library's rate: eight pages a workgroup after a beginning of 8 us); 8
 // groups of 16 behind 4,000, 300 own, 4 tokens each, 118 (76 GFLOP, 58 us); 2 of 128 behind
-// 16,300, 1,000 own, 209 (153 GFLOP, 117 us). The large ones are bound by the instructions of a
-// page, half as many matrix instructions again as the formula has: weights are two operands.
+// 16,300, 1,000 own, 208 (153 GFLOP, 117 us). The large ones are bound by the instructions of a
+// page, half as many matrix instructions again as the formula has, as weights are two operands: the
+// matrix unit has 49% of the time, other vector instructions 33%.
 #include <stddef.h>
 
 #include "attend_tile.h"
@@ -35,7 +36,7 @@ constexpr int kGrid = kShares / 2;      // workgroups
 constexpr int kGridWaves = 8;
 constexpr int kGridThreads = kGridWaves * 64;
 constexpr int kPageRing = 3;
-constexpr float kRise = 12.f;           // (8: 186 us where this takes 184)
+constexpr float kRise = 12.f;           // (8: 64 sequences 49.7 us where this takes 48.5)
 
 // The plan: what share found, and the parts of an attention.
 struct PlanHeader {
@@ -333,8 +334,8 @@ constexpr int kLeast = 11;
 static_assert(kLeast >= kCost64.page && kLeast >= kCost16.page, "");
 // How many workgroups take part. No share is shorter than a page's time (so that every one
 // between a unit's first and last has a part of it), and few pages are left to many only as
-// far as the parts are joined in less time than that saves (18: 4 sequences of 1,000 14.4 us, with
-// 11 13.4).
+// far as the parts are joined in less time than that saves (15: 4 sequences of 1,000 14.4 us, with
+// 11 13.5).
 __device__ __forceinline__ int shares_of(int total) {
     const int n = total / kLeast;
     return n < 1 ? total > 0 : n < kGrid ? n : kGrid;
@@ -525,9 +526,9 @@ __device__ __forceinline__ bool locate(const SharedParams& P, PageLds& L, int wg
     at.shares = shares_of(at.total);
     if (wg >= at.shares) return false;
     // Workgroups that are one die's take shares that follow each other, so that they meet a
-    // group's pages in one L2 (eight groups of 16 sequences with 4 tokens fetch 76 MB where they
-    // took 239, 101 us and 103); not where a group has most of the work: the eight dies come to its
-    // pages in turn then, unit after unit (16 sequences of 4,100 21.8 us, and 22.4).
+    // group's pages in one L2 (eight groups of 16 sequences with 4 tokens fetch 77 MB where they
+    // took 239, 119 us and 121); not where a group has most of the work: the eight dies come to its
+    // pages in turn then, unit after unit (16 sequences of 4,100 21.1 us, and 21.7).
     const bool spread = at.shares < kGrid || 2 * (int64_t)most > at.total;
     at.wg = spread ? wg : (wg & 7) * (kGrid / 8) + (wg >> 3);
     const int off = Split(at.total, at.shares).first(at.wg) - (before + incl - n);
@@ -668,7 +669,7 @@ __device__ __forceinline__ void issue_page(const SharedParams& P, PageLds& L, in
 //
 // The weights are two operands, bf16 and what that leaves: 16 bits, as in attend16, so that what
 // a sequence gets does not lose bits when other requests make the units higher. (With the first
-// alone a page takes 4,450 cycles, 64 sequences 44 us for 48, 256 176 for 209, and sums of weights
+// alone a page takes 4,450 cycles, 64 sequences 44 us for 48, 256 177 for 208, and sums of weights
 // that nearly cancel are lost.)
 //
 // A page takes 5,500 cycles, of which the matrix unit has 3,264 (102 instructions of 16 cycles of
@@ -1231,9 +1232,9 @@ __global__ __launch_bounds__(kGridThreads, 1) void shared_kernel(SharedParams P)
 // Adds the parts of 16 rows, those over common pages first: lane (g, n) has four columns of row
 // n. A wave 64 columns and all parts of their rows, or, where there are few rows of many parts, an
 // eighth of the parts, and the workgroup's eight waves their sum (shared and joined, 64 sequences
-// of 16 heads 47.0 us and 48.2 in one wave each; 256 sequences 182 us and 180).
+// of 16 heads 48.5 us and 50.3 in one wave each; 256 sequences 209 us and 207).
 constexpr int kJoinParts = 2;                   // on their way together (four: more registers,
-                                                // 8,192 rows 109.1 us where this takes 108.3)
+                                                // the same time)
 constexpr int64_t kManyRows = 2048;
 template <bool kSplit>
 __global__ __launch_bounds__(kGridThreads) void join_kernel(SharedParams P) {

@@ -8,7 +8,7 @@
 // One pass: a row's values stay in registers from their load to h, so x, y and a gate of
 // every token are read once, x' and h written once, and those bytes are the bound. All
 // arithmetic is fp32; x' and h are each rounded once, and h is taken from x' before its
-// rounding. Measured: a row of 2,048 values 2.5 us, 250 rows 4.6; 16,000 rows
+// rounding. Measured: a row of 2,048 values 2.6 us, 250 rows 4.5; 16,000 rows
 // (328 MB, with a gate of every token) 61 us, 5.4 TB/s, where a large copy reaches 5.1.
 #include <math.h>
 

@@ -3,9 +3,9 @@
 //
 // A pair (a, b) of a head's values becomes (a cos - b sin, b cos + a sin), with the angle
 // of its position and frequency; the bytes of x and out bound many tokens, a launch's
-// latency few. An angle costs some sixty instructions and serves all heads of its token, so
+// latency few. An angle costs some seventy-five instructions and serves all heads of its token, so
 // a thread takes the same four pairs of several heads where there are enough tokens. Measured: one
-// token of 16 heads 2.6 us, 2,000 5.4; 8,001 whole heads of 192 fp32 values (197 MB) 39 us, a
+// token of 16 heads 2.6 us, 2,000 5.7; 8,001 whole heads of 192 fp32 values (197 MB) 39 us, a
 // large copy's 5.1 TB/s.
 #include <math.h>
 

@@ -577,7 +577,7 @@ int fleet_cache_share(const fleet_cache* cache, const int32_t* groups, int32_t n
 /* fleet_cache_attend without a window, the pages that a group shares read once for all
  * its rows: what it takes, sees and leaves is as there, for less time the more sequences
  * share and the more of their positions (16 heads, one layer: 4 sequences of 1,040
- * 13 us as there; 64 behind 8,192 48 for 62; 256 behind two times 16,300 210 for 382). The
+ * 13 us as there; 64 behind 8,192 48 for 62; 256 behind two times 16,300 208 for 382). The
  * probabilities have 16 bits in the second product, whatever else is in the call. plan: as
  * fleet_cache_share left it, for at least as many tokens and heads. n_tokens *
  * n_heads <= 2^20, (n_tokens * n_heads / 32 + 2 * n_seqs) * (11 * max_pages + 36) < 2^31. */
